@@ -65,7 +65,7 @@ def draw(rng):
             case = {"op": op, "rows": _spread(rng, 1, 16384), "cols": _spread(rng, 32, 28672, 32), "dtype": rng.choice(["f32", "f16", "bf16"])}
             cost, most = case["rows"] * case["cols"], _LARGEST_ROUND_TRIP
         elif op == "mx_product":
-            case = {"op": op, "M": _spread(rng, 1, 8192), "N": _spread(rng, 16, 28672), "K": _spread(rng, 32, 28672, 32), "dtype": rng.choice(["f16", "bf16"])}
+            case = {"op": op, "M": _spread(rng, 1, 8192), "N": _spread(rng, 16, 28672), "K": _spread(rng, 32, 28672, 32), "dtype": rng.choice(["f32", "f16", "bf16"])}
             cost, most = case["M"] * case["N"] * case["K"], _LARGEST_PRODUCT
         else:
             case = {"op": op, "M": _spread(rng, 1, 8192), "I": _spread(rng, 64, 28672, 8), "K": _spread(rng, 64, 8192, 8), "dtype": rng.choice(["f16", "bf16"]),
