@@ -32,7 +32,8 @@ typedef enum {
   QL_I8 = 3,
   QL_I4 = 4,     /* two values per byte, first element in the low nibble */
   QL_F8E4M3 = 5, /* e4m3fn: no infinities, 0x7F/0xFF are NaN, largest finite 448 */
-  QL_F4E2M1 = 6  /* e2m1fn (0, 0.5, 1, 1.5, 2, 3, 4, 6 and negatives): two per byte, first element in the low nibble */
+  QL_F4E2M1 = 6, /* e2m1fn (0, 0.5, 1, 1.5, 2, 3, 4, 6 and negatives): two per byte, first element in the low nibble */
+  QL_F8E8M0 = 7  /* e8m0fnu: byte b stands for 2^(b - 127), 0xFF for NaN; only block scales of the MXFP4 entries */
 } ql_dtype;
 
 typedef enum {
@@ -140,6 +141,18 @@ QL_API int ql_dequantize_nvfp4(const ql_tensor *data, const ql_tensor *scales, c
  * use ql_linear).  Takes scratch for the re-ordered scales from the stream-ordered allocator. */
 QL_API int ql_gemm_nvfp4(const ql_tensor *a, const ql_tensor *a_scales, const ql_tensor *a_global, const ql_tensor *b,
                          const ql_tensor *b_scales, const ql_tensor *b_global, ql_tensor *y, void *stream);
+
+/* Microscaled 4-bit floating point (the OCP MX format MXFP4; no reference operator): blocks of 32 values along the last
+ * axis share one e8m0 scale.  With m = max|block|:
+ *   scale = 2^max(floor(log2 m) - 2, -127)    (2^-127 for a block of zeros),
+ *   data  = e2m1(input / scale), round to nearest even, saturating at +-6, signs of zeros kept.
+ * The division is by a power of two, so data and scales are the format's, bit for bit.  A block that holds an infinity or
+ * a NaN gets the scale NaN and zero data: it dequantizes to NaN.  input: f32 | f16 | bf16 [..., K], K % 32 == 0;
+ * data: QL_F4E2M1 of the input's shape (buffer of numel / 2 bytes); scales: QL_F8E8M0 [..., K / 32].
+ * ql_dequantize_mxfp4: output = data * scale, rounded to f32 | f16 | bf16.
+ * 16-byte aligned floating-point buffers and 4-byte aligned data (QL_ERR_UNSUPPORTED otherwise). */
+QL_API int ql_quantize_mxfp4(const ql_tensor *input, ql_tensor *data, ql_tensor *scales, void *stream);
+QL_API int ql_dequantize_mxfp4(const ql_tensor *data, const ql_tensor *scales, ql_tensor *output, void *stream);
 
 /* Weight-only linear layers, Y[M,N] = X[M,K] . dequantize(W)[N,K]^T with f32 accumulation
  * (linear.py:140-151 with quant_dtype set and no input scale).

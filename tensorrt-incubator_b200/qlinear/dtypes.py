@@ -25,7 +25,8 @@ bfloat16 = dtype("bfloat16", _lib.BF16, torch.bfloat16, 16)
 int8 = dtype("int8", _lib.I8, torch.int8, 8)
 int4 = dtype("int4", _lib.I4, None, 4)
 float8 = dtype("float8", _lib.F8E4M3, torch.float8_e4m3fn, 8)
-float4 = dtype("float4", _lib.F4E2M1, None, 4)   # e2m1; only produced by dynamic_quantize
+float4 = dtype("float4", _lib.F4E2M1, None, 4)   # e2m1; only produced by dynamic_quantize and quantize_mxfp4
+float8_e8m0 = dtype("float8_e8m0", _lib.F8E8M0, torch.float8_e8m0fnu, 8)   # powers of two; only MXFP4 block scales
 
 # plain types `cast` converts between (no kernel of this library involved)
 int32 = dtype("int32", -1, torch.int32, 32)
@@ -36,7 +37,7 @@ QUANTIZABLE_DTYPES = (float32, float16, bfloat16)
 QUANTIZED_DTYPES = (int8, int4, float8)
 MAXBOUND = {int8: 127.0, int4: 7.0, float8: 448.0}
 
-_BY_TORCH = {d.torch: d for d in (float32, float16, bfloat16, int8, float8, int32, int64, bool)}
+_BY_TORCH = {d.torch: d for d in (float32, float16, bfloat16, int8, float8, float8_e8m0, int32, int64, bool)}
 
 
 def from_torch(t) -> dtype:

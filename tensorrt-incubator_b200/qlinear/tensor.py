@@ -107,3 +107,16 @@ def empty_quantized(shape, qdtype: dt.dtype, device):
         n = math.prod(shape)
         return Int4Tensor(torch.empty((n + 1) // 2, dtype=torch.uint8, device=device), shape)
     return torch.empty(tuple(shape), dtype=qdtype.torch, device=device)
+
+
+def call_on(device, fn, *args, same_device=()) -> None:
+    """fn(*args, the current stream of `device`) with `device` current, whichever device was; every tensor of
+    `same_device` has to live there."""
+    for t in same_device:
+        if t.device != device:
+            raise _lib.QlError(_lib.ERR_INVALID_ARGUMENT, f"tensors must live on one device, got {device} and {t.device}")
+    if device.index is None or device.index == torch.cuda.current_device():
+        _lib.check(fn(*args, current_stream(device)))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, current_stream(device)))
