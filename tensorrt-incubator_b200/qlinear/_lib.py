@@ -71,6 +71,7 @@ SIGNATURES = {
     "ql_gemm_nvfp4": ([_T, _T, _T, _T, _T, _T, _T, _S], ctypes.c_int),
     "ql_quantize_mxfp4": ([_T, _T, _T, _S], ctypes.c_int),
     "ql_dequantize_mxfp4": ([_T, _T, _T, _S], ctypes.c_int),
+    "ql_gemm_mxfp4": ([_T, _T, _T, _T, _T, _S], ctypes.c_int),
     "ql_linear_w8a16": ([_T, _T, _T, _T, _S], ctypes.c_int),
     "ql_linear_w4a16": ([_T, _T, _T, _T, _S], ctypes.c_int),
     "ql_linear_weight_only": ([_T, _T, _T, _T, ctypes.c_uint32, _S], ctypes.c_int),

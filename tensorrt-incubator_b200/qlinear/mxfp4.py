@@ -40,3 +40,20 @@ def dequantize_mxfp4(data: Float4Tensor, scales: torch.Tensor, dtype: dt.dtype =
     s = scales.contiguous()   # kept alive across the call: a view only borrows the pointer
     call_on(data.device, _lib.lib().ql_dequantize_mxfp4, ql_view(data), ql_view(s), ql_view(y), same_device=(s, y))
     return y
+
+
+def gemm_mxfp4(a: Float4Tensor, a_scales: torch.Tensor, b: Float4Tensor, b_scales: torch.Tensor, out_dtype: dt.dtype = dt.bfloat16,
+               out=None) -> torch.Tensor:
+    """dequantize_mxfp4(a) @ dequantize_mxfp4(b)^T on the block-scaled tensor cores: a [M, K] (activations, any M from one
+    token up), b [N, K] (weights) and their scales as quantize_mxfp4 returns them; f32 sums, one rounding to `out_dtype`
+    (float32, float16 or bfloat16)."""
+    for t, what in ((a, "a"), (a_scales, "a_scales"), (b, "b"), (b_scales, "b_scales")):
+        require_cuda(t, what)
+    if not isinstance(a, Float4Tensor) or not isinstance(b, Float4Tensor):
+        raise QuantizeError("gemm_mxfp4: a and b must be Float4Tensor, as quantize_mxfp4 returns them")
+    if out is None and out_dtype not in dt.QUANTIZABLE_DTYPES:
+        raise QuantizeError(f"Unsupported data type in gemm_mxfp4. Supported data types are: {dt.QUANTIZABLE_DTYPES}. Got out_dtype={out_dtype}")
+    y = out if out is not None else torch.empty((a.shape[0], b.shape[0]), dtype=out_dtype.torch, device=a.device)
+    sa, sb = a_scales.contiguous(), b_scales.contiguous()   # kept alive across the call: a view only borrows the pointer
+    call_on(a.device, _lib.lib().ql_gemm_mxfp4, ql_view(a), ql_view(sa), ql_view(b), ql_view(sb), ql_view(y), same_device=(sa, b, sb, y))
+    return y

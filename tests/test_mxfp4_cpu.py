@@ -60,3 +60,23 @@ def test_quantize_and_dequantize_argument_rules():
         assert "aligned" in _err(call(_t(_lib.F32, [4, 64], 0x1008), q, s))
         assert "aligned" in _err(call(x, _t(_lib.F4E2M1, [4, 64], 0x1002), s))
         assert call(_t(_lib.F32, [0, 64], None), _t(_lib.F4E2M1, [0, 64], None), _t(_lib.F8E8M0, [0, 2], None)) == 0
+
+
+def test_product_argument_rules():
+    L = _lib.lib()
+    a, sa, b, sb, y = _t(_lib.F4E2M1, [4, 64]), _t(_lib.F8E8M0, [4, 2]), _t(_lib.F4E2M1, [8, 64]), _t(_lib.F8E8M0, [8, 2]), _t(_lib.BF16, [4, 8])
+    call = lambda a=a, sa=sa, b=b, sb=sb, y=y: L.ql_gemm_mxfp4(a, sa, b, sb, y, None)
+    assert "a is null" in _err(call(sa=None)) and "b is null" in _err(call(b=None))
+    assert "data must be f4E2M1FN" in _err(call(a=_t(_lib.I4, [4, 64])))
+    assert "scales f8E8M0FNU" in _err(call(sb=_t(_lib.F8E4M3, [8, 2])))
+    assert "must be 2-D" in _err(call(a=_t(_lib.F4E2M1, [256])))
+    assert "one entry per block of 32" in _err(call(sa=_t(_lib.F8E8M0, [4, 4])))
+    assert "one entry per block of 32" in _err(call(a=_t(_lib.F4E2M1, [4, 48]), sa=_t(_lib.F8E8M0, [4, 1])))
+    assert "inner dimensions differ" in _err(call(b=_t(_lib.F4E2M1, [8, 32]), sb=_t(_lib.F8E8M0, [8, 1])))
+    assert "y must be [M,N]" in _err(call(y=_t(_lib.BF16, [8, 4])))
+    assert "f32, f16 or bf16" in _err(call(y=_t(_lib.I8, [4, 8])))
+    assert "no data pointer" in _err(call(y=_t(_lib.BF16, [4, 8], None)))
+    assert "non-zero K" in _err(call(a=_t(_lib.F4E2M1, [4, 0], None), sa=_t(_lib.F8E8M0, [4, 0], None), b=_t(_lib.F4E2M1, [8, 0], None), sb=_t(_lib.F8E8M0, [8, 0], None)))
+    assert "16-byte aligned" in _err(call(b=_t(_lib.F4E2M1, [8, 64], 0x1008)))
+    assert "aligned to its type" in _err(call(y=_t(_lib.BF16, [4, 8], 0x1001)))
+    assert call(a=_t(_lib.F4E2M1, [0, 64], None), sa=_t(_lib.F8E8M0, [0, 2], None), y=_t(_lib.BF16, [0, 8], None)) == 0

@@ -1,0 +1,146 @@
+"""The MXFP4 product against the product in float64 of the very same operands.
+
+Bound: products of two e2m1 values under power-of-two scales are exact; an MMA adds 64 of them to the f32 accumulator and
+may truncate where it aligns them, at most 2 steps of 2^-23 of the largest magnitude in the sum, which S = sum |a||b|
+bounds.  With K / 64 MMAs and up to 8 partial sums added at the end, |error| <= (K / 64 + 8) 2^-22 S; the result type's
+rounding, half a step (eps / 2 of the value, or half the smallest subnormal), comes on top."""
+import numpy as np
+import pytest
+import torch
+
+import mx_reference as mx
+import qlinear as ql
+from helpers import randn
+
+pytestmark = pytest.mark.gpu
+
+
+def operand(rows, K, seed, std=1.0):
+    x = randn((rows, K), torch.float32, seed, std) * torch.exp(0.7 * randn((K,), torch.float32, seed + 1))
+    return ql.quantize_mxfp4(x)
+
+
+def wide(data, scales):
+    codes = mx.unpack(data.packed.cpu().numpy(), data.shape)
+    return torch.from_numpy(mx.values(codes, scales.view(torch.uint8).cpu().numpy())).cuda()
+
+
+def check(y, a, sa, b, sb, K):
+    A, B = wide(a, sa), wide(b, sb)
+    want, S = A @ B.T, A.abs() @ B.abs().T
+    f = torch.finfo(y.dtype)
+    bound = (K / 64 + 8) * 2.0 ** -22 * S
+    if y.dtype != torch.float32:
+        bound = bound + f.eps / 2 * want.abs() + f.smallest_normal * f.eps / 2
+    bad = ~((y.double() - want).abs() <= bound)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} off, worst {float((y.double() - want).abs().max())}, first {bad.nonzero()[0].tolist()}"
+    assert ql.lib().ql_gemm_status(None) == 0
+
+
+def guarded(M, N, dtype):
+    """A result with NaN rows before and behind it, to see what is written."""
+    whole = torch.full((M + 2, N), float("nan"), dtype=dtype, device="cuda")
+    return whole, whole[1:M + 1]
+
+
+# rows, columns and K with tails; one token; K of one block, of less and more than a 256-value step; scale rows of every alignment
+SMALL = [(1, 128, 256), (1, 1, 32), (3, 200, 96), (16, 129, 512), (17, 64, 2048), (32, 1000, 4128), (33, 130, 288), (64, 127, 1024), (65, 300, 320),
+         (128, 128, 8192), (129, 500, 1056), (333, 1001, 2080), (5, 4096, 11008), (300, 40, 64)]
+
+
+@pytest.mark.parametrize("M,N,K", SMALL)
+@pytest.mark.parametrize("out", [torch.float32, torch.float16, torch.bfloat16])
+def test_few_tiles(M, N, K, out):
+    a, sa = operand(M, K, 5000 + M)
+    b, sb = operand(N, K, 6000 + N, K ** -0.5)
+    whole, y = guarded(M, N, out)
+    ql.gemm_mxfp4(a, sa, b, sb, out=y)
+    check(y, a, sa, b, sb, K)
+    assert torch.isnan(whole[0]).all() and torch.isnan(whole[-1]).all()
+    again = ql.gemm_mxfp4(a, sa, b, sb, out_dtype=ql.dtypes.from_torch(out))
+    assert torch.equal(again, y)   # the same bits on every run
+
+
+# at least 148 tiles of 128 x 224: scales of whole 16-byte rows, and padded ones
+@pytest.mark.parametrize("M,N,K", [(2048, 4096, 512), (1700, 2600, 1056), (4100, 1120, 32), (2048, 2300, 2048), (640, 6700, 4640)])
+@pytest.mark.parametrize("out", [torch.float32, torch.float16, torch.bfloat16])
+def test_many_tiles(M, N, K, out):
+    a, sa = operand(M, K, 5100 + M)
+    b, sb = operand(N, K, 6100 + N, K ** -0.5)
+    whole, y = guarded(M, N, out)
+    ql.gemm_mxfp4(a, sa, b, sb, out=y)
+    check(y, a, sa, b, sb, K)
+    assert torch.isnan(whole[0]).all() and torch.isnan(whole[-1]).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(2, 200, 288), (600, 9000, 288)])
+def test_scales_of_every_size_and_nan(M, N, K):
+    """Scales from 2^-100 to 2^100 that cancel in the product; a NaN scale spoils its own row or column only."""
+    a, sa = operand(M, K, 5200)
+    b, sb = operand(N, K, 6200)
+    g = torch.Generator().manual_seed(7)
+    e = torch.randint(-100, 101, (K // 32,), generator=g)
+    sa8 = (sa.view(torch.uint8).int() + e.cuda()).to(torch.uint8).view(torch.float8_e8m0fnu)
+    sb8 = (sb.view(torch.uint8).int() - e.cuda()).to(torch.uint8).view(torch.float8_e8m0fnu)
+    y = ql.gemm_mxfp4(a, sa8, b, sb8, out_dtype=ql.float32)
+    check(y, a, sa8, b, sb8, K)
+    assert torch.equal(y, ql.gemm_mxfp4(a, sa, b, sb, out_dtype=ql.float32))
+    sa8.view(torch.uint8)[1, 3] = 255
+    sb8.view(torch.uint8)[7, 0] = 255
+    z = ql.gemm_mxfp4(a, sa8, b, sb8, out_dtype=ql.float32)
+    spoiled = torch.zeros_like(z, dtype=torch.bool)
+    spoiled[1], spoiled[:, 7] = True, True
+    assert torch.equal(torch.isnan(z), spoiled) and torch.equal(z[~spoiled], y[~spoiled])
+
+
+def test_streams_capture_and_interleaved_calls():
+    """Calls on two streams at once, and two captured graphs replayed in turn, do not disturb one another."""
+    cases = [(1, 4096, 8192), (700, 6000, 1056)]
+    ops = [(operand(M, K, 5300 + i), operand(N, K, 6300 + i, K ** -0.5)) for i, (M, N, K) in enumerate(cases)]
+    call = lambda i: ql.gemm_mxfp4(*ops[i][0], *ops[i][1])
+    want = [call(0), call(1)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(i))
+        graphs.append(g)
+    for _ in range(3):
+        for y in outs:
+            y.fill_(float("nan"))
+        for i, g in enumerate(graphs):
+            with torch.cuda.stream(streams[i]):
+                streams[i].wait_stream(torch.cuda.default_stream())
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(outs[i], want[i]) for i in range(2))
+    assert ql.lib().ql_gemm_status(None) == 0
+
+
+def test_empty_and_refused():
+    a, sa = operand(4, 64, 5400)
+    b, sb = operand(8, 64, 6400)
+    none = ql.quantize_mxfp4(torch.empty((0, 64), device="cuda"))
+    assert ql.gemm_mxfp4(*none, b, sb).shape == (0, 8) and ql.gemm_mxfp4(a, sa, *none).shape == (4, 0)
+    with pytest.raises(ql.QuantizeError, match="Float4Tensor"):
+        ql.gemm_mxfp4(torch.ones((4, 64), device="cuda"), sa, b, sb)
+    with pytest.raises(ql.QuantizeError, match="Unsupported data type"):
+        ql.gemm_mxfp4(a, sa, b, sb, out_dtype=ql.int8)
+    with pytest.raises(ql.QlError, match="one entry per block of 32"):
+        ql.gemm_mxfp4(a, sb, b, sb)
+    with pytest.raises(ql.QlError, match=r"y must be \[M,N\]"):
+        ql.gemm_mxfp4(a, sa, b, sb, out=torch.empty((8, 4), device="cuda"))
+    with pytest.raises(ql.QlError, match="one device"):
+        ql.gemm_mxfp4(a, sa, b, sb, out=torch.empty((4, 8)))
+    c, sc = ql.dynamic_quantize(torch.ones((8, 64), device="cuda"))   # NVFP4 scales are no MXFP4 scales
+    with pytest.raises(ql.QlError, match="f8E8M0FNU"):
+        ql.gemm_mxfp4(a, sa, c, sc)
