@@ -156,9 +156,8 @@ QL_API int ql_dequantize_mxfp4(const ql_tensor *data, const ql_tensor *scales, q
 
 /* Block-scaled MXFP4 product: Y[M,N] = dq(a)[M,K] . dq(b)[N,K]^T of operands as ql_quantize_mxfp4 writes them, the block
  * scales applied by the tensor core (tcgen05.mma kind::mxf4, f32 accumulation), one rounding to y's type.  a, b: QL_F4E2M1
- * [M,K], [N,K], 16-byte aligned; *_scales: QL_F8E8M0 [rows, K/32]; y: f32 | f16 | bf16.  K > 0, K % 32 == 0; M and N any.  A NaN
- * scale makes its row (a) or column (b) of Y NaN.  Large products whose scales have K % 512 != 0 or are not 16-byte aligned
- * take scratch for a padded copy of the scales from the stream-ordered allocator. */
+ * [M,K], [N,K], 16-byte aligned; *_scales: QL_F8E8M0 [rows, K/32], 4-byte aligned; y: f32 | f16 | bf16.  K > 0, K % 32 == 0; M and N any.  A NaN
+ * scale makes its row (a) or column (b) of Y NaN.  One launch, no scratch. */
 QL_API int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, const ql_tensor *b, const ql_tensor *b_scales,
                          ql_tensor *y, void *stream);
 

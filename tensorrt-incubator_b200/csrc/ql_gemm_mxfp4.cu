@@ -56,13 +56,30 @@ template <int N> __device__ __forceinline__ uint32_t mx_idesc(uint32_t byte) {
 __device__ __forceinline__ void tmem_store_4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// One lane of a converged warp.  The roles that issue copies and MMAs run as whole warps and elect a lane only around the
+// instruction: their operands are then provably the same in all lanes and stay in uniform registers.  Inside a branch that
+// one lane alone takes, every descriptor word is moved there first: 111 cycles per MMA, against the 57 to 112 it needs.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 // A warp's wait with one answer for all lanes: what follows is executed by the whole warp or by none of it.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code));
 }
+// A wait that only the clock ends: for what this CTA has in flight itself.
+__device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity))
+    if (clock64() - t0 > kWaitLimitCycles) return false;
+  return true;
+}
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// the four MMAs of one k step
+// The four MMAs of one k step, issued by one lane of a converged warp.
 template <int N>
 __device__ __forceinline__ void mx_k_step(uint32_t tmem_d, uint32_t a_addr, uint32_t b_addr, uint32_t t_sfa, uint32_t t_sfb, int sfb_cols, bool first) {
   const uint64_t adesc = make_smem_desc(a_addr), bdesc = make_smem_desc(b_addr);
@@ -78,72 +95,129 @@ __device__ __forceinline__ void store_y(void *Y, int dtype, size_t i, float v) {
   else store_y<__nv_bfloat16>(Y, i, v);
 }
 
-// The 8 scale bytes of one row and k step (zeros beyond the row's end and beyond the operand).
-__device__ __forceinline__ uint2 load_row_scales(const uint8_t *sf, int row, int rows, int kb, int ks, int vec) {
-  uint2 v = make_uint2(0u, 0u);
-  if (row >= rows) return v;
-  const int b0 = ks * kScaleBytes;
-  const uint8_t *p = sf + (size_t)row * kb + b0;
-  if (vec == 8) return __ldg(reinterpret_cast<const uint2 *>(p));
-  if (vec == 4) {
-    v.x = __ldg(reinterpret_cast<const uint32_t *>(p));
-    if (b0 + 4 < kb) v.y = __ldg(reinterpret_cast<const uint32_t *>(p) + 1);
-    return v;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    if (b0 + i < kb) v.x |= (uint32_t)__ldg(p + i) << (8 * i);
-    if (b0 + 4 + i < kb) v.y |= (uint32_t)__ldg(p + 4 + i) << (8 * i);
-  }
+__device__ __forceinline__ uint32_t ldg32_if(const void *p, bool on) {
+  uint32_t v;
+  asm("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.nc.b32 %0, [%1];\n\t}" : "=r"(v) : "l"(p), "r"((int)on));
   return v;
 }
+// up to four neighbouring values of y
+__device__ __forceinline__ void store_y4(const MxArgs &args, size_t i, const float4 &v, int n, bool vec) {
+  if (vec && args.y_dtype == QL_F32) *reinterpret_cast<float4 *>(static_cast<float *>(args.Y) + i) = v;
+  else if (vec && args.y_dtype == QL_F16) *reinterpret_cast<uint2 *>(static_cast<__half *>(args.Y) + i) = make_uint2(pack2<__half>(v.x, v.y), pack2<__half>(v.z, v.w));
+  else if (vec) *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(args.Y) + i) = make_uint2(pack2<__nv_bfloat16>(v.x, v.y), pack2<__nv_bfloat16>(v.z, v.w));
+  else {
+    const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (j < n) store_y(args.Y, args.y_dtype, i + j, f[j]);
+  }
+}
+
+__device__ __forceinline__ uint32_t ldg8_if(const void *p, bool on) {
+  uint32_t v;
+  asm("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.nc.u8 %0, [%1];\n\t}" : "=r"(v) : "l"(p), "r"((int)on));
+  return v;
+}
+// The scale bytes of four k steps of one row: the first `n` of 32 bytes from p on, zeros beyond.  Loading and shifting are
+// apart, so that the loads of several rows are in flight together, and the loads are predicated, not branched around: a
+// branch or a use between them makes each wait for the one before.
+// WIDE: rows lie on multiples of 8 bytes.  Else only the operand does, on a multiple of 4: the aligned words that hold the
+// bytes are read, and of a word that reaches beyond the operand (`left` bytes from p on) just the bytes inside.
+template <bool WIDE> struct RowScales {
+  uint32_t r[WIDE ? 8 : 9];
+  int n, off;
+  __device__ __forceinline__ void load(const uint8_t *p, int n_, long long left) {
+    n = n_;
+    off = WIDE ? 0 : (int)(reinterpret_cast<uintptr_t>(p) & 3);
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2)
+        asm("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %3, %4;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t@p ld.global.nc.v2.b32 {%0, %1}, [%2];\n\t}"
+            : "=r"(r[i]), "=r"(r[i + 1])
+            : "l"(p + 4 * i), "r"(4 * i), "r"(n));
+    } else {
+      const uint8_t *q = p - off;
+      const int inside = left > 64 ? 64 : (int)left + off; // bytes of the operand from q on
+#pragma unroll
+      for (int i = 0; i < 9; i++) r[i] = ldg32_if(q + 4 * i, 4 * i < n + off && 4 * i + 4 <= inside);
+      const int cut = inside & ~3; // the word that reaches beyond, if it is wanted
+      const bool wanted = cut < 36 && cut < n + off;
+#pragma unroll
+      for (int j = 0; j < 3; j++) {
+        uint32_t v = ldg8_if(q + cut + j, wanted && cut + j < inside) << (8 * j);
+#pragma unroll
+        for (int i = 0; i < 9; i++)
+          if (4 * i == cut && wanted) r[i] |= v;
+      }
+    }
+  }
+  __device__ __forceinline__ uint32_t word(int i) const {
+    if constexpr (WIDE) return r[i];
+    const uint32_t w = __funnelshift_r(r[i], r[i + 1], 8 * off);
+    const int here = n - 4 * i; // valid bytes of this word
+    return here >= 4 ? w : (here <= 0 ? 0u : w & ((1u << (8 * here)) - 1u));
+  }
+};
 
 // ------------------------------------------------------------------------------------------------------------------
 // split kernel: 128 rows of the weights x TN tokens, K over the CTAs of a cluster
 // ------------------------------------------------------------------------------------------------------------------
 constexpr int kSplitThreads = 192;
 constexpr int kMaxSplit = 8;
+constexpr int kFetchSteps = 4;      // k steps whose scales travel together: 32 bytes, a whole sector, of every row
+constexpr int kScPitch = 40;
 
+constexpr int kSplitSlots = 2;      // groups of k steps whose scales lie in tensor memory at once
+constexpr int kSplitMaxStages = 16;
+
+// Fixed parts first, then the ring: `stages` of (rows of the weights rounded up to 8) + TN rows of 128 bytes.  The MMA reads
+// 128 rows of the first operand whatever `rows` is; what it reads beyond them (other stages, the slack behind the last one)
+// ends up in accumulator rows nobody looks at.
 template <int TN> struct SplitSmem {
-  static constexpr int kStages = 4;
-  static constexpr int kStageBytes = MX_A_BYTES + TN * BK_BYTES;
-  static constexpr int kTiles = kStages * kStageBytes;
-  static_assert(TN * BM * 4 <= kTiles && kStageBytes % 1024 == 0, "the partial sums reuse the ring");
-  static constexpr int kBarriers = kTiles; // full[S], empty[S], sfull[2], sempty[2], tfull
-  static constexpr int kTmemPtr = kBarriers + (2 * kStages + 5) * 8;
+  static constexpr int kParts = 0;                         // partial sums of this CTA's tokens, [split][TN / split][128]
+  static constexpr int kScales = kParts + TN * BM * 4;     // two groups of four k steps' scales
+  static constexpr int kScaleGroup = (BM + TN) * kScPitch;
+  static constexpr int kBarriers = kScales + 2 * kScaleGroup; // full[16], empty[16], sfull[2], sempty[2], tfull
+  static constexpr int kTmemPtr = kBarriers + (2 * kSplitMaxStages + 2 * kSplitSlots + 1) * 8;
   static constexpr int kAbort = kTmemPtr + 4;
-  static constexpr int kDynamic = kAbort + 4 + 1024;
+  static constexpr int kRing = (kAbort + 4 + 1023) / 1024 * 1024;
+  static constexpr int stage_bytes(int rows) { return ((rows + 7) / 8 * 8 + TN) * BK_BYTES; }
+  static constexpr int total(int rows, int stages) { return kRing + stages * stage_bytes(rows) + MX_A_BYTES + 1024; }
 };
 
-template <int TN>
+template <int TN, bool WIDE>
 __global__ void __launch_bounds__(kSplitThreads)
-gemm_mxfp4_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const MxArgs args, int split, int vec_a, int vec_b) {
+gemm_mxfp4_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const MxArgs args, int rows, int stages, int split_log2) {
   using L = SplitSmem<TN>;
-  constexpr int ST = L::kStages;
-  constexpr uint32_t kSfCol0 = TN;                         // two slots of 16 columns: 8 of the weights' scales, 8 of the tokens'
-  constexpr uint32_t kTmemCols = TN + 32 <= 64 ? 64 : (TN + 32 <= 128 ? 128 : 256);
+  constexpr int ST = kSplitMaxStages, SL = kSplitSlots;
+  const int stage_bytes = L::stage_bytes(rows), b_off = stage_bytes - TN * BK_BYTES;
+  constexpr int TN_LOG2 = TN == 16 ? 4 : (TN == 32 ? 5 : (TN == 64 ? 6 : 7));
+  constexpr uint32_t kSfCol0 = TN;                         // two slots of four k steps, 16 columns each: 8 of the weights' scales, 8 of the tokens'
+  constexpr uint32_t kSlotCols = 16 * kFetchSteps, kTmemCols = 256;
+  static_assert(kSfCol0 + SL * kSlotCols <= kTmemCols, "tensor memory");
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t smem_base = smem_u32(smem), bar_base = smem_base + L::kBarriers;
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
   auto empty_bar = [&](int s) { return bar_base + 8u * (ST + s); };
   auto sfull_bar = [&](int s) { return bar_base + 8u * (2 * ST + s); };
-  auto sempty_bar = [&](int s) { return bar_base + 8u * (2 * ST + 2 + s); };
-  const uint32_t tfull_bar = bar_base + 8u * (2 * ST + 4);
+  auto sempty_bar = [&](int s) { return bar_base + 8u * (2 * ST + SL + s); };
+  const uint32_t tfull_bar = bar_base + 8u * (2 * ST + 2 * SL);
   volatile uint32_t *tmem_ptr_smem = reinterpret_cast<volatile uint32_t *>(smem + L::kTmemPtr);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::kAbort);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = blockIdx.x % split, tile = blockIdx.x / split;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int split = 1 << split_log2;
+  const int rank = blockIdx.x & (split - 1), tile = blockIdx.x >> split_log2;
   const int wt = tile % args.tiles_a, xt = tile / args.tiles_a;
   const int ks0 = (int)((long long)args.num_ks * rank / split), ks1 = (int)((long long)args.num_ks * (rank + 1) / split);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < ST; s++) {
+    for (int s = 0; s < stages; s++) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
     }
-    for (int s = 0; s < 2; s++) {
+    for (int s = 0; s < SL; s++) {
       mbar_init(sfull_bar(s), 4);
       mbar_init(sempty_bar(s), 1);
     }
@@ -158,105 +232,134 @@ gemm_mxfp4_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_ptr_smem;
+  if (split > 1) cluster_arrive(); // waited for before the first store into a partner: the partner has started by then
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr_smem, 0);
 
   if (warp == 0) {
     // ------------------------------------------------------------------ producer
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int issued = 0;
-      bool ok = true;
-      for (int ks = ks0; ks < ks1; ks++) {
-        if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, args.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
-        const uint32_t a_dst = smem_base + stage * L::kStageBytes;
-        mbar_expect_tx(full_bar(stage), L::kStageBytes);
-        tma_load_2d(a_dst, &map_w, full_bar(stage), ks * BK_BYTES, wt * BM); // coordinates in bytes of packed e2m1
-        tma_load_2d(a_dst + MX_A_BYTES, &map_x, full_bar(stage), ks * BK_BYTES, xt * TN);
-        issued++;
-        if (++stage == ST) { stage = 0; phase ^= 1; }
+    int stage = 0, issued = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int ks = ks0; ks < ks1; ks++) {
+      if (!warp_wait(empty_bar(stage), phase ^ 1, abort_flag, args.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+      if (elect_one()) {
+        const uint32_t a_dst = smem_base + L::kRing + stage * stage_bytes;
+        mbar_expect_tx(full_bar(stage), (uint32_t)(rows + TN) * BK_BYTES);
+        tma_load_2d(a_dst, &map_w, full_bar(stage), ks * BK_BYTES, wt * rows); // coordinates in bytes of packed e2m1
+        tma_load_2d(a_dst + b_off, &map_x, full_bar(stage), ks * BK_BYTES, xt * TN);
       }
-      if (!ok) { // let the loads in flight land before the shared memory goes away
-        const int pending = issued < ST ? issued : ST;
-        for (int i = 0; i < pending; i++) {
-          stage = (stage == 0) ? ST - 1 : stage - 1;
-          if (stage == ST - 1) phase ^= 1;
-          const long long t0 = clock64();
-          while (!mbar_try_wait(full_bar(stage), phase) && clock64() - t0 < kWaitLimitCycles) {}
-        }
+      __syncwarp();
+      issued++;
+      if (++stage == stages) { stage = 0; phase ^= 1; }
+    }
+    if (!ok) { // let the loads in flight land before the shared memory goes away
+      const int pending = issued < stages ? issued : stages;
+      for (int i = 0; i < pending; i++) {
+        stage = (stage == 0) ? stages - 1 : stage - 1;
+        if (stage == stages - 1) phase ^= 1;
+        bounded_wait(full_bar(stage), phase);
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issue
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int ks = ks0; ks < ks1; ks++) {
-        const int it = ks - ks0, slot = it & 1;
-        if (!mbar_wait(full_bar(stage), phase, abort_flag, args.status, ST_TIMEOUT_FULL)) break;
-        if (!mbar_wait(sfull_bar(slot), (it >> 1) & 1, abort_flag, args.status, ST_TIMEOUT_FULL)) break;
-        tc_fence_after();
-        const uint32_t a_addr = smem_base + stage * L::kStageBytes, t_sf = tmem_base + kSfCol0 + 16 * slot;
-        mx_k_step<TN>(tmem_base, a_addr, a_addr + MX_A_BYTES, t_sf, t_sf + 8, 4, it == 0);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int ks = ks0; ks < ks1; ks++) {
+      const int it = ks - ks0, group = it / kFetchSteps, slot = group & 1, q = it % kFetchSteps;
+      if (q == 0 && !warp_wait(sfull_bar(slot), (group >> 1) & 1, abort_flag, args.status, ST_TIMEOUT_FULL)) break;
+      if (!warp_wait(full_bar(stage), phase, abort_flag, args.status, ST_TIMEOUT_FULL)) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t a_addr = smem_base + L::kRing + stage * stage_bytes, t_sf = tmem_base + kSfCol0 + slot * kSlotCols + 16 * q;
+        mx_k_step<TN>(tmem_base, a_addr, a_addr + b_off, t_sf, t_sf + 8, 4, it == 0);
         tc_commit(empty_bar(stage));
-        tc_commit(sempty_bar(slot));
-        if (++stage == ST) { stage = 0; phase ^= 1; }
+        if (q == kFetchSteps - 1) tc_commit(sempty_bar(slot));
       }
-      tc_commit(tfull_bar);
-      // every MMA issued above is done with shared and tensor memory before this thread goes on, after an abort too
-      const long long t0 = clock64();
-      while (!mbar_try_wait(tfull_bar, 0)) {
-        if (clock64() - t0 > kWaitLimitCycles) { atomicCAS(args.status, 0, ST_TIMEOUT_DRAIN); break; }
-      }
+      __syncwarp();
+      if (++stage == stages) { stage = 0; phase ^= 1; }
     }
+    // every MMA issued above is done with shared and tensor memory before this warp goes on, after an abort too
+    if (elect_one()) tc_commit(tfull_bar);
+    __syncwarp();
+    if (!bounded_wait(tfull_bar, 0) && lane == 0) atomicCAS(args.status, 0, ST_TIMEOUT_DRAIN);
   } else {
     // ------------------------------------------------------------------ scales, then the accumulator (warps 2..5)
     const int quad = warp & 3;
     const uint32_t quarter = (uint32_t)(quad * 32) << 16;
+    // The 128 threads fetch four k steps of scales together, a row each, two groups ahead; they hand them over through
+    // shared memory (rows 40 bytes apart: conflict-free both ways), and each warp stores the rows its lanes hold, one
+    // hand-over to the MMA thread per group.  (Each warp loading all rows for itself is four times the L1 look-ups, one per
+    // row and step: 1 us per k step at TN = 128.  A hand-over per k step: 0.4 us per step, a latency.)
     constexpr int XR = TN <= 32 ? 1 : TN / 32; // rows of the token operand a lane carries
-    uint2 a[4], b[XR];
-    auto fetch = [&](int ks) {
-#pragma unroll
-      for (int c = 0; c < 4; c++) a[c] = load_row_scales(args.sfa, wt * BM + c * 32 + lane, args.N, args.kb, ks, vec_a);
-#pragma unroll
-      for (int c = 0; c < XR; c++) {
-        const int r = c * 32 + lane;
-        b[c] = r < TN ? load_row_scales(args.sfb, xt * TN + r, args.M, args.kb, ks, vec_b) : make_uint2(0u, 0u);
-      }
+    const int tid = quad * 32 + lane;
+    RowScales<WIDE> a[2], b[2];
+    const long long row_a = (long long)wt * rows + tid, row_b = (long long)xt * TN + tid;
+    const bool has_a = tid < rows && row_a < args.N, has_b = tid < TN && row_b < args.M;
+    auto fetch = [&](int ks, RowScales<WIDE> &fa, RowScales<WIDE> &fb) {
+      const int b0 = ks * kScaleBytes, n = min(args.kb, ks1 * kScaleBytes) - b0;
+      const long long at_a = has_a ? row_a * args.kb + b0 : 0, at_b = has_b ? row_b * args.kb + b0 : 0;
+      fa.load(args.sfa + at_a, has_a ? n : 0, (long long)args.N * args.kb - at_a);
+      fb.load(args.sfb + at_b, has_b ? n : 0, (long long)args.M * args.kb - at_b);
     };
-    if (ks0 < ks1) fetch(ks0);
-    for (int ks = ks0; ks < ks1; ks++) {
-      const int it = ks - ks0, slot = it & 1;
-      uint2 pa[4], pb[4];
+    bool ok = true;
+    auto hand_over = [&](int ks, int slot, uint32_t parity, RowScales<WIDE> &fa, RowScales<WIDE> &fb) {
+      uint8_t *buf = smem + L::kScales + slot * L::kScaleGroup;
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        pa[c] = a[c];
-        pb[c] = c < XR ? b[c < XR ? c : 0] : make_uint2(0u, 0u);
+      for (int q = 0; q < kFetchSteps; q++) {
+        *reinterpret_cast<uint2 *>(buf + tid * kScPitch + q * 8) = make_uint2(fa.word(2 * q), fa.word(2 * q + 1));
+        if (tid < TN) *reinterpret_cast<uint2 *>(buf + (BM + tid) * kScPitch + q * 8) = make_uint2(fb.word(2 * q), fb.word(2 * q + 1));
       }
-      if (ks + 1 < ks1) fetch(ks + 1); // in flight while this step's slot is waited for
-      if (!warp_wait(sempty_bar(slot), ((it >> 1) & 1) ^ 1, abort_flag, args.status, ST_TIMEOUT_EMPTY)) break;
-      const uint32_t t = tmem_base + quarter + kSfCol0 + 16 * slot;
-      tmem_store_4(t, pa[0].x, pa[1].x, pa[2].x, pa[3].x);
-      tmem_store_4(t + 4, pa[0].y, pa[1].y, pa[2].y, pa[3].y);
-      tmem_store_4(t + 8, pb[0].x, pb[1].x, pb[2].x, pb[3].x);
-      tmem_store_4(t + 12, pb[0].y, pb[1].y, pb[2].y, pb[3].y);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      fetch(ks + 2 * kFetchSteps, fa, fb);
+      ok = warp_wait(sempty_bar(slot), parity, abort_flag, args.status, ST_TIMEOUT_EMPTY);
+      if (!ok) return;
+      const uint32_t t = tmem_base + quarter + kSfCol0 + slot * kSlotCols;
+#pragma unroll
+      for (int q = 0; q < kFetchSteps; q++) {
+        uint2 pa[4], pb[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          pa[c] = *reinterpret_cast<const uint2 *>(buf + (c * 32 + lane) * kScPitch + q * 8);
+          pb[c] = make_uint2(0u, 0u);
+          if (c < XR && c * 32 + lane < TN) pb[c] = *reinterpret_cast<const uint2 *>(buf + (BM + c * 32 + lane) * kScPitch + q * 8);
+        }
+        tmem_store_4(t + 16 * q, pa[0].x, pa[1].x, pa[2].x, pa[3].x);
+        tmem_store_4(t + 16 * q + 4, pa[0].y, pa[1].y, pa[2].y, pa[3].y);
+        tmem_store_4(t + 16 * q + 8, pb[0].x, pb[1].x, pb[2].x, pb[3].x);
+        tmem_store_4(t + 16 * q + 12, pb[0].y, pb[1].y, pb[2].y, pb[3].y);
+      }
       tmem_store_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(sfull_bar(slot));
+    };
+    fetch(ks0, a[0], b[0]);
+    fetch(ks0 + kFetchSteps, a[1], b[1]);
+    uint32_t parity = 1;
+    for (int ks = ks0; ks < ks1 && ok; ks += 2 * kFetchSteps, parity ^= 1) {
+      hand_over(ks, 0, parity, a[0], b[0]);
+      if (ok && ks + kFetchSteps < ks1) hand_over(ks + kFetchSteps, 1, parity, a[1], b[1]);
     }
     warp_wait(tfull_bar, 0, abort_flag, args.status, ST_TIMEOUT_TMEM_FULL);
     tc_fence_after();
     // lane = row of the weights = column of Y, so a warp's store of one token is contiguous
-    const int n = wt * BM + quad * 32 + lane;
-    float *part = reinterpret_cast<float *>(smem); // [TN][128]: the ring is free once the MMAs are done
+    const int row = quad * 32 + lane, n = row < rows ? wt * rows + row : args.N;
+    const int tokens = min(TN, args.M - xt * TN), per_log2 = TN_LOG2 - split_log2, per = 1 << per_log2; // CTA o adds up tokens [o * per, (o + 1) * per)
+    if (split > 1) cluster_wait();
 #pragma unroll 1
     for (int c = 0; c < TN / 16; c++) {
+      if (c * 16 >= tokens) break;
       uint32_t r[16];
       tmem_load_16(tmem_base + quarter + c * 16, r);
       if (split > 1) {
 #pragma unroll
-        for (int j = 0; j < 16; j++) part[(c * 16 + j) * BM + quad * 32 + lane] = __uint_as_float(r[j]);
+        for (int j = 0; j < 16; j++) {
+          const int t = c * 16 + j;
+          if (t < tokens) {
+            const uint32_t local = smem_base + (uint32_t)(L::kParts + ((rank * per + (t & (per - 1))) * BM + row) * 4);
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(local, (uint32_t)(t >> per_log2))), "f"(__uint_as_float(r[j])) : "memory");
+          }
+        }
       } else if (n < args.N) {
         const int m = xt * TN + c * 16;
 #pragma unroll
@@ -266,26 +369,28 @@ gemm_mxfp4_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     }
     tc_fence_before();
   }
-  __syncthreads();
   if (split > 1) {
-    cluster_sync_all(); // every CTA's partial sums are in its shared memory
-    const int t0 = TN * rank / split, t1 = TN * (rank + 1) / split;
-    for (int i = threadIdx.x; i < (t1 - t0) * BM; i += kSplitThreads) {
-      const int t = t0 + i / BM, row = i % BM;
-      const int m = xt * TN + t, n = wt * BM + row;
-      if (m >= args.M || n >= args.N) continue;
-      const uint32_t local = smem_base + (uint32_t)(t * BM + row) * 4u;
-      float p[kMaxSplit], v = 0.f;
+    if (warp < 2) cluster_wait();
+    __syncwarp();
+    cluster_sync_all(); // every part has arrived
+    const int per = TN >> split_log2, t0 = rank * per, t1 = min(t0 + per, args.M - xt * TN);
+    // four neighbouring columns of Y a thread: rows is a multiple of 4
+    const float4 *parts = reinterpret_cast<const float4 *>(smem + L::kParts);
+    const bool vec = args.N % 4 == 0 && (reinterpret_cast<uintptr_t>(args.Y) & 15) == 0;
+    for (int i = threadIdx.x; i < (t1 - t0) * (BM / 4); i += kSplitThreads) {
+      const int row = i % (BM / 4) * 4, n = wt * rows + row;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int s = 0; s < kMaxSplit; s++)
-        if (s < split) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p[s]) : "r"(map_to_cta(local, (uint32_t)s)));
-#pragma unroll
-      for (int s = 0; s < kMaxSplit; s++)
-        if (s < split) v += p[s];
-      store_y(args.Y, args.y_dtype, (size_t)m * args.N + n, v);
+      for (int p = 0; p < kMaxSplit; p++) {
+        if (p < split) {
+          const float4 w = parts[p * per * (BM / 4) + i];
+          v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+        }
+      }
+      if (row < rows && n < args.N) store_y4(args, (size_t)(xt * TN + t0 + i / (BM / 4)) * args.N + n, v, vec ? 4 : min(4, args.N - n), vec);
     }
-    cluster_sync_all(); // a CTA's shared memory stays until its partners have read it
   }
+  __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
@@ -301,40 +406,56 @@ constexpr int TSTAGES = 4;
 constexpr int T_STAGE_BYTES = MX_A_BYTES + TBN * BK_BYTES;
 constexpr int kScSteps = 4;         // k steps whose scales travel together: 32 bytes, a whole sector, of every row
 constexpr int T_SC_ROWS = BM + TBN;
-constexpr int T_SC_BYTES = T_SC_ROWS * 32;
+constexpr int T_SC_ODD = T_SC_ROWS / 2 * 32;               // SC_PAIRS: 32 bytes of the even rows, then 48 of the odd ones
+constexpr int T_SC_BYTES = T_SC_ODD + T_SC_ROWS / 2 * 48;
 struct TileSmem {
   static constexpr int kScales = TSTAGES * T_STAGE_BYTES;
-  static constexpr int kBarriers = kScales + 2 * T_SC_BYTES; // full[S], empty[S], tfull[2], tempty[2], scfull[2], scempty[2], sfull[2], sempty[2], drain
+  static constexpr int kStaging = kScales + 2 * T_SC_BYTES;   // the epilogue's: 32 rows x 33 words a warp
+  static constexpr int kBarriers = kStaging + 4 * 32 * 33 * 4; // full[S], empty[S], tfull[2], tempty[2], scfull[2], scempty[2], sfull[2], sempty[2], drain
   static constexpr int kTmemPtr = kBarriers + (2 * TSTAGES + 13) * 8;
   static constexpr int kAbort = kTmemPtr + 4;
   static constexpr int kDynamic = kAbort + 4 + 1024;
 };
 static_assert(TileSmem::kDynamic <= 232448 && T_STAGE_BYTES % 1024 == 0 && T_SC_BYTES % 128 == 0, "tile shape");
 
-// 32 columns of one accumulator row, rounded to y's type and stored
+// 32 columns of one accumulator row a lane, rounded to y's type and stored in whole 16-byte pieces
 template <typename OutT>
-__device__ __forceinline__ void mx_store_chunk(OutT *Y, const uint32_t (&r)[32], int m, int n, int N, bool vec) {
-  OutT *y = Y + (size_t)m * (size_t)N + n;
-  if (vec && n + 32 <= N) {
-    if constexpr (sizeof(OutT) == 4) {
+__device__ __forceinline__ void mx_store_chunk(OutT *y, const uint32_t (&r)[32]) {
+  if constexpr (sizeof(OutT) == 4) {
 #pragma unroll
-      for (int j = 0; j < 32; j += 4) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]));
-    } else {
-      auto two = [&](int j) { return pack2<OutT>(__uint_as_float(r[j]), __uint_as_float(r[j + 1])); };
-#pragma unroll
-      for (int j = 0; j < 32; j += 8) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
-    }
+    for (int j = 0; j < 32; j += 4) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]));
   } else {
+    auto two = [&](int j) { return pack2<OutT>(__uint_as_float(r[j]), __uint_as_float(r[j + 1])); };
 #pragma unroll
-    for (int j = 0; j < 32; j++)
-      if (n + j < N) y[j] = FloatIO<OutT>::from_f32(__uint_as_float(r[j]));
+    for (int j = 0; j < 32; j += 8) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
   }
 }
+// The same 32 x 32 values where rows are not aligned or the chunk is cut: turned in shared memory, so that a warp's store is
+// one row's run of columns.  (A lane storing its own row value by value took 40 us on 333 x 1001 x 2080.)
+__device__ __forceinline__ void mx_store_rows(const MxArgs &args, float *stage, const uint32_t (&r)[32], int m0, int n0, int lane) {
+#pragma unroll
+  for (int j = 0; j < 32; j++) stage[lane * 33 + j] = __uint_as_float(r[j]);
+  __syncwarp();
+  const int n = n0 + lane;
+#pragma unroll 8
+  for (int i = 0; i < 32; i++)
+    if (m0 + i < args.M && n < args.N) store_y(args.Y, args.y_dtype, (size_t)(m0 + i) * args.N + n, stage[i * 33 + lane]);
+  __syncwarp();
+}
 
+// How the scales reach shared memory, 32 bytes (four k steps) of each of a tile's 352 rows at a time.  The copy engine wants
+// rows a multiple of 16 bytes apart.  SC_ROWS: they are.  SC_PAIRS: they are an odd multiple of 8 bytes long (K = 11008, say),
+// so the even rows form one matrix and the odd rows, seen from 8 bytes before the first, another.  SC_WORDS: any other length;
+// the scale warps load them, three rows a thread, one group ahead.  2000 x 4096: K = 11264 65.6 us, 11008 (pairs) 62.4 us,
+// 11040 (words) 111 us; the warps loading 8 bytes at a time took 88 us at K = 11008.
+enum { SC_ROWS, SC_PAIRS, SC_WORDS };
+template <int SC>
 __global__ void __launch_bounds__(kTileThreads, 1)
 gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sa,
-                        const __grid_constant__ CUtensorMap map_sb, const MxArgs args) {
+                        const __grid_constant__ CUtensorMap map_sb, const __grid_constant__ CUtensorMap map_sa_odd, const __grid_constant__ CUtensorMap map_sb_odd,
+                        const MxArgs args) {
   using L = TileSmem;
+  constexpr bool COPY = SC != SC_WORDS;
   constexpr uint32_t kTmemCols = 512; // 2 x 224 accumulator columns, then two slots of 32: 8 columns of A's scales, 16 of B's
   constexpr uint32_t kSfCol0 = 2 * TBN;
   extern __shared__ uint8_t smem_raw[];
@@ -352,7 +473,7 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
   volatile uint32_t *tmem_ptr_smem = reinterpret_cast<volatile uint32_t *>(smem + L::kTmemPtr);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::kAbort);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int num_tiles = args.tiles_a * args.tiles_b;
 
   if (threadIdx.x == 0) {
@@ -379,125 +500,185 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_ptr_smem;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr_smem, 0);
 
   if (warp == 0) {
     // ------------------------------------------------------------------ producer
-    if (lane == 0) {
-      int stage = 0, sc = 0;
-      uint32_t phase = 0, sc_phase = 0;
-      long long issued = 0, sc_issued = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-        const int mt = tile % args.tiles_a, nt = tile / args.tiles_a; // row tiles of one column tile run side by side: B stays in L2
-        for (int ks = 0; ks < args.num_ks; ks++) {
-          if (ks % kScSteps == 0) {
-            if (!mbar_wait(scempty_bar(sc), sc_phase ^ 1, abort_flag, args.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+    int stage = 0, sc = 0;
+    uint32_t phase = 0, sc_phase = 0;
+    long long issued = 0, sc_issued = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      const int mt = tile % args.tiles_a, nt = tile / args.tiles_a; // row tiles of one column tile run side by side: B stays in L2
+      for (int ks = 0; ks < args.num_ks; ks++) {
+        if (COPY && ks % kScSteps == 0) {
+          if (!warp_wait(scempty_bar(sc), sc_phase ^ 1, abort_flag, args.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+          if (elect_one()) {
             const uint32_t dst = smem_base + L::kScales + sc * T_SC_BYTES;
-            mbar_expect_tx(scfull_bar(sc), T_SC_BYTES);
-            tma_load_2d(dst, &map_sa, scfull_bar(sc), ks * kScaleBytes, mt * BM);
-            tma_load_2d(dst + BM * 32, &map_sb, scfull_bar(sc), ks * kScaleBytes, nt * TBN);
-            sc_issued++;
-            if (++sc == 2) { sc = 0; sc_phase ^= 1; }
+            if (SC == SC_ROWS) {
+              mbar_expect_tx(scfull_bar(sc), T_SC_ROWS * 32);
+              tma_load_2d(dst, &map_sa, scfull_bar(sc), ks * kScaleBytes, mt * BM);
+              tma_load_2d(dst + BM * 32, &map_sb, scfull_bar(sc), ks * kScaleBytes, nt * TBN);
+            } else {
+              mbar_expect_tx(scfull_bar(sc), T_SC_BYTES);
+              tma_load_2d(dst, &map_sa, scfull_bar(sc), ks * kScaleBytes, mt * (BM / 2));
+              tma_load_2d(dst + BM / 2 * 32, &map_sb, scfull_bar(sc), ks * kScaleBytes, nt * (TBN / 2));
+              tma_load_2d(dst + T_SC_ODD, &map_sa_odd, scfull_bar(sc), ks * kScaleBytes, mt * (BM / 2)); // from 8 bytes before
+              tma_load_2d(dst + T_SC_ODD + BM / 2 * 48, &map_sb_odd, scfull_bar(sc), ks * kScaleBytes, nt * (TBN / 2));
+            }
           }
-          if (!mbar_wait(empty_bar(stage), phase ^ 1, abort_flag, args.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+          __syncwarp();
+          sc_issued++;
+          if (++sc == 2) { sc = 0; sc_phase ^= 1; }
+        }
+        if (!warp_wait(empty_bar(stage), phase ^ 1, abort_flag, args.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+        if (elect_one()) {
           const uint32_t a_dst = smem_base + stage * T_STAGE_BYTES;
           mbar_expect_tx(full_bar(stage), T_STAGE_BYTES);
           tma_load_2d(a_dst, &map_a, full_bar(stage), ks * BK_BYTES, mt * BM); // coordinates in bytes of packed e2m1
           tma_load_2d(a_dst + MX_A_BYTES, &map_b, full_bar(stage), ks * BK_BYTES, nt * TBN);
-          issued++;
-          if (++stage == TSTAGES) { stage = 0; phase ^= 1; }
         }
+        __syncwarp();
+        issued++;
+        if (++stage == TSTAGES) { stage = 0; phase ^= 1; }
       }
-      if (!ok) { // let the loads in flight land before the shared memory goes away
-        const long long pending = issued < TSTAGES ? issued : TSTAGES, sc_pending = sc_issued < 2 ? sc_issued : 2;
-        for (long long i = 0; i < pending; i++) {
-          stage = (stage == 0) ? TSTAGES - 1 : stage - 1;
-          if (stage == TSTAGES - 1) phase ^= 1;
-          const long long t0 = clock64();
-          while (!mbar_try_wait(full_bar(stage), phase) && clock64() - t0 < kWaitLimitCycles) {}
-        }
-        for (long long i = 0; i < sc_pending; i++) {
-          sc ^= 1;
-          if (sc == 1) sc_phase ^= 1;
-          const long long t0 = clock64();
-          while (!mbar_try_wait(scfull_bar(sc), sc_phase) && clock64() - t0 < kWaitLimitCycles) {}
-        }
+    }
+    if (!ok) { // let the loads in flight land before the shared memory goes away
+      const long long pending = issued < TSTAGES ? issued : TSTAGES, sc_pending = sc_issued < 2 ? sc_issued : 2;
+      for (long long i = 0; i < pending; i++) {
+        stage = (stage == 0) ? TSTAGES - 1 : stage - 1;
+        if (stage == TSTAGES - 1) phase ^= 1;
+        bounded_wait(full_bar(stage), phase);
+      }
+      for (long long i = 0; i < sc_pending; i++) {
+        sc ^= 1;
+        if (sc == 1) sc_phase ^= 1;
+        bounded_wait(scfull_bar(sc), sc_phase);
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issue
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      int it = 0;
-      long long step = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, it++) {
-        const int buf = it & 1;
-        if (!mbar_wait(tempty_bar(buf), ((it >> 1) & 1) ^ 1, abort_flag, args.status, ST_TIMEOUT_TMEM_EMPTY)) { ok = false; break; }
-        for (int ks = 0; ks < args.num_ks; ks++, step++) {
-          const int slot = (int)(step & 1);
-          if (!mbar_wait(full_bar(stage), phase, abort_flag, args.status, ST_TIMEOUT_FULL)) { ok = false; break; }
-          if (!mbar_wait(sfull_bar(slot), (uint32_t)((step >> 1) & 1), abort_flag, args.status, ST_TIMEOUT_FULL)) { ok = false; break; }
-          tc_fence_after();
+    int stage = 0, it = 0;
+    uint32_t phase = 0, step = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, it++) {
+      const int buf = it & 1;
+      if (!warp_wait(tempty_bar(buf), ((it >> 1) & 1) ^ 1, abort_flag, args.status, ST_TIMEOUT_TMEM_EMPTY)) { ok = false; break; }
+      for (int ks = 0; ks < args.num_ks; ks++, step++) {
+        const int slot = (int)(step & 1);
+        if (!warp_wait(sfull_bar(slot), (step >> 1) & 1, abort_flag, args.status, ST_TIMEOUT_FULL)) { ok = false; break; }
+        if (!warp_wait(full_bar(stage), phase, abort_flag, args.status, ST_TIMEOUT_FULL)) { ok = false; break; }
+        tc_fence_after();
+        if (elect_one()) {
           const uint32_t a_addr = smem_base + stage * T_STAGE_BYTES, t_sf = tmem_base + kSfCol0 + 32 * slot;
           mx_k_step<TBN>(tmem_base + (uint32_t)(buf * TBN), a_addr, a_addr + MX_A_BYTES, t_sf, t_sf + 8, 8, ks == 0);
           tc_commit(empty_bar(stage));
           tc_commit(sempty_bar(slot));
-          if (++stage == TSTAGES) { stage = 0; phase ^= 1; }
+          if (ks == args.num_ks - 1) tc_commit(tfull_bar(buf));
         }
-        if (ok) tc_commit(tfull_bar(buf));
-      }
-      tc_commit(drain_bar); // every MMA issued above has to finish before tensor memory is released
-      const long long t0 = clock64();
-      while (!mbar_try_wait(drain_bar, 0)) {
-        if (clock64() - t0 > kWaitLimitCycles) { atomicCAS(args.status, 0, ST_TIMEOUT_DRAIN); break; }
+        __syncwarp();
+        if (++stage == TSTAGES) { stage = 0; phase ^= 1; }
       }
     }
+    if (elect_one()) tc_commit(drain_bar); // every MMA issued above has to finish before tensor memory is released
+    __syncwarp();
+    if (!bounded_wait(drain_bar, 0) && lane == 0) atomicCAS(args.status, 0, ST_TIMEOUT_DRAIN);
   } else if (warp >= 6) {
     // ------------------------------------------------------------------ scales (warps 6..9, one per quarter of the lanes)
     const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
-    int sc = 0;
-    uint32_t sc_phase = 0;
-    long long step = 0;
+    uint32_t step = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-      for (int ks = 0; ks < args.num_ks && ok; ks += kScSteps) {
-        if (!warp_wait(scfull_bar(sc), sc_phase, abort_flag, args.status, ST_TIMEOUT_FULL)) { ok = false; break; }
-        uint32_t w[T_SC_ROWS / 32][8]; // rows lane, lane + 32, ... : the words of four k steps
-        const uint8_t *src = smem + L::kScales + sc * T_SC_BYTES + lane * 32;
+    const int tid = (warp & 3) * 32 + lane;
+    // groups of four k steps, tile after tile; a cursor for what is fetched ahead
+    const int groups = (args.num_ks + kScSteps - 1) / kScSteps;
+    int f_tile = blockIdx.x, f_group = 0;
+    RowScales<false> own[3]; // !COPY: the next group; rows tid, tid + 128, tid + 256 of the tile's 352
+    auto fetch = [&]() {
+      const int mt = f_tile % args.tiles_a, nt = f_tile / args.tiles_a, b0 = f_group * kScSteps * kScaleBytes, n = args.kb - b0;
+#pragma unroll
+      for (int i = 0; i < 3; i++) {
+        const int r = tid + 128 * i; // 0..127: A's rows; then B's
+        const long long row = i == 0 ? (long long)mt * BM + r : (long long)nt * TBN + (r - BM);
+        const bool has = f_tile < num_tiles && r < T_SC_ROWS && row < (i == 0 ? args.M : args.N);
+        const long long at = has ? row * args.kb + b0 : 0;
+        own[i].load((i == 0 ? args.sfa : args.sfb) + at, has ? n : 0, (long long)(i == 0 ? args.M : args.N) * args.kb - at);
+      }
+      if (++f_group == groups) f_group = 0, f_tile += gridDim.x;
+    };
+    auto hand_over = [&](int ks, int sc, uint32_t sc_phase) {
+      if (COPY) {
+        ok = warp_wait(scfull_bar(sc), sc_phase, abort_flag, args.status, ST_TIMEOUT_FULL);
+        if (!ok) return;
+      } else {
+        // a buffer is rewritten two groups later: the barrier between, which every warp passes after reading the group
+        // before it, keeps the two apart
+#pragma unroll
+        for (int i = 0; i < 3; i++) {
+          if (tid + 128 * i < T_SC_ROWS) {
+            uint4 *dst = reinterpret_cast<uint4 *>(smem + L::kScales + sc * T_SC_BYTES + (tid + 128 * i) * 32);
+            dst[0] = make_uint4(own[i].word(0), own[i].word(1), own[i].word(2), own[i].word(3));
+            dst[1] = make_uint4(own[i].word(4), own[i].word(5), own[i].word(6), own[i].word(7));
+          }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        fetch();
+      }
+      uint32_t w[T_SC_ROWS / 32][8]; // rows lane, lane + 32, ... : the words of four k steps
+      const uint8_t *buf = smem + L::kScales + sc * T_SC_BYTES;
+      if (SC == SC_PAIRS) {
+        const uint8_t *src = lane & 1 ? buf + T_SC_ODD + (lane >> 1) * 48 + 8 : buf + (lane >> 1) * 32;
+        const int step16 = lane & 1 ? 16 * 48 : 16 * 32; // to the row 32 further on
 #pragma unroll
         for (int c = 0; c < T_SC_ROWS / 32; c++) {
-          const uint4 lo = *reinterpret_cast<const uint4 *>(src + c * 1024), hi = *reinterpret_cast<const uint4 *>(src + c * 1024 + 16);
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const uint2 v = *reinterpret_cast<const uint2 *>(src + c * step16 + 8 * j);
+            w[c][2 * j] = v.x, w[c][2 * j + 1] = v.y;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < T_SC_ROWS / 32; c++) {
+          const uint8_t *src = buf + (c * 32 + lane) * 32;
+          const uint4 lo = *reinterpret_cast<const uint4 *>(src), hi = *reinterpret_cast<const uint4 *>(src + 16);
           w[c][0] = lo.x, w[c][1] = lo.y, w[c][2] = lo.z, w[c][3] = lo.w;
           w[c][4] = hi.x, w[c][5] = hi.y, w[c][6] = hi.z, w[c][7] = hi.w;
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(scempty_bar(sc));
-        if (++sc == 2) { sc = 0; sc_phase ^= 1; }
+      }
+      __syncwarp();
+      if (COPY && lane == 0) mbar_arrive(scempty_bar(sc));
 #pragma unroll
-        for (int q = 0; q < kScSteps; q++) {
-          if (ok && ks + q < args.num_ks) {
-            const int slot = (int)(step & 1);
-            if (!warp_wait(sempty_bar(slot), (uint32_t)((step >> 1) & 1) ^ 1u, abort_flag, args.status, ST_TIMEOUT_EMPTY)) ok = false;
-            if (ok) {
-              const uint32_t t = tmem_base + quarter + kSfCol0 + 32 * slot;
+      for (int q = 0; q < kScSteps; q++) {
+        if (ok && ks + q < args.num_ks) {
+          const int slot = (int)(step & 1);
+          ok = warp_wait(sempty_bar(slot), ((step >> 1) & 1) ^ 1u, abort_flag, args.status, ST_TIMEOUT_EMPTY);
+          if (ok) {
+            const uint32_t t = tmem_base + quarter + kSfCol0 + 32 * slot;
 #pragma unroll
-              for (int j = 0; j < 2; j++) { // two MMAs' worth of cells: A's rows, B's first 128 rows, B's last 96
-                tmem_store_4(t + 4 * j, w[0][2 * q + j], w[1][2 * q + j], w[2][2 * q + j], w[3][2 * q + j]);
-                tmem_store_4(t + 8 + 8 * j, w[4][2 * q + j], w[5][2 * q + j], w[6][2 * q + j], w[7][2 * q + j]);
-                tmem_store_4(t + 12 + 8 * j, w[8][2 * q + j], w[9][2 * q + j], w[10][2 * q + j], 0u);
-              }
-              tmem_store_wait();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(sfull_bar(slot));
-              step++;
+            for (int j = 0; j < 2; j++) { // two MMAs' worth of cells: A's rows, B's first 128 rows, B's last 96
+              tmem_store_4(t + 4 * j, w[0][2 * q + j], w[1][2 * q + j], w[2][2 * q + j], w[3][2 * q + j]);
+              tmem_store_4(t + 8 + 8 * j, w[4][2 * q + j], w[5][2 * q + j], w[6][2 * q + j], w[7][2 * q + j]);
+              tmem_store_4(t + 12 + 8 * j, w[8][2 * q + j], w[9][2 * q + j], w[10][2 * q + j], 0u);
             }
+            tmem_store_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sfull_bar(slot));
+            step++;
           }
         }
       }
+    };
+    if (!COPY) fetch();
+    const int mine = blockIdx.x < num_tiles ? (num_tiles - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
+    const long long total = (long long)mine * groups;
+    int group = 0;
+    uint32_t sc_phase = 0;
+    for (long long i = 0; i < total && ok; i += 2, sc_phase ^= 1) {
+      hand_over(group * kScSteps, 0, sc_phase);
+      if (++group == groups) group = 0;
+      if (ok && i + 1 < total) hand_over(group * kScSteps, 1, sc_phase);
+      if (++group == groups) group = 0;
     }
   } else {
     // ------------------------------------------------------------------ epilogue (warps 2..5)
@@ -516,10 +697,14 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
         uint32_t r[32];
         tmem_load_32(taddr + c * 32, r);
         const int n = nt * TBN + c * 32;
-        if (m < args.M && n < args.N) {
-          if (args.y_dtype == QL_F32) mx_store_chunk(static_cast<float *>(args.Y), r, m, n, args.N, vec);
-          else if (args.y_dtype == QL_F16) mx_store_chunk(static_cast<__half *>(args.Y), r, m, n, args.N, vec);
-          else mx_store_chunk(static_cast<__nv_bfloat16 *>(args.Y), r, m, n, args.N, vec);
+        if (n >= args.N) break;
+        if (!vec || n + 32 > args.N) {
+          mx_store_rows(args, reinterpret_cast<float *>(smem + L::kStaging) + quad * 32 * 33, r, m - lane, n, lane);
+        } else if (m < args.M) {
+          const size_t at = (size_t)m * (size_t)args.N + n;
+          if (args.y_dtype == QL_F32) mx_store_chunk(static_cast<float *>(args.Y) + at, r);
+          else if (args.y_dtype == QL_F16) mx_store_chunk(static_cast<__half *>(args.Y) + at, r);
+          else mx_store_chunk(static_cast<__nv_bfloat16 *>(args.Y) + at, r);
         }
       }
       tc_fence_before();
@@ -533,22 +718,6 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
-  }
-}
-
-// Row-major scales with rows padded to `pitch` bytes (zeros), so that the copy engine can address them: both operands.
-__global__ void __launch_bounds__(256) mx_pad_scales_kernel(const uint8_t *__restrict__ a, int64_t rows_a, const uint8_t *__restrict__ b, int64_t rows_b, int kb, int pitch,
-                                                            uint32_t *__restrict__ out) {
-  const int64_t words = (rows_a + rows_b) * (pitch / 4);
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / (pitch / 4);
-    const int b0 = (int)(i % (pitch / 4)) * 4;
-    const uint8_t *p = row < rows_a ? a + row * kb : b + (row - rows_a) * kb;
-    uint32_t w = 0;
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (b0 + j < kb) w |= (uint32_t)p[b0 + j] << (8 * j);
-    out[i] = w;
   }
 }
 
@@ -573,75 +742,158 @@ template <typename K> int allow_smem(K kern, int bytes, bool (&configured)[64]) 
   return QL_OK;
 }
 
-int scale_vec(const uint8_t *p, int kb) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p) | (uintptr_t)kb;
-  return a % 8 == 0 ? 8 : (a % 4 == 0 ? 4 : 1);
+bool scales_on_multiple(const MxArgs &args, int of) {
+  return ((reinterpret_cast<uintptr_t>(args.sfa) | reinterpret_cast<uintptr_t>(args.sfb) | (uintptr_t)args.kb) & (uintptr_t)(of - 1)) == 0;
+}
+
+// Clusters of 2^log2 CTAs that the device holds at once at one CTA per SM (a part of the machine with a number of SMs that is
+// no multiple of the cluster leaves some idle: 148, 74, 33, 15 on B200).
+template <int TN, bool WIDE> int resident_clusters(int log2) {
+  static int cached[64][4] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
+  int &n = cached[dev][log2];
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * sm_count() << log2), 1, 1);
+    cfg.blockDim = dim3(kSplitThreads, 1, 1);
+    cfg.dynamicSmemBytes = 232448;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 1u << log2, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int got = 0;
+    if (cudaOccupancyMaxActiveClusters(&got, gemm_mxfp4_split_kernel<TN, WIDE>, &cfg) != cudaSuccess || got < 1) {
+      cudaGetLastError();
+      got = sm_count() >> log2;
+    }
+    n = got;
+  }
+  return n;
+}
+
+struct SplitPlan {
+  int co, log2, rows, stages;
+  double us;
+};
+
+// How to cut a product of few tiles: `rows` of the weights per CTA, 2^log2 CTAs sharing K, `co` CTAs per SM.  The estimate
+// of each choice's time comes from measurements on B200 (graph-replayed calls, cold weights): 3.3 us fixed; per k step
+// 0.33 us, 0.0029 us more for every token row beyond 16, or what one SM's share of memory bandwidth (48 KB/us) takes;
+// 1.2 us + 0.033 us per token row to add up the parts of a cluster.  Examples (us; M, N, K):
+//   1 x 28672 x 8192    100 rows, 2 CTAs per SM 23.5   |  128 rows, 1 per SM (two waves) 30.8  |  K over 4 CTAs 31.5
+//   1 x 4096 x 4096     128 rows, K over 4 CTAs 6.4    |  28 rows, K whole 9.4
+//   24 x 4096 x 11008   128 rows, K over 4 CTAs 11.0   |  28 rows, K whole 18.3
+// Rows are spread so that one wave of CTAs covers the weights: an MMA's rows beyond them cost nothing here, a second wave
+// does.
+template <int TN, bool WIDE> SplitPlan plan_split(int M, int N, int num_ks) {
+  using L = SplitSmem<TN>;
+  const int64_t tiles_x = (M + TN - 1) / TN;
+  SplitPlan best = {1, 0, BM, 1, 1e30};
+  for (int co = 1; co <= (TN <= 32 ? 2 : 1); co++) {
+    for (int log2 = 0; log2 < 4 && (log2 == 0 || num_ks >= (2 << log2)); log2++) {
+      const int fit = resident_clusters<TN, WIDE>(log2) * co;
+      const int64_t per_x = fit / tiles_x, want = per_x < 1 ? BM : (N + per_x - 1) / per_x;
+      const int rows = ((int)(want > BM ? BM : (want < 16 ? 16 : want)) + 3) / 4 * 4;
+      const int64_t tiles = (int64_t)((N + rows - 1) / rows) * tiles_x, waves = (tiles + fit - 1) / fit;
+      const int steps = (num_ks + (1 << log2) - 1) >> log2;
+      const double latency = 0.33 + 0.0029 * (TN - 16), bandwidth = (double)(rows + TN) * BK_BYTES * co / 48e3;
+      const double us = (double)waves * (3.3 + 0.5 * (co - 1) + (log2 ? 1.2 + 0.033 * TN : 0.0) + steps * (latency > bandwidth ? latency : bandwidth));
+      if (us < best.us) {
+        int stages = (232448 / co - 2048 - L::total(rows, 0)) / L::stage_bytes(rows);
+        stages = stages > kSplitMaxStages ? kSplitMaxStages : stages;
+        best = {co, log2, rows, stages > steps ? steps : stages, us};
+      }
+    }
+  }
+  return best;
 }
 
 // args: the weights are operand a here
-template <int TN> int launch_split(const void *w, const void *x, MxArgs args, int64_t K, cudaStream_t st) {
+template <int TN, bool WIDE> int launch_split_as(const void *w, const void *x, MxArgs args, int64_t K, const SplitPlan &plan, cudaStream_t st) {
   using L = SplitSmem<TN>;
-  static bool configured[64] = {false};
-  int rc = allow_smem(gemm_mxfp4_split_kernel<TN>, L::kDynamic, configured);
-  if (rc != QL_OK) return rc;
-  CUtensorMap mw, mx;
-  if ((rc = make_map(&mw, KIND_F8, w, args.N, K / 2, BM)) != QL_OK) return rc;
-  if ((rc = make_map(&mx, KIND_F8, x, args.M, K / 2, TN)) != QL_OK) return rc;
-  args.tiles_a = (args.N + BM - 1) / BM;
+  auto kern = gemm_mxfp4_split_kernel<TN, WIDE>;
+  int rc;
+  args.tiles_a = (args.N + plan.rows - 1) / plan.rows;
   args.tiles_b = (args.M + TN - 1) / TN;
-  const int64_t tiles = (int64_t)args.tiles_a * args.tiles_b;
-  // K is shared by more CTAs while the machine is not full and every CTA keeps two k steps
-  int split = 1;
-  while (split < kMaxSplit && tiles * split < 2ll * sm_count() && args.num_ks / (2 * split) >= 2) split *= 2;
+  CUtensorMap mw, mx;
+  if ((rc = make_map(&mw, KIND_F8, w, args.N, K / 2, plan.rows)) != QL_OK) return rc;
+  if ((rc = make_map(&mx, KIND_F8, x, args.M, K / 2, TN)) != QL_OK) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * split), 1, 1);
+  cfg.gridDim = dim3((unsigned)(((int64_t)args.tiles_a * args.tiles_b) << plan.log2), 1, 1);
   cfg.blockDim = dim3(kSplitThreads, 1, 1);
-  cfg.dynamicSmemBytes = L::kDynamic;
+  cfg.dynamicSmemBytes = L::total(plan.rows, plan.stages);
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)split, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  attr.val.clusterDim.x = 1u << plan.log2, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_mxfp4_split_kernel<TN>, mw, mx, args, split, scale_vec(args.sfa, args.kb), scale_vec(args.sfb, args.kb)));
+  QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, mw, mx, args, plan.rows, plan.stages, plan.log2));
   count_launches(1);
   return QL_OK;
 }
-
-int launch_tiles(const void *a, const void *b, MxArgs args, int64_t K, cudaStream_t st) {
-  static bool configured[64] = {false};
-  int rc = allow_smem(gemm_mxfp4_tiles_kernel, TileSmem::kDynamic, configured);
+// Runs the split kernel where its estimate is below `limit_us`, else says so in *ran.
+template <int TN> int launch_split(const void *w, const void *x, const MxArgs &args, int64_t K, double limit_us, bool *ran, cudaStream_t st) {
+  const bool wide = scales_on_multiple(args, 8);
+  // the occupancy query needs the kernels' shared-memory limit raised first
+  static bool configured_f[64] = {false}, configured_g[64] = {false};
+  int rc = wide ? allow_smem(gemm_mxfp4_split_kernel<TN, true>, 232448, configured_f) : allow_smem(gemm_mxfp4_split_kernel<TN, false>, 232448, configured_g);
   if (rc != QL_OK) return rc;
-  CUtensorMap ma, mb, msa, msb;
+  const SplitPlan plan = wide ? plan_split<TN, true>(args.M, args.N, args.num_ks) : plan_split<TN, false>(args.M, args.N, args.num_ks);
+  *ran = plan.us <= limit_us;
+  if (!*ran) return QL_OK;
+  return wide ? launch_split_as<TN, true>(w, x, args, K, plan, st) : launch_split_as<TN, false>(w, x, args, K, plan, st);
+}
+
+// [rows, row_bytes] bytes, rows `pitch` bytes apart, box = [box_rows, box_bytes], no swizzle
+int make_map_strided(CUtensorMap *map, const void *ptr, int64_t rows, int64_t row_bytes, int64_t pitch, int box_bytes, int box_rows) {
+  EncodeTiledFn enc;
+  int rc = get_encode_fn(&enc);
+  if (rc != QL_OK) return rc;
+  cuuint64_t dims[2] = {(cuuint64_t)row_bytes, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)pitch};
+  cuuint32_t box[2] = {(cuuint32_t)box_bytes, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(QL_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return QL_OK;
+}
+
+template <int SC> int launch_tiles_as(const void *a, const void *b, MxArgs args, int64_t K, cudaStream_t st) {
+  static bool configured[64] = {false};
+  int rc = allow_smem(gemm_mxfp4_tiles_kernel<SC>, TileSmem::kDynamic, configured);
+  if (rc != QL_OK) return rc;
+  CUtensorMap ma, mb, msa, msb, msa_odd, msb_odd;
   if ((rc = make_map(&ma, KIND_F8, a, args.M, K / 2, BM)) != QL_OK) return rc;
   if ((rc = make_map(&mb, KIND_F8, b, args.N, K / 2, TBN)) != QL_OK) return rc;
-  // the copy engine takes rows of whole 16-byte units from a 16-byte aligned base; other scales are padded first
-  uint8_t *scratch = nullptr;
-  int pitch = args.kb;
-  if (args.kb % 16 != 0 || !aligned16(args.sfa) || !aligned16(args.sfb)) {
-    pitch = (args.kb + 15) / 16 * 16;
-    keep_scratch_pool_warm();
-    QL_CUDA_TRY(cudaMallocAsync(&scratch, (size_t)((int64_t)args.M + args.N) * pitch, st));
-    const int64_t words = ((int64_t)args.M + args.N) * (pitch / 4), blocks = (words + 255) / 256, cap = (int64_t)sm_count() * 16;
-    mx_pad_scales_kernel<<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, st>>>(args.sfa, args.M, args.sfb, args.N, args.kb, pitch, reinterpret_cast<uint32_t *>(scratch));
-    count_launches(1);
-    args.sfa = scratch;
-    args.sfb = scratch + (int64_t)args.M * pitch;
+  msa = ma, msb = mb, msa_odd = ma, msb_odd = mb; // whatever the variant does not use
+  if (SC == SC_ROWS) {
+    if ((rc = make_map_bytes(&msa, args.sfa, args.M, args.kb, 32, BM)) != QL_OK) return rc;
+    if ((rc = make_map_bytes(&msb, args.sfb, args.N, args.kb, 32, TBN)) != QL_OK) return rc;
+  } else if (SC == SC_PAIRS) {
+    const int64_t kb = args.kb;
+    if ((rc = make_map_strided(&msa, args.sfa, (args.M + 1) / 2, kb, 2 * kb, 32, BM / 2)) != QL_OK) return rc;
+    if ((rc = make_map_strided(&msb, args.sfb, (args.N + 1) / 2, kb, 2 * kb, 32, TBN / 2)) != QL_OK) return rc;
+    if ((rc = make_map_strided(&msa_odd, args.sfa + kb - 8, args.M / 2, kb + 8, 2 * kb, 48, BM / 2)) != QL_OK) return rc;
+    if ((rc = make_map_strided(&msb_odd, args.sfb + kb - 8, args.N / 2, kb + 8, 2 * kb, 48, TBN / 2)) != QL_OK) return rc;
   }
-  if ((rc = make_map_bytes(&msa, args.sfa, args.M, pitch, 32, BM)) == QL_OK && (rc = make_map_bytes(&msb, args.sfb, args.N, pitch, 32, TBN)) == QL_OK) {
-    args.tiles_a = (args.M + BM - 1) / BM;
-    args.tiles_b = (args.N + TBN - 1) / TBN;
-    const int64_t tiles = (int64_t)args.tiles_a * args.tiles_b;
-    gemm_mxfp4_tiles_kernel<<<(unsigned)(tiles < sm_count() ? tiles : sm_count()), kTileThreads, TileSmem::kDynamic, st>>>(ma, mb, msa, msb, args);
-    count_launches(1);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) rc = cuda_error(e, "gemm_mxfp4_tiles_kernel");
-  }
-  if (scratch) {
-    const cudaError_t e = cudaFreeAsync(scratch, st);
-    if (rc == QL_OK && e != cudaSuccess) return cuda_error(e, "cudaFreeAsync");
-  }
-  return rc;
+  args.tiles_a = (args.M + BM - 1) / BM;
+  args.tiles_b = (args.N + TBN - 1) / TBN;
+  const int64_t tiles = (int64_t)args.tiles_a * args.tiles_b;
+  gemm_mxfp4_tiles_kernel<SC><<<(unsigned)(tiles < sm_count() ? tiles : sm_count()), kTileThreads, TileSmem::kDynamic, st>>>(
+      ma, mb, msa, msb, msa_odd, msb_odd, args);
+  count_launches(1);
+  QL_CUDA_TRY(cudaGetLastError());
+  return QL_OK;
+}
+int launch_tiles(const void *a, const void *b, const MxArgs &args, int64_t K, cudaStream_t st) {
+  const bool bases = aligned16(args.sfa) && aligned16(args.sfb);
+  if (bases && args.kb % 16 == 0) return launch_tiles_as<SC_ROWS>(a, b, args, K, st);
+  if (bases && args.kb % 16 == 8 && args.M > 1 && args.N > 1) return launch_tiles_as<SC_PAIRS>(a, b, args, K, st); // an odd row exists
+  return launch_tiles_as<SC_WORDS>(a, b, args, K, st);
 }
 
 } // namespace
@@ -662,6 +914,7 @@ extern "C" int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, cons
   if (!y->data) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: y has no data pointer", op);
   if (K == 0) return set_error(QL_ERR_UNSUPPORTED, "%s: needs a non-zero K", op);
   if (!aligned16(a->data) || !aligned16(b->data)) return set_error(QL_ERR_UNSUPPORTED, "%s: needs 16-byte aligned operands", op);
+  if ((reinterpret_cast<uintptr_t>(a_scales->data) | reinterpret_cast<uintptr_t>(b_scales->data)) & 3) return set_error(QL_ERR_UNSUPPORTED, "%s: needs 4-byte aligned scales", op);
   if (reinterpret_cast<uintptr_t>(y->data) % (y->dtype == QL_F32 ? 4 : 2)) return set_error(QL_ERR_UNSUPPORTED, "%s: y is not aligned to its type", op);
   if (M > (1 << 30) || N > (1 << 30) || K > (1 << 30)) return set_error(QL_ERR_UNSUPPORTED, "%s: dimension too large", op);
   cudaStream_t st = (cudaStream_t)stream;
@@ -678,15 +931,20 @@ extern "C" int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, cons
   if (!args.status) return set_error(QL_ERR_CUDA, "%s: could not allocate the device status word", op);
   const int64_t tiles = ((M + BM - 1) / BM) * ((N + TBN - 1) / TBN);
   if (tiles >= (1ll << 30)) return set_error(QL_ERR_UNSUPPORTED, "%s: too many output tiles", op);
-  if (M > 128 && tiles >= sm_count()) {
-    args.sfa = static_cast<const uint8_t *>(a_scales->data);
-    args.sfb = static_cast<const uint8_t *>(b_scales->data);
-    return launch_tiles(a->data, b->data, args, K, st);
-  }
-  args.sfa = static_cast<const uint8_t *>(b_scales->data); // the weights are the 128-row operand
+  // The tiles kernel takes 4 us and 0.56 us per k step and tile of an SM (1 us where its warps load the scales); the split
+  // kernel what plan_split says.  Up to 32 tokens the tiles are mostly padding and the split kernel is the better one
+  // throughout.  128 x 4096 x 4096: split 11.7 us, tiles 13.2; 128 x 28672 x 8192: 45.7 and 27.8; 333 x 1001 x 2080: 13.3, 17.4.
+  const int64_t per_sm = (tiles + sm_count() - 1) / sm_count();
+  const double tiles_us = M <= 32 ? 1e30 : 4.0 + (K % 256 == 0 ? 0.56 : 1.0) * (double)per_sm * args.num_ks;
+  args.sfa = static_cast<const uint8_t *>(b_scales->data); // the weights are the 128-row operand of the split kernel
   args.sfb = static_cast<const uint8_t *>(a_scales->data);
-  if (M <= 16) return launch_split<16>(b->data, a->data, args, K, st);
-  if (M <= 32) return launch_split<32>(b->data, a->data, args, K, st);
-  if (M <= 64) return launch_split<64>(b->data, a->data, args, K, st);
-  return launch_split<128>(b->data, a->data, args, K, st);
+  bool ran = false;
+  rc = M <= 16   ? launch_split<16>(b->data, a->data, args, K, tiles_us, &ran, st)
+       : M <= 32 ? launch_split<32>(b->data, a->data, args, K, tiles_us, &ran, st)
+       : M <= 64 ? launch_split<64>(b->data, a->data, args, K, tiles_us, &ran, st)
+                 : launch_split<128>(b->data, a->data, args, K, tiles_us, &ran, st);
+  if (rc != QL_OK || ran) return rc;
+  args.sfa = static_cast<const uint8_t *>(a_scales->data);
+  args.sfb = static_cast<const uint8_t *>(b_scales->data);
+  return launch_tiles(a->data, b->data, args, K, st);
 }

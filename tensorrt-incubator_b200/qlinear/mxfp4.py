@@ -54,6 +54,7 @@ def gemm_mxfp4(a: Float4Tensor, a_scales: torch.Tensor, b: Float4Tensor, b_scale
     if out is None and out_dtype not in dt.QUANTIZABLE_DTYPES:
         raise QuantizeError(f"Unsupported data type in gemm_mxfp4. Supported data types are: {dt.QUANTIZABLE_DTYPES}. Got out_dtype={out_dtype}")
     y = out if out is not None else torch.empty((a.shape[0], b.shape[0]), dtype=out_dtype.torch, device=a.device)
-    sa, sb = a_scales.contiguous(), b_scales.contiguous()   # kept alive across the call: a view only borrows the pointer
+    # dense, on a multiple of 4 bytes (a slice of rows need not be); kept alive across the call: a view only borrows the pointer
+    sa, sb = (s if s.data_ptr() % 4 == 0 else s.clone() for s in (a_scales.contiguous(), b_scales.contiguous()))
     call_on(a.device, _lib.lib().ql_gemm_mxfp4, ql_view(a), ql_view(sa), ql_view(b), ql_view(sb), ql_view(y), same_device=(sa, b, sb, y))
     return y

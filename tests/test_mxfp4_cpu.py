@@ -78,5 +78,6 @@ def test_product_argument_rules():
     assert "no data pointer" in _err(call(y=_t(_lib.BF16, [4, 8], None)))
     assert "non-zero K" in _err(call(a=_t(_lib.F4E2M1, [4, 0], None), sa=_t(_lib.F8E8M0, [4, 0], None), b=_t(_lib.F4E2M1, [8, 0], None), sb=_t(_lib.F8E8M0, [8, 0], None)))
     assert "16-byte aligned" in _err(call(b=_t(_lib.F4E2M1, [8, 64], 0x1008)))
+    assert "4-byte aligned scales" in _err(call(sb=_t(_lib.F8E8M0, [8, 2], 0x1002)))
     assert "aligned to its type" in _err(call(y=_t(_lib.BF16, [4, 8], 0x1001)))
     assert call(a=_t(_lib.F4E2M1, [0, 64], None), sa=_t(_lib.F8E8M0, [0, 2], None), y=_t(_lib.BF16, [0, 8], None)) == 0

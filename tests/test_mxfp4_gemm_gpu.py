@@ -62,7 +62,7 @@ def test_few_tiles(M, N, K, out):
 
 
 # at least 148 tiles of 128 x 224: scales of whole 16-byte rows, and padded ones
-@pytest.mark.parametrize("M,N,K", [(2048, 4096, 512), (1700, 2600, 1056), (4100, 1120, 32), (2048, 2300, 2048), (640, 6700, 4640)])
+@pytest.mark.parametrize("M,N,K", [(2048, 4096, 512), (1700, 2600, 1056), (4100, 1120, 32), (2048, 2300, 2048), (640, 6700, 4640), (1701, 2601, 1280), (2047, 2305, 11008)])
 @pytest.mark.parametrize("out", [torch.float32, torch.float16, torch.bfloat16])
 def test_many_tiles(M, N, K, out):
     a, sa = operand(M, K, 5100 + M)
@@ -91,6 +91,18 @@ def test_scales_of_every_size_and_nan(M, N, K):
     spoiled = torch.zeros_like(z, dtype=torch.bool)
     spoiled[1], spoiled[:, 7] = True, True
     assert torch.equal(torch.isnan(z), spoiled) and torch.equal(z[~spoiled], y[~spoiled])
+
+
+@pytest.mark.parametrize("M,N", [(3, 70), (700, 9000)])
+def test_sliced_operands(M, N):
+    """Row slices: data start on whole rows of 16 bytes, scale rows of 33 and 5 bytes anywhere (a copy is made of those)."""
+    for K in (1056, 160):
+        a, sa = operand(M + 5, K, 5250)
+        b, sb = operand(N + 5, K, 6250, K ** -0.5)
+        part = lambda t, lo, n: ql.Float4Tensor(t.packed[lo * K // 2:(lo + n) * K // 2], (n, K))
+        for lo in (1, 2, 4):
+            a2, sa2, b2, sb2 = part(a, lo, M), sa[lo:lo + M], part(b, lo, N), sb[lo:lo + N]
+            check(ql.gemm_mxfp4(a2, sa2, b2, sb2, out_dtype=ql.float32), a2, sa2, b2, sb2, K)
 
 
 def test_streams_capture_and_interleaved_calls():
