@@ -161,6 +161,28 @@ QL_API int ql_dequantize_mxfp4(const ql_tensor *data, const ql_tensor *scales, q
 QL_API int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, const ql_tensor *b, const ql_tensor *b_scales,
                          ql_tensor *y, void *stream);
 
+/* Gated projection of a feed-forward block in 16 bits (the unquantized counterpart of ql_gemm_fp8_swiglu):
+ *   h[M,I] = act(x w_gate^T) * (x w_up^T),   x [M,K], w_gate and w_up [I,K] (Linear's [out, in] layout), all f16 or all bf16,
+ * both products, the activation and the gate's product in one kernel, from f32 sums with one rounding. */
+typedef enum {
+  QL_ACT_SILU = 0,      /* z / (1 + e^-z) */
+  QL_ACT_GELU = 1,      /* z Phi(z) */
+  QL_ACT_GELU_TANH = 2, /* z / 2 (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+  QL_ACT_RELU = 3
+} ql_activation;
+QL_API int ql_gated_linear(const ql_tensor *x, const ql_tensor *w_gate, const ql_tensor *w_up, int32_t activation,
+                           ql_tensor *h, void *stream);
+/* Its backward pass: the gradients of x, w_gate and w_up from grad = the gradient of h [M,I], all of x's type.  dx may be
+ * null, and so may dw_gate and dw_up together.  Nothing is kept from the forward pass: both projections are computed again;
+ * their gradients are formed in f32 and rounded once to x's type as operands of the second products, which sum in f32.
+ * `workspace`: 256-byte aligned device memory of at least the bytes the query gives; free again when the call's work on the
+ * stream is done.  K and I multiples of 8, 16-byte aligned tensors (QL_ERR_UNSUPPORTED otherwise); M any. */
+QL_API int ql_gated_linear_backward_workspace(const ql_tensor *x, const ql_tensor *w_gate, int32_t want_dx, int32_t want_dw,
+                                              int64_t *bytes);
+QL_API int ql_gated_linear_backward(const ql_tensor *grad, const ql_tensor *x, const ql_tensor *w_gate, const ql_tensor *w_up,
+                                    int32_t activation, ql_tensor *dx, ql_tensor *dw_gate, ql_tensor *dw_up, void *workspace,
+                                    int64_t workspace_bytes, void *stream);
+
 /* Weight-only linear layers, Y[M,N] = X[M,K] . dequantize(W)[N,K]^T with f32 accumulation
  * (linear.py:140-151 with quant_dtype set and no input scale).
  *   w8: W int8 [N,K], scale [N] per output channel (weight_quant_dim = 0)

@@ -1,0 +1,1067 @@
+// Gated projection of a feed-forward block in 16 bits and its backward pass (sm_100a only):
+//     H = act(G) * U,   G = X Wg^T,  U = X Wu^T          X [M,K], Wg and Wu [I,K], H [M,I]; act: silu, gelu, gelu_tanh, relu
+//     dG = dH * U * act'(G),  dU = dH * act(G),  dX = dG Wg + dU Wu,  dWg = dG^T X,  dWu = dU^T X
+// the unquantized counterpart of the fp8 block's gate/up projection (ql_gemm_fp8_swiglu), weights as they are stored.
+//
+// Forward: both projections are one product with the gate rows as one half of the B operand and the up rows as the other;
+// activation and product are formed from the f32 accumulators, and H is rounded once.  G and U never reach memory.
+// Backward: nothing of size M x I is kept from the forward pass.  A first kernel repeats the two projections and forms dG and
+// dU in its epilogue from the f32 accumulators and dH; both are rounded to the operands' type, being the operands of the
+// second kernel, which computes dX and both weight gradients in one launch.  Keeping G and U in 16 bits would save the third
+// of the backward pass that repeats them and would add their two roundings to the one of dG and dU.
+//
+// Kernels:
+//   gated_split     few tokens (decoding): the weights are the 128-row operand (gate rows, then up rows of the same channels),
+//                   up to 128 tokens the other; a cluster of CTAs shares K and adds its parts in rank order through
+//                   distributed shared memory.  Bound by reading the weights once.
+//   gated_pair      many tokens: persistent CTA pairs (cta_group::2) on 256 tokens x 128 channels, six stages; CTA 0 of a
+//                   pair loads the gate rows, CTA 1 the up rows, so each holds half of the B tile.  Bound by the tensor cores.
+//   gated_grads     the second products, persistent CTA pairs on 256 x 256 tiles.  dX reads dG, dU along their rows (K-major)
+//                   and the weights across (MN-major); the weight gradients read both operands across.  All through the
+//                   same 128-byte-swizzled tiles: for an operand whose rows run along the reduction a tile is 64 rows of
+//                   128 bytes per 64 columns, and the descriptor says so.  No operand is transposed in memory.
+//   grads_reduce    adds the f32 parts of units whose reduction was cut, in order.
+// Every wait is bounded, as in the other tensor-core kernels.
+#include <cuda.h>
+#include <string.h>
+
+#include <type_traits>
+
+#include "ql_common.cuh"
+#include "ql_tc_common.cuh"
+
+namespace ql {
+namespace {
+
+enum { ACT_SILU = 0, ACT_GELU = 1, ACT_GELU_TANH = 2, ACT_RELU = 3 };
+
+// act(z).  The fast exponential and division are a few ulp off in f32; the result is rounded to 16 bits.
+template <int ACT> __device__ __forceinline__ float act_value(float z) {
+  if constexpr (ACT == ACT_SILU) return __fdividef(z, 1.f + __expf(-z));
+  else if constexpr (ACT == ACT_GELU) return 0.5f * z * erfcf(-0.70710678f * z);
+  else if constexpr (ACT == ACT_GELU_TANH) return __fdividef(z, 1.f + __expf(-1.5957691f * (z + 0.044715f * z * z * z))); // (1 + tanh y) / 2 = 1 / (1 + e^-2y)
+  else return z < 0.f ? 0.f : z; // a NaN stays one
+}
+// act(z) and act'(z)
+template <int ACT> __device__ __forceinline__ void act_both(float z, float &a, float &d) {
+  if constexpr (ACT == ACT_SILU) {
+    const float s = __fdividef(1.f, 1.f + __expf(-z));
+    a = z * s;
+    d = s * (1.f + z * (1.f - s));
+  } else if constexpr (ACT == ACT_GELU) {
+    const float c = 0.5f * erfcf(-0.70710678f * z);
+    a = z * c;
+    d = c + z * 0.39894228f * __expf(-0.5f * z * z);
+  } else if constexpr (ACT == ACT_GELU_TANH) {
+    const float s = __fdividef(1.f, 1.f + __expf(-1.5957691f * (z + 0.044715f * z * z * z)));
+    a = z * s;
+    d = s + z * s * (1.f - s) * 1.5957691f * (1.f + 0.134145f * z * z);
+  } else {
+    a = z < 0.f ? 0.f : z;
+    d = z > 0.f ? 1.f : 0.f;
+  }
+}
+// f(activation as a template argument), chosen once for a whole chunk of values
+template <typename F> __device__ __forceinline__ void with_act(int act, F &&f) {
+  switch (act) {
+  case ACT_SILU: f(std::integral_constant<int, ACT_SILU>{}); break;
+  case ACT_GELU: f(std::integral_constant<int, ACT_GELU>{}); break;
+  case ACT_GELU_TANH: f(std::integral_constant<int, ACT_GELU_TANH>{}); break;
+  default: f(std::integral_constant<int, ACT_RELU>{}); break;
+  }
+}
+
+template <typename T> constexpr uint32_t kTypeBits = FloatIO<T>::kDtype == QL_BF16 ? (1u << 7 | 1u << 10) : 0u; // operand formats of kind::f16
+
+// Instruction descriptor of kind::f16: f32 accumulation, N >> 3 at bit 17, M >> 4 at bit 24, operand A (bit 15) or B (bit 16)
+// MN-major.
+template <typename T> __device__ __forceinline__ uint32_t f16_idesc(int m, int n, bool a_mn, bool b_mn) {
+  return 1u << 4 | kTypeBits<T> | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24 | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+}
+// Descriptor of an MN-major tile as [64-column groups][64 rows of 128 bytes], 128-byte swizzle: 64 columns further on is 8192
+// bytes (leading byte offset), 8 rows of the reduction further on is 1024 (stride byte offset).
+__device__ __forceinline__ uint64_t make_mn_desc(uint32_t addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr >> 4) & 0x3FFF);
+  d |= (uint64_t)(8192 >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+__device__ __forceinline__ void mma_f16_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+
+constexpr int G_TILE = 128 * BK_BYTES;      // 16 KiB: one CTA's half of an operand tile, 128 rows x 64 values or 64 x 128
+constexpr int G_STAGE = 2 * G_TILE;
+constexpr int G_STAGES = 6;
+constexpr int kPairThreads = 192;           // producer, MMA, four epilogue warps
+constexpr int G_N = 256;                    // columns of the pair's accumulator
+
+struct PairSmem {
+  static constexpr int kStaging = G_STAGES * G_STAGE;       // the epilogue's: 4 warps x 2 x 4096 bytes
+  static constexpr int kBarriers = kStaging + 4 * 2 * 4096; // full[S], empty[S], tfull[2], tempty[2], drain
+  static constexpr int kTmemPtr = kBarriers + (2 * G_STAGES + 5) * 8;
+  static constexpr int kAbort = kTmemPtr + 4;
+  static constexpr int kDynamic = kAbort + 4 + 1024;
+};
+static_assert(PairSmem::kDynamic <= 232448, "shared memory");
+
+// 32 rows x 128 bytes of a warp, parked with the copy engine's swizzle and written out by one bulk tensor store (whole lines,
+// clipped at the matrix's edges); two buffers.
+struct Parked {
+  uint8_t *base;
+  __device__ __forceinline__ void put(int buf, int lane, int piece, const uint4 &v) {
+    *reinterpret_cast<uint4 *>(base + buf * 4096 + lane * 128 + ((piece ^ (lane & 7)) << 4)) = v;
+  }
+  __device__ __forceinline__ void send(int buf, const CUtensorMap *map, int lane, int x, int y) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(map, smem_u32(base + buf * 4096), x, y);
+      bulk_commit();
+    }
+  }
+  template <int PENDING> __device__ __forceinline__ void reusable(int lane) { // the buffer about to be rewritten has been read
+    if (lane == 0) bulk_wait_read<PENDING>();
+    __syncwarp();
+  }
+  __device__ __forceinline__ void finish(int lane) {
+    if (lane == 0) bulk_wait_all<0>();
+    __syncwarp();
+  }
+};
+
+// What the two pair kernels share: barriers, tensor memory, the ring.  Both CTAs' loads complete on the leader's barriers.
+struct Pair {
+  uint8_t *smem;
+  uint32_t base, bars, tmem, rank;
+  volatile int *abort_flag;
+  int *status;
+  int warp, lane;
+  __device__ __forceinline__ uint32_t full(int s) const { return bars + 8u * s; }
+  __device__ __forceinline__ uint32_t empty(int s) const { return bars + 8u * (G_STAGES + s); }
+  __device__ __forceinline__ uint32_t tfull(int b) const { return bars + 8u * (2 * G_STAGES + b); }
+  __device__ __forceinline__ uint32_t tempty(int b) const { return bars + 8u * (2 * G_STAGES + 2 + b); }
+  __device__ __forceinline__ uint32_t drain() const { return bars + 8u * (2 * G_STAGES + 4); }
+
+  __device__ __forceinline__ void start(uint8_t *raw, int *status_) {
+    smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    base = smem_u32(smem);
+    bars = base + PairSmem::kBarriers;
+    abort_flag = reinterpret_cast<volatile int *>(smem + PairSmem::kAbort);
+    status = status_;
+    warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    lane = threadIdx.x & 31;
+    rank = cluster_ctarank();
+    volatile uint32_t *tmem_ptr = reinterpret_cast<volatile uint32_t *>(smem + PairSmem::kTmemPtr);
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < G_STAGES; s++) {
+        mbar_init(full(s), 1);
+        mbar_init(empty(s), 1);
+      }
+      for (int b = 0; b < 2; b++) {
+        mbar_init(tfull(b), 1);
+        mbar_init(tempty(b), 8); // four epilogue warps in each CTA of the pair
+      }
+      mbar_init(drain(), 1);
+      *abort_flag = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32((const void *)tmem_ptr)) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all(); // the partner's barriers exist before anything is signalled across the pair
+    tc_fence_after();
+    tmem = __shfl_sync(0xffffffffu, *tmem_ptr, 0);
+  }
+  __device__ __forceinline__ void end() {
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all(); // neither CTA may leave while the pair's MMAs or barriers can still touch it
+    if (warp == 1) {
+      tc_fence_after();
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+  }
+  // after a failed wait of the producer: tells the partner, and lets what this ring still expects land
+  __device__ __forceinline__ void producer_gives_up(int stage, uint32_t phase, long long issued) {
+    if (lane == 0) signal_partner_abort(smem_u32((const void *)abort_flag), rank);
+    if (rank != 0) return;
+    const long long pending = issued < G_STAGES ? issued : G_STAGES;
+    for (long long i = 0; i < pending; i++) {
+      stage = (stage == 0) ? G_STAGES - 1 : stage - 1;
+      if (stage == G_STAGES - 1) phase ^= 1;
+      bounded_wait(full(stage), phase);
+    }
+  }
+  __device__ __forceinline__ void drain_mmas() {
+    if (elect_one()) tc_commit_pair(map_to_cta(drain(), 0));
+    __syncwarp();
+    if (!bounded_wait(drain(), 0) && lane == 0) atomicCAS(status, 0, ST_TIMEOUT_DRAIN);
+  }
+};
+
+// ------------------------------------------------------------------------------------------------------------------
+// the two projections of many tokens: forward (H), or dG and dU
+// ------------------------------------------------------------------------------------------------------------------
+struct ProjArgs {
+  const void *dh; // backward: [M, I]
+  int M, I, K;
+  int act;
+  int num_kb; // steps of 64 values of K
+  int tiles_m, tiles_n, group_m;
+  int *status;
+};
+
+// Bands of `group_m` row tiles walk all column tiles together, so the band's rows stay in L2.
+__device__ __forceinline__ void band_coords(int tile, int tiles_m, int tiles_n, int group_m, int *mt, int *nt) {
+  const int per_group = group_m * tiles_n, grp = tile / per_group, first = grp * group_m, size = min(group_m, tiles_m - first), local = tile - grp * per_group;
+  *mt = first + local % size;
+  *nt = local / size;
+}
+
+template <typename T, bool BACKWARD>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_gate, const __grid_constant__ CUtensorMap map_up,
+                  const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_out2, const ProjArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  Pair p;
+  p.start(smem_raw, args.status);
+  const int cluster_id = blockIdx.x >> 1, num_clusters = gridDim.x >> 1, num_tiles = args.tiles_m * args.tiles_n;
+
+  if (p.warp == 0) {
+    // ------------------------------------------------------------------ producer (both CTAs)
+    int stage = 0;
+    uint32_t phase = 0;
+    long long issued = 0;
+    bool ok = true;
+    const CUtensorMap *map_w = p.rank == 0 ? &map_gate : &map_up;
+    for (int tile = cluster_id; tile < num_tiles && ok; tile += num_clusters) {
+      int mt, nt;
+      band_coords(tile, args.tiles_m, args.tiles_n, args.group_m, &mt, &nt);
+      const int m0 = mt * 256 + (int)p.rank * 128, n0 = nt * 128;
+      for (int kb = 0; kb < args.num_kb; kb++) {
+        if (!warp_wait(p.empty(stage), phase ^ 1, p.abort_flag, p.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+        if (elect_one()) {
+          const uint32_t dst = p.base + stage * G_STAGE, bar = map_to_cta(p.full(stage), 0);
+          if (p.rank == 0) mbar_expect_tx(p.full(stage), 2 * G_STAGE);
+          tma_load_2d_pair(dst, &map_x, bar, kb * 64, m0);
+          tma_load_2d_pair(dst + G_TILE, map_w, bar, kb * 64, n0);
+        }
+        __syncwarp();
+        issued++;
+        if (++stage == G_STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+    if (!ok) p.producer_gives_up(stage, phase, issued);
+  } else if (p.warp == 1) {
+    // ------------------------------------------------------------------ MMA issue (leader only)
+    if (p.rank == 0) {
+      const uint32_t idesc = f16_idesc<T>(256, G_N, false, false);
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = cluster_id; tile < num_tiles && ok; tile += num_clusters, it++) {
+        const int buf = it & 1;
+        if (!warp_wait(p.tempty(buf), ((it >> 1) & 1) ^ 1, p.abort_flag, p.status, ST_TIMEOUT_TMEM_EMPTY)) { ok = false; break; }
+        for (int kb = 0; kb < args.num_kb; kb++) {
+          if (!warp_wait(p.full(stage), phase, p.abort_flag, p.status, ST_TIMEOUT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t a = p.base + stage * G_STAGE;
+            const uint64_t adesc = make_smem_desc(a), bdesc = make_smem_desc(a + G_TILE);
+#pragma unroll
+            for (int k = 0; k < 4; k++) mma_f16_pair(p.tmem + (uint32_t)(buf * G_N), adesc + 2 * k, bdesc + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+            tc_commit_pair(map_to_cta(p.empty(stage), 0));
+            tc_commit_pair(map_to_cta(p.empty(stage), 1));
+            if (kb == args.num_kb - 1) {
+              tc_commit_pair(map_to_cta(p.tfull(buf), 0));
+              tc_commit_pair(map_to_cta(p.tfull(buf), 1));
+            }
+          }
+          __syncwarp();
+          if (++stage == G_STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok && p.lane == 0) signal_partner_abort(smem_u32((const void *)p.abort_flag), p.rank);
+      p.drain_mmas();
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue (warps 2..5, both CTAs)
+    const int quad = p.warp & 3, lane = p.lane;
+    Parked out{p.smem + PairSmem::kStaging + quad * 8192};
+    int it = 0;
+    bool ok = true;
+    for (int tile = cluster_id; tile < num_tiles; tile += num_clusters, it++) {
+      const int buf = it & 1;
+      int mt, nt;
+      band_coords(tile, args.tiles_m, args.tiles_n, args.group_m, &mt, &nt);
+      const int m0 = mt * 256 + (int)p.rank * 128 + quad * 32, m = m0 + lane;
+      ok = warp_wait(p.tfull(buf), (it >> 1) & 1, p.abort_flag, p.status, ST_TIMEOUT_TMEM_FULL);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t taddr = p.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * G_N);
+#pragma unroll 1
+      for (int c = 0; c < 4; c++) { // 32 channels: gate in columns 32 c, up in columns 128 + 32 c
+        const int n = nt * 128 + c * 32, half = c & 1;
+        uint4 dh[4];
+        if constexpr (BACKWARD) {
+          const T *row = static_cast<const T *>(args.dh) + (size_t)m * (size_t)args.I + n;
+#pragma unroll
+          for (int j = 0; j < 4; j++) dh[j] = m < args.M && n + 8 * j < args.I ? __ldcs(reinterpret_cast<const uint4 *>(row) + j) : make_uint4(0u, 0u, 0u, 0u);
+        }
+        uint32_t g[32], u[32];
+        tmem_load_32(taddr + c * 32, g);
+        tmem_load_32(taddr + 128 + c * 32, u);
+        if constexpr (!BACKWARD) {
+          if (half == 0) out.reusable<1>(lane);
+          with_act(args.act, [&](auto act) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) g[j] = __float_as_uint(act_value<decltype(act)::value>(__uint_as_float(g[j])) * __uint_as_float(u[j]));
+          });
+          auto two = [&](int j) { return pack2<T>(__uint_as_float(g[j]), __uint_as_float(g[j + 1])); };
+          const int b = (c >> 1) & 1;
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) out.put(b, lane, half * 4 + (j >> 3), make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
+          if (half == 1) out.send(b, &map_out, lane, n - 32, m0);
+        } else {
+          if (half == 0) out.reusable<0>(lane); // both buffers: dG in one, dU in the other
+          const T *d = reinterpret_cast<const T *>(dh);
+          with_act(args.act, [&](auto act) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+              float a, da;
+              const float dv = FloatIO<T>::to_f32(d[j]);
+              act_both<decltype(act)::value>(__uint_as_float(g[j]), a, da);
+              g[j] = __float_as_uint(dv * __uint_as_float(u[j]) * da);
+              u[j] = __float_as_uint(dv * a);
+            }
+          });
+          auto two = [&](const uint32_t (&v)[32], int j) { return pack2<T>(__uint_as_float(v[j]), __uint_as_float(v[j + 1])); };
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            out.put(0, lane, half * 4 + (j >> 3), make_uint4(two(g, j), two(g, j + 2), two(g, j + 4), two(g, j + 6)));
+            out.put(1, lane, half * 4 + (j >> 3), make_uint4(two(u, j), two(u, j + 2), two(u, j + 4), two(u, j + 6)));
+          }
+          if (half == 1) {
+            out.send(0, &map_out, lane, n - 32, m0);
+            out.send(1, &map_out2, lane, n - 32, m0);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_cta(p.tempty(buf), 0)); // the leader owns the accumulator hand-over
+    }
+    out.finish(lane);
+    if (!ok && lane == 0) signal_partner_abort(smem_u32((const void *)p.abort_flag), p.rank);
+  }
+  p.end();
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// dX and both weight gradients
+// ------------------------------------------------------------------------------------------------------------------
+struct GradArgs {
+  int M, I, K;
+  // units: a 256 x 256 tile and one of `*_split` parts of its reduction
+  int x_tiles_m, x_tiles_n, x_steps, x_split, x_units;   // dX [M, K]: steps of 64 channels, the gate's first, then the up's
+  int w_tiles_m, w_tiles_n, w_steps, w_split, w_units;   // dWg and dWu [I, K] each: steps of 64 tokens
+  int heavy, heavy_w;                                    // the first `heavy` clusters have one dX unit more and `heavy_w` weight units
+  int x_per;                                             // dX units of the others
+  int group_m;
+  float *x_parts, *w_parts;                              // [split][M][K], [split][2][I][K], null where nothing is cut
+  int *status;
+};
+
+struct Unit {
+  bool is_x;
+  int row0, col0;       // of the output (dW: of dWg, or of dWu when `up`)
+  bool up;
+  int step0, step1, part;
+};
+
+// The j-th unit of cluster c: its dX units, then its weight units.  Neighbouring clusters hold neighbouring tiles.
+__device__ __forceinline__ bool get_unit(const GradArgs &a, int c, int clusters, int j, Unit *u) {
+  const int nx = a.x_per + (c < a.heavy ? 1 : 0);
+  if (j < nx) {
+    const int unit = c + j * clusters, tiles = a.x_tiles_m * a.x_tiles_n, tile = unit % tiles;
+    int mt, nt;
+    band_coords(tile, a.x_tiles_m, a.x_tiles_n, a.group_m, &mt, &nt);
+    u->is_x = true, u->up = false, u->row0 = mt * 256, u->col0 = nt * 256, u->part = unit / tiles;
+    u->step0 = (int)((long long)a.x_steps * u->part / a.x_split), u->step1 = (int)((long long)a.x_steps * (u->part + 1) / a.x_split);
+    return true;
+  }
+  j -= nx;
+  int unit;
+  if (c < a.heavy) {
+    if (j >= a.heavy_w) return false;
+    unit = j * a.heavy + c;
+  } else {
+    unit = a.heavy * a.heavy_w + j * (clusters - a.heavy) + (c - a.heavy);
+  }
+  if (unit >= a.w_units) return false;
+  const int tiles = 2 * a.w_tiles_m * a.w_tiles_n, tile = unit % tiles;
+  int mt, nt;
+  band_coords(tile, 2 * a.w_tiles_m, a.w_tiles_n, a.group_m, &mt, &nt);
+  u->is_x = false, u->up = mt >= a.w_tiles_m, u->row0 = (u->up ? mt - a.w_tiles_m : mt) * 256, u->col0 = nt * 256, u->part = unit / tiles;
+  u->step0 = (int)((long long)a.w_steps * u->part / a.w_split), u->step1 = (int)((long long)a.w_steps * (u->part + 1) / a.w_split);
+  return true;
+}
+
+// Maps: d*_k see dG / dU as tiles of 128 rows x 64 columns (K-major), d*_mn, w*_mn, x_mn as 64 rows x 64 columns.
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+gated_grads_kernel(const __grid_constant__ CUtensorMap map_dg_k, const __grid_constant__ CUtensorMap map_du_k, const __grid_constant__ CUtensorMap map_dg_mn,
+                   const __grid_constant__ CUtensorMap map_du_mn, const __grid_constant__ CUtensorMap map_wg_mn, const __grid_constant__ CUtensorMap map_wu_mn,
+                   const __grid_constant__ CUtensorMap map_x_mn, const __grid_constant__ CUtensorMap map_dx, const __grid_constant__ CUtensorMap map_dwg,
+                   const __grid_constant__ CUtensorMap map_dwu, const GradArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  Pair p;
+  p.start(smem_raw, args.status);
+  const int cluster_id = blockIdx.x >> 1, num_clusters = gridDim.x >> 1;
+  Unit u;
+
+  if (p.warp == 0) {
+    // ------------------------------------------------------------------ producer (both CTAs)
+    int stage = 0;
+    uint32_t phase = 0;
+    long long issued = 0;
+    bool ok = true;
+    const int half_steps = args.x_steps / 2; // steps of the gate's channels
+    for (int j = 0; ok && get_unit(args, cluster_id, num_clusters, j, &u); j++) {
+      const int r0 = u.row0 + (int)p.rank * 128, c0 = u.col0 + (int)p.rank * 128;
+      for (int s = u.step0; s < u.step1; s++) {
+        if (!warp_wait(p.empty(stage), phase ^ 1, p.abort_flag, p.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+        if (elect_one()) {
+          const uint32_t a = p.base + stage * G_STAGE, b = a + G_TILE, bar = map_to_cta(p.full(stage), 0);
+          if (p.rank == 0) mbar_expect_tx(p.full(stage), 2 * G_STAGE);
+          if (u.is_x) {
+            const bool up = s >= half_steps;
+            const int i0 = (up ? s - half_steps : s) * 64;
+            tma_load_2d_pair(a, up ? &map_du_k : &map_dg_k, bar, i0, r0);
+            const CUtensorMap *w = up ? &map_wu_mn : &map_wg_mn;
+            tma_load_2d_pair(b, w, bar, c0, i0);
+            tma_load_2d_pair(b + 8192, w, bar, c0 + 64, i0);
+          } else {
+            const CUtensorMap *d = u.up ? &map_du_mn : &map_dg_mn;
+            tma_load_2d_pair(a, d, bar, r0, s * 64);
+            tma_load_2d_pair(a + 8192, d, bar, r0 + 64, s * 64);
+            tma_load_2d_pair(b, &map_x_mn, bar, c0, s * 64);
+            tma_load_2d_pair(b + 8192, &map_x_mn, bar, c0 + 64, s * 64);
+          }
+        }
+        __syncwarp();
+        issued++;
+        if (++stage == G_STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+    if (!ok) p.producer_gives_up(stage, phase, issued);
+  } else if (p.warp == 1) {
+    // ------------------------------------------------------------------ MMA issue (leader only)
+    if (p.rank == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int j = 0; ok && get_unit(args, cluster_id, num_clusters, j, &u); j++) {
+        const int buf = j & 1;
+        const uint32_t idesc = f16_idesc<T>(256, G_N, !u.is_x, true);
+        if (!warp_wait(p.tempty(buf), ((j >> 1) & 1) ^ 1, p.abort_flag, p.status, ST_TIMEOUT_TMEM_EMPTY)) { ok = false; break; }
+        for (int s = u.step0; s < u.step1; s++) {
+          if (!warp_wait(p.full(stage), phase, p.abort_flag, p.status, ST_TIMEOUT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t a = p.base + stage * G_STAGE;
+            // 16 values of the reduction further on: 32 bytes along a row, or 16 rows of 128 bytes
+            const uint64_t adesc = u.is_x ? make_smem_desc(a) : make_mn_desc(a), bdesc = make_mn_desc(a + G_TILE);
+            const uint64_t astep = u.is_x ? 2 : 128;
+#pragma unroll
+            for (int k = 0; k < 4; k++) mma_f16_pair(p.tmem + (uint32_t)(buf * G_N), adesc + astep * k, bdesc + 128 * k, idesc, (s > u.step0 || k) ? 1u : 0u);
+            tc_commit_pair(map_to_cta(p.empty(stage), 0));
+            tc_commit_pair(map_to_cta(p.empty(stage), 1));
+            if (s == u.step1 - 1) {
+              tc_commit_pair(map_to_cta(p.tfull(buf), 0));
+              tc_commit_pair(map_to_cta(p.tfull(buf), 1));
+            }
+          }
+          __syncwarp();
+          if (++stage == G_STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok && p.lane == 0) signal_partner_abort(smem_u32((const void *)p.abort_flag), p.rank);
+      p.drain_mmas();
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue (warps 2..5, both CTAs)
+    const int quad = p.warp & 3, lane = p.lane;
+    Parked out{p.smem + PairSmem::kStaging + quad * 8192};
+    bool ok = true;
+    for (int j = 0; get_unit(args, cluster_id, num_clusters, j, &u); j++) {
+      const int buf = j & 1;
+      ok = warp_wait(p.tfull(buf), (j >> 1) & 1, p.abort_flag, p.status, ST_TIMEOUT_TMEM_FULL);
+      if (!ok) break;
+      tc_fence_after();
+      const int r0 = u.row0 + (int)p.rank * 128 + quad * 32, r = r0 + lane, rows = u.is_x ? args.M : args.I;
+      const uint32_t taddr = p.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * G_N);
+      float *parts = u.is_x ? args.x_parts : args.w_parts;
+      if (parts) { // f32 part of a cut reduction: [part][dX, or dWg and dWu]
+        parts += ((size_t)(u.is_x ? u.part : 2 * u.part + (u.up ? 1 : 0)) * (size_t)rows + (size_t)r) * (size_t)args.K;
+      }
+      const CUtensorMap *map = u.is_x ? &map_dx : (u.up ? &map_dwu : &map_dwg);
+#pragma unroll 1
+      for (int c = 0; c < G_N / 32; c++) {
+        const int n = u.col0 + c * 32, half = c & 1, b = (c >> 1) & 1;
+        uint32_t v[32];
+        tmem_load_32(taddr + c * 32, v);
+        if (parts) {
+          if (r < rows) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) // K is a multiple of 8
+              if (n + i < args.K) __stcs(reinterpret_cast<uint4 *>(parts + n + i), make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+          }
+        } else {
+          if (half == 0) out.reusable<1>(lane);
+          auto two = [&](int i) { return pack2<T>(__uint_as_float(v[i]), __uint_as_float(v[i + 1])); };
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) out.put(b, lane, half * 4 + (i >> 3), make_uint4(two(i), two(i + 2), two(i + 4), two(i + 6)));
+          if (half == 1) out.send(b, map, lane, n - 32, r0);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(map_to_cta(p.tempty(buf), 0));
+    }
+    out.finish(lane);
+    if (!ok && lane == 0) signal_partner_abort(smem_u32((const void *)p.abort_flag), p.rank);
+  }
+  p.end();
+}
+
+// out[i] = sum over p of parts[p][i], p rising; blocks below `x_blocks` add dX, the others dWg and then dWu
+template <typename T>
+__global__ void __launch_bounds__(256) grads_reduce_kernel(const float4 *__restrict__ x_parts, int x_split, T *__restrict__ dx, int64_t nx4, const float4 *__restrict__ w_parts,
+                                                           int w_split, T *__restrict__ dwg, T *__restrict__ dwu, int64_t nw4) {
+  const int64_t n = (x_parts ? nx4 : 0) + (w_parts ? 2 * nw4 : 0);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const bool is_x = x_parts && i < nx4;
+    const int64_t j = is_x ? i : i - (x_parts ? nx4 : 0);
+    const float4 *src = is_x ? x_parts + j : w_parts + j;
+    const int64_t stride = is_x ? nx4 : 2 * nw4;
+    const int split = is_x ? x_split : w_split;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < split; p++) {
+      const float4 w = __ldcs(src + p * stride);
+      v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+    }
+    T *out = is_x ? dx : (j < nw4 ? dwg : dwu);
+    const int64_t at = is_x || j < nw4 ? j : j - nw4;
+    reinterpret_cast<uint2 *>(out)[at] = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------------
+// few tokens: the weights as the 128-row operand, K over the CTAs of a cluster
+// ------------------------------------------------------------------------------------------------------------------
+constexpr int kSplitThreads = 192;
+constexpr int kSplitMaxStages = 16;
+constexpr int kMaxSplit = 8;
+
+struct SplitArgs {
+  void *h;
+  int M, I;
+  int act;
+  int num_kb;
+  int tiles_c; // tiles of channels
+  int *status;
+};
+
+// Fixed parts first, then the ring: `stages` of (channels rounded up to 8) gate rows, as many up rows and TN tokens of 128
+// bytes each.  The MMA reads 128 rows whatever there is of them; the rest lands in accumulator rows nobody looks at.
+template <int TN> struct SplitSmem {
+  static constexpr int kParts = 0;                      // this CTA's tokens, [split][TN / split][128]
+  static constexpr int kBarriers = kParts + TN * BM * 4; // full[16], empty[16], tfull
+  static constexpr int kTmemPtr = kBarriers + (2 * kSplitMaxStages + 1) * 8;
+  static constexpr int kAbort = kTmemPtr + 4;
+  static constexpr int kRing = (kAbort + 4 + 1023) / 1024 * 1024;
+  static constexpr int stage_bytes(int channels) { return ((channels + 7) / 8 * 16 + TN) * BK_BYTES; }
+  static constexpr int total(int channels, int stages) { return kRing + stages * stage_bytes(channels) + BM * BK_BYTES + 1024; }
+};
+
+template <typename T, int TN>
+__global__ void __launch_bounds__(kSplitThreads)
+gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__ CUtensorMap map_up, const __grid_constant__ CUtensorMap map_x,
+                   const SplitArgs args, int channels, int stages, int split_log2) {
+  using L = SplitSmem<TN>;
+  constexpr int TN_LOG2 = TN == 16 ? 4 : (TN == 32 ? 5 : (TN == 64 ? 6 : 7));
+  constexpr uint32_t kTmemCols = TN < 32 ? 32 : TN;
+  const int c8 = (channels + 7) / 8 * 8, stage_bytes = L::stage_bytes(channels), x_off = stage_bytes - TN * BK_BYTES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t smem_base = smem_u32(smem), bar_base = smem_base + L::kBarriers;
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (kSplitMaxStages + s); };
+  const uint32_t tfull_bar = bar_base + 8u * (2 * kSplitMaxStages);
+  volatile uint32_t *tmem_ptr_smem = reinterpret_cast<volatile uint32_t *>(smem + L::kTmemPtr);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::kAbort);
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int split = 1 << split_log2;
+  const int rank = blockIdx.x & (split - 1), tile = blockIdx.x >> split_log2;
+  const int ct = tile % args.tiles_c, xt = tile / args.tiles_c;
+  const int kb0 = (int)((long long)args.num_kb * rank / split), kb1 = (int)((long long)args.num_kb * (rank + 1) / split);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; s++) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(tfull_bar, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)tmem_ptr_smem)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (split > 1) cluster_arrive(); // waited for before the first store into a partner: the partner has started by then
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr_smem, 0);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ producer
+    int stage = 0, issued = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; kb++) {
+      if (!warp_wait(empty_bar(stage), phase ^ 1, abort_flag, args.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+      if (elect_one()) {
+        const uint32_t dst = smem_base + L::kRing + stage * stage_bytes;
+        mbar_expect_tx(full_bar(stage), (uint32_t)(2 * channels + TN) * BK_BYTES);
+        tma_load_2d(dst, &map_gate, full_bar(stage), kb * 64, ct * channels);
+        tma_load_2d(dst + c8 * BK_BYTES, &map_up, full_bar(stage), kb * 64, ct * channels);
+        tma_load_2d(dst + x_off, &map_x, full_bar(stage), kb * 64, xt * TN);
+      }
+      __syncwarp();
+      issued++;
+      if (++stage == stages) { stage = 0; phase ^= 1; }
+    }
+    if (!ok) { // let the loads in flight land before the shared memory goes away
+      const int pending = issued < stages ? issued : stages;
+      for (int i = 0; i < pending; i++) {
+        stage = (stage == 0) ? stages - 1 : stage - 1;
+        if (stage == stages - 1) phase ^= 1;
+        bounded_wait(full_bar(stage), phase);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issue
+    const uint32_t idesc = f16_idesc<T>(BM, TN, false, false);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; kb++) {
+      if (!warp_wait(full_bar(stage), phase, abort_flag, args.status, ST_TIMEOUT_FULL)) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t a = smem_base + L::kRing + stage * stage_bytes;
+        const uint64_t adesc = make_smem_desc(a), bdesc = make_smem_desc(a + x_off);
+#pragma unroll
+        for (int k = 0; k < 4; k++) tc_mma<KIND_F16>(tmem_base, adesc + 2 * k, bdesc + 2 * k, idesc, (kb > kb0 || k) ? 1u : 0u);
+        tc_commit(empty_bar(stage));
+      }
+      __syncwarp();
+      if (++stage == stages) { stage = 0; phase ^= 1; }
+    }
+    // every MMA issued above is done with shared and tensor memory before this warp goes on, after an abort too
+    if (elect_one()) tc_commit(tfull_bar);
+    __syncwarp();
+    if (!bounded_wait(tfull_bar, 0) && lane == 0) atomicCAS(args.status, 0, ST_TIMEOUT_DRAIN);
+    if (split > 1) cluster_wait();
+  } else {
+    // ------------------------------------------------------------------ the accumulator (warps 2..5)
+    const int quad = warp & 3, row = quad * 32 + lane;
+    warp_wait(tfull_bar, 0, abort_flag, args.status, ST_TIMEOUT_TMEM_FULL);
+    tc_fence_after();
+    const int tokens = min(TN, args.M - xt * TN), per_log2 = TN_LOG2 - split_log2, per = 1 << per_log2; // CTA o adds up tokens [o * per, (o + 1) * per)
+    if (split > 1) cluster_wait();
+#pragma unroll 1
+    for (int c = 0; c < TN / 16; c++) {
+      if (c * 16 >= tokens) break;
+      uint32_t r[16];
+      tmem_load_16(tmem_base + ((uint32_t)(quad * 32) << 16) + c * 16, r);
+#pragma unroll
+      for (int j = 0; j < 16; j++) {
+        const int t = c * 16 + j;
+        if (t < tokens) {
+          const uint32_t local = smem_base + (uint32_t)(L::kParts + ((rank * per + (t & (per - 1))) * BM + row) * 4);
+          if (split > 1) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(local, (uint32_t)(t >> per_log2))), "f"(__uint_as_float(r[j])) : "memory");
+          else asm volatile("st.shared.f32 [%0], %1;" ::"r"(local), "f"(__uint_as_float(r[j])) : "memory");
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  if (split > 1 && warp == 0) cluster_wait();
+  __syncthreads();
+  if (split > 1) cluster_sync_all(); // every part has arrived
+  {
+    const int per = TN >> split_log2, t0 = rank * per, t1 = min(t0 + per, args.M - xt * TN);
+    const float *parts = reinterpret_cast<const float *>(smem + L::kParts);
+    T *h = static_cast<T *>(args.h);
+    with_act(args.act, [&](auto act) {
+      for (int i = threadIdx.x; i < (t1 - t0) * 64; i += kSplitThreads) {
+        const int t = i / 64, ch = i % 64, n = ct * channels + ch;
+        if (ch >= channels || n >= args.I) continue;
+        float g = 0.f, u = 0.f;
+#pragma unroll
+        for (int p = 0; p < kMaxSplit; p++) {
+          if (p < split) {
+            g += parts[(p * per + t) * BM + ch];
+            u += parts[(p * per + t) * BM + c8 + ch];
+          }
+        }
+        h[(size_t)(xt * TN + t0 + t) * (size_t)args.I + n] = FloatIO<T>::from_f32(act_value<decltype(act)::value>(g) * u);
+      }
+    });
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+  }
+}
+
+// ----------------------------------------------------------------------------------------------
+// host side
+// ----------------------------------------------------------------------------------------------
+template <typename T> constexpr int kMapKind = FloatIO<T>::kDtype == QL_BF16 ? KIND_BF16 : KIND_F16;
+
+template <typename K> int resident(K kern, int threads, int smem, int cluster) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * sm_count() * cluster), 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)cluster, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = sm_count() / cluster;
+  }
+  return n;
+}
+// clusters (of `cluster` CTAs, one CTA per SM) of a kernel the current device holds at once; asked once
+template <typename K> int resident_cached(K kern, int threads, int smem, int cluster, int (&cache)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sm_count() / cluster;
+  if (cache[dev] == 0) cache[dev] = resident(kern, threads, smem, cluster);
+  return cache[dev];
+}
+
+// A band of rows of A stays L2-resident: about 16 MiB of it, four row tiles of 256 at the least.
+int band(int64_t row_bytes, int tiles_m) {
+  int64_t g = (16ll << 20) / (256 * row_bytes);
+  g = g < 4 ? 4 : g;
+  return (int)(g > tiles_m ? (tiles_m < 1 ? 1 : tiles_m) : g);
+}
+
+template <typename T, bool BACKWARD>
+int launch_pair(const void *x, const void *wg, const void *wu, const void *dh, void *out, void *out2, int M, int I, int K, int act, cudaStream_t st) {
+  auto kern = gated_pair_kernel<T, BACKWARD>;
+  static bool configured[64] = {false};
+  static int cache[64] = {0};
+  int rc = allow_smem(kern, PairSmem::kDynamic, configured);
+  if (rc != QL_OK) return rc;
+  ProjArgs a;
+  a.dh = dh;
+  a.M = M, a.I = I, a.K = K, a.act = act;
+  a.num_kb = (K + 63) / 64;
+  a.tiles_m = (M + 255) / 256;
+  a.tiles_n = (I + 127) / 128;
+  a.group_m = band((int64_t)K * 2, a.tiles_m);
+  a.status = device_status_word();
+  if (!a.status) return set_error(QL_ERR_CUDA, "gated_linear: could not allocate the device status word");
+  CUtensorMap mx, mg, mu, mo, mo2;
+  const int kind = kMapKind<T>, dtype = FloatIO<T>::kDtype;
+  if ((rc = make_map(&mx, kind, x, M, K, 128)) != QL_OK) return rc;
+  if ((rc = make_map(&mg, kind, wg, I, K, 128)) != QL_OK) return rc;
+  if ((rc = make_map(&mu, kind, wu, I, K, 128)) != QL_OK) return rc;
+  if ((rc = make_map_out(&mo, dtype, out, M, I, I)) != QL_OK) return rc;
+  if ((rc = make_map_out(&mo2, dtype, out2 ? out2 : out, M, I, I)) != QL_OK) return rc;
+  const int pairs = resident_cached(kern, kPairThreads, PairSmem::kDynamic, 2, cache), tiles = a.tiles_m * a.tiles_n;
+  kern<<<2 * (tiles < pairs ? tiles : pairs), kPairThreads, PairSmem::kDynamic, st>>>(mx, mg, mu, mo, mo2, a);
+  count_launches(1);
+  QL_CUDA_TRY(cudaGetLastError());
+  return QL_OK;
+}
+
+struct SplitPlan {
+  int co, log2, channels, stages;
+  double us;
+};
+
+template <typename T, int TN> SplitPlan plan_split(int M, int I, int num_kb) {
+  using L = SplitSmem<TN>;
+  static int cache[4][64] = {};
+  const int64_t tiles_x = (M + TN - 1) / TN;
+  SplitPlan best = {1, 0, 64, 1, 1e30};
+  for (int co = 1; co <= (TN <= 32 ? 2 : 1); co++) {
+    for (int log2 = 0; log2 < 4 && (log2 == 0 || num_kb >= (4 << log2)); log2++) {
+      const int fit = resident_cached(gated_split_kernel<T, TN>, kSplitThreads, 232448, 1 << log2, cache[log2]) * co;
+      const int64_t per_x = fit / tiles_x, want = per_x < 1 ? 64 : (I + per_x - 1) / per_x;
+      const int channels = (int)(want > 64 ? 64 : (want < 8 ? 8 : want));
+      const int64_t tiles = (int64_t)((I + channels - 1) / channels) * tiles_x, waves = (tiles + fit - 1) / fit;
+      const int steps = (num_kb + (1 << log2) - 1) >> log2;
+      const double latency = 0.2 + 0.0029 * (TN - 16), bandwidth = (double)(2 * channels + TN) * BK_BYTES * co / 48e3;
+      const double us = (double)waves * (3.3 + 0.5 * (co - 1) + (log2 ? 1.2 + 0.033 * TN : 0.0) + steps * (latency > bandwidth ? latency : bandwidth));
+      if (us < best.us) {
+        int stages = (232448 / co - 2048 - L::total(channels, 0)) / L::stage_bytes(channels);
+        stages = stages > kSplitMaxStages ? kSplitMaxStages : stages;
+        best = {co, log2, channels, stages > steps ? steps : stages, us};
+      }
+    }
+  }
+  return best;
+}
+
+// Runs the split kernel where its estimate is below `limit_us`, else says so in *ran.
+template <typename T, int TN>
+int launch_split(const void *x, const void *wg, const void *wu, void *h, int M, int I, int K, int act, double limit_us, bool *ran, cudaStream_t st) {
+  using L = SplitSmem<TN>;
+  auto kern = gated_split_kernel<T, TN>;
+  static bool configured[64] = {false};
+  int rc = allow_smem(kern, 232448, configured);
+  if (rc != QL_OK) return rc;
+  SplitArgs a;
+  a.h = h;
+  a.M = M, a.I = I, a.act = act;
+  a.num_kb = (K + 63) / 64;
+  const SplitPlan plan = plan_split<T, TN>(M, I, a.num_kb);
+  *ran = plan.us <= limit_us;
+  if (!*ran) return QL_OK;
+  a.tiles_c = (I + plan.channels - 1) / plan.channels;
+  a.status = device_status_word();
+  if (!a.status) return set_error(QL_ERR_CUDA, "gated_linear: could not allocate the device status word");
+  CUtensorMap mg, mu, mx;
+  const int kind = kMapKind<T>;
+  if ((rc = make_map(&mg, kind, wg, I, K, plan.channels)) != QL_OK) return rc;
+  if ((rc = make_map(&mu, kind, wu, I, K, plan.channels)) != QL_OK) return rc;
+  if ((rc = make_map(&mx, kind, x, M, K, TN)) != QL_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(((int64_t)a.tiles_c * ((M + TN - 1) / TN)) << plan.log2), 1, 1);
+  cfg.blockDim = dim3(kSplitThreads, 1, 1);
+  cfg.dynamicSmemBytes = L::total(plan.channels, plan.stages);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 1u << plan.log2, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, mg, mu, mx, a, plan.channels, plan.stages, plan.log2));
+  count_launches(1);
+  return QL_OK;
+}
+
+template <typename T>
+int forward(const void *x, const void *wg, const void *wu, void *h, int M, int I, int K, int act, cudaStream_t st) {
+  const int64_t tiles = (int64_t)((M + 255) / 256) * ((I + 127) / 128), per = (tiles + sm_count() / 2 - 1) / (sm_count() / 2);
+  const double pair_us = M <= 32 ? 1e30 : 6.0 + 0.3 * (double)per * ((K + 63) / 64);
+  bool ran = false;
+  int rc;
+  if (M <= 16) rc = launch_split<T, 16>(x, wg, wu, h, M, I, K, act, pair_us, &ran, st);
+  else if (M <= 32) rc = launch_split<T, 32>(x, wg, wu, h, M, I, K, act, pair_us, &ran, st);
+  else if (M <= 64) rc = launch_split<T, 64>(x, wg, wu, h, M, I, K, act, pair_us, &ran, st);
+  else rc = launch_split<T, 128>(x, wg, wu, h, M, I, K, act, pair_us, &ran, st);
+  if (rc != QL_OK || ran) return rc;
+  return launch_pair<T, false>(x, wg, wu, nullptr, h, nullptr, M, I, K, act, st);
+}
+
+// How the units of the second products are cut and dealt out (see GradArgs), for `pairs` CTA pairs.
+struct GradPlan {
+  GradArgs a;
+  int64_t x_part_floats, w_part_floats;
+};
+GradPlan plan_grads(int M, int I, int K, bool want_x, bool want_w, int pairs) {
+  GradPlan p;
+  GradArgs &a = p.a;
+  a.M = M, a.I = I, a.K = K;
+  a.x_tiles_m = (M + 255) / 256, a.x_tiles_n = a.w_tiles_n = (K + 255) / 256, a.w_tiles_m = (I + 255) / 256;
+  a.x_steps = 2 * ((I + 63) / 64), a.w_steps = (M + 63) / 64;
+  const int64_t x_tiles = want_x ? (int64_t)a.x_tiles_m * a.x_tiles_n : 0, w_tiles = want_w ? 2ll * a.w_tiles_m * a.w_tiles_n : 0;
+  // A unit costs its steps and about 8 more to start and write out.  A reduction is cut where its tiles alone would leave
+  // pairs idle: into units of at least 8 steps, no longer than a pair's share of all steps.
+  const int64_t share = (x_tiles * a.x_steps + w_tiles * a.w_steps + pairs - 1) / pairs;
+  auto cut = [&](int64_t tiles, int steps) {
+    if (tiles == 0 || tiles >= pairs) return 1;
+    const int64_t len = share < 8 ? 8 : share;
+    int64_t s = (steps + len - 1) / len;
+    const int64_t most = steps / 8 < 1 ? 1 : steps / 8;
+    s = s > most ? most : s;
+    return (int)(s > 32 ? 32 : s);
+  };
+  a.x_split = cut(x_tiles, a.x_steps), a.w_split = cut(w_tiles, a.w_steps);
+  a.x_units = (int)(x_tiles * a.x_split), a.w_units = (int)(w_tiles * a.w_split);
+  a.x_per = a.x_units / pairs, a.heavy = a.x_units % pairs;
+  // weight units of a heavy cluster: as many fewer as one dX unit is worth
+  const double ux = (double)a.x_steps / a.x_split + 8, uw = (double)a.w_steps / a.w_split + 8;
+  double hw = (a.w_units - (pairs - a.heavy) * ux / uw) / pairs;
+  a.heavy_w = a.heavy == 0 ? 0 : (int)(hw < 0 ? 0 : hw + 0.5);
+  if ((int64_t)a.heavy * a.heavy_w > a.w_units) a.heavy_w = a.w_units / a.heavy;
+  a.group_m = 8;
+  a.x_parts = a.w_parts = nullptr;
+  p.x_part_floats = a.x_split > 1 ? (int64_t)a.x_split * M * K : 0;
+  p.w_part_floats = a.w_split > 1 ? 2ll * a.w_split * I * K : 0;
+  return p;
+}
+
+int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+
+template <typename T> int grad_pairs() {
+  static bool configured[64] = {false};
+  static int cache[64] = {0};
+  if (allow_smem(gated_grads_kernel<T>, PairSmem::kDynamic, configured) != QL_OK) return sm_count() / 2;
+  return resident_cached(gated_grads_kernel<T>, kPairThreads, PairSmem::kDynamic, 2, cache);
+}
+int pairs_of(int dtype) { return dtype == QL_BF16 ? grad_pairs<__nv_bfloat16>() : grad_pairs<__half>(); }
+
+template <typename T>
+int backward(const void *dh, const void *x, const void *wg, const void *wu, void *dx, void *dwg, void *dwu, int M, int I, int K, int act, uint8_t *ws, const GradPlan &plan,
+             cudaStream_t st) {
+  const int64_t mi = align256((int64_t)M * I * 2);
+  void *dg = ws, *du = ws + mi;
+  int rc = launch_pair<T, true>(x, wg, wu, dh, dg, du, M, I, K, act, st);
+  if (rc != QL_OK || (!dx && !dwg)) return rc;
+  GradArgs a = plan.a;
+  a.status = device_status_word();
+  uint8_t *parts = ws + 2 * mi;
+  if (plan.x_part_floats) a.x_parts = reinterpret_cast<float *>(parts);
+  if (plan.w_part_floats) a.w_parts = reinterpret_cast<float *>(parts + align256(plan.x_part_floats * 4));
+  CUtensorMap dgk, duk, dgm, dum, wgm, wum, xm, mx, mg, mu;
+  const int kind = kMapKind<T>, dtype = FloatIO<T>::kDtype;
+  if ((rc = make_map(&dgk, kind, dg, M, I, 128)) != QL_OK) return rc;
+  if ((rc = make_map(&duk, kind, du, M, I, 128)) != QL_OK) return rc;
+  if ((rc = make_map(&dgm, kind, dg, M, I, 64)) != QL_OK) return rc;
+  if ((rc = make_map(&dum, kind, du, M, I, 64)) != QL_OK) return rc;
+  if ((rc = make_map(&wgm, kind, wg, I, K, 64)) != QL_OK) return rc;
+  if ((rc = make_map(&wum, kind, wu, I, K, 64)) != QL_OK) return rc;
+  if ((rc = make_map(&xm, kind, x, M, K, 64)) != QL_OK) return rc;
+  mx = mg = mu = xm; // what is not wanted is not written
+  if (dx && (rc = make_map_out(&mx, dtype, dx, M, K, K)) != QL_OK) return rc;
+  if (dwg && (rc = make_map_out(&mg, dtype, dwg, I, K, K)) != QL_OK) return rc;
+  if (dwu && (rc = make_map_out(&mu, dtype, dwu, I, K, K)) != QL_OK) return rc;
+  const int pairs = grad_pairs<T>(); // get_unit deals the units out over exactly this many
+  gated_grads_kernel<T><<<2 * pairs, kPairThreads, PairSmem::kDynamic, st>>>(dgk, duk, dgm, dum, wgm, wum, xm, mx, mg, mu, a);
+  count_launches(1);
+  QL_CUDA_TRY(cudaGetLastError());
+  if (a.x_parts || a.w_parts) {
+    const int64_t nx4 = (int64_t)M * K / 4, nw4 = (int64_t)I * K / 4, n = (a.x_parts ? nx4 : 0) + (a.w_parts ? 2 * nw4 : 0);
+    const int64_t blocks = (n + 255) / 256, cap = (int64_t)sm_count() * 8;
+    grads_reduce_kernel<T><<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, st>>>(reinterpret_cast<const float4 *>(a.x_parts), a.x_split, static_cast<T *>(dx), nx4,
+                                                                                reinterpret_cast<const float4 *>(a.w_parts), a.w_split, static_cast<T *>(dwg),
+                                                                                static_cast<T *>(dwu), nw4);
+    count_launches(1);
+    QL_CUDA_TRY(cudaGetLastError());
+  }
+  return QL_OK;
+}
+
+// Shapes and types of x [M,K], the two weights [I,K] and a matrix [M,I].
+int check_gated(const char *op, const ql_tensor *x, const ql_tensor *wg, const ql_tensor *wu, const ql_tensor *h, const char *h_name, int act) {
+  const ql_tensor *t[4] = {x, wg, wu, h};
+  const char *name[4] = {"x", "w_gate", "w_up", h_name};
+  for (int i = 0; i < 4; i++) {
+    if (!t[i]) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: %s is null", op, name[i]);
+    if (t[i]->rank != 2 || t[i]->shape[0] < 0 || t[i]->shape[1] < 0) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: %s must be a 2-D tensor", op, name[i]);
+    if (t[i]->dtype != QL_F16 && t[i]->dtype != QL_BF16) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: %s must be f16 or bf16", op, name[i]);
+    if (t[i]->dtype != x->dtype) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: %s and x must be of one type", op, name[i]);
+    if (t[i]->shape[0] > (1 << 30) || t[i]->shape[1] > (1 << 30)) return set_error(QL_ERR_UNSUPPORTED, "%s: dimension of %s too large", op, name[i]);
+  }
+  if (act < ACT_SILU || act > ACT_RELU) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", op, act);
+  const int64_t M = x->shape[0], K = x->shape[1], I = wg->shape[0];
+  if (wg->shape[1] != K || wu->shape[0] != I || wu->shape[1] != K)
+    return set_error(QL_ERR_INVALID_ARGUMENT, "%s: w_gate and w_up must both be [I,K] with K = %lld", op, (long long)K);
+  if (h->shape[0] != M || h->shape[1] != I) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: %s must be [M,I] = [%lld,%lld]", op, h_name, (long long)M, (long long)I);
+  for (int i = 0; i < 4; i++) {
+    if (numel(t[i]) > 0 && !t[i]->data) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: %s has no data pointer", op, name[i]);
+    if (!aligned16(t[i]->data)) return set_error(QL_ERR_UNSUPPORTED, "%s: %s must be 16-byte aligned", op, name[i]);
+  }
+  if (K % 8 != 0 || I % 8 != 0) return set_error(QL_ERR_UNSUPPORTED, "%s: needs K (%lld) and I (%lld) to be multiples of 8", op, (long long)K, (long long)I);
+  return QL_OK;
+}
+
+} // namespace
+} // namespace ql
+
+using namespace ql;
+
+extern "C" int ql_gated_linear(const ql_tensor *x, const ql_tensor *w_gate, const ql_tensor *w_up, int32_t activation, ql_tensor *h, void *stream) {
+  const char *op = "gated_linear";
+  const int rc = check_gated(op, x, w_gate, w_up, h, "h", activation);
+  if (rc != QL_OK) return rc;
+  const int M = (int)x->shape[0], K = (int)x->shape[1], I = (int)w_gate->shape[0];
+  cudaStream_t st = (cudaStream_t)stream;
+  if (M == 0 || I == 0) return QL_OK;
+  if (K == 0) { // act(0) * 0
+    QL_CUDA_TRY(cudaMemsetAsync(h->data, 0, (size_t)numel(h) * 2, st));
+    return QL_OK;
+  }
+  return x->dtype == QL_BF16 ? forward<__nv_bfloat16>(x->data, w_gate->data, w_up->data, h->data, M, I, K, activation, st)
+                             : forward<__half>(x->data, w_gate->data, w_up->data, h->data, M, I, K, activation, st);
+}
+
+extern "C" int ql_gated_linear_backward_workspace(const ql_tensor *x, const ql_tensor *w_gate, int32_t want_dx, int32_t want_dw, int64_t *bytes) {
+  const char *op = "gated_linear_backward_workspace";
+  if (!x || !w_gate || !bytes || x->rank != 2 || w_gate->rank != 2) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: needs x [M,K], w_gate [I,K] and a place for the size", op);
+  const int64_t M = x->shape[0], K = x->shape[1], I = w_gate->shape[0];
+  if (M < 0 || K < 0 || I < 0 || M > (1 << 30) || K > (1 << 30) || I > (1 << 30)) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: bad shape", op);
+  *bytes = 0;
+  if (M == 0 || K == 0 || I == 0) return QL_OK;
+  const GradPlan p = plan_grads((int)M, (int)I, (int)K, want_dx != 0, want_dw != 0, pairs_of(x->dtype));
+  *bytes = 2 * align256(M * I * 2) + align256(p.x_part_floats * 4) + align256(p.w_part_floats * 4);
+  return QL_OK;
+}
+
+extern "C" int ql_gated_linear_backward(const ql_tensor *grad, const ql_tensor *x, const ql_tensor *w_gate, const ql_tensor *w_up, int32_t activation, ql_tensor *dx,
+                                        ql_tensor *dw_gate, ql_tensor *dw_up, void *workspace, int64_t workspace_bytes, void *stream) {
+  const char *op = "gated_linear_backward";
+  int rc = check_gated(op, x, w_gate, w_up, grad, "grad", activation);
+  if (rc != QL_OK) return rc;
+  if ((dw_gate == nullptr) != (dw_up == nullptr)) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: dw_gate and dw_up go together", op);
+  const ql_tensor *out[3] = {dx, dw_gate, dw_up}, *like[3] = {x, w_gate, w_up};
+  const char *name[3] = {"dx", "dw_gate", "dw_up"};
+  for (int i = 0; i < 3; i++) {
+    if (!out[i]) continue;
+    if (out[i]->dtype != x->dtype || out[i]->rank != 2 || out[i]->shape[0] != like[i]->shape[0] || out[i]->shape[1] != like[i]->shape[1])
+      return set_error(QL_ERR_INVALID_ARGUMENT, "%s: %s must have the type and shape of what it is the gradient of", op, name[i]);
+    if (numel(out[i]) > 0 && !out[i]->data) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: %s has no data pointer", op, name[i]);
+    if (!aligned16(out[i]->data)) return set_error(QL_ERR_UNSUPPORTED, "%s: %s must be 16-byte aligned", op, name[i]);
+  }
+  const int M = (int)x->shape[0], K = (int)x->shape[1], I = (int)w_gate->shape[0];
+  cudaStream_t st = (cudaStream_t)stream;
+  if (M == 0 || I == 0 || K == 0) { // sums over nothing
+    for (int i = 0; i < 3; i++)
+      if (out[i] && numel(out[i]) > 0) QL_CUDA_TRY(cudaMemsetAsync(out[i]->data, 0, (size_t)numel(out[i]) * 2, st));
+    return QL_OK;
+  }
+  if (!dx && !dw_gate) return QL_OK;
+  int64_t need = 0;
+  if ((rc = ql_gated_linear_backward_workspace(x, w_gate, dx != nullptr, dw_gate != nullptr, &need)) != QL_OK) return rc;
+  if (!workspace || workspace_bytes < need) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %lld bytes, got %lld", op, (long long)need, (long long)(workspace ? workspace_bytes : 0));
+  if (reinterpret_cast<uintptr_t>(workspace) & 255) return set_error(QL_ERR_UNSUPPORTED, "%s: the workspace must be 256-byte aligned", op);
+  if (!device_status_word()) return set_error(QL_ERR_CUDA, "%s: could not allocate the device status word", op);
+  const GradPlan plan = plan_grads(M, I, K, dx != nullptr, dw_gate != nullptr, pairs_of(x->dtype));
+  void *p[3] = {dx ? dx->data : nullptr, dw_gate ? dw_gate->data : nullptr, dw_up ? dw_up->data : nullptr};
+  uint8_t *ws = static_cast<uint8_t *>(workspace);
+  return x->dtype == QL_BF16 ? backward<__nv_bfloat16>(grad->data, x->data, w_gate->data, w_up->data, p[0], p[1], p[2], M, I, K, activation, ws, plan, st)
+                             : backward<__half>(grad->data, x->data, w_gate->data, w_up->data, p[0], p[1], p[2], M, I, K, activation, ws, plan, st);
+}

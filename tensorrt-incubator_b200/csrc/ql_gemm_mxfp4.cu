@@ -56,27 +56,6 @@ template <int N> __device__ __forceinline__ uint32_t mx_idesc(uint32_t byte) {
 __device__ __forceinline__ void tmem_store_4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// One lane of a converged warp.  The roles that issue copies and MMAs run as whole warps and elect a lane only around the
-// instruction: their operands are then provably the same in all lanes and stay in uniform registers.  Inside a branch that
-// one lane alone takes, every descriptor word is moved there first: 111 cycles per MMA, against the 57 to 112 it needs.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
-  return p != 0;
-}
-// A warp's wait with one answer for all lanes: what follows is executed by the whole warp or by none of it.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code));
-}
-// A wait that only the clock ends: for what this CTA has in flight itself.
-__device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity) {
-  const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity))
-    if (clock64() - t0 > kWaitLimitCycles) return false;
-  return true;
-}
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // The four MMAs of one k step, issued by one lane of a converged warp.
@@ -182,7 +161,12 @@ template <int TN> struct SplitSmem {
   static constexpr int kAbort = kTmemPtr + 4;
   static constexpr int kRing = (kAbort + 4 + 1023) / 1024 * 1024;
   static constexpr int stage_bytes(int rows) { return ((rows + 7) / 8 * 8 + TN) * BK_BYTES; }
-  static constexpr int total(int rows, int stages) { return kRing + stages * stage_bytes(rows) + MX_A_BYTES + 1024; }
+  // At least a third of an SM's shared memory: two CTAs of 256 columns fill tensor memory, and a third one waiting for columns
+  // while its cluster partners wait for it could wait for good.
+  static constexpr int total(int rows, int stages) {
+    const int n = kRing + stages * stage_bytes(rows) + MX_A_BYTES + 1024;
+    return n < 79872 ? 79872 : n;
+  }
 };
 
 template <int TN, bool WIDE>
@@ -732,16 +716,6 @@ int check_mx_operand(const char *op, const char *name, const ql_tensor *d, const
   return QL_OK;
 }
 
-template <typename K> int allow_smem(K kern, int bytes, bool (&configured)[64]) {
-  int dev = 0;
-  QL_CUDA_TRY(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64 || !configured[dev]) {
-    QL_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    if (dev >= 0 && dev < 64) configured[dev] = true;
-  }
-  return QL_OK;
-}
-
 bool scales_on_multiple(const MxArgs &args, int of) {
   return ((reinterpret_cast<uintptr_t>(args.sfa) | reinterpret_cast<uintptr_t>(args.sfb) | (uintptr_t)args.kb) & (uintptr_t)(of - 1)) == 0;
 }
@@ -801,7 +775,7 @@ template <int TN, bool WIDE> SplitPlan plan_split(int M, int N, int num_ks) {
       const double latency = 0.33 + 0.0029 * (TN - 16), bandwidth = (double)(rows + TN) * BK_BYTES * co / 48e3;
       const double us = (double)waves * (3.3 + 0.5 * (co - 1) + (log2 ? 1.2 + 0.033 * TN : 0.0) + steps * (latency > bandwidth ? latency : bandwidth));
       if (us < best.us) {
-        int stages = (232448 / co - 2048 - L::total(rows, 0)) / L::stage_bytes(rows);
+        int stages = (232448 / co - 2048 - (L::kRing + MX_A_BYTES + 1024)) / L::stage_bytes(rows);
         stages = stages > kSplitMaxStages ? kSplitMaxStages : stages;
         best = {co, log2, rows, stages > steps ? steps : stages, us};
       }

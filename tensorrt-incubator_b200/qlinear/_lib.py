@@ -18,6 +18,7 @@ F32, F16, BF16, I8, I4, F8E4M3, F4E2M1, F8E8M0 = 0, 1, 2, 3, 4, 5, 6, 7
 # ql_status
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_CUDA, ERR_NO_DEVICE, ERR_DEVICE_TIMEOUT = range(6)
 # ql_fp8_mode
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}  # ql_activation
 FP8_MODES = {"direct": 0, "via_f16": 1, "stablehlo": 2}
 
 
@@ -72,6 +73,9 @@ SIGNATURES = {
     "ql_quantize_mxfp4": ([_T, _T, _T, _S], ctypes.c_int),
     "ql_dequantize_mxfp4": ([_T, _T, _T, _S], ctypes.c_int),
     "ql_gemm_mxfp4": ([_T, _T, _T, _T, _T, _S], ctypes.c_int),
+    "ql_gated_linear": ([_T, _T, _T, ctypes.c_int32, _T, _S], ctypes.c_int),
+    "ql_gated_linear_backward_workspace": ([_T, _T, ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(ctypes.c_int64)], ctypes.c_int),
+    "ql_gated_linear_backward": ([_T, _T, _T, _T, ctypes.c_int32, _T, _T, _T, ctypes.c_void_p, ctypes.c_int64, _S], ctypes.c_int),
     "ql_linear_w8a16": ([_T, _T, _T, _T, _S], ctypes.c_int),
     "ql_linear_w4a16": ([_T, _T, _T, _T, _S], ctypes.c_int),
     "ql_linear_weight_only": ([_T, _T, _T, _T, ctypes.c_uint32, _S], ctypes.c_int),

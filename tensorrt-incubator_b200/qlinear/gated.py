@@ -1,0 +1,69 @@
+"""Gated projection of a feed-forward block in 16 bits, and its backward pass: the unquantized counterpart of the fp8 block's
+gate/up projection (mlp.gemm_fp8_swiglu), for the block that a quantized one is made from, compared with or trained as.  The
+reference has no such operator; its pieces are tp.Linear and the activations of its frontend."""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .ops import QuantizeError
+from .tensor import call_on, ql_view, require_cuda
+
+
+def _activation(name: str) -> int:
+    try:
+        return _lib.ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise QuantizeError(f"Unknown activation {name!r}: one of {tuple(_lib.ACTIVATIONS)}.") from None
+
+
+def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
+    require_cuda(t, what)
+    if t.dim() == 0:
+        raise QuantizeError(f"{what} must have at least 1 dimension.")
+    return t.reshape(-1, t.shape[-1]).contiguous() if t.numel() else t.reshape(t.shape[:-1].numel(), t.shape[-1])
+
+
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu", *, out=None) -> torch.Tensor:
+    """act(x @ w_gate^T) * (x @ w_up^T): x [..., K], w_gate and w_up [I, K], all float16 or all bfloat16; both products,
+    `activation` ("silu", "gelu", "gelu_tanh" or "relu") and the gate's product in one kernel, f32 sums, one rounding.  K and
+    I are multiples of 8; any number of rows from none up."""
+    act = _activation(activation)
+    x2 = _rows(x, "x")
+    wg, wu = w_gate.contiguous(), w_up.contiguous()   # kept alive across the call: a view only borrows the pointer
+    h = out if out is not None else torch.empty(x.shape[:-1] + wg.shape[:1], dtype=x.dtype, device=x.device)
+    if out is not None and tuple(out.shape) != tuple(x.shape[:-1] + wg.shape[:1]):
+        raise QuantizeError(f"out must have shape {tuple(x.shape[:-1] + wg.shape[:1])}, got {tuple(out.shape)}.")
+    ql_view(h)   # a result that is not dense is refused here: reshape would copy it
+    call_on(x.device, _lib.lib().ql_gated_linear, ql_view(x2), ql_view(wg), ql_view(wu), act, ql_view(h.reshape(x2.shape[0], wg.shape[0])),
+            same_device=(wg, wu, h))
+    return h
+
+
+def gated_linear_backward(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu", *,
+                          need_input_grad: bool = True, need_weight_grad: bool = True):
+    """(dx, dw_gate, dw_up) of gated_linear from `grad`, the gradient of its result [..., I]; None for what is not needed.
+    Nothing is kept from the forward pass: the projections are computed again, their gradients are formed in f32 and rounded
+    once to the operands' type for the second products.  Gradients have the type of what they belong to."""
+    act = _activation(activation)
+    x2, g2 = _rows(x, "x"), _rows(grad, "grad")
+    if grad.shape[:-1] != x.shape[:-1]:
+        raise QuantizeError(f"grad and x must have the same leading dimensions, got {tuple(grad.shape)} and {tuple(x.shape)}.")
+    wg, wu = w_gate.contiguous(), w_up.contiguous()
+    dx = torch.empty(x2.shape, dtype=x.dtype, device=x.device) if need_input_grad else None
+    dwg = torch.empty(wg.shape, dtype=x.dtype, device=x.device) if need_weight_grad else None
+    dwu = torch.empty(wu.shape, dtype=x.dtype, device=x.device) if need_weight_grad else None
+    v = lambda t: ql_view(t) if t is not None else None
+    size = ctypes.c_int64()
+
+    def run(stream):   # with the tensors' device current: the plan behind the size depends on the device
+        rc = _lib.lib().ql_gated_linear_backward_workspace(ql_view(x2), ql_view(wg), need_input_grad, need_weight_grad, ctypes.byref(size))
+        if rc != _lib.OK:
+            return rc
+        ws = torch.empty(size.value, dtype=torch.uint8, device=x.device)
+        return _lib.lib().ql_gated_linear_backward(ql_view(g2), ql_view(x2), ql_view(wg), ql_view(wu), act, v(dx), v(dwg), v(dwu),
+                                                   ws.data_ptr() or None, size.value, stream)
+    call_on(x.device, run, same_device=(g2, wg, wu))
+    return (dx.reshape(x.shape) if dx is not None else None), dwg, dwu
