@@ -157,9 +157,13 @@ QL_API int ql_dequantize_mxfp4(const ql_tensor *data, const ql_tensor *scales, q
 /* Block-scaled MXFP4 product: Y[M,N] = dq(a)[M,K] . dq(b)[N,K]^T of operands as ql_quantize_mxfp4 writes them, the block
  * scales applied by the tensor core (tcgen05.mma kind::mxf4, f32 accumulation), one rounding to y's type.  a, b: QL_F4E2M1
  * [M,K], [N,K], 16-byte aligned; *_scales: QL_F8E8M0 [rows, K/32], 4-byte aligned; y: f32 | f16 | bf16.  K > 0, K % 32 == 0; M and N any.  A NaN
- * scale makes its row (a) or column (b) of Y NaN.  One launch, no scratch. */
+ * scale makes its row (a) or column (b) of Y NaN.  `workspace`: 16-byte aligned device memory of at least the bytes the query
+ * gives (0 for most calls: it holds a padded copy of scales whose rows are no multiple of 16 bytes or not aligned, of more
+ * than 32 tokens); free again when the call's work on the stream is done. */
+QL_API int ql_gemm_mxfp4_workspace(const ql_tensor *a, const ql_tensor *a_scales, const ql_tensor *b, const ql_tensor *b_scales,
+                                   int64_t *bytes);
 QL_API int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, const ql_tensor *b, const ql_tensor *b_scales,
-                         ql_tensor *y, void *stream);
+                         ql_tensor *y, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* Gated projection of a feed-forward block in 16 bits (the unquantized counterpart of ql_gemm_fp8_swiglu):
  *   h[M,I] = act(x w_gate^T) * (x w_up^T),   x [M,K], w_gate and w_up [I,K] (Linear's [out, in] layout), all f16 or all bf16,

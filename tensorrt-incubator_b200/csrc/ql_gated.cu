@@ -279,11 +279,9 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             const uint64_t adesc = make_smem_desc(a), bdesc = make_smem_desc(a + G_TILE);
 #pragma unroll
             for (int k = 0; k < 4; k++) mma_f16_pair(p.tmem + (uint32_t)(buf * G_N), adesc + 2 * k, bdesc + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
-            tc_commit_pair(map_to_cta(p.empty(stage), 0));
-            tc_commit_pair(map_to_cta(p.empty(stage), 1));
+            tc_commit_both(p.empty(stage));
             if (kb == args.num_kb - 1) {
-              tc_commit_pair(map_to_cta(p.tfull(buf), 0));
-              tc_commit_pair(map_to_cta(p.tfull(buf), 1));
+              tc_commit_both(p.tfull(buf));
             }
           }
           __syncwarp();
@@ -358,7 +356,7 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_to_cta(p.tempty(buf), 0)); // the leader owns the accumulator hand-over
+      if (lane == 0) mbar_arrive_remote(map_to_cta(p.tempty(buf), 0)); // the leader owns the accumulator hand-over
     }
     out.finish(lane);
     if (!ok && lane == 0) signal_partner_abort(smem_u32((const void *)p.abort_flag), p.rank);
@@ -484,11 +482,9 @@ gated_grads_kernel(const __grid_constant__ CUtensorMap map_dg_k, const __grid_co
             const uint64_t astep = u.is_x ? 2 : 128;
 #pragma unroll
             for (int k = 0; k < 4; k++) mma_f16_pair(p.tmem + (uint32_t)(buf * G_N), adesc + astep * k, bdesc + 128 * k, idesc, (s > u.step0 || k) ? 1u : 0u);
-            tc_commit_pair(map_to_cta(p.empty(stage), 0));
-            tc_commit_pair(map_to_cta(p.empty(stage), 1));
+            tc_commit_both(p.empty(stage));
             if (s == u.step1 - 1) {
-              tc_commit_pair(map_to_cta(p.tfull(buf), 0));
-              tc_commit_pair(map_to_cta(p.tfull(buf), 1));
+              tc_commit_both(p.tfull(buf));
             }
           }
           __syncwarp();
@@ -536,7 +532,7 @@ gated_grads_kernel(const __grid_constant__ CUtensorMap map_dg_k, const __grid_co
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_to_cta(p.tempty(buf), 0));
+      if (lane == 0) mbar_arrive_remote(map_to_cta(p.tempty(buf), 0));
     }
     out.finish(lane);
     if (!ok && lane == 0) signal_partner_abort(smem_u32((const void *)p.abort_flag), p.rank);
@@ -768,9 +764,10 @@ template <typename K> int resident_cached(K kern, int threads, int smem, int clu
   return cache[dev];
 }
 
-// A band of rows of A stays L2-resident: about 16 MiB of it, four row tiles of 256 at the least.
+// A band of rows of A stays L2-resident: about 32 MiB of it, four row tiles of 256 at the least.  4096 x 28672 x 8192: bands
+// of 16, 32, 64 and 128 MiB 3.00, 2.78, 2.81 and 2.83 ms; 4096 x 11008 x 4096: 522, 501, 504 and 509 us.
 int band(int64_t row_bytes, int tiles_m) {
-  int64_t g = (16ll << 20) / (256 * row_bytes);
+  int64_t g = (32ll << 20) / (256 * row_bytes);
   g = g < 4 ? 4 : g;
   return (int)(g > tiles_m ? (tiles_m < 1 ? 1 : tiles_m) : g);
 }
@@ -917,7 +914,7 @@ GradPlan plan_grads(int M, int I, int K, bool want_x, bool want_w, int pairs) {
   double hw = (a.w_units - (pairs - a.heavy) * ux / uw) / pairs;
   a.heavy_w = a.heavy == 0 ? 0 : (int)(hw < 0 ? 0 : hw + 0.5);
   if ((int64_t)a.heavy * a.heavy_w > a.w_units) a.heavy_w = a.w_units / a.heavy;
-  a.group_m = 8;
+  a.group_m = 8; // row tiles walked together; 4, 8, 16, 32 on 4096 x 11008 x 4096: 1.62, 1.55, 1.59, 1.54 ms; on 1024 x 28672 x 8192: 2.12, 2.10, 2.10, 2.20
   a.x_parts = a.w_parts = nullptr;
   p.x_part_floats = a.x_split > 1 ? (int64_t)a.x_split * M * K : 0;
   p.w_part_floats = a.w_split > 1 ? 2ll * a.w_split * I * K : 0;

@@ -16,7 +16,10 @@
 //   split   few output tiles (decoding, short prompts): the weights are the 128-row operand and up to 128 tokens the other;
 //           a cluster of up to 8 CTAs shares the K axis of one tile and adds its parts through distributed shared memory,
 //           in rank order (the same bits on every run).
-//   tiles   many output tiles: one persistent CTA per SM on 128 x 224 tiles.
+//   tiles   many output tiles, persistent: one CTA per SM on 128 x 208 tiles, or CTA pairs on 256 x 208 tiles.  In a pair
+//           (tcgen05.mma.cta_group::2, issued by its leader) each CTA holds its own 128 rows of A and half of the B tile, so
+//           per MMA it reads 232 rows of operands from shared memory instead of 336; the scales of all 208 columns are needed
+//           by both.
 // Every wait is bounded, as in the other tensor-core kernels.
 #include <cuda.h>
 #include <string.h>
@@ -29,6 +32,7 @@ namespace {
 
 constexpr int kKStep = 256;           // values of K per pipeline stage: 128 bytes of e2m1
 constexpr int kScaleBytes = 8;        // scales of one row and k step
+constexpr int kSplitOnly = 32;        // up to so many tokens the split kernel is always the one
 constexpr int MX_A_BYTES = BM * BK_BYTES;
 
 struct MxArgs {
@@ -42,29 +46,46 @@ struct MxArgs {
   int *status;
 };
 
+template <bool PAIR>
 __device__ __forceinline__ void mx_mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
-               ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
-               : "memory");
+  if constexpr (PAIR)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+                 ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+                 : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+                 ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb)
+                 : "memory");
 }
 // e2m1 operands (format 1), both K-major, e8m0 scales (bit 23), N >> 3 at bit 17, M >> 4 at bit 24, dense K = 64; the byte
 // offset (0 or 2) of the scales within their cells at bits 29 (A) and 4 (B)
-template <int N> __device__ __forceinline__ uint32_t mx_idesc(uint32_t byte) {
-  return 1u << 7 | 1u << 10 | (uint32_t)(N >> 3) << 17 | 1u << 23 | (uint32_t)(BM >> 4) << 24 | byte << 29 | byte << 4;
+template <int M, int N> __device__ __forceinline__ uint32_t mx_idesc(uint32_t byte) {
+  return 1u << 7 | 1u << 10 | (uint32_t)(N >> 3) << 17 | 1u << 23 | (uint32_t)(M >> 4) << 24 | byte << 29 | byte << 4;
 }
 __device__ __forceinline__ void tmem_store_4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ void tmem_store_16(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f, uint32_t g, uint32_t h, uint32_t i, uint32_t j,
+                                              uint32_t k, uint32_t l, uint32_t m, uint32_t n, uint32_t o, uint32_t p) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+               ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d), "r"(e), "r"(f), "r"(g), "r"(h), "r"(i), "r"(j), "r"(k), "r"(l), "r"(m), "r"(n), "r"(o), "r"(p)
+               : "memory");
+}
+// A look at a barrier, without waiting
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// The four MMAs of one k step, issued by one lane of a converged warp.
-template <int N>
-__device__ __forceinline__ void mx_k_step(uint32_t tmem_d, uint32_t a_addr, uint32_t b_addr, uint32_t t_sfa, uint32_t t_sfb, int sfb_cols, bool first) {
-  const uint64_t adesc = make_smem_desc(a_addr), bdesc = make_smem_desc(b_addr);
-#pragma unroll
-  for (int j = 0; j < 4; j++) // 64 values = 32 bytes of K each; two MMAs share one set of scale cells
-    mx_mma(tmem_d, adesc + 2 * j, bdesc + 2 * j, mx_idesc<N>((j & 1) * 2), t_sfa + 4 * (j >> 1), t_sfb + sfb_cols * (j >> 1), (first && j == 0) ? 0u : 1u);
+// MMA j (0..3) of a k step, issued by one lane of a converged warp: 64 values = 32 bytes of K; two MMAs share one set of
+// scale cells.
+template <int N, bool PAIR>
+__device__ __forceinline__ void mx_k_mma(int j, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t t_sfa, uint32_t t_sfb, int sfb_cols, uint32_t accumulate) {
+  mx_mma<PAIR>(tmem_d, adesc + 2 * j, bdesc + 2 * j, mx_idesc<PAIR ? 2 * BM : BM, N>((j & 1) * 2), t_sfa + 4 * (j >> 1), t_sfb + sfb_cols * (j >> 1), accumulate);
 }
 
 template <typename OutT> __device__ __forceinline__ void store_y(void *Y, size_t i, float v) { static_cast<OutT *>(Y)[i] = FloatIO<OutT>::from_f32(v); }
@@ -76,7 +97,7 @@ __device__ __forceinline__ void store_y(void *Y, int dtype, size_t i, float v) {
 
 __device__ __forceinline__ uint32_t ldg32_if(const void *p, bool on) {
   uint32_t v;
-  asm("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.nc.b32 %0, [%1];\n\t}" : "=r"(v) : "l"(p), "r"((int)on));
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.nc.b32 %0, [%1];\n\t}" : "=r"(v) : "l"(p), "r"((int)on));
   return v;
 }
 // up to four neighbouring values of y
@@ -94,7 +115,7 @@ __device__ __forceinline__ void store_y4(const MxArgs &args, size_t i, const flo
 
 __device__ __forceinline__ uint32_t ldg8_if(const void *p, bool on) {
   uint32_t v;
-  asm("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.nc.u8 %0, [%1];\n\t}" : "=r"(v) : "l"(p), "r"((int)on));
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.nc.u8 %0, [%1];\n\t}" : "=r"(v) : "l"(p), "r"((int)on));
   return v;
 }
 // The scale bytes of four k steps of one row: the first `n` of 32 bytes from p on, zeros beyond.  Loading and shifting are
@@ -111,7 +132,7 @@ template <bool WIDE> struct RowScales {
     if constexpr (WIDE) {
 #pragma unroll
       for (int i = 0; i < 8; i += 2)
-        asm("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %3, %4;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t@p ld.global.nc.v2.b32 {%0, %1}, [%2];\n\t}"
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.s32 p, %3, %4;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t@p ld.global.nc.v2.b32 {%0, %1}, [%2];\n\t}"
             : "=r"(r[i]), "=r"(r[i + 1])
             : "l"(p + 4 * i), "r"(4 * i), "r"(n));
     } else {
@@ -255,7 +276,9 @@ gemm_mxfp4_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
       tc_fence_after();
       if (elect_one()) {
         const uint32_t a_addr = smem_base + L::kRing + stage * stage_bytes, t_sf = tmem_base + kSfCol0 + slot * kSlotCols + 16 * q;
-        mx_k_step<TN>(tmem_base, a_addr, a_addr + b_off, t_sf, t_sf + 8, 4, it == 0);
+        const uint64_t adesc = make_smem_desc(a_addr), bdesc = make_smem_desc(a_addr + b_off);
+#pragma unroll
+        for (int j = 0; j < 4; j++) mx_k_mma<TN, false>(j, tmem_base, adesc, bdesc, t_sf, t_sf + 8, 4, (it | j) != 0 ? 1u : 0u);
         tc_commit(empty_bar(stage));
         if (q == kFetchSteps - 1) tc_commit(sempty_bar(slot));
       }
@@ -382,65 +405,67 @@ gemm_mxfp4_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// tiles kernel: persistent, 128 x 224
+// tiles kernel: persistent, 128 x 208, or 256 x 208 by CTA pairs
 // ------------------------------------------------------------------------------------------------------------------
-constexpr int TBN = 224;            // widest tile whose two accumulators leave room for two slots of scales
+// The width leaves tensor memory, beside two accumulators, 96 columns: two slots of the scales of two k steps.  With 224 there
+// is room for two slots of one step, and refilling one (the commit, the hand-over, the store) takes longer than a step.
+constexpr int TBN = 208;
 constexpr int kTileThreads = 320;   // producer, MMA, four epilogue warps, four scale warps
-constexpr int TSTAGES = 4;
-constexpr int T_STAGE_BYTES = MX_A_BYTES + TBN * BK_BYTES;
 constexpr int kScSteps = 4;         // k steps whose scales travel together: 32 bytes, a whole sector, of every row
+constexpr int kSlotSteps = 2;       // k steps of one stage and of one slot: 16 columns of A's scales, then 32 of B's (8 per pair of MMAs, 6.5 used)
+constexpr int kSlotCols = 48;
 constexpr int T_SC_ROWS = BM + TBN;
-constexpr int T_SC_ODD = T_SC_ROWS / 2 * 32;               // SC_PAIRS: 32 bytes of the even rows, then 48 of the odd ones
-constexpr int T_SC_BYTES = T_SC_ODD + T_SC_ROWS / 2 * 48;
-struct TileSmem {
-  static constexpr int kScales = TSTAGES * T_STAGE_BYTES;
+constexpr int T_SC_LANES = (T_SC_ROWS + 31) / 32; // rows a lane carries (of the last, half the lanes' are past the tile)
+constexpr int T_SC_BYTES = T_SC_LANES * 32 * 32;  // with room for those
+template <bool PAIR> struct TileSmem {
+  static constexpr int kStages = PAIR ? 3 : 2; // of two k steps: half as many barriers to look at and to signal as with one
+  static constexpr int kRowsB = PAIR ? TBN / 2 : TBN;                     // rows of the B tile one CTA holds
+  static constexpr int kTileB = kRowsB * BK_BYTES;
+  static constexpr int kStageBytes = kSlotSteps * (MX_A_BYTES + kTileB);  // A's tiles, then B's
+  static constexpr int kScales = kStages * kStageBytes;
   static constexpr int kStaging = kScales + 2 * T_SC_BYTES;   // the epilogue's: 32 rows x 33 words a warp
   static constexpr int kBarriers = kStaging + 4 * 32 * 33 * 4; // full[S], empty[S], tfull[2], tempty[2], scfull[2], scempty[2], sfull[2], sempty[2], drain
-  static constexpr int kTmemPtr = kBarriers + (2 * TSTAGES + 13) * 8;
+  static constexpr int kTmemPtr = kBarriers + (2 * kStages + 13) * 8;
   static constexpr int kAbort = kTmemPtr + 4;
   static constexpr int kDynamic = kAbort + 4 + 1024;
+  static_assert(kDynamic <= 232448 && kStageBytes % 1024 == 0 && T_SC_BYTES % 128 == 0, "tile shape");
 };
-static_assert(TileSmem::kDynamic <= 232448 && T_STAGE_BYTES % 1024 == 0 && T_SC_BYTES % 128 == 0, "tile shape");
 
-// 32 columns of one accumulator row a lane, rounded to y's type and stored in whole 16-byte pieces
+// 32 columns (or the first 16) of one accumulator row a lane, rounded to y's type and stored in whole 16-byte pieces
 template <typename OutT>
-__device__ __forceinline__ void mx_store_chunk(OutT *y, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void mx_store_chunk(OutT *y, const uint32_t (&r)[32], bool whole) {
   if constexpr (sizeof(OutT) == 4) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]));
+    for (int j = 0; j < 32; j += 4)
+      if (j < 16 || whole) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]));
   } else {
     auto two = [&](int j) { return pack2<OutT>(__uint_as_float(r[j]), __uint_as_float(r[j + 1])); };
 #pragma unroll
-    for (int j = 0; j < 32; j += 8) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
+    for (int j = 0; j < 32; j += 8)
+      if (j < 16 || whole) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
   }
 }
 // The same 32 x 32 values where rows are not aligned or the chunk is cut: turned in shared memory, so that a warp's store is
 // one row's run of columns.  (A lane storing its own row value by value took 40 us on 333 x 1001 x 2080.)
-__device__ __forceinline__ void mx_store_rows(const MxArgs &args, float *stage, const uint32_t (&r)[32], int m0, int n0, int lane) {
+__device__ __forceinline__ void mx_store_rows(const MxArgs &args, float *stage, const uint32_t (&r)[32], int m0, int n0, int end, int lane) {
 #pragma unroll
   for (int j = 0; j < 32; j++) stage[lane * 33 + j] = __uint_as_float(r[j]);
   __syncwarp();
   const int n = n0 + lane;
 #pragma unroll 8
   for (int i = 0; i < 32; i++)
-    if (m0 + i < args.M && n < args.N) store_y(args.Y, args.y_dtype, (size_t)(m0 + i) * args.N + n, stage[i * 33 + lane]);
+    if (m0 + i < args.M && n < end) store_y(args.Y, args.y_dtype, (size_t)(m0 + i) * args.N + n, stage[i * 33 + lane]);
   __syncwarp();
 }
 
-// How the scales reach shared memory, 32 bytes (four k steps) of each of a tile's 352 rows at a time.  The copy engine wants
-// rows a multiple of 16 bytes apart.  SC_ROWS: they are.  SC_PAIRS: they are an odd multiple of 8 bytes long (K = 11008, say),
-// so the even rows form one matrix and the odd rows, seen from 8 bytes before the first, another.  SC_WORDS: any other length;
-// the scale warps load them, three rows a thread, one group ahead.  2000 x 4096: K = 11264 65.6 us, 11008 (pairs) 62.4 us,
-// 11040 (words) 111 us; the warps loading 8 bytes at a time took 88 us at K = 11008.
-enum { SC_ROWS, SC_PAIRS, SC_WORDS };
-template <int SC>
+template <bool PAIR>
 __global__ void __launch_bounds__(kTileThreads, 1)
 gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sa,
-                        const __grid_constant__ CUtensorMap map_sb, const __grid_constant__ CUtensorMap map_sa_odd, const __grid_constant__ CUtensorMap map_sb_odd,
-                        const MxArgs args) {
-  using L = TileSmem;
-  constexpr bool COPY = SC != SC_WORDS;
-  constexpr uint32_t kTmemCols = 512; // 2 x 224 accumulator columns, then two slots of 32: 8 columns of A's scales, 16 of B's
+                        const __grid_constant__ CUtensorMap map_sb, const MxArgs args) {
+  using L = TileSmem<PAIR>;
+  constexpr int TSTAGES = L::kStages;
+  constexpr uint32_t kTmemCols = 512; // two accumulators, two slots of scales
+  static_assert(2 * TBN + 2 * kSlotCols <= 512, "tensor memory");
   constexpr uint32_t kSfCol0 = 2 * TBN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -458,7 +483,23 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::kAbort);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int num_tiles = args.tiles_a * args.tiles_b;
+  const int num_tiles = args.tiles_a * args.tiles_b; // tiles_a counts 256 rows for a pair
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0;
+  const int first_tile = PAIR ? blockIdx.x >> 1 : blockIdx.x, tile_stride = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int row_tile = PAIR ? 2 : 1; // this CTA's rows are the 128-row tile row_tile * mt + rank
+  auto arrive_leader = [&](uint32_t bar) { // the pair's leader owns what the MMAs wait for
+    if (PAIR) mbar_arrive_remote(map_to_cta(bar, 0));
+    else mbar_arrive(bar);
+  };
+  auto commit_all = [&](uint32_t bar) { // to the same barrier of both CTAs
+    if (PAIR)
+      tc_commit_both(bar);
+    else
+      tc_commit(bar);
+  };
+  auto tell_partner = [&]() {
+    if (PAIR && lane == 0) signal_partner_abort(smem_u32((const void *)abort_flag), rank);
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < TSTAGES; s++) {
@@ -467,10 +508,10 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(tfull_bar(b), 1);
-      mbar_init(tempty_bar(b), 4);
+      mbar_init(tempty_bar(b), PAIR ? 8 : 4);
       mbar_init(scfull_bar(b), 1);
       mbar_init(scempty_bar(b), 4);
-      mbar_init(sfull_bar(b), 4);
+      mbar_init(sfull_bar(b), PAIR ? 8 : 4);
       mbar_init(sempty_bar(b), 1);
     }
     mbar_init(drain_bar, 1);
@@ -478,11 +519,17 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)tmem_ptr_smem)), "r"(kTmemCols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)tmem_ptr_smem)), "r"(kTmemCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32((const void *)tmem_ptr_smem)), "r"(kTmemCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync_all(); // the partner's barriers exist before anything is signalled across the pair
   tc_fence_after();
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr_smem, 0);
 
@@ -492,24 +539,16 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
     uint32_t phase = 0, sc_phase = 0;
     long long issued = 0, sc_issued = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+    for (int tile = first_tile; tile < num_tiles && ok; tile += tile_stride) {
       const int mt = tile % args.tiles_a, nt = tile / args.tiles_a; // row tiles of one column tile run side by side: B stays in L2
-      for (int ks = 0; ks < args.num_ks; ks++) {
-        if (COPY && ks % kScSteps == 0) {
+      for (int ks = 0; ks < args.num_ks; ks += kSlotSteps) { // a second step beyond K is loaded as zeros
+        if (ks % kScSteps == 0) {
           if (!warp_wait(scempty_bar(sc), sc_phase ^ 1, abort_flag, args.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
           if (elect_one()) {
             const uint32_t dst = smem_base + L::kScales + sc * T_SC_BYTES;
-            if (SC == SC_ROWS) {
-              mbar_expect_tx(scfull_bar(sc), T_SC_ROWS * 32);
-              tma_load_2d(dst, &map_sa, scfull_bar(sc), ks * kScaleBytes, mt * BM);
-              tma_load_2d(dst + BM * 32, &map_sb, scfull_bar(sc), ks * kScaleBytes, nt * TBN);
-            } else {
-              mbar_expect_tx(scfull_bar(sc), T_SC_BYTES);
-              tma_load_2d(dst, &map_sa, scfull_bar(sc), ks * kScaleBytes, mt * (BM / 2));
-              tma_load_2d(dst + BM / 2 * 32, &map_sb, scfull_bar(sc), ks * kScaleBytes, nt * (TBN / 2));
-              tma_load_2d(dst + T_SC_ODD, &map_sa_odd, scfull_bar(sc), ks * kScaleBytes, mt * (BM / 2)); // from 8 bytes before
-              tma_load_2d(dst + T_SC_ODD + BM / 2 * 48, &map_sb_odd, scfull_bar(sc), ks * kScaleBytes, nt * (TBN / 2));
-            }
+            mbar_expect_tx(scfull_bar(sc), T_SC_ROWS * 32);
+            tma_load_2d(dst, &map_sa, scfull_bar(sc), ks * kScaleBytes, (row_tile * mt + rank) * BM);
+            tma_load_2d(dst + BM * 32, &map_sb, scfull_bar(sc), ks * kScaleBytes, nt * TBN);
           }
           __syncwarp();
           sc_issued++;
@@ -517,10 +556,20 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
         }
         if (!warp_wait(empty_bar(stage), phase ^ 1, abort_flag, args.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
         if (elect_one()) {
-          const uint32_t a_dst = smem_base + stage * T_STAGE_BYTES;
-          mbar_expect_tx(full_bar(stage), T_STAGE_BYTES);
-          tma_load_2d(a_dst, &map_a, full_bar(stage), ks * BK_BYTES, mt * BM); // coordinates in bytes of packed e2m1
-          tma_load_2d(a_dst + MX_A_BYTES, &map_b, full_bar(stage), ks * BK_BYTES, nt * TBN);
+          const uint32_t a_dst = smem_base + stage * L::kStageBytes, b_dst = a_dst + kSlotSteps * MX_A_BYTES;
+          const uint32_t bar = PAIR ? map_to_cta(full_bar(stage), 0) : full_bar(stage); // a pair's bytes all land on the leader's barrier
+          if (rank == 0) mbar_expect_tx(full_bar(stage), (PAIR ? 2 : 1) * L::kStageBytes);
+#pragma unroll
+          for (int q = 0; q < kSlotSteps; q++) { // coordinates in bytes of packed e2m1
+            const int x = (ks + q) * BK_BYTES;
+            if (PAIR) {
+              tma_load_2d_pair(a_dst + q * MX_A_BYTES, &map_a, bar, x, (2 * mt + rank) * BM);
+              tma_load_2d_pair(b_dst + q * L::kTileB, &map_b, bar, x, nt * TBN + rank * L::kRowsB);
+            } else {
+              tma_load_2d(a_dst + q * MX_A_BYTES, &map_a, bar, x, mt * BM);
+              tma_load_2d(b_dst + q * L::kTileB, &map_b, bar, x, nt * TBN);
+            }
+          }
         }
         __syncwarp();
         issued++;
@@ -528,8 +577,9 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
       }
     }
     if (!ok) { // let the loads in flight land before the shared memory goes away
+      tell_partner();
       const long long pending = issued < TSTAGES ? issued : TSTAGES, sc_pending = sc_issued < 2 ? sc_issued : 2;
-      for (long long i = 0; i < pending; i++) {
+      for (long long i = 0; i < pending && rank == 0; i++) { // a pair's loads complete on its leader's barriers
         stage = (stage == 0) ? TSTAGES - 1 : stage - 1;
         if (stage == TSTAGES - 1) phase ^= 1;
         bounded_wait(full_bar(stage), phase);
@@ -541,120 +591,107 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issue
-    int stage = 0, it = 0;
-    uint32_t phase = 0, step = 0;
-    bool ok = true;
-    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, it++) {
-      const int buf = it & 1;
-      if (!warp_wait(tempty_bar(buf), ((it >> 1) & 1) ^ 1, abort_flag, args.status, ST_TIMEOUT_TMEM_EMPTY)) { ok = false; break; }
-      for (int ks = 0; ks < args.num_ks; ks++, step++) {
-        const int slot = (int)(step & 1);
-        if (!warp_wait(sfull_bar(slot), (step >> 1) & 1, abort_flag, args.status, ST_TIMEOUT_FULL)) { ok = false; break; }
-        if (!warp_wait(full_bar(stage), phase, abort_flag, args.status, ST_TIMEOUT_FULL)) { ok = false; break; }
-        tc_fence_after();
-        if (elect_one()) {
-          const uint32_t a_addr = smem_base + stage * T_STAGE_BYTES, t_sf = tmem_base + kSfCol0 + 32 * slot;
-          mx_k_step<TBN>(tmem_base + (uint32_t)(buf * TBN), a_addr, a_addr + MX_A_BYTES, t_sf, t_sf + 8, 8, ks == 0);
-          tc_commit(empty_bar(stage));
-          tc_commit(sempty_bar(slot));
-          if (ks == args.num_ks - 1) tc_commit(tfull_bar(buf));
+    // ------------------------------------------------------------------ MMA issue (a pair's leader)
+    // The tensor core takes the next MMA when it starts the one before, so whatever this warp does between two MMAs has one
+    // MMA's time (104 cycles) to hide in.  A look at a barrier takes about 80: the ones for the next stage and slot go between
+    // the MMAs of this one, and only what was not ready then is waited for.  (Both waits ahead of the MMAs left the tensor
+    // core idle for half of every k step.)
+    if (rank == 0) {
+      const bool leader = elect_one();
+      int stage = 0, it = 0;
+      uint32_t phase = 0, half = 0; // half: slots used so far
+      bool ok = true, data_ready = false, scales_ready = false;
+      for (int tile = first_tile; tile < num_tiles && ok; tile += tile_stride, it++) {
+        const int buf = it & 1;
+        if (!warp_wait(tempty_bar(buf), ((it >> 1) & 1) ^ 1, abort_flag, args.status, ST_TIMEOUT_TMEM_EMPTY)) { ok = false; break; }
+        const uint32_t tmem_d = tmem_base + (uint32_t)(buf * TBN);
+        for (int ks = 0; ks < args.num_ks; ks += kSlotSteps) {
+          const int slot = (int)(half & 1);
+          if (!scales_ready && !warp_wait(sfull_bar(slot), (half >> 1) & 1, abort_flag, args.status, ST_TIMEOUT_FULL)) { ok = false; break; }
+          if (!data_ready && !warp_wait(full_bar(stage), phase, abort_flag, args.status, ST_TIMEOUT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a_addr = smem_base + stage * L::kStageBytes, t_sfa = tmem_base + kSfCol0 + kSlotCols * slot, t_sfb = t_sfa + 16;
+          const uint64_t adesc = make_smem_desc(a_addr), bdesc = make_smem_desc(a_addr + kSlotSteps * MX_A_BYTES);
+          const int cur = stage;
+          if (++stage == TSTAGES) { stage = 0; phase ^= 1; }
+          half++;
+          if (leader) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) mx_k_mma<TBN, PAIR>(j, tmem_d, adesc, bdesc, t_sfa, t_sfb, 8, (ks | j) != 0 ? 1u : 0u);
+            mx_k_mma<TBN, PAIR>(0, tmem_d, adesc + (MX_A_BYTES >> 4), bdesc + (L::kTileB >> 4), t_sfa + 8, t_sfb + 16, 8, 1u);
+          }
+          __syncwarp();
+          data_ready = __all_sync(0xffffffffu, mbar_test_wait(full_bar(stage), phase));
+          if (leader) {
+            mx_k_mma<TBN, PAIR>(1, tmem_d, adesc + (MX_A_BYTES >> 4), bdesc + (L::kTileB >> 4), t_sfa + 8, t_sfb + 16, 8, 1u);
+            mx_k_mma<TBN, PAIR>(2, tmem_d, adesc + (MX_A_BYTES >> 4), bdesc + (L::kTileB >> 4), t_sfa + 8, t_sfb + 16, 8, 1u);
+          }
+          __syncwarp();
+          scales_ready = __all_sync(0xffffffffu, mbar_test_wait(sfull_bar((int)(half & 1)), (half >> 1) & 1));
+          if (leader) {
+            mx_k_mma<TBN, PAIR>(3, tmem_d, adesc + (MX_A_BYTES >> 4), bdesc + (L::kTileB >> 4), t_sfa + 8, t_sfb + 16, 8, 1u);
+            commit_all(sempty_bar(slot));
+            commit_all(empty_bar(cur));
+            if (ks + kSlotSteps >= args.num_ks) commit_all(tfull_bar(buf));
+          }
+          __syncwarp();
         }
-        __syncwarp();
-        if (++stage == TSTAGES) { stage = 0; phase ^= 1; }
       }
+      if (!ok) tell_partner();
+      if (elect_one()) { // every MMA issued above has to finish before tensor memory is released
+        if (PAIR) tc_commit_pair(map_to_cta(drain_bar, 0));
+        else tc_commit(drain_bar);
+      }
+      __syncwarp();
+      if (!bounded_wait(drain_bar, 0) && lane == 0) atomicCAS(args.status, 0, ST_TIMEOUT_DRAIN);
     }
-    if (elect_one()) tc_commit(drain_bar); // every MMA issued above has to finish before tensor memory is released
-    __syncwarp();
-    if (!bounded_wait(drain_bar, 0) && lane == 0) atomicCAS(args.status, 0, ST_TIMEOUT_DRAIN);
   } else if (warp >= 6) {
     // ------------------------------------------------------------------ scales (warps 6..9, one per quarter of the lanes)
     const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
-    uint32_t step = 0;
+    uint32_t half = 0; // slots filled so far
     bool ok = true;
-    const int tid = (warp & 3) * 32 + lane;
-    // groups of four k steps, tile after tile; a cursor for what is fetched ahead
-    const int groups = (args.num_ks + kScSteps - 1) / kScSteps;
-    int f_tile = blockIdx.x, f_group = 0;
-    RowScales<false> own[3]; // !COPY: the next group; rows tid, tid + 128, tid + 256 of the tile's 352
-    auto fetch = [&]() {
-      const int mt = f_tile % args.tiles_a, nt = f_tile / args.tiles_a, b0 = f_group * kScSteps * kScaleBytes, n = args.kb - b0;
-#pragma unroll
-      for (int i = 0; i < 3; i++) {
-        const int r = tid + 128 * i; // 0..127: A's rows; then B's
-        const long long row = i == 0 ? (long long)mt * BM + r : (long long)nt * TBN + (r - BM);
-        const bool has = f_tile < num_tiles && r < T_SC_ROWS && row < (i == 0 ? args.M : args.N);
-        const long long at = has ? row * args.kb + b0 : 0;
-        own[i].load((i == 0 ? args.sfa : args.sfb) + at, has ? n : 0, (long long)(i == 0 ? args.M : args.N) * args.kb - at);
-      }
-      if (++f_group == groups) f_group = 0, f_tile += gridDim.x;
-    };
+    const int groups = (args.num_ks + kScSteps - 1) / kScSteps; // of four k steps, in a tile
     auto hand_over = [&](int ks, int sc, uint32_t sc_phase) {
-      if (COPY) {
-        ok = warp_wait(scfull_bar(sc), sc_phase, abort_flag, args.status, ST_TIMEOUT_FULL);
-        if (!ok) return;
-      } else {
-        // a buffer is rewritten two groups later: the barrier between, which every warp passes after reading the group
-        // before it, keeps the two apart
-#pragma unroll
-        for (int i = 0; i < 3; i++) {
-          if (tid + 128 * i < T_SC_ROWS) {
-            uint4 *dst = reinterpret_cast<uint4 *>(smem + L::kScales + sc * T_SC_BYTES + (tid + 128 * i) * 32);
-            dst[0] = make_uint4(own[i].word(0), own[i].word(1), own[i].word(2), own[i].word(3));
-            dst[1] = make_uint4(own[i].word(4), own[i].word(5), own[i].word(6), own[i].word(7));
-          }
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        fetch();
-      }
-      uint32_t w[T_SC_ROWS / 32][8]; // rows lane, lane + 32, ... : the words of four k steps
+      ok = warp_wait(scfull_bar(sc), sc_phase, abort_flag, args.status, ST_TIMEOUT_FULL);
+      if (!ok) return;
       const uint8_t *buf = smem + L::kScales + sc * T_SC_BYTES;
-      if (SC == SC_PAIRS) {
-        const uint8_t *src = lane & 1 ? buf + T_SC_ODD + (lane >> 1) * 48 + 8 : buf + (lane >> 1) * 32;
-        const int step16 = lane & 1 ? 16 * 48 : 16 * 32; // to the row 32 further on
+#pragma unroll 1
+      for (int h = 0; h < kScSteps / kSlotSteps; h++) {
+        const bool more = ok && ks + h * kSlotSteps < args.num_ks;
+        uint32_t w[T_SC_LANES][4]; // rows lane, lane + 32, ... : the words of two k steps
+        if (more) {
 #pragma unroll
-        for (int c = 0; c < T_SC_ROWS / 32; c++) {
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const uint2 v = *reinterpret_cast<const uint2 *>(src + c * step16 + 8 * j);
-            w[c][2 * j] = v.x, w[c][2 * j + 1] = v.y;
+          for (int c = 0; c < T_SC_LANES; c++) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(buf + (c * 32 + lane) * 32 + 16 * h);
+            w[c][0] = v.x, w[c][1] = v.y, w[c][2] = v.z, w[c][3] = v.w;
           }
         }
-      } else {
-#pragma unroll
-        for (int c = 0; c < T_SC_ROWS / 32; c++) {
-          const uint8_t *src = buf + (c * 32 + lane) * 32;
-          const uint4 lo = *reinterpret_cast<const uint4 *>(src), hi = *reinterpret_cast<const uint4 *>(src + 16);
-          w[c][0] = lo.x, w[c][1] = lo.y, w[c][2] = lo.z, w[c][3] = lo.w;
-          w[c][4] = hi.x, w[c][5] = hi.y, w[c][6] = hi.z, w[c][7] = hi.w;
+        if (h == kScSteps / kSlotSteps - 1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(scempty_bar(sc));
         }
-      }
-      __syncwarp();
-      if (COPY && lane == 0) mbar_arrive(scempty_bar(sc));
-#pragma unroll
-      for (int q = 0; q < kScSteps; q++) {
-        if (ok && ks + q < args.num_ks) {
-          const int slot = (int)(step & 1);
-          ok = warp_wait(sempty_bar(slot), ((step >> 1) & 1) ^ 1u, abort_flag, args.status, ST_TIMEOUT_EMPTY);
+        if (more) {
+          const int slot = (int)(half & 1);
+          ok = warp_wait(sempty_bar(slot), ((half >> 1) & 1) ^ 1u, abort_flag, args.status, ST_TIMEOUT_EMPTY);
           if (ok) {
-            const uint32_t t = tmem_base + quarter + kSfCol0 + 32 * slot;
+            // of each k step and pair of MMAs (word j): four cells of A's rows, seven of B's
+            const uint32_t t = tmem_base + quarter + kSfCol0 + kSlotCols * slot;
+            tmem_store_16(t, w[0][0], w[1][0], w[2][0], w[3][0], w[0][1], w[1][1], w[2][1], w[3][1], w[0][2], w[1][2], w[2][2], w[3][2], w[0][3], w[1][3], w[2][3], w[3][3]);
 #pragma unroll
-            for (int j = 0; j < 2; j++) { // two MMAs' worth of cells: A's rows, B's first 128 rows, B's last 96
-              tmem_store_4(t + 4 * j, w[0][2 * q + j], w[1][2 * q + j], w[2][2 * q + j], w[3][2 * q + j]);
-              tmem_store_4(t + 8 + 8 * j, w[4][2 * q + j], w[5][2 * q + j], w[6][2 * q + j], w[7][2 * q + j]);
-              tmem_store_4(t + 12 + 8 * j, w[8][2 * q + j], w[9][2 * q + j], w[10][2 * q + j], 0u);
+            for (int q = 0; q < kSlotSteps; q++) {
+              auto v = [&](int c, int j) { return w[4 + c][2 * q + j]; };
+              tmem_store_16(t + 16 + 16 * q, v(0, 0), v(1, 0), v(2, 0), v(3, 0), v(4, 0), v(5, 0), v(6, 0), 0u, v(0, 1), v(1, 1), v(2, 1), v(3, 1), v(4, 1), v(5, 1), v(6, 1), 0u);
             }
             tmem_store_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(sfull_bar(slot));
-            step++;
+            if (lane == 0) arrive_leader(sfull_bar(slot));
+            half++;
           }
         }
       }
     };
-    if (!COPY) fetch();
-    const int mine = blockIdx.x < num_tiles ? (num_tiles - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
+    const int mine = first_tile < num_tiles ? (num_tiles - first_tile + tile_stride - 1) / tile_stride : 0;
     const long long total = (long long)mine * groups;
     int group = 0;
     uint32_t sc_phase = 0;
@@ -664,44 +701,48 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
       if (ok && i + 1 < total) hand_over(group * kScSteps, 1, sc_phase);
       if (++group == groups) group = 0;
     }
+    if (!ok) tell_partner();
   } else {
     // ------------------------------------------------------------------ epilogue (warps 2..5)
     const int quad = warp & 3;
     const bool vec = (reinterpret_cast<uintptr_t>(args.Y) & 15) == 0 && args.N % (args.y_dtype == QL_F32 ? 4 : 8) == 0;
     int it = 0;
-    for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, it++) {
+    for (int tile = first_tile; tile < num_tiles; tile += tile_stride, it++) {
       const int buf = it & 1;
       const int mt = tile % args.tiles_a, nt = tile / args.tiles_a;
-      if (!warp_wait(tfull_bar(buf), (it >> 1) & 1, abort_flag, args.status, ST_TIMEOUT_TMEM_FULL)) break;
+      if (!warp_wait(tfull_bar(buf), (it >> 1) & 1, abort_flag, args.status, ST_TIMEOUT_TMEM_FULL)) { tell_partner(); break; }
       tc_fence_after();
-      const int m = mt * BM + quad * 32 + lane;
+      const int m = (row_tile * mt + (int)rank) * BM + quad * 32 + lane;
       const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * TBN);
 #pragma unroll 1
-      for (int c = 0; c < TBN / 32; c++) {
+      for (int c = 0; c < (TBN + 31) / 32; c++) {
         uint32_t r[32];
-        tmem_load_32(taddr + c * 32, r);
-        const int n = nt * TBN + c * 32;
-        if (n >= args.N) break;
-        if (!vec || n + 32 > args.N) {
-          mx_store_rows(args, reinterpret_cast<float *>(smem + L::kStaging) + quad * 32 * 33, r, m - lane, n, lane);
+        tmem_load_32(taddr + c * 32, r); // of the last chunk half the columns are the next accumulator's, or scales: not stored
+        const int n = nt * TBN + c * 32, end = min(args.N, nt * TBN + TBN);
+        if (n >= end) break;
+        const bool whole = n + 32 <= end;
+        if (!vec || !(whole || n + 16 == end)) {
+          mx_store_rows(args, reinterpret_cast<float *>(smem + L::kStaging) + quad * 32 * 33, r, m - lane, n, end, lane);
         } else if (m < args.M) {
           const size_t at = (size_t)m * (size_t)args.N + n;
-          if (args.y_dtype == QL_F32) mx_store_chunk(static_cast<float *>(args.Y) + at, r);
-          else if (args.y_dtype == QL_F16) mx_store_chunk(static_cast<__half *>(args.Y) + at, r);
-          else mx_store_chunk(static_cast<__nv_bfloat16 *>(args.Y) + at, r);
+          if (args.y_dtype == QL_F32) mx_store_chunk(static_cast<float *>(args.Y) + at, r, whole);
+          else if (args.y_dtype == QL_F16) mx_store_chunk(static_cast<__half *>(args.Y) + at, r, whole);
+          else mx_store_chunk(static_cast<__nv_bfloat16 *>(args.Y) + at, r, whole);
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(tempty_bar(buf));
+      if (lane == 0) arrive_leader(tempty_bar(buf));
     }
   }
 
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync_all(); // neither CTA may leave while the pair's MMAs or barriers can still touch it
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
   }
 }
 
@@ -821,53 +862,71 @@ template <int TN> int launch_split(const void *w, const void *x, const MxArgs &a
   return wide ? launch_split_as<TN, true>(w, x, args, K, plan, st) : launch_split_as<TN, false>(w, x, args, K, plan, st);
 }
 
-// [rows, row_bytes] bytes, rows `pitch` bytes apart, box = [box_rows, box_bytes], no swizzle
-int make_map_strided(CUtensorMap *map, const void *ptr, int64_t rows, int64_t row_bytes, int64_t pitch, int box_bytes, int box_rows) {
-  EncodeTiledFn enc;
-  int rc = get_encode_fn(&enc);
-  if (rc != QL_OK) return rc;
-  cuuint64_t dims[2] = {(cuuint64_t)row_bytes, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)pitch};
-  cuuint32_t box[2] = {(cuuint32_t)box_bytes, (cuuint32_t)box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_error(QL_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
-  return QL_OK;
+// Rows of scale bytes, `pitch` bytes apart and zero-padded, of both operands: 16 bytes a thread.
+__global__ void __launch_bounds__(256) mx_pad_scales_kernel(const uint8_t *__restrict__ a, int rows_a, const uint8_t *__restrict__ b, int rows_b, int kb, int units,
+                                                            uint4 *__restrict__ out) {
+  const int unit = blockIdx.x * 32 + threadIdx.x % 32, b0 = unit * 16; // a warp takes 512 bytes of a row, a block eight rows
+  if (unit >= units) return;
+  for (int64_t row = (int64_t)blockIdx.y * 8 + threadIdx.x / 32; row < (int64_t)rows_a + rows_b; row += (int64_t)gridDim.y * 8) {
+    const uint8_t *p = (row < rows_a ? a + row * kb : b + (row - rows_a) * kb) + b0;
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    if (b0 + 16 <= kb && (reinterpret_cast<uintptr_t>(p) & 3) == 0) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) w[j] = __ldg(reinterpret_cast<const uint32_t *>(p) + j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        if (b0 + j < kb) w[j / 4] |= (uint32_t)__ldg(p + j) << (8 * (j % 4));
+    }
+    out[row * units + unit] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
 }
 
-template <int SC> int launch_tiles_as(const void *a, const void *b, MxArgs args, int64_t K, cudaStream_t st) {
+// The copy engine takes rows of whole 16-byte units from a 16-byte aligned base.  Other scales are copied into such rows first
+// (in the caller's workspace): 2000 x 4096 x 11040 51 us, against 47 at K = 11264 and 150 with the scale warps loading them.
+int padded_pitch(int64_t kb) { return (int)((kb + 15) / 16 * 16); }
+bool needs_padding(const MxArgs &args) { return args.kb % 16 != 0 || !aligned16(args.sfa) || !aligned16(args.sfb); }
+int64_t padded_bytes(int64_t M, int64_t N, int64_t kb) { return (M + N) * padded_pitch(kb); }
+
+template <bool PAIR> int launch_tiles(const void *a, const void *b, MxArgs args, int64_t K, void *workspace, cudaStream_t st) {
+  using L = TileSmem<PAIR>;
   static bool configured[64] = {false};
-  int rc = allow_smem(gemm_mxfp4_tiles_kernel<SC>, TileSmem::kDynamic, configured);
+  int rc = allow_smem(gemm_mxfp4_tiles_kernel<PAIR>, L::kDynamic, configured);
   if (rc != QL_OK) return rc;
-  CUtensorMap ma, mb, msa, msb, msa_odd, msb_odd;
-  if ((rc = make_map(&ma, KIND_F8, a, args.M, K / 2, BM)) != QL_OK) return rc;
-  if ((rc = make_map(&mb, KIND_F8, b, args.N, K / 2, TBN)) != QL_OK) return rc;
-  msa = ma, msb = mb, msa_odd = ma, msb_odd = mb; // whatever the variant does not use
-  if (SC == SC_ROWS) {
-    if ((rc = make_map_bytes(&msa, args.sfa, args.M, args.kb, 32, BM)) != QL_OK) return rc;
-    if ((rc = make_map_bytes(&msb, args.sfb, args.N, args.kb, 32, TBN)) != QL_OK) return rc;
-  } else if (SC == SC_PAIRS) {
-    const int64_t kb = args.kb;
-    if ((rc = make_map_strided(&msa, args.sfa, (args.M + 1) / 2, kb, 2 * kb, 32, BM / 2)) != QL_OK) return rc;
-    if ((rc = make_map_strided(&msb, args.sfb, (args.N + 1) / 2, kb, 2 * kb, 32, TBN / 2)) != QL_OK) return rc;
-    if ((rc = make_map_strided(&msa_odd, args.sfa + kb - 8, args.M / 2, kb + 8, 2 * kb, 48, BM / 2)) != QL_OK) return rc;
-    if ((rc = make_map_strided(&msb_odd, args.sfb + kb - 8, args.N / 2, kb + 8, 2 * kb, 48, TBN / 2)) != QL_OK) return rc;
+  int pitch = args.kb;
+  if (needs_padding(args)) {
+    pitch = padded_pitch(args.kb);
+    const int units = pitch / 16;
+    const int64_t row_blocks = ((int64_t)args.M + args.N + 7) / 8;
+    const dim3 grid((unsigned)((units + 31) / 32), (unsigned)(row_blocks < 65535 ? row_blocks : 65535));
+    mx_pad_scales_kernel<<<grid, 256, 0, st>>>(args.sfa, args.M, args.sfb, args.N, args.kb, units, static_cast<uint4 *>(workspace));
+    count_launches(1);
+    QL_CUDA_TRY(cudaGetLastError());
+    args.sfa = static_cast<const uint8_t *>(workspace);
+    args.sfb = args.sfa + (int64_t)args.M * pitch;
   }
-  args.tiles_a = (args.M + BM - 1) / BM;
+  CUtensorMap ma, mb, msa, msb;
+  if ((rc = make_map(&ma, KIND_F8, a, args.M, K / 2, BM)) != QL_OK) return rc;
+  if ((rc = make_map(&mb, KIND_F8, b, args.N, K / 2, L::kRowsB)) != QL_OK) return rc;
+  if ((rc = make_map_bytes(&msa, args.sfa, args.M, pitch, 32, BM)) != QL_OK) return rc;
+  if ((rc = make_map_bytes(&msb, args.sfb, args.N, pitch, 32, TBN)) != QL_OK) return rc;
+  args.tiles_a = (args.M + (PAIR ? 2 : 1) * BM - 1) / ((PAIR ? 2 : 1) * BM);
   args.tiles_b = (args.N + TBN - 1) / TBN;
   const int64_t tiles = (int64_t)args.tiles_a * args.tiles_b;
-  gemm_mxfp4_tiles_kernel<SC><<<(unsigned)(tiles < sm_count() ? tiles : sm_count()), kTileThreads, TileSmem::kDynamic, st>>>(
-      ma, mb, msa, msb, msa_odd, msb_odd, args);
+  const int units = PAIR ? sm_count() / 2 : sm_count();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((PAIR ? 2 : 1) * (tiles < units ? tiles : units)), 1, 1);
+  cfg.blockDim = dim3(kTileThreads, 1, 1);
+  cfg.dynamicSmemBytes = L::kDynamic;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = PAIR ? 2 : 1, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_mxfp4_tiles_kernel<PAIR>, ma, mb, msa, msb, args));
   count_launches(1);
-  QL_CUDA_TRY(cudaGetLastError());
   return QL_OK;
-}
-int launch_tiles(const void *a, const void *b, const MxArgs &args, int64_t K, cudaStream_t st) {
-  const bool bases = aligned16(args.sfa) && aligned16(args.sfb);
-  if (bases && args.kb % 16 == 0) return launch_tiles_as<SC_ROWS>(a, b, args, K, st);
-  if (bases && args.kb % 16 == 8 && args.M > 1 && args.N > 1) return launch_tiles_as<SC_PAIRS>(a, b, args, K, st); // an odd row exists
-  return launch_tiles_as<SC_WORDS>(a, b, args, K, st);
 }
 
 } // namespace
@@ -875,7 +934,20 @@ int launch_tiles(const void *a, const void *b, const MxArgs &args, int64_t K, cu
 
 using namespace ql;
 
-extern "C" int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, const ql_tensor *b, const ql_tensor *b_scales, ql_tensor *y, void *stream) {
+extern "C" int ql_gemm_mxfp4_workspace(const ql_tensor *a, const ql_tensor *a_scales, const ql_tensor *b, const ql_tensor *b_scales, int64_t *bytes) {
+  const char *op = "gemm_mxfp4_workspace";
+  int rc;
+  if ((rc = check_mx_operand(op, "a", a, a_scales)) != QL_OK) return rc;
+  if ((rc = check_mx_operand(op, "b", b, b_scales)) != QL_OK) return rc;
+  if (!bytes) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: no place for the size", op);
+  const int64_t M = a->shape[0], N = b->shape[0], kb = a->shape[1] / 32;
+  const bool rows16 = kb % 16 == 0 && aligned16(a_scales->data) && aligned16(b_scales->data);
+  *bytes = rows16 || M <= kSplitOnly || N == 0 ? 0 : padded_bytes(M, N, kb);
+  return QL_OK;
+}
+
+extern "C" int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, const ql_tensor *b, const ql_tensor *b_scales, ql_tensor *y, void *workspace, int64_t workspace_bytes,
+                             void *stream) {
   const char *op = "gemm_mxfp4";
   int rc;
   if ((rc = check_mx_operand(op, "a", a, a_scales)) != QL_OK) return rc;
@@ -891,6 +963,11 @@ extern "C" int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, cons
   if ((reinterpret_cast<uintptr_t>(a_scales->data) | reinterpret_cast<uintptr_t>(b_scales->data)) & 3) return set_error(QL_ERR_UNSUPPORTED, "%s: needs 4-byte aligned scales", op);
   if (reinterpret_cast<uintptr_t>(y->data) % (y->dtype == QL_F32 ? 4 : 2)) return set_error(QL_ERR_UNSUPPORTED, "%s: y is not aligned to its type", op);
   if (M > (1 << 30) || N > (1 << 30) || K > (1 << 30)) return set_error(QL_ERR_UNSUPPORTED, "%s: dimension too large", op);
+  int64_t need = 0;
+  if ((rc = ql_gemm_mxfp4_workspace(a, a_scales, b, b_scales, &need)) != QL_OK) return rc;
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return set_error(QL_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %lld bytes, got %lld", op, (long long)need, (long long)(workspace ? workspace_bytes : 0));
+  if (need > 0 && !aligned16(workspace)) return set_error(QL_ERR_UNSUPPORTED, "%s: the workspace must be 16-byte aligned", op);
   cudaStream_t st = (cudaStream_t)stream;
 
   MxArgs args;
@@ -903,13 +980,15 @@ extern "C" int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, cons
   args.tiles_a = args.tiles_b = 0;
   args.status = device_status_word();
   if (!args.status) return set_error(QL_ERR_CUDA, "%s: could not allocate the device status word", op);
-  const int64_t tiles = ((M + BM - 1) / BM) * ((N + TBN - 1) / TBN);
+  // Pairs of the tiles kernel take 4.5 us and 0.45 us per k step and tile of a pair, its single CTAs 0.56; the split kernel what
+  // plan_split says.  Up to 32 tokens the tiles are mostly padding and the split kernel is the better one throughout; up to
+  // 128 a pair's second half would be.  128 x 4096 x 4096: split 11.7 us, tiles 12.7; 128 x 28672 x 8192: 45.7, 28.0 (pairs 32);
+  // 512 x 11008 x 4096: single CTAs 21.9, pairs 20.4; 8192 x 28672 x 8192: 920, 800.
+  const bool pairs = M > BM;
+  const int64_t row_tiles = pairs ? (M + 2 * BM - 1) / (2 * BM) : (M + BM - 1) / BM, units = pairs ? sm_count() / 2 : sm_count();
+  const int64_t tiles = row_tiles * ((N + TBN - 1) / TBN);
   if (tiles >= (1ll << 30)) return set_error(QL_ERR_UNSUPPORTED, "%s: too many output tiles", op);
-  // The tiles kernel takes 4 us and 0.56 us per k step and tile of an SM (1 us where its warps load the scales); the split
-  // kernel what plan_split says.  Up to 32 tokens the tiles are mostly padding and the split kernel is the better one
-  // throughout.  128 x 4096 x 4096: split 11.7 us, tiles 13.2; 128 x 28672 x 8192: 45.7 and 27.8; 333 x 1001 x 2080: 13.3, 17.4.
-  const int64_t per_sm = (tiles + sm_count() - 1) / sm_count();
-  const double tiles_us = M <= 32 ? 1e30 : 4.0 + (K % 256 == 0 ? 0.56 : 1.0) * (double)per_sm * args.num_ks;
+  const double tiles_us = M <= kSplitOnly ? 1e30 : 4.5 + (need > 0 ? 3.0 : 0.0) + (pairs ? 0.45 : 0.56) * (double)((tiles + units - 1) / units) * args.num_ks;
   args.sfa = static_cast<const uint8_t *>(b_scales->data); // the weights are the 128-row operand of the split kernel
   args.sfb = static_cast<const uint8_t *>(a_scales->data);
   bool ran = false;
@@ -920,5 +999,5 @@ extern "C" int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, cons
   if (rc != QL_OK || ran) return rc;
   args.sfa = static_cast<const uint8_t *>(a_scales->data);
   args.sfb = static_cast<const uint8_t *>(b_scales->data);
-  return launch_tiles(a->data, b->data, args, K, st);
+  return pairs ? launch_tiles<true>(a->data, b->data, args, K, workspace, st) : launch_tiles<false>(a->data, b->data, args, K, workspace, st);
 }

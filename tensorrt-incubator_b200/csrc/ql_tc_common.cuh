@@ -227,6 +227,15 @@ __device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity) {
     if (clock64() - t0 > kWaitLimitCycles) return false;
   return true;
 }
+// The same barrier of both CTAs of a pair, in one instruction (`bar` is this CTA's address of it).
+__device__ __forceinline__ void tc_commit_both(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+// Arrival at a barrier of another CTA of the cluster that need not publish this thread's writes: what it announces, stores to
+// tensor memory, is ordered by the tcgen05 fences.  The release at cluster scope of mbar_arrive_cluster takes about 1000 cycles.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 

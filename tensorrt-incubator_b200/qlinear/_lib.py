@@ -72,7 +72,8 @@ SIGNATURES = {
     "ql_gemm_nvfp4": ([_T, _T, _T, _T, _T, _T, _T, _S], ctypes.c_int),
     "ql_quantize_mxfp4": ([_T, _T, _T, _S], ctypes.c_int),
     "ql_dequantize_mxfp4": ([_T, _T, _T, _S], ctypes.c_int),
-    "ql_gemm_mxfp4": ([_T, _T, _T, _T, _T, _S], ctypes.c_int),
+    "ql_gemm_mxfp4_workspace": ([_T, _T, _T, _T, ctypes.POINTER(ctypes.c_int64)], ctypes.c_int),
+    "ql_gemm_mxfp4": ([_T, _T, _T, _T, _T, ctypes.c_void_p, ctypes.c_int64, _S], ctypes.c_int),
     "ql_gated_linear": ([_T, _T, _T, ctypes.c_int32, _T, _S], ctypes.c_int),
     "ql_gated_linear_backward_workspace": ([_T, _T, ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(ctypes.c_int64)], ctypes.c_int),
     "ql_gated_linear_backward": ([_T, _T, _T, _T, ctypes.c_int32, _T, _T, _T, ctypes.c_void_p, ctypes.c_int64, _S], ctypes.c_int),
@@ -134,16 +135,10 @@ def check(rc: int) -> None:
 
 
 def make_tensor(ptr: int, dtype: int, shape) -> QlTensor:
-    t = QlTensor()
-    t.data = ptr
-    t.dtype = dtype
-    shape = tuple(int(s) for s in shape)
-    if len(shape) > QL_MAX_RANK:
-        raise QlError(ERR_INVALID_ARGUMENT, f"rank {len(shape)} exceeds {QL_MAX_RANK}")
-    t.rank = len(shape)
-    for i, s in enumerate(shape):
-        t.shape[i] = s
-    return t
+    rank = len(shape)
+    if rank > QL_MAX_RANK:
+        raise QlError(ERR_INVALID_ARGUMENT, f"rank {rank} exceeds {QL_MAX_RANK}")
+    return QlTensor(ptr, dtype, rank, tuple(shape))   # one call: the rest of the shape is zero
 
 
 def make_attrs(axis=None, fp8_mode="direct") -> QlQdqAttrs:

@@ -21,6 +21,8 @@ def _activation(name: str) -> int:
 
 def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
     require_cuda(t, what)
+    if t.dim() == 2:
+        return t.contiguous()
     if t.dim() == 0:
         raise QuantizeError(f"{what} must have at least 1 dimension.")
     return t.reshape(-1, t.shape[-1]).contiguous() if t.numel() else t.reshape(t.shape[:-1].numel(), t.shape[-1])
@@ -33,13 +35,17 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
     act = _activation(activation)
     x2 = _rows(x, "x")
     wg, wu = w_gate.contiguous(), w_up.contiguous()   # kept alive across the call: a view only borrows the pointer
-    h = out if out is not None else torch.empty(x.shape[:-1] + wg.shape[:1], dtype=x.dtype, device=x.device)
-    if out is not None and tuple(out.shape) != tuple(x.shape[:-1] + wg.shape[:1]):
-        raise QuantizeError(f"out must have shape {tuple(x.shape[:-1] + wg.shape[:1])}, got {tuple(out.shape)}.")
-    ql_view(h)   # a result that is not dense is refused here: reshape would copy it
-    call_on(x.device, _lib.lib().ql_gated_linear, ql_view(x2), ql_view(wg), ql_view(wu), act, ql_view(h.reshape(x2.shape[0], wg.shape[0])),
-            same_device=(wg, wu, h))
-    return h
+    rows, I = x2.shape[0], wg.shape[0]
+    if out is None:
+        h = torch.empty(rows, I, dtype=x.dtype, device=x.device)
+    else:
+        if tuple(out.shape) != tuple(x.shape[:-1]) + (I,):
+            raise QuantizeError(f"out must have shape {tuple(x.shape[:-1]) + (I,)}, got {tuple(out.shape)}.")
+        if not out.is_contiguous():
+            raise QuantizeError("out must be contiguous (dense row-major).")
+        h = out.view(rows, I)
+    call_on(x.device, _lib.lib().ql_gated_linear, ql_view(x2), ql_view(wg), ql_view(wu), act, ql_view(h), same_device=(wg, wu, h))
+    return out if out is not None else (h if x.dim() == 2 else h.view(x.shape[:-1] + (I,)))
 
 
 def gated_linear_backward(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu", *,
@@ -55,15 +61,16 @@ def gated_linear_backward(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Ten
     dx = torch.empty(x2.shape, dtype=x.dtype, device=x.device) if need_input_grad else None
     dwg = torch.empty(wg.shape, dtype=x.dtype, device=x.device) if need_weight_grad else None
     dwu = torch.empty(wu.shape, dtype=x.dtype, device=x.device) if need_weight_grad else None
-    v = lambda t: ql_view(t) if t is not None else None
+    vx, vg = ql_view(x2), ql_view(wg)
+    out = [ql_view(t) if t is not None else None for t in (dx, dwg, dwu)]
     size = ctypes.c_int64()
+    L = _lib.lib()
 
     def run(stream):   # with the tensors' device current: the plan behind the size depends on the device
-        rc = _lib.lib().ql_gated_linear_backward_workspace(ql_view(x2), ql_view(wg), need_input_grad, need_weight_grad, ctypes.byref(size))
+        rc = L.ql_gated_linear_backward_workspace(vx, vg, need_input_grad, need_weight_grad, ctypes.byref(size))
         if rc != _lib.OK:
             return rc
         ws = torch.empty(size.value, dtype=torch.uint8, device=x.device)
-        return _lib.lib().ql_gated_linear_backward(ql_view(g2), ql_view(x2), ql_view(wg), ql_view(wu), act, v(dx), v(dwg), v(dwu),
-                                                   ws.data_ptr() or None, size.value, stream)
+        return L.ql_gated_linear_backward(ql_view(g2), vx, vg, ql_view(wu), act, *out, ws.data_ptr() or None, size.value, stream)
     call_on(x.device, run, same_device=(g2, wg, wu))
     return (dx.reshape(x.shape) if dx is not None else None), dwg, dwu

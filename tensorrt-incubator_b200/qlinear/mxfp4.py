@@ -3,6 +3,8 @@ scale (a power of two) per block.  Data are Float4Tensor, as dynamic_quantize's 
 torch.float8_e8m0fnu.  The reference has no such operator; NVFP4 (ops.dynamic_quantize) is its nearest relative."""
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -47,14 +49,23 @@ def gemm_mxfp4(a: Float4Tensor, a_scales: torch.Tensor, b: Float4Tensor, b_scale
     """dequantize_mxfp4(a) @ dequantize_mxfp4(b)^T on the block-scaled tensor cores: a [M, K] (activations, any M from one
     token up), b [N, K] (weights) and their scales as quantize_mxfp4 returns them; f32 sums, one rounding to `out_dtype`
     (float32, float16 or bfloat16)."""
-    for t, what in ((a, "a"), (a_scales, "a_scales"), (b, "b"), (b_scales, "b_scales")):
-        require_cuda(t, what)
+    require_cuda(a, "a")
+    require_cuda(b, "b")
     if not isinstance(a, Float4Tensor) or not isinstance(b, Float4Tensor):
         raise QuantizeError("gemm_mxfp4: a and b must be Float4Tensor, as quantize_mxfp4 returns them")
     if out is None and out_dtype not in dt.QUANTIZABLE_DTYPES:
         raise QuantizeError(f"Unsupported data type in gemm_mxfp4. Supported data types are: {dt.QUANTIZABLE_DTYPES}. Got out_dtype={out_dtype}")
-    y = out if out is not None else torch.empty((a.shape[0], b.shape[0]), dtype=out_dtype.torch, device=a.device)
+    y = out if out is not None else torch.empty(a.shape[0], b.shape[0], dtype=out_dtype.torch, device=a.device)
     # dense, on a multiple of 4 bytes (a slice of rows need not be); kept alive across the call: a view only borrows the pointer
     sa, sb = (s if s.data_ptr() % 4 == 0 else s.clone() for s in (a_scales.contiguous(), b_scales.contiguous()))
-    call_on(a.device, _lib.lib().ql_gemm_mxfp4, ql_view(a), ql_view(sa), ql_view(b), ql_view(sb), ql_view(y), same_device=(sa, b, sb, y))
+    L = _lib.lib()
+    va, vsa, vb, vsb = ql_view(a), ql_view(sa), ql_view(b), ql_view(sb)
+    ws = None
+    if sa.shape[-1] % 16 or (sa.data_ptr() | sb.data_ptr()) % 16:   # rows the kernel for many tokens wants a padded copy of
+        size = ctypes.c_int64()
+        _lib.check(L.ql_gemm_mxfp4_workspace(va, vsa, vb, vsb, ctypes.byref(size)))
+        if size.value:
+            ws = torch.empty(size.value, dtype=torch.uint8, device=a.device)
+    call_on(a.device, L.ql_gemm_mxfp4, va, vsa, vb, vsb, ql_view(y), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+            same_device=(sa, b, sb, y))
     return y

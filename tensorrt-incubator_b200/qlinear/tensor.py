@@ -83,13 +83,11 @@ def dtype_of(t) -> dt.dtype:
 
 def ql_view(t) -> _lib.QlTensor:
     """QlTensor over a CUDA torch tensor or Int4Tensor (no copy; the caller keeps `t` alive)."""
-    if isinstance(t, Int4Tensor):
-        return _lib.make_tensor(t.packed.data_ptr(), _lib.I4, t.shape)
-    if isinstance(t, Float4Tensor):
-        return _lib.make_tensor(t.packed.data_ptr(), _lib.F4E2M1, t.shape)
-    if not t.is_contiguous():
-        raise _lib.QlError(_lib.ERR_INVALID_ARGUMENT, "tensors must be contiguous (dense row-major)")
-    return _lib.make_tensor(t.data_ptr(), dt.from_torch(t.dtype).code, t.shape)
+    if isinstance(t, torch.Tensor):
+        if not t.is_contiguous():
+            raise _lib.QlError(_lib.ERR_INVALID_ARGUMENT, "tensors must be contiguous (dense row-major)")
+        return _lib.make_tensor(t.data_ptr(), dt.from_torch(t.dtype).code, t.shape)
+    return _lib.make_tensor(t.packed.data_ptr(), _lib.I4 if isinstance(t, Int4Tensor) else _lib.F4E2M1, t.shape)
 
 
 def require_cuda(t, what: str) -> None:
@@ -99,7 +97,12 @@ def require_cuda(t, what: str) -> None:
 
 
 def current_stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The handle of `device`'s current stream (what torch.cuda.current_stream(device).cuda_stream is, without building the
+    stream object: 0.1 us instead of 3 on every launch)."""
+    index = device.index if isinstance(device, torch.device) else None
+    if index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def empty_quantized(shape, qdtype: dt.dtype, device):
@@ -116,7 +119,9 @@ def call_on(device, fn, *args, same_device=()) -> None:
         if t.device != device:
             raise _lib.QlError(_lib.ERR_INVALID_ARGUMENT, f"tensors must live on one device, got {device} and {t.device}")
     if device.index is None or device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, current_stream(device)))
+        rc = fn(*args, current_stream(device))
+        if rc != _lib.OK:
+            _lib.check(rc)
     else:
         with torch.cuda.device(device):
             _lib.check(fn(*args, current_stream(device)))

@@ -285,7 +285,7 @@ def test_refusals():
         ql.gated_linear(x, w, w[:4])
     with pytest.raises(ql.QuantizeError, match="out must have shape"):
         ql.gated_linear(x, w, w, out=torch.empty((4, 16), dtype=torch.bfloat16, device="cuda"))
-    with pytest.raises(ql.QlError, match="contiguous"):
+    with pytest.raises(ql.QuantizeError, match="contiguous"):
         ql.gated_linear(x, w, w, out=torch.empty((8, 4), dtype=torch.bfloat16, device="cuda").t())
     with pytest.raises(ql.QlError, match="one device"):
         ql.gated_linear(x, w, w.cpu())

@@ -1,5 +1,7 @@
 """MXFP4 without a GPU: the host restatement on hand-worked blocks, and what the entry points refuse before they touch
 a device."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -65,7 +67,7 @@ def test_quantize_and_dequantize_argument_rules():
 def test_product_argument_rules():
     L = _lib.lib()
     a, sa, b, sb, y = _t(_lib.F4E2M1, [4, 64]), _t(_lib.F8E8M0, [4, 2]), _t(_lib.F4E2M1, [8, 64]), _t(_lib.F8E8M0, [8, 2]), _t(_lib.BF16, [4, 8])
-    call = lambda a=a, sa=sa, b=b, sb=sb, y=y: L.ql_gemm_mxfp4(a, sa, b, sb, y, None)
+    call = lambda a=a, sa=sa, b=b, sb=sb, y=y, ws=None, n=0: L.ql_gemm_mxfp4(a, sa, b, sb, y, ws, n, None)
     assert "a is null" in _err(call(sa=None)) and "b is null" in _err(call(b=None))
     assert "data must be f4E2M1FN" in _err(call(a=_t(_lib.I4, [4, 64])))
     assert "scales f8E8M0FNU" in _err(call(sb=_t(_lib.F8E4M3, [8, 2])))
@@ -81,3 +83,12 @@ def test_product_argument_rules():
     assert "4-byte aligned scales" in _err(call(sb=_t(_lib.F8E8M0, [8, 2], 0x1002)))
     assert "aligned to its type" in _err(call(y=_t(_lib.BF16, [4, 8], 0x1001)))
     assert call(a=_t(_lib.F4E2M1, [0, 64], None), sa=_t(_lib.F8E8M0, [0, 2], None), y=_t(_lib.BF16, [0, 8], None)) == 0
+    # many tokens whose scale rows are no multiple of 16 bytes: a workspace for a padded copy
+    size = ctypes.c_int64(-1)
+    many = dict(a=_t(_lib.F4E2M1, [40, 96]), sa=_t(_lib.F8E8M0, [40, 3]), b=_t(_lib.F4E2M1, [8, 96]), sb=_t(_lib.F8E8M0, [8, 3]))
+    assert L.ql_gemm_mxfp4_workspace(*many.values(), ctypes.byref(size)) == 0 and size.value == 48 * 16
+    y = _t(_lib.BF16, [40, 8])
+    assert "needs a workspace of 768 bytes" in _err(call(**many, y=y)) and "needs a workspace of 768 bytes" in _err(call(**many, y=y, ws=0x1000, n=767))
+    assert "16-byte aligned" in _err(call(**many, y=y, ws=0x1008, n=768))
+    assert L.ql_gemm_mxfp4_workspace(a, sa, b, sb, ctypes.byref(size)) == 0 and size.value == 0
+    assert "no place for the size" in _err(L.ql_gemm_mxfp4_workspace(a, sa, b, sb, None))
