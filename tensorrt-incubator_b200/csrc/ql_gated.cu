@@ -302,6 +302,14 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       int mt, nt;
       band_coords(tile, args.tiles_m, args.tiles_n, args.group_m, &mt, &nt);
       const int m0 = mt * 256 + (int)p.rank * 128 + quad * 32, m = m0 + lane;
+      uint4 ahead[4]; // dH of the next chunk, on its way while this one is worked on
+      auto fetch = [&](int c) {
+        const int n = nt * 128 + c * 32;
+        const T *row = static_cast<const T *>(args.dh) + (size_t)m * (size_t)args.I + n;
+#pragma unroll
+        for (int j = 0; j < 4; j++) ahead[j] = c < 4 && m < args.M && n + 8 * j < args.I ? __ldcs(reinterpret_cast<const uint4 *>(row) + j) : make_uint4(0u, 0u, 0u, 0u);
+      };
+      if constexpr (BACKWARD) fetch(0);
       ok = warp_wait(p.tfull(buf), (it >> 1) & 1, p.abort_flag, p.status, ST_TIMEOUT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after();
@@ -311,9 +319,9 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         const int n = nt * 128 + c * 32, half = c & 1;
         uint4 dh[4];
         if constexpr (BACKWARD) {
-          const T *row = static_cast<const T *>(args.dh) + (size_t)m * (size_t)args.I + n;
 #pragma unroll
-          for (int j = 0; j < 4; j++) dh[j] = m < args.M && n + 8 * j < args.I ? __ldcs(reinterpret_cast<const uint4 *>(row) + j) : make_uint4(0u, 0u, 0u, 0u);
+          for (int j = 0; j < 4; j++) dh[j] = ahead[j];
+          fetch(c + 1);
         }
         uint32_t g[32], u[32];
         tmem_load_32(taddr + c * 32, g);
@@ -372,8 +380,9 @@ struct GradArgs {
   // units: a 256 x 256 tile and one of `*_split` parts of its reduction
   int x_tiles_m, x_tiles_n, x_steps, x_split, x_units;   // dX [M, K]: steps of 64 channels, the gate's first, then the up's
   int w_tiles_m, w_tiles_n, w_steps, w_split, w_units;   // dWg and dWu [I, K] each: steps of 64 tokens
-  int heavy, heavy_w;                                    // the first `heavy` clusters have one dX unit more and `heavy_w` weight units
-  int x_per;                                             // dX units of the others
+  int x_per;                                             // dX units of a cluster; one more for the first `heavy` ones,
+  int heavy, heavy_w;                                    // which then have `heavy_w` weight units, the others the rest.
+  int mixed;                                             // instead: units of one length, all dealt out in turn
   int group_m;
   float *x_parts, *w_parts;                              // [split][M][K], [split][2][I][K], null where nothing is cut
   int *status;
@@ -388,9 +397,9 @@ struct Unit {
 
 // The j-th unit of cluster c: its dX units, then its weight units.  Neighbouring clusters hold neighbouring tiles.
 __device__ __forceinline__ bool get_unit(const GradArgs &a, int c, int clusters, int j, Unit *u) {
-  const int nx = a.x_per + (c < a.heavy ? 1 : 0);
-  if (j < nx) {
-    const int unit = c + j * clusters, tiles = a.x_tiles_m * a.x_tiles_n, tile = unit % tiles;
+  const int turn = c + j * clusters, nx = a.x_per + (c < a.heavy ? 1 : 0);
+  if (a.mixed ? turn < a.x_units : j < nx) {
+    const int unit = turn, tiles = a.x_tiles_m * a.x_tiles_n, tile = unit % tiles;
     int mt, nt;
     band_coords(tile, a.x_tiles_m, a.x_tiles_n, a.group_m, &mt, &nt);
     u->is_x = true, u->up = false, u->row0 = mt * 256, u->col0 = nt * 256, u->part = unit / tiles;
@@ -399,7 +408,9 @@ __device__ __forceinline__ bool get_unit(const GradArgs &a, int c, int clusters,
   }
   j -= nx;
   int unit;
-  if (c < a.heavy) {
+  if (a.mixed) {
+    unit = turn - a.x_units;
+  } else if (c < a.heavy) {
     if (j >= a.heavy_w) return false;
     unit = j * a.heavy + c;
   } else {
@@ -895,29 +906,40 @@ GradPlan plan_grads(int M, int I, int K, bool want_x, bool want_w, int pairs) {
   a.x_tiles_m = (M + 255) / 256, a.x_tiles_n = a.w_tiles_n = (K + 255) / 256, a.w_tiles_m = (I + 255) / 256;
   a.x_steps = 2 * ((I + 63) / 64), a.w_steps = (M + 63) / 64;
   const int64_t x_tiles = want_x ? (int64_t)a.x_tiles_m * a.x_tiles_n : 0, w_tiles = want_w ? 2ll * a.w_tiles_m * a.w_tiles_n : 0;
-  // A unit costs its steps and about 8 more to start and write out.  A reduction is cut where its tiles alone would leave
-  // pairs idle: into units of at least 8 steps, no longer than a pair's share of all steps.
+  // A unit costs its steps and about 8 more to start and write out.  With two tiles a pair or more, dX's long units come first,
+  // cut to a pair's share of all steps where they are fewer than the pairs, and a pair that has one more of them gets as many
+  // fewer of the weights' as that is worth.  With fewer tiles both reductions are cut into units of one length, dealt out in
+  // turn: the length, of the share and fractions of it down to 8, that makes the longest pair's time the shortest.
+  // 8192 x 1024 x 512 84 us so, 153 dealt out the first way; 512 x 11008 x 4096 235 us the first way, 250 the second.
   const int64_t share = (x_tiles * a.x_steps + w_tiles * a.w_steps + pairs - 1) / pairs;
-  auto cut = [&](int64_t tiles, int steps) {
-    if (tiles == 0 || tiles >= pairs) return 1;
-    const int64_t len = share < 8 ? 8 : share;
-    int64_t s = (steps + len - 1) / len;
-    const int64_t most = steps / 8 < 1 ? 1 : steps / 8;
-    s = s > most ? most : s;
-    return (int)(s > 32 ? 32 : s);
+  auto cut = [&](int64_t tiles, int steps, int64_t len) { // what is not wanted has no units and no parts
+    if (tiles == 0) return 1;
+    const int64_t n = (steps + len - 1) / len;
+    return (int)(n > 32 ? 32 : n);
   };
-  a.x_split = cut(x_tiles, a.x_steps), a.w_split = cut(w_tiles, a.w_steps);
+  a.mixed = x_tiles + w_tiles < 2 * pairs;
+  if (a.mixed) {
+    int64_t best = INT64_MAX;
+    for (int part = 1; part <= 4; part++) {
+      const int64_t len = share / part < 8 ? 8 : share / part;
+      const int xs = cut(x_tiles, a.x_steps, len), ws = cut(w_tiles, a.w_steps, len);
+      const int64_t x_len = x_tiles ? (a.x_steps + xs - 1) / xs : 0, w_len = w_tiles ? (a.w_steps + ws - 1) / ws : 0;
+      const int64_t cost = (x_tiles * xs + w_tiles * ws + pairs - 1) / pairs * ((x_len > w_len ? x_len : w_len) + 8);
+      if (cost < best) best = cost, a.x_split = xs, a.w_split = ws;
+    }
+  } else {
+    a.x_split = x_tiles >= pairs ? 1 : cut(x_tiles, a.x_steps, share < 8 ? 8 : share);
+    a.w_split = w_tiles >= pairs ? 1 : cut(w_tiles, a.w_steps, share < 8 ? 8 : share);
+  }
   a.x_units = (int)(x_tiles * a.x_split), a.w_units = (int)(w_tiles * a.w_split);
   a.x_per = a.x_units / pairs, a.heavy = a.x_units % pairs;
-  // weight units of a heavy cluster: as many fewer as one dX unit is worth
   const double ux = (double)a.x_steps / a.x_split + 8, uw = (double)a.w_steps / a.w_split + 8;
-  double hw = (a.w_units - (pairs - a.heavy) * ux / uw) / pairs;
-  a.heavy_w = a.heavy == 0 ? 0 : (int)(hw < 0 ? 0 : hw + 0.5);
-  if ((int64_t)a.heavy * a.heavy_w > a.w_units) a.heavy_w = a.w_units / a.heavy;
+  const double hw = (a.w_units - (pairs - a.heavy) * ux / uw) / pairs;
+  a.heavy_w = hw < 0 ? 0 : (int)(hw + 0.5);
   a.group_m = 8; // row tiles walked together; 4, 8, 16, 32 on 4096 x 11008 x 4096: 1.62, 1.55, 1.59, 1.54 ms; on 1024 x 28672 x 8192: 2.12, 2.10, 2.10, 2.20
   a.x_parts = a.w_parts = nullptr;
-  p.x_part_floats = a.x_split > 1 ? (int64_t)a.x_split * M * K : 0;
-  p.w_part_floats = a.w_split > 1 ? 2ll * a.w_split * I * K : 0;
+  p.x_part_floats = x_tiles > 0 && a.x_split > 1 ? (int64_t)a.x_split * M * K : 0;
+  p.w_part_floats = w_tiles > 0 && a.w_split > 1 ? 2ll * a.w_split * I * K : 0;
   return p;
 }
 
