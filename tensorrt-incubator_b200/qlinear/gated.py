@@ -4,6 +4,7 @@ reference has no such operator; its pieces are tp.Linear and the activations of 
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -26,6 +27,15 @@ def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
     if t.dim() == 0:
         raise QuantizeError(f"{what} must have at least 1 dimension.")
     return t.reshape(-1, t.shape[-1]).contiguous() if t.numel() else t.reshape(t.shape[:-1].numel(), t.shape[-1])
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(x_shape, w_shape, dtype: int, want_dx: bool, want_dw: bool, device_index: int) -> int:
+    """ql_gated_linear_backward_workspace, asked once per shape (and device, which is the current one)."""
+    size = ctypes.c_int64()
+    _lib.check(_lib.lib().ql_gated_linear_backward_workspace(_lib.make_tensor(None, dtype, x_shape), _lib.make_tensor(None, dtype, w_shape), want_dx, want_dw,
+                                                             ctypes.byref(size)))
+    return size.value
 
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu", *, out=None) -> torch.Tensor:
@@ -63,14 +73,11 @@ def gated_linear_backward(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Ten
     dwu = torch.empty(wu.shape, dtype=x.dtype, device=x.device) if need_weight_grad else None
     vx, vg = ql_view(x2), ql_view(wg)
     out = [ql_view(t) if t is not None else None for t in (dx, dwg, dwu)]
-    size = ctypes.c_int64()
     L = _lib.lib()
 
-    def run(stream):   # with the tensors' device current: the plan behind the size depends on the device
-        rc = L.ql_gated_linear_backward_workspace(vx, vg, need_input_grad, need_weight_grad, ctypes.byref(size))
-        if rc != _lib.OK:
-            return rc
-        ws = torch.empty(size.value, dtype=torch.uint8, device=x.device)
-        return L.ql_gated_linear_backward(ql_view(g2), vx, vg, ql_view(wu), act, *out, ws.data_ptr() or None, size.value, stream)
+    def run(stream):   # with the tensors' device current: the plan behind the workspace's size depends on the device
+        size = _workspace_bytes(tuple(x2.shape), tuple(wg.shape), vx.dtype, need_input_grad, need_weight_grad, x.device.index)
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        return L.ql_gated_linear_backward(ql_view(g2), vx, vg, ql_view(wu), act, *out, ws.data_ptr() or None, size, stream)
     call_on(x.device, run, same_device=(g2, wg, wu))
     return (dx.reshape(x.shape) if dx is not None else None), dwg, dwu
