@@ -63,8 +63,14 @@ int *device_status_word() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
   if (!words[dev]) {
-    if (cudaMalloc(&words[dev], sizeof(int)) != cudaSuccess) return nullptr;
-    cudaMemset(words[dev], 0, sizeof(int));
+    // the first call may come while a stream is captured: the allocation is no part of what is captured
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    int *word = nullptr;
+    const bool ok = cudaMalloc(&word, sizeof(int)) == cudaSuccess && cudaMemset(word, 0, sizeof(int)) == cudaSuccess;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (!ok) return nullptr;
+    words[dev] = word;
   }
   return words[dev];
 }

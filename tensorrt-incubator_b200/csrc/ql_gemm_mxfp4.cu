@@ -182,11 +182,12 @@ template <int TN> struct SplitSmem {
   static constexpr int kAbort = kTmemPtr + 4;
   static constexpr int kRing = (kAbort + 4 + 1023) / 1024 * 1024;
   static constexpr int stage_bytes(int rows) { return ((rows + 7) / 8 * 8 + TN) * BK_BYTES; }
-  // At least a third of an SM's shared memory: two CTAs of 256 columns fill tensor memory, and a third one waiting for columns
-  // while its cluster partners wait for it could wait for good.
+  // At least half of an SM's shared memory, as it takes half of its tensor memory: what fits beside it then finds the columns it
+  // needs.  A CTA waiting for columns while its cluster partners wait for it could wait for good.
+  static constexpr int kHalf = 232448 / 2 - 2048;
   static constexpr int total(int rows, int stages) {
     const int n = kRing + stages * stage_bytes(rows) + MX_A_BYTES + 1024;
-    return n < 79872 ? 79872 : n;
+    return n < kHalf ? kHalf : n;
   }
 };
 

@@ -13,6 +13,7 @@ from .ops import QuantizeError
 from .tensor import Float4Tensor, call_on, ql_view, require_cuda
 
 BLOCK = 32
+_FLOATS = frozenset((torch.float32, torch.float16, torch.bfloat16))
 
 
 def quantize_mxfp4(input: torch.Tensor):
@@ -20,15 +21,15 @@ def quantize_mxfp4(input: torch.Tensor):
     2^(floor(log2 max|block b|) - 2), at least 2^-127, and data the block over its scale in e2m1, rounded half to even and
     saturated.  A block with an infinity or a NaN in it gets a NaN scale."""
     require_cuda(input, "input")
-    if input.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    if input.dtype not in _FLOATS:
         raise QuantizeError(f"Input does not have a valid dtype in quantize_mxfp4. input.dtype must be one of {dt.QUANTIZABLE_DTYPES}, got {input.dtype}")
-    if input.dim() == 0 or input.shape[-1] % BLOCK:
-        raise QuantizeError(f"the last dimension must be divisible by {BLOCK}, got shape {tuple(input.shape)}.")
-    x = input.contiguous()
-    shape = x.shape
-    data = Float4Tensor(torch.empty(x.numel() // 2, dtype=torch.uint8, device=x.device), shape)
-    scales = torch.empty(shape[:-1] + (shape[-1] // BLOCK,), dtype=torch.float8_e8m0fnu, device=x.device)
-    call_on(x.device, _lib.lib().ql_quantize_mxfp4, ql_view(x), ql_view(data), ql_view(scales))
+    shape = tuple(input.shape)
+    if not shape or shape[-1] % BLOCK:
+        raise QuantizeError(f"the last dimension must be divisible by {BLOCK}, got shape {shape}.")
+    x, device = input.contiguous(), input.device
+    data = Float4Tensor(torch.empty(x.numel() // 2, dtype=torch.uint8, device=device), shape)
+    scales = torch.empty(*shape[:-1], shape[-1] // BLOCK, dtype=torch.float8_e8m0fnu, device=device)
+    call_on(device, _lib.lib().ql_quantize_mxfp4, ql_view(x), ql_view(data), ql_view(scales))
     return data, scales
 
 
@@ -38,7 +39,7 @@ def dequantize_mxfp4(data: Float4Tensor, scales: torch.Tensor, dtype: dt.dtype =
     require_cuda(scales, "scales")
     if dtype not in dt.QUANTIZABLE_DTYPES:
         raise QuantizeError(f"Unsupported data type in dequantize_mxfp4. Supported data types are: {dt.QUANTIZABLE_DTYPES}. Got dtype={dtype}")
-    y = out if out is not None else torch.empty(data.shape, dtype=dtype.torch, device=data.device)
+    y = out if out is not None else torch.empty(*data.shape, dtype=dtype.torch, device=data.device)
     s = scales.contiguous()   # kept alive across the call: a view only borrows the pointer
     call_on(data.device, _lib.lib().ql_dequantize_mxfp4, ql_view(data), ql_view(s), ql_view(y), same_device=(s, y))
     return y

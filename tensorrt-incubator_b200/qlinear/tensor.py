@@ -54,7 +54,7 @@ class Float4Tensor:
     _VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
     def __init__(self, packed: torch.Tensor, shape):
-        self.shape = tuple(int(s) for s in shape)
+        self.shape = tuple(map(int, shape))
         assert packed.dtype == torch.uint8 and packed.numel() * 2 == math.prod(self.shape)
         self.packed = packed.contiguous()
 
@@ -118,7 +118,8 @@ def call_on(device, fn, *args, same_device=()) -> None:
     for t in same_device:
         if t.device != device:
             raise _lib.QlError(_lib.ERR_INVALID_ARGUMENT, f"tensors must live on one device, got {device} and {t.device}")
-    if device.index is None or device.index == torch.cuda.current_device():
+    index = device.index
+    if index is None or index == torch._C._cuda_getDevice():   # what torch.cuda.current_device() returns, without its start-up check
         rc = fn(*args, current_stream(device))
         if rc != _lib.OK:
             _lib.check(rc)
