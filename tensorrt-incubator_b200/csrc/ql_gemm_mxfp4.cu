@@ -424,42 +424,39 @@ template <bool PAIR> struct TileSmem {
   static constexpr int kTileB = kRowsB * BK_BYTES;
   static constexpr int kStageBytes = kSlotSteps * (MX_A_BYTES + kTileB);  // A's tiles, then B's
   static constexpr int kScales = kStages * kStageBytes;
-  static constexpr int kStaging = kScales + 2 * T_SC_BYTES;   // the epilogue's: 32 rows x 33 words a warp
-  static constexpr int kBarriers = kStaging + 4 * 32 * 33 * 4; // full[S], empty[S], tfull[2], tempty[2], scfull[2], scempty[2], sfull[2], sempty[2], drain
+  static constexpr int kBarriers = kScales + 2 * T_SC_BYTES; // full[S], empty[S], tfull[2], tempty[2], scfull[2], scempty[2], sfull[2], sempty[2], drain
   static constexpr int kTmemPtr = kBarriers + (2 * kStages + 13) * 8;
   static constexpr int kAbort = kTmemPtr + 4;
   static constexpr int kDynamic = kAbort + 4 + 1024;
   static_assert(kDynamic <= 232448 && kStageBytes % 1024 == 0 && T_SC_BYTES % 128 == 0, "tile shape");
 };
 
-// 32 columns (or the first 16) of one accumulator row a lane, rounded to y's type and stored in whole 16-byte pieces
+// `cols` (a multiple of the 16-byte piece, at most 32) columns of one accumulator row a lane, rounded to y's type
 template <typename OutT>
-__device__ __forceinline__ void mx_store_chunk(OutT *y, const uint32_t (&r)[32], bool whole) {
+__device__ __forceinline__ void mx_store_chunk(OutT *y, const uint32_t (&r)[32], int cols) {
   if constexpr (sizeof(OutT) == 4) {
 #pragma unroll
     for (int j = 0; j < 32; j += 4)
-      if (j < 16 || whole) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]));
+      if (j < cols) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]));
   } else {
     auto two = [&](int j) { return pack2<OutT>(__uint_as_float(r[j]), __uint_as_float(r[j + 1])); };
 #pragma unroll
     for (int j = 0; j < 32; j += 8)
-      if (j < 16 || whole) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
+      if (j < cols) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
   }
 }
-// The same 32 x 32 values where rows are not aligned or the chunk is cut: turned in shared memory, so that a warp's store is
-// one row's run of columns.  (A lane storing its own row value by value took 40 us on 333 x 1001 x 2080.)
-__device__ __forceinline__ void mx_store_rows(const MxArgs &args, float *stage, const uint32_t (&r)[32], int m0, int n0, int end, int lane) {
+// TURNED: 32 rows of Y, a lane its column of them, so that a warp's store is a row's run of 32 columns
+template <typename OutT>
+__device__ __forceinline__ void mx_store_turned(OutT *y, const uint32_t (&r)[32], int rows, size_t pitch) {
 #pragma unroll
-  for (int j = 0; j < 32; j++) stage[lane * 33 + j] = __uint_as_float(r[j]);
-  __syncwarp();
-  const int n = n0 + lane;
-#pragma unroll 8
-  for (int i = 0; i < 32; i++)
-    if (m0 + i < args.M && n < end) store_y(args.Y, args.y_dtype, (size_t)(m0 + i) * args.N + n, stage[i * 33 + lane]);
-  __syncwarp();
+  for (int j = 0; j < 32; j++)
+    if (j < rows) y[(size_t)j * pitch] = FloatIO<OutT>::from_f32(__uint_as_float(r[j]));
 }
 
-template <bool PAIR>
+// TURNED: operand a are the weights and operand b the activations (args.M, args.N: rows of a and b; Y is [N, M]).  For rows of
+// Y that are no multiple of 16 bytes, where a lane that holds a row of Y could only store it value by value, far apart:
+// 4571 x 5597 x 160 takes 39 us turned, 88 through a staging buffer in shared memory.
+template <bool PAIR, bool TURNED>
 __global__ void __launch_bounds__(kTileThreads, 1)
 gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sa,
                         const __grid_constant__ CUtensorMap map_sb, const MxArgs args) {
@@ -706,7 +703,6 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
   } else {
     // ------------------------------------------------------------------ epilogue (warps 2..5)
     const int quad = warp & 3;
-    const bool vec = (reinterpret_cast<uintptr_t>(args.Y) & 15) == 0 && args.N % (args.y_dtype == QL_F32 ? 4 : 8) == 0;
     int it = 0;
     for (int tile = first_tile; tile < num_tiles; tile += tile_stride, it++) {
       const int buf = it & 1;
@@ -719,16 +715,17 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
       for (int c = 0; c < (TBN + 31) / 32; c++) {
         uint32_t r[32];
         tmem_load_32(taddr + c * 32, r); // of the last chunk half the columns are the next accumulator's, or scales: not stored
-        const int n = nt * TBN + c * 32, end = min(args.N, nt * TBN + TBN);
-        if (n >= end) break;
-        const bool whole = n + 32 <= end;
-        if (!vec || !(whole || n + 16 == end)) {
-          mx_store_rows(args, reinterpret_cast<float *>(smem + L::kStaging) + quad * 32 * 33, r, m - lane, n, end, lane);
-        } else if (m < args.M) {
-          const size_t at = (size_t)m * (size_t)args.N + n;
-          if (args.y_dtype == QL_F32) mx_store_chunk(static_cast<float *>(args.Y) + at, r, whole);
-          else if (args.y_dtype == QL_F16) mx_store_chunk(static_cast<__half *>(args.Y) + at, r, whole);
-          else mx_store_chunk(static_cast<__nv_bfloat16 *>(args.Y) + at, r, whole);
+        const int n = nt * TBN + c * 32, cols = min(min(args.N, nt * TBN + TBN) - n, 32);
+        if (cols <= 0) break;
+        if (m < args.M) {
+          const size_t at = TURNED ? (size_t)n * (size_t)args.M + m : (size_t)m * (size_t)args.N + n;
+          auto store = [&](auto *y) {
+            if constexpr (TURNED) mx_store_turned(y, r, cols, (size_t)args.M);
+            else mx_store_chunk(y, r, cols);
+          };
+          if (args.y_dtype == QL_F32) store(static_cast<float *>(args.Y) + at);
+          else if (args.y_dtype == QL_F16) store(static_cast<__half *>(args.Y) + at);
+          else store(static_cast<__nv_bfloat16 *>(args.Y) + at);
         }
       }
       tc_fence_before();
@@ -889,10 +886,11 @@ int padded_pitch(int64_t kb) { return (int)((kb + 15) / 16 * 16); }
 bool needs_padding(const MxArgs &args) { return args.kb % 16 != 0 || !aligned16(args.sfa) || !aligned16(args.sfb); }
 int64_t padded_bytes(int64_t M, int64_t N, int64_t kb) { return (M + N) * padded_pitch(kb); }
 
-template <bool PAIR> int launch_tiles(const void *a, const void *b, MxArgs args, int64_t K, void *workspace, cudaStream_t st) {
+// args: operands a and b as the kernel takes them (TURNED: the weights first)
+template <bool PAIR, bool TURNED> int launch_tiles(const void *a, const void *b, MxArgs args, int64_t K, void *workspace, cudaStream_t st) {
   using L = TileSmem<PAIR>;
   static bool configured[64] = {false};
-  int rc = allow_smem(gemm_mxfp4_tiles_kernel<PAIR>, L::kDynamic, configured);
+  int rc = allow_smem(gemm_mxfp4_tiles_kernel<PAIR, TURNED>, L::kDynamic, configured);
   if (rc != QL_OK) return rc;
   int pitch = args.kb;
   if (needs_padding(args)) {
@@ -925,7 +923,7 @@ template <bool PAIR> int launch_tiles(const void *a, const void *b, MxArgs args,
   attr.val.clusterDim.x = PAIR ? 2 : 1, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_mxfp4_tiles_kernel<PAIR>, ma, mb, msa, msb, args));
+  QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_mxfp4_tiles_kernel<PAIR, TURNED>, ma, mb, msa, msb, args));
   count_launches(1);
   return QL_OK;
 }
@@ -983,11 +981,13 @@ extern "C" int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, cons
   if (!args.status) return set_error(QL_ERR_CUDA, "%s: could not allocate the device status word", op);
   // Pairs of the tiles kernel take 4.5 us and 0.45 us per k step and tile of a pair, its single CTAs 0.56; the split kernel what
   // plan_split says.  Up to 32 tokens the tiles are mostly padding and the split kernel is the better one throughout; up to
-  // 128 a pair's second half would be.  128 x 4096 x 4096: split 11.7 us, tiles 12.7; 128 x 28672 x 8192: 45.7, 28.0 (pairs 32);
-  // 512 x 11008 x 4096: single CTAs 21.9, pairs 20.4; 8192 x 28672 x 8192: 920, 800.
-  const bool pairs = M > BM;
-  const int64_t row_tiles = pairs ? (M + 2 * BM - 1) / (2 * BM) : (M + BM - 1) / BM, units = pairs ? sm_count() / 2 : sm_count();
-  const int64_t tiles = row_tiles * ((N + TBN - 1) / TBN);
+  // 128 rows of the first operand a pair's second half would be.  128 x 4096 x 4096: split 11.7 us, tiles 12.7; 128 x 28672 x
+  // 8192: 45.7, 28.0 (pairs 32); 512 x 11008 x 4096: single CTAs 21.9, pairs 20.4; 8192 x 28672 x 8192: 920, 800.
+  const bool turned = N % (y->dtype == QL_F32 ? 4 : 8) != 0 || !aligned16(y->data);
+  const int64_t R = turned ? N : M, C = turned ? M : N; // rows of the tiles kernel's operands
+  const bool pairs = R > BM;
+  const int64_t row_tiles = pairs ? (R + 2 * BM - 1) / (2 * BM) : (R + BM - 1) / BM, units = pairs ? sm_count() / 2 : sm_count();
+  const int64_t tiles = row_tiles * ((C + TBN - 1) / TBN);
   if (tiles >= (1ll << 30)) return set_error(QL_ERR_UNSUPPORTED, "%s: too many output tiles", op);
   const double tiles_us = M <= kSplitOnly ? 1e30 : 4.5 + (need > 0 ? 3.0 : 0.0) + (pairs ? 0.45 : 0.56) * (double)((tiles + units - 1) / units) * args.num_ks;
   args.sfa = static_cast<const uint8_t *>(b_scales->data); // the weights are the 128-row operand of the split kernel
@@ -998,7 +998,11 @@ extern "C" int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, cons
        : M <= 64 ? launch_split<64>(b->data, a->data, args, K, tiles_us, &ran, st)
                  : launch_split<128>(b->data, a->data, args, K, tiles_us, &ran, st);
   if (rc != QL_OK || ran) return rc;
+  if (turned) {
+    args.M = (int)N, args.N = (int)M;
+    return pairs ? launch_tiles<true, true>(b->data, a->data, args, K, workspace, st) : launch_tiles<false, true>(b->data, a->data, args, K, workspace, st);
+  }
   args.sfa = static_cast<const uint8_t *>(a_scales->data);
   args.sfb = static_cast<const uint8_t *>(b_scales->data);
-  return pairs ? launch_tiles<true>(a->data, b->data, args, K, workspace, st) : launch_tiles<false>(a->data, b->data, args, K, workspace, st);
+  return pairs ? launch_tiles<true, false>(a->data, b->data, args, K, workspace, st) : launch_tiles<false, false>(a->data, b->data, args, K, workspace, st);
 }
