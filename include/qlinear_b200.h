@@ -179,8 +179,9 @@ QL_API int ql_gated_linear(const ql_tensor *x, const ql_tensor *w_gate, const ql
 /* Its backward pass: the gradients of x, w_gate and w_up from grad = the gradient of h [M,I], all of x's type.  dx may be
  * null, and so may dw_gate and dw_up together.  Nothing is kept from the forward pass: both projections are computed again;
  * their gradients are formed in f32 and rounded once to x's type as operands of the second products, which sum in f32.
- * `workspace`: 256-byte aligned device memory of at least the bytes the query gives; free again when the call's work on the
- * stream is done.  K and I multiples of 8, 16-byte aligned tensors (QL_ERR_UNSUPPORTED otherwise); M any. */
+ * Results must not overlap inputs.  `workspace`: 256-byte aligned device memory of at least the bytes the query gives; free
+ * again when the call's work on the stream is done.  K and I multiples of 8, 16-byte aligned tensors (QL_ERR_UNSUPPORTED
+ * otherwise); M any. */
 QL_API int ql_gated_linear_backward_workspace(const ql_tensor *x, const ql_tensor *w_gate, int32_t want_dx, int32_t want_dw,
                                               int64_t *bytes);
 QL_API int ql_gated_linear_backward(const ql_tensor *grad, const ql_tensor *x, const ql_tensor *w_gate, const ql_tensor *w_up,

@@ -61,8 +61,9 @@ def test_few_tiles(M, N, K, out):
     assert torch.equal(again, y)   # the same bits on every run
 
 
-# at least 148 tiles of 128 x 224: scales of whole 16-byte rows, and padded ones
-@pytest.mark.parametrize("M,N,K", [(2048, 4096, 512), (1700, 2600, 1056), (4100, 1120, 32), (2048, 2300, 2048), (640, 6700, 4640), (1701, 2601, 1280), (2047, 2305, 11008)])
+# many tiles: scales of whole 16-byte rows and padded ones, rows of Y of whole 16-byte pieces and of odd lengths
+@pytest.mark.parametrize("M,N,K", [(2048, 4096, 512), (1700, 2600, 1056), (4100, 1120, 32), (2048, 2300, 2048), (640, 6700, 4640), (1701, 2601, 1280), (2047, 2305, 11008), (130, 4099, 544), (257, 2001, 1024), (2048, 1000, 4096), (70, 9000, 4096),
+                                   (128, 11000, 8192), (3000, 101, 8192), (33, 9001, 4128), (40000, 101, 1024), (20000, 3, 4096)])
 @pytest.mark.parametrize("out", [torch.float32, torch.float16, torch.bfloat16])
 def test_many_tiles(M, N, K, out):
     a, sa = operand(M, K, 5100 + M)
@@ -136,6 +137,46 @@ def test_streams_capture_and_interleaved_calls():
         torch.cuda.synchronize()
         assert all(torch.equal(outs[i], want[i]) for i in range(2))
     assert ql.lib().ql_gemm_status(None) == 0
+
+
+@pytest.mark.parametrize("N", [32768, 32771])
+def test_offsets_beyond_32_bits(N):
+    """Y of more than 2^31 values, rows of whole 16-byte pieces and odd ones: its last rows are what the same rows alone give
+    (the few rows go through the other kernel: products of one block are exact in f32 either way)."""
+    M, K = 70000, 32
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GB")
+    a, sa = operand(M, K, 5500)
+    b, sb = operand(N, K, 6500)
+    y = ql.gemm_mxfp4(a, sa, b, sb)
+    tail = ql.Float4Tensor(a.packed[-20 * K // 2:], (20, K))
+    assert torch.equal(y[-20:], ql.gemm_mxfp4(tail, sa[-20:], b, sb))
+    assert torch.equal(y[40000:40020], ql.gemm_mxfp4(ql.Float4Tensor(a.packed[40000 * K // 2:40020 * K // 2], (20, K)), sa[40000:40020], b, sb))
+
+
+def test_calls_from_several_threads():
+    """Host threads share nothing but caches: each on its own stream, few rows and many."""
+    import threading
+    shapes = [(1, 500, 1056), (40, 3000, 512), (300, 5000, 288), (300, 5001, 288)]
+    ops = [(operand(M, K, 5600 + i), operand(N, K, 6600 + i, K ** -0.5)) for i, (M, N, K) in enumerate(shapes)]
+    want = [ql.gemm_mxfp4(*a, *b) for a, b in ops]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(seed):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for k in range(12):
+                i = (seed + k) % len(ops)
+                y = ql.gemm_mxfp4(*ops[i][0], *ops[i][1])
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(y, want[i]):
+                    wrong.append(i)
+    threads = [threading.Thread(target=work, args=(s,)) for s in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_empty_and_refused():
