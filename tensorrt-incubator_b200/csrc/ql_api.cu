@@ -59,20 +59,29 @@ int sm_count() {
 
 int *device_status_word() {
   // one word per device, allocated on first use and kept for the life of the process
-  static int *words[64] = {nullptr};
+  static std::atomic<int *> words[64];
+  static std::mutex first_use;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
-  if (!words[dev]) {
-    // the first call may come while a stream is captured: the allocation is no part of what is captured
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    int *word = nullptr;
-    const bool ok = cudaMalloc(&word, sizeof(int)) == cudaSuccess && cudaMemset(word, 0, sizeof(int)) == cudaSuccess;
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    if (!ok) return nullptr;
-    words[dev] = word;
+  if (int *word = words[dev].load(std::memory_order_acquire)) return word;
+  std::lock_guard<std::mutex> lock(first_use);
+  if (int *word = words[dev].load(std::memory_order_relaxed)) return word;
+  // The first call may come while a stream is captured.  The allocation is no part of what is captured, and the word is
+  // cleared on a stream of its own: work on the default stream would end the capture of a stream that synchronises with it.
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  int *word = nullptr;
+  cudaStream_t own = nullptr;
+  const bool ok = cudaMalloc(&word, sizeof(int)) == cudaSuccess && cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking) == cudaSuccess &&
+                  cudaMemsetAsync(word, 0, sizeof(int), own) == cudaSuccess && cudaStreamSynchronize(own) == cudaSuccess;
+  if (own) cudaStreamDestroy(own);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (!ok) {
+    if (word) cudaFree(word);
+    return nullptr;
   }
-  return words[dev];
+  words[dev].store(word, std::memory_order_release);
+  return word;
 }
 
 // kernels (ql_qdq.cu)

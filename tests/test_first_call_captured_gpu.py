@@ -39,3 +39,16 @@ assert ql.lib().ql_gemm_status(None) == 0
 def test_first_call_is_captured(what):
     r = subprocess.run([sys.executable, "-c", PROGRAM, os.path.join(ROOT, "tensorrt-incubator_b200"), what], capture_output=True, text=True, timeout=240)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("what", ["product", "gated"])
+def test_first_call_is_captured_on_a_stream_that_synchronises_with_the_default_one(what):
+    """Such a stream's capture ends where the process touches the default stream meanwhile."""
+    program = PROGRAM.replace("g = torch.cuda.CUDAGraph()", """
+import ctypes
+rt, stream = ctypes.CDLL("libcudart.so.12"), ctypes.c_void_p()
+assert rt.cudaStreamCreate(ctypes.byref(stream)) == 0
+g = torch.cuda.CUDAGraph()""").replace("with torch.cuda.graph(g):", "with torch.cuda.graph(g, stream=torch.cuda.ExternalStream(stream.value)):")
+    assert program.count("ExternalStream") == 1 and program.count("cudaStreamCreate") == 1
+    r = subprocess.run([sys.executable, "-c", program, os.path.join(ROOT, "tensorrt-incubator_b200"), what], capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0, r.stdout + r.stderr
