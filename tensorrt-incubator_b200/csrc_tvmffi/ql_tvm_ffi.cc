@@ -17,7 +17,13 @@
 //   ql_gemm_nvfp4(a_u8, a_scales, a_global | None, b_u8, b_scales, b_global | None, y)
 //   ql_rmsnorm_quant_fp8(x, eps, q, scale)    ql_gemm_fp8_swiglu(xq, wq, sx, sw, act, row_amax)
 //   ql_quantize_rows_fp8(act, row_amax, q, scale)
-// uint8 tensors are raw bytes: e4m3 bit patterns, or two int4 / e2m1 values per byte where the signature says so.
+//   ql_quantize_mxfp4(input, data_u8[..., K/2], scales_u8)       ql_dequantize_mxfp4(data_u8, scales_u8, output)
+//   ql_gemm_mxfp4(a_u8, a_scales_u8, b_u8, b_scales_u8, y, workspace_u8 | None)   ql_gemm_mxfp4_workspace(a_u8, ..., b_scales_u8) -> bytes
+//   ql_gated_linear(x, w_gate, w_up, activation, h)              activation: the number of ql_activation
+//   ql_gated_linear_backward(grad, x, w_gate, w_up, activation, dx | None, dw_gate | None, dw_up | None, workspace_u8 | None)
+//   ql_gated_linear_backward_workspace(x, w_gate, want_dx, want_dw) -> bytes
+// uint8 tensors are raw bytes: e4m3 bit patterns (e8m0 ones: the MXFP4 scales), or two int4 / e2m1 values per byte where the
+// signature says so.
 // Errors become a raised TVM-FFI error (non-zero return), never an abort.
 #include <dlpack/dlpack.h>
 #include <tvm/ffi/c_api.h>
@@ -49,7 +55,9 @@ bool int_arg(const TVMFFIAny &a, int64_t *out) {
   return false;
 }
 
-// DLTensor -> ql_tensor.  `packed` reinterprets a uint8 [..., K/2] tensor as int4 (1) or e2m1 (2) [..., K].
+// DLTensor -> ql_tensor.  `packed` reinterprets a uint8 [..., K/2] tensor as int4 (1) or e2m1 (2) [..., K], or takes uint8 for
+// e8m0 (kE8M0).
+constexpr int kE8M0 = 3;
 bool to_ql(const DLTensor *t, ql_tensor *out, int packed, char *why, size_t why_len) {
   if (!t) {
     snprintf(why, why_len, "expected a tensor argument");
@@ -80,6 +88,8 @@ bool to_ql(const DLTensor *t, ql_tensor *out, int packed, char *why, size_t why_
     else if (d.code == kDLInt && d.bits == 8) q = QL_I8;
     else if (d.code == kDLInt && d.bits == 4) q = QL_I4;
     else if (d.code == kDLFloat8_e4m3fn && d.bits == 8) q = QL_F8E4M3;
+    else if (d.code == kDLFloat8_e8m0fnu && d.bits == 8) q = QL_F8E8M0;
+    else if (d.code == kDLUInt && d.bits == 8 && packed == kE8M0) q = QL_F8E8M0;
     else if (d.code == kDLUInt && d.bits == 8) q = packed == 1 ? QL_I4 : packed == 2 ? QL_F4E2M1 : QL_F8E4M3; // raw bytes
   }
   if (q < 0) {
@@ -90,11 +100,25 @@ bool to_ql(const DLTensor *t, ql_tensor *out, int packed, char *why, size_t why_
   out->dtype = q;
   out->rank = t->ndim;
   for (int i = 0; i < t->ndim; i++) out->shape[i] = t->shape[i];
-  if (packed && d.code == kDLUInt && t->ndim >= 1) out->shape[t->ndim - 1] *= 2;
+  if (packed && packed != kE8M0 && d.code == kDLUInt && t->ndim >= 1) out->shape[t->ndim - 1] *= 2;
   return true;
 }
 
 void *stream_of(const DLTensor *t) { return TVMFFIEnvGetStream(t->device.device_type, t->device.device_id); }
+
+// bytes of a workspace given as a tensor of bytes (none: 0)
+int64_t byte_count(const ql_tensor *t) {
+  int64_t n = t ? 1 : 0;
+  for (int i = 0; t && i < t->rank; i++) n *= t->shape[i];
+  return t && (t->dtype == QL_F8E4M3 || t->dtype == QL_I8) ? n : 0;
+}
+
+int int_result(TVMFFIAny *ret, int64_t v) {
+  ret->type_index = kTVMFFIInt;
+  ret->zero_padding = 0;
+  ret->v_int64 = v;
+  return 0;
+}
 
 int finish(int rc) {
   if (rc == QL_OK) return 0;
@@ -273,5 +297,87 @@ TVM_FFI_DLL_EXPORT int __tvm_ffi_ql_quantize_rows_fp8(void *, const TVMFFIAny *a
   QL_TENSOR(2, q, 0)
   QL_TENSOR(3, scale, 0)
   return finish(ql_quantize_rows_fp8(&a, &amax, &q, &scale, stream_of(a_dl)));
+}
+
+TVM_FFI_DLL_EXPORT int __tvm_ffi_ql_quantize_mxfp4(void *, const TVMFFIAny *args, int32_t n, TVMFFIAny *) {
+  char why[160];
+  if (n != 3) return fail("expected (input, data, scales)");
+  QL_TENSOR(0, in, 0)
+  QL_TENSOR(1, data, 2)
+  QL_TENSOR(2, scales, kE8M0)
+  return finish(ql_quantize_mxfp4(&in, &data, &scales, stream_of(in_dl)));
+}
+
+TVM_FFI_DLL_EXPORT int __tvm_ffi_ql_dequantize_mxfp4(void *, const TVMFFIAny *args, int32_t n, TVMFFIAny *) {
+  char why[160];
+  if (n != 3) return fail("expected (data, scales, output)");
+  QL_TENSOR(0, data, 2)
+  QL_TENSOR(1, scales, kE8M0)
+  QL_TENSOR(2, out, 0)
+  return finish(ql_dequantize_mxfp4(&data, &scales, &out, stream_of(data_dl)));
+}
+
+TVM_FFI_DLL_EXPORT int __tvm_ffi_ql_gemm_mxfp4_workspace(void *, const TVMFFIAny *args, int32_t n, TVMFFIAny *ret) {
+  char why[160];
+  if (n != 4) return fail("expected (a, a_scales, b, b_scales)");
+  QL_TENSOR(0, a, 2)
+  QL_TENSOR(1, sa, kE8M0)
+  QL_TENSOR(2, b, 2)
+  QL_TENSOR(3, sb, kE8M0)
+  int64_t bytes = 0;
+  const int rc = finish(ql_gemm_mxfp4_workspace(&a, &sa, &b, &sb, &bytes));
+  return rc == 0 ? int_result(ret, bytes) : rc;
+}
+
+TVM_FFI_DLL_EXPORT int __tvm_ffi_ql_gemm_mxfp4(void *, const TVMFFIAny *args, int32_t n, TVMFFIAny *) {
+  char why[160];
+  if (n != 6) return fail("expected (a, a_scales, b, b_scales, y, workspace | None)");
+  QL_TENSOR(0, a, 2)
+  QL_TENSOR(1, sa, kE8M0)
+  QL_TENSOR(2, b, 2)
+  QL_TENSOR(3, sb, kE8M0)
+  QL_TENSOR(4, y, 0)
+  QL_OPTIONAL(5, ws)
+  return finish(ql_gemm_mxfp4(&a, &sa, &b, &sb, &y, ws_p ? ws.data : nullptr, byte_count(ws_p), stream_of(a_dl)));
+}
+
+TVM_FFI_DLL_EXPORT int __tvm_ffi_ql_gated_linear(void *, const TVMFFIAny *args, int32_t n, TVMFFIAny *) {
+  char why[160];
+  if (n != 5) return fail("expected (x, w_gate, w_up, activation, h)");
+  QL_TENSOR(0, x, 0)
+  QL_TENSOR(1, wg, 0)
+  QL_TENSOR(2, wu, 0)
+  int64_t act;
+  if (!int_arg(args[3], &act)) return fail("activation must be an integer");
+  QL_TENSOR(4, h, 0)
+  return finish(ql_gated_linear(&x, &wg, &wu, (int32_t)act, &h, stream_of(x_dl)));
+}
+
+TVM_FFI_DLL_EXPORT int __tvm_ffi_ql_gated_linear_backward_workspace(void *, const TVMFFIAny *args, int32_t n, TVMFFIAny *ret) {
+  char why[160];
+  if (n != 4) return fail("expected (x, w_gate, want_dx, want_dw)");
+  QL_TENSOR(0, x, 0)
+  QL_TENSOR(1, wg, 0)
+  int64_t want_dx, want_dw, bytes = 0;
+  if (!int_arg(args[2], &want_dx) || !int_arg(args[3], &want_dw)) return fail("want_dx and want_dw must be integers");
+  const int rc = finish(ql_gated_linear_backward_workspace(&x, &wg, want_dx != 0, want_dw != 0, &bytes));
+  return rc == 0 ? int_result(ret, bytes) : rc;
+}
+
+TVM_FFI_DLL_EXPORT int __tvm_ffi_ql_gated_linear_backward(void *, const TVMFFIAny *args, int32_t n, TVMFFIAny *) {
+  char why[160];
+  if (n != 9) return fail("expected (grad, x, w_gate, w_up, activation, dx | None, dw_gate | None, dw_up | None, workspace | None)");
+  QL_TENSOR(0, grad, 0)
+  QL_TENSOR(1, x, 0)
+  QL_TENSOR(2, wg, 0)
+  QL_TENSOR(3, wu, 0)
+  int64_t act;
+  if (!int_arg(args[4], &act)) return fail("activation must be an integer");
+  QL_OPTIONAL(5, dx)
+  QL_OPTIONAL(6, dwg)
+  QL_OPTIONAL(7, dwu)
+  QL_OPTIONAL(8, ws)
+  return finish(ql_gated_linear_backward(&grad, &x, &wg, &wu, (int32_t)act, dx_p ? &dx : nullptr, dwg_p ? &dwg : nullptr, dwu_p ? &dwu : nullptr, ws_p ? ws.data : nullptr,
+                                         byte_count(ws_p), stream_of(x_dl)));
 }
 }

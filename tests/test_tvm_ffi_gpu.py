@@ -116,3 +116,58 @@ def test_linear_matmul_nvfp4_and_mlp_stages_through_tvm_ffi():
     assert torch.equal(act, wact) and torch.equal(amax, wamax) and torch.equal(aq, waq.view(torch.uint8)) and torch.equal(sa2, wsa)
     with pytest.raises(Exception, match="expected"):
         mod.ql_matmul(x, x)
+
+
+def test_plugin_exports_the_microscaled_and_gated_functions():
+    if not os.path.exists(PLUGIN):
+        pytest.skip("plug-in not built (tvm_ffi headers missing at build time)")
+    import ctypes
+    L = ctypes.CDLL(PLUGIN)
+    for name in ("ql_quantize_mxfp4", "ql_dequantize_mxfp4", "ql_gemm_mxfp4", "ql_gemm_mxfp4_workspace", "ql_gated_linear",
+                 "ql_gated_linear_backward", "ql_gated_linear_backward_workspace"):
+        assert hasattr(L, "__tvm_ffi_" + name)
+
+
+@pytest.mark.gpu
+def test_mxfp4_and_gated_projection_through_tvm_ffi():
+    """Same bits as the operator layer, with the workspaces a caller allocates from the queries."""
+    if not os.path.exists(PLUGIN):
+        pytest.skip("plug-in not built")
+    mod = tvm_ffi.load_module(PLUGIN)
+    g = torch.Generator(device="cpu").manual_seed(23)
+    u8 = lambda *shape: torch.empty(shape, dtype=torch.uint8, device="cuda")
+    a = torch.randn((40, 96), generator=g).to(torch.bfloat16).cuda()
+    b = torch.randn((72, 96), generator=g).to(torch.bfloat16).cuda()
+    qa, sa, qb, sb = u8(40, 48), u8(40, 3), u8(72, 48), u8(72, 3)
+    mod.ql_quantize_mxfp4(a, qa, sa)
+    mod.ql_quantize_mxfp4(b, qb, sb)
+    n = mod.ql_gemm_mxfp4_workspace(qa, sa, qb, sb)
+    assert n > 0   # rows of three scale bytes
+    y, back = torch.empty((40, 72), device="cuda"), torch.empty((40, 96), dtype=torch.float16, device="cuda")
+    mod.ql_gemm_mxfp4(qa, sa, qb, sb, y, u8(n))
+    mod.ql_dequantize_mxfp4(qa, sa, back)
+    fa, fsa = ql.quantize_mxfp4(a)
+    fb, fsb = ql.quantize_mxfp4(b)
+    assert torch.equal(qa.reshape(-1), fa.packed.reshape(-1)) and torch.equal(sa, fsa.view(torch.uint8))
+    assert torch.equal(y, ql.gemm_mxfp4(fa, fsa, fb, fsb, ql.float32)) and torch.equal(back, ql.dequantize_mxfp4(fa, fsa, ql.float16))
+    with pytest.raises(Exception, match="needs a workspace"):
+        mod.ql_gemm_mxfp4(qa, sa, qb, sb, y, None)
+    one = torch.empty((1, 72), dtype=torch.bfloat16, device="cuda")
+    mod.ql_gemm_mxfp4(qa[:1], sa[:1], qb, sb, one, None)   # one token needs none
+    assert torch.equal(one, ql.gemm_mxfp4(ql.Float4Tensor(qa[:1].reshape(-1), (1, 96)), fsa[:1], fb, fsb))
+
+    x = torch.randn((24, 64), generator=g).to(torch.float16).cuda()
+    wg, wu = (torch.randn((2, 136, 64), generator=g) / 8).to(torch.float16).cuda()
+    dh = torch.randn((24, 136), generator=g).to(torch.float16).cuda()
+    h, dx, dwg, dwu = torch.empty_like(dh), torch.empty_like(x), torch.empty_like(wg), torch.empty_like(wu)
+    mod.ql_gated_linear(x, wg, wu, 1, h)
+    ws = u8(mod.ql_gated_linear_backward_workspace(x, wg, 1, 1))
+    mod.ql_gated_linear_backward(dh, x, wg, wu, 1, dx, dwg, dwu, ws)
+    assert torch.equal(h, ql.gated_linear(x, wg, wu, "gelu"))
+    for got, want in zip((dx, dwg, dwu), ql.gated_linear_backward(dh, x, wg, wu, "gelu")):
+        assert torch.equal(got, want)
+    dx.zero_()
+    mod.ql_gated_linear_backward(dh, x, wg, wu, 1, dx, None, None, u8(mod.ql_gated_linear_backward_workspace(x, wg, 1, 0)))
+    assert torch.equal(dx, ql.gated_linear_backward(dh, x, wg, wu, "gelu", need_weight_grad=False)[0])
+    with pytest.raises(Exception, match="unknown activation"):
+        mod.ql_gated_linear(x, wg, wu, 9, h)
