@@ -150,16 +150,17 @@ QL_API int ql_gemm_nvfp4(const ql_tensor *a, const ql_tensor *a_scales, const ql
  * a NaN gets the scale NaN and zero data: it dequantizes to NaN.  input: f32 | f16 | bf16 [..., K], K % 32 == 0;
  * data: QL_F4E2M1 of the input's shape (buffer of numel / 2 bytes); scales: QL_F8E8M0 [..., K / 32].
  * ql_dequantize_mxfp4: output = data * scale, rounded to f32 | f16 | bf16.
- * 16-byte aligned floating-point buffers and 4-byte aligned data (QL_ERR_UNSUPPORTED otherwise). */
+ * 16-byte aligned floating-point buffers and 4-byte aligned data (QL_ERR_UNSUPPORTED otherwise); results overlap nothing
+ * else (QL_ERR_INVALID_ARGUMENT, as in the three entries below). */
 QL_API int ql_quantize_mxfp4(const ql_tensor *input, ql_tensor *data, ql_tensor *scales, void *stream);
 QL_API int ql_dequantize_mxfp4(const ql_tensor *data, const ql_tensor *scales, ql_tensor *output, void *stream);
 
 /* Block-scaled MXFP4 product: Y[M,N] = dq(a)[M,K] . dq(b)[N,K]^T of operands as ql_quantize_mxfp4 writes them, the block
  * scales applied by the tensor core (tcgen05.mma kind::mxf4, f32 accumulation), one rounding to y's type.  a, b: QL_F4E2M1
- * [M,K], [N,K], 16-byte aligned; *_scales: QL_F8E8M0 [rows, K/32], 4-byte aligned; y: f32 | f16 | bf16.  K > 0, K % 32 == 0; M and N any.  A NaN
- * scale makes its row (a) or column (b) of Y NaN.  `workspace`: 16-byte aligned device memory of at least the bytes the query
- * gives (0 for most calls: it holds a padded copy of scales whose rows are no multiple of 16 bytes or not aligned, of more
- * than 32 tokens); free again when the call's work on the stream is done. */
+ * [M,K], [N,K], 16-byte aligned; *_scales: QL_F8E8M0 [rows, K/32], 4-byte aligned; y: f32 | f16 | bf16.  K > 0, K % 32 == 0;
+ * M and N any.  A NaN scale makes its row (a) or column (b) of Y NaN.  `workspace`: 16-byte aligned device memory of at least
+ * the bytes the query gives (0 for most calls: it holds a padded copy of scales whose rows are no multiple of 16 bytes or not
+ * aligned, of more than 32 tokens); free again when the call's work on the stream is done. */
 QL_API int ql_gemm_mxfp4_workspace(const ql_tensor *a, const ql_tensor *a_scales, const ql_tensor *b, const ql_tensor *b_scales,
                                    int64_t *bytes);
 QL_API int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, const ql_tensor *b, const ql_tensor *b_scales,
@@ -167,7 +168,8 @@ QL_API int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, const ql
 
 /* Gated projection of a feed-forward block in 16 bits (the unquantized counterpart of ql_gemm_fp8_swiglu):
  *   h[M,I] = act(x w_gate^T) * (x w_up^T),   x [M,K], w_gate and w_up [I,K] (Linear's [out, in] layout), all f16 or all bf16,
- * both products, the activation and the gate's product in one kernel, from f32 sums with one rounding. */
+ * both products, the activation and the gate's product in one kernel, from f32 sums with one rounding.  K and I multiples of
+ * 8, 16-byte aligned tensors (QL_ERR_UNSUPPORTED otherwise), here and in the backward pass; M any. */
 typedef enum {
   QL_ACT_SILU = 0,      /* z / (1 + e^-z) */
   QL_ACT_GELU = 1,      /* z Phi(z) */
@@ -179,9 +181,8 @@ QL_API int ql_gated_linear(const ql_tensor *x, const ql_tensor *w_gate, const ql
 /* Its backward pass: the gradients of x, w_gate and w_up from grad = the gradient of h [M,I], all of x's type.  dx may be
  * null, and so may dw_gate and dw_up together.  Nothing is kept from the forward pass: both projections are computed again;
  * their gradients are formed in f32 and rounded once to x's type as operands of the second products, which sum in f32.
- * Results must not overlap inputs.  `workspace`: 256-byte aligned device memory of at least the bytes the query gives; free
- * again when the call's work on the stream is done.  K and I multiples of 8, 16-byte aligned tensors (QL_ERR_UNSUPPORTED
- * otherwise); M any. */
+ * `workspace`: 256-byte aligned device memory of at least the bytes the query gives; free again when the call's work on the
+ * stream is done. */
 QL_API int ql_gated_linear_backward_workspace(const ql_tensor *x, const ql_tensor *w_gate, int32_t want_dx, int32_t want_dw,
                                               int64_t *bytes);
 QL_API int ql_gated_linear_backward(const ql_tensor *grad, const ql_tensor *x, const ql_tensor *w_gate, const ql_tensor *w_up,

@@ -36,6 +36,16 @@ static inline int64_t numel(const ql_tensor *t) {
 static inline bool is_float_dtype(int d) { return d == QL_F32 || d == QL_F16 || d == QL_BF16; }
 static inline bool is_quant_dtype(int d) { return d == QL_I8 || d == QL_I4 || d == QL_F8E4M3; }
 static inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static inline int64_t byte_size(const ql_tensor *t) {
+  const int bits = t->dtype == QL_F32 ? 32 : (t->dtype == QL_F16 || t->dtype == QL_BF16 ? 16 : (t->dtype == QL_I4 || t->dtype == QL_F4E2M1 ? 4 : 8));
+  return (numel(t) * bits + 7) / 8;
+}
+// Do two tensors share memory?  A null or an empty one shares none.
+static inline bool overlap(const ql_tensor *a, const ql_tensor *b) {
+  if (!a || !b || byte_size(a) == 0 || byte_size(b) == 0) return false;
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a->data), pb = reinterpret_cast<uintptr_t>(b->data);
+  return pa < pb + (uintptr_t)byte_size(b) && pb < pa + (uintptr_t)byte_size(a);
+}
 
 // Where the scale of element i lives:  idx(i) = ((i / a) % b) * c + (i % d) / e
 //   per-tensor            a=1 b=1 c=0 d=1 e=1

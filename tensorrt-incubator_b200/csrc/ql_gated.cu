@@ -76,10 +76,11 @@ template <int ACT> __device__ __forceinline__ void act_both(float z, float &a, f
   } else if constexpr (ACT == ACT_GELU_TANH) {
     const float s = __fdividef(1.f, 1.f + __expf(-1.5957691f * (z + 0.044715f * z * z * z)));
     a = z * s;
-    d = s + z * s * (1.f - s) * 1.5957691f * (1.f + 0.134145f * z * z);
+    const float b = fminf(fmaxf(z, -32.f), 32.f); // beyond, s (1 - s) is 0 in f32, and z^2 need not be finite; a NaN is s's too
+    d = s + b * s * (1.f - s) * 1.5957691f * (1.f + 0.134145f * b * b);
   } else {
     a = z < 0.f ? 0.f : z;
-    d = z > 0.f ? 1.f : 0.f;
+    d = z > 0.f ? 1.f : a; // 0, or z's NaN
   }
 }
 // f(activation as a template argument), chosen once for a whole chunk of values
@@ -1076,6 +1077,7 @@ extern "C" int ql_gated_linear(const ql_tensor *x, const ql_tensor *w_gate, cons
   const int M = (int)x->shape[0], K = (int)x->shape[1], I = (int)w_gate->shape[0];
   cudaStream_t st = (cudaStream_t)stream;
   if (M == 0 || I == 0) return QL_OK;
+  if (overlap(h, x) || overlap(h, w_gate) || overlap(h, w_up)) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: h must not overlap an operand", op);
   if (K == 0) { // act(0) * 0
     QL_CUDA_TRY(cudaMemsetAsync(h->data, 0, (size_t)numel(h) * 2, st));
     return QL_OK;
@@ -1123,6 +1125,13 @@ extern "C" int ql_gated_linear_backward(const ql_tensor *grad, const ql_tensor *
   if ((rc = ql_gated_linear_backward_workspace(x, w_gate, dx != nullptr, dw_gate != nullptr, &need)) != QL_OK) return rc;
   if (!workspace || workspace_bytes < need) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %lld bytes, got %lld", op, (long long)need, (long long)(workspace ? workspace_bytes : 0));
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return set_error(QL_ERR_UNSUPPORTED, "%s: the workspace must be 256-byte aligned", op);
+  const ql_tensor *in[4] = {grad, x, w_gate, w_up};
+  for (int i = 0; i < 3; i++) {
+    for (int j = 0; j < 4; j++)
+      if (overlap(out[i], in[j])) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: %s must not overlap an operand", op, name[i]);
+    for (int j = 0; j < i; j++)
+      if (overlap(out[i], out[j])) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: %s and %s must not overlap", op, name[j], name[i]);
+  }
   if (!device_status_word()) return set_error(QL_ERR_CUDA, "%s: could not allocate the device status word", op);
   const GradPlan plan = plan_grads(M, I, K, dx != nullptr, dw_gate != nullptr, pairs_of(x->dtype));
   void *p[3] = {dx ? dx->data : nullptr, dw_gate ? dw_gate->data : nullptr, dw_up ? dw_up->data : nullptr};

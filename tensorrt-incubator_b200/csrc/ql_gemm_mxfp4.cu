@@ -967,6 +967,7 @@ extern "C" int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, cons
   if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(QL_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %lld bytes, got %lld", op, (long long)need, (long long)(workspace ? workspace_bytes : 0));
   if (need > 0 && !aligned16(workspace)) return set_error(QL_ERR_UNSUPPORTED, "%s: the workspace must be 16-byte aligned", op);
+  if (overlap(y, a) || overlap(y, a_scales) || overlap(y, b) || overlap(y, b_scales)) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: y must not overlap an operand", op);
   cudaStream_t st = (cudaStream_t)stream;
 
   MxArgs args;

@@ -166,6 +166,7 @@ extern "C" int ql_quantize_mxfp4(const ql_tensor *input, ql_tensor *data, ql_ten
   if (rc != QL_OK) return rc;
   const int64_t n8 = numel(input) / 8;
   if (n8 == 0) return QL_OK;
+  if (overlap(data, input) || overlap(scales, input) || overlap(data, scales)) return set_error(QL_ERR_INVALID_ARGUMENT, "quantize_mxfp4: input and results must not overlap");
   cudaStream_t st = (cudaStream_t)stream;
   uint32_t *q = static_cast<uint32_t *>(data->data);
   uint8_t *s = static_cast<uint8_t *>(scales->data);
@@ -182,6 +183,7 @@ extern "C" int ql_dequantize_mxfp4(const ql_tensor *data, const ql_tensor *scale
   if (rc != QL_OK) return rc;
   const int64_t n8 = numel(output) / 8;
   if (n8 == 0) return QL_OK;
+  if (overlap(output, data) || overlap(output, scales)) return set_error(QL_ERR_INVALID_ARGUMENT, "dequantize_mxfp4: output must not overlap data or scales");
   cudaStream_t st = (cudaStream_t)stream;
   const uint32_t *q = static_cast<const uint32_t *>(data->data);
   const uint8_t *s = static_cast<const uint8_t *>(scales->data);

@@ -45,7 +45,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
     act = _activation(activation)
     x2 = _rows(x, "x")
     wg, wu = w_gate.contiguous(), w_up.contiguous()   # kept alive across the call: a view only borrows the pointer
-    rows, I = x2.shape[0], wg.shape[0]
+    rows, I = x2.shape[0], wg.shape[0] if wg.dim() else 0   # what is no matrix the entry refuses
     if out is None:
         h = torch.empty(rows, I, dtype=x.dtype, device=x.device)
     else:

@@ -56,6 +56,8 @@ def gemm_mxfp4(a: Float4Tensor, a_scales: torch.Tensor, b: Float4Tensor, b_scale
         raise QuantizeError("gemm_mxfp4: a and b must be Float4Tensor, as quantize_mxfp4 returns them")
     if out is None and out_dtype not in dt.QUANTIZABLE_DTYPES:
         raise QuantizeError(f"Unsupported data type in gemm_mxfp4. Supported data types are: {dt.QUANTIZABLE_DTYPES}. Got out_dtype={out_dtype}")
+    if len(a.shape) != 2 or len(b.shape) != 2 or a_scales.dim() != 2 or b_scales.dim() != 2:
+        raise QuantizeError("gemm_mxfp4: data and scales must be 2-D")
     y = out if out is not None else torch.empty(a.shape[0], b.shape[0], dtype=out_dtype.torch, device=a.device)
     # dense, on a multiple of 4 bytes (a slice of rows need not be); kept alive across the call: a view only borrows the pointer
     sa, sb = (s if s.data_ptr() % 4 == 0 else s.clone() for s in (a_scales.contiguous(), b_scales.contiguous()))

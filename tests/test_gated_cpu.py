@@ -79,3 +79,21 @@ def test_backward_argument_rules():
     assert L.ql_gated_linear_backward_workspace(_t(B, [0, 16], None), t["wg"], 1, 1, ctypes.byref(n)) == 0 and n.value == 0
     assert "needs x" in _err(L.ql_gated_linear_backward_workspace(None, t["wg"], 1, 1, ctypes.byref(n)))
     assert call(dx=None, dg=None, du=None) == 0   # nothing asked for
+
+
+def test_results_that_share_memory_are_refused():
+    """Addresses only: the refusals come before anything is launched."""
+    L = _lib.lib()
+    x, wg, wu = _t(B, [4, 16], 0x10000), _t(B, [8, 16], 0x20000), _t(B, [8, 16], 0x30000)
+    for ptr in (0x10000, 0x10000 + 4 * 16 * 2 - 16, 0x20000 - 16, 0x30000 + 8 * 16 * 2 - 16):
+        assert "h must not overlap an operand" in _err(L.ql_gated_linear(x, wg, wu, 0, _t(B, [4, 8], ptr), None))
+    n = ctypes.c_int64()
+    assert L.ql_gated_linear_backward_workspace(x, wg, 1, 1, ctypes.byref(n)) == 0
+
+    def call(dx=0x50000, dwg=0x60000, dwu=0x70000):
+        return L.ql_gated_linear_backward(_t(B, [4, 8], 0x40000), x, wg, wu, 0, _t(B, [4, 16], dx), _t(B, [8, 16], dwg), _t(B, [8, 16], dwu), 0x100000, n.value, None)
+    assert "dx must not overlap an operand" in _err(call(dx=0x10000))
+    assert "dw_gate must not overlap an operand" in _err(call(dwg=0x40000))
+    assert "dw_up must not overlap an operand" in _err(call(dwu=0x30000 - 16))
+    assert "dw_gate and dw_up must not overlap" in _err(call(dwu=0x60000))
+    assert "dx and dw_gate must not overlap" in _err(call(dx=0x60010))

@@ -295,3 +295,52 @@ def test_refusals():
         ql.gated_linear_backward(torch.ones((4, 16), dtype=torch.bfloat16, device="cuda"), x, w, w)
     with pytest.raises(ql.QlError, match="16-byte aligned"):
         ql.gated_linear(torch.ones(4 * 16 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(4, 16), w, w)
+
+
+@pytest.mark.parametrize("M", [21, 300])
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh", "relu"])
+def test_gates_of_every_size(activation, M):
+    """One channel whose gate and up are values of x themselves, so that G and U are exact: gates from 2^-20 to 2^66, where a
+    square is no f32 any more.  h is rounded once, dG and dU once and then again, unchanged, as the one term of dX's sum.  In
+    f32 before that: a few ulp, of an exponential of up to 80 about 80 2^-23, far below the rounding's 2^-8; beyond 80 the true
+    values are below 2^-110."""
+    z = torch.tensor([s * v for v in (2.0 ** -20, 0.25, 1.0, 2.5, 6.0, 12.0, 40.0, 80.0, 2.0 ** 20, 2.0 ** 66) for s in (1, -1)] + [0.0])
+    z = z.repeat(-(-M // len(z)))[:M].double()
+    x, wg, wu = torch.zeros(M, 8, dtype=torch.bfloat16, device="cuda"), *torch.zeros(2, 8, 8, dtype=torch.bfloat16, device="cuda")
+    x[:, 0], x[:, 1], wg[0, 0], wu[0, 1] = z.to(torch.bfloat16).cuda(), 1.5, 1.0, 1.0
+    grad = torch.zeros(M, 8, dtype=torch.bfloat16, device="cuda")
+    grad[:, 0] = 0.75
+    z = x[:, 0].double().cpu()
+    if activation == "silu":
+        s = 1 / (1 + torch.exp(-z))
+        a, d = z * s, s + z * s * (1 / (1 + torch.exp(z)))
+    elif activation == "gelu":
+        c = torch.special.erfc(-z / 2 ** 0.5) / 2
+        a, d = z * c, c + z * torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5
+    elif activation == "gelu_tanh":
+        k = (2 / torch.pi) ** 0.5
+        y = 2 * k * (z + 0.044715 * z ** 3)
+        s = 1 / (1 + torch.exp(-y))
+        a, d = z * s, s + torch.where(z.abs() < 1e3, z * s / (1 + torch.exp(y)) * 2 * k * (1 + 0.134145 * z * z), torch.zeros_like(z))
+    else:
+        a, d = z.clamp(min=0), (z > 0).double()
+    h = ql.gated_linear(x, wg, wu, activation)[:, 0].double().cpu()
+    dx = ql.gated_linear_backward(grad, x, wg, wu, activation, need_weight_grad=False)[0].double().cpu()
+    close = lambda got, want: torch.allclose(got, want, rtol=2.0 ** -8 + 2.0 ** -12, atol=2.0 ** -108)
+    assert close(h, 1.5 * a)
+    assert close(dx[:, 0], 0.75 * 1.5 * d)
+    assert close(dx[:, 1], 0.75 * a)
+
+
+@pytest.mark.parametrize("M", [16, 300])
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh", "relu"])
+def test_a_nan_weight_spoils_its_channel_only(activation, M):
+    x, wg, wu = randn((M, 16), torch.float16, 8500), randn((24, 16), torch.float16, 8501, 0.25), randn((24, 16), torch.float16, 8502, 0.25)
+    grad = randn((M, 24), torch.float16, 8503)
+    wg[5, 3] = float("nan")
+    h = ql.gated_linear(x, wg, wu, activation)
+    _, dwg, dwu = ql.gated_linear_backward(grad, x, wg, wu, activation, need_input_grad=False)
+    channel = torch.arange(24, device="cuda") == 5
+    assert torch.equal(h.isnan(), channel.expand(M, 24))
+    for g in (dwg, dwu):
+        assert torch.equal(g.isnan(), channel[:, None].expand(24, 16))

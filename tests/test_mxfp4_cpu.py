@@ -92,3 +92,27 @@ def test_product_argument_rules():
     assert "16-byte aligned" in _err(call(**many, y=y, ws=0x1008, n=768))
     assert L.ql_gemm_mxfp4_workspace(a, sa, b, sb, ctypes.byref(size)) == 0 and size.value == 0
     assert "no place for the size" in _err(L.ql_gemm_mxfp4_workspace(a, sa, b, sb, None))
+
+
+def test_results_that_share_memory_are_refused():
+    """Addresses only: the refusals come before anything is launched."""
+    L = _lib.lib()
+    x, q, s = _t(_lib.F32, [4, 64], 0x10000), _t(_lib.F4E2M1, [4, 64], 0x20000), _t(_lib.F8E8M0, [4, 2], 0x30000)
+    assert "must not overlap" in _err(L.ql_quantize_mxfp4(x, _t(_lib.F4E2M1, [4, 64], 0x10000), s, None))
+    assert "must not overlap" in _err(L.ql_quantize_mxfp4(x, q, _t(_lib.F8E8M0, [4, 2], 0x10000 + 1023), None))
+    assert "must not overlap" in _err(L.ql_quantize_mxfp4(x, q, _t(_lib.F8E8M0, [4, 2], 0x20000 + 127), None))
+    assert "must not overlap" in _err(L.ql_dequantize_mxfp4(q, s, _t(_lib.F32, [4, 64], 0x20000 - 512), None))
+    assert "must not overlap" in _err(L.ql_dequantize_mxfp4(q, s, _t(_lib.BF16, [4, 64], 0x30000), None))
+    b, sb = _t(_lib.F4E2M1, [8, 64], 0x40000), _t(_lib.F8E8M0, [8, 2], 0x50000)
+    for ptr in (0x20000, 0x30000, 0x40000 + 256 - 2, 0x50000 - 62):
+        assert "must not overlap" in _err(L.ql_gemm_mxfp4(q, s, b, sb, _t(_lib.BF16, [4, 8], ptr), None, 0, None))
+
+
+def test_python_layer_refuses_scales_of_other_ranks():
+    class OnGpu(ql.Float4Tensor):   # passes for one in GPU memory; the refusal comes before anything is read
+        device = torch.device("cuda", 0)
+    a = OnGpu(torch.zeros(64, dtype=torch.uint8), (4, 32))
+    s = torch.zeros(4, 1, dtype=torch.uint8).view(torch.float8_e8m0fnu)
+    for bad in ((a, s.view(4), a, s), (a, s, a, s[0, 0])):
+        with pytest.raises(ql.QuantizeError, match="must be 2-D"):
+            ql.gemm_mxfp4(*bad)
