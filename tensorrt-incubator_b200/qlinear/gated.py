@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from .ops import QuantizeError
-from .tensor import call_on, ql_view, require_cuda
+from .tensor import call_on, empty, ql_view, require_cuda
 
 
 def _activation(name: str) -> int:
@@ -47,7 +47,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
     wg, wu = w_gate.contiguous(), w_up.contiguous()   # kept alive across the call: a view only borrows the pointer
     rows, I = x2.shape[0], wg.shape[0] if wg.dim() else 0   # what is no matrix the entry refuses
     if out is None:
-        h = torch.empty(rows, I, dtype=x.dtype, device=x.device)
+        h = empty((rows, I), x.dtype, x.device)
     else:
         if tuple(out.shape) != tuple(x.shape[:-1]) + (I,):
             raise QuantizeError(f"out must have shape {tuple(x.shape[:-1]) + (I,)}, got {tuple(out.shape)}.")
@@ -68,16 +68,17 @@ def gated_linear_backward(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Ten
     if grad.shape[:-1] != x.shape[:-1]:
         raise QuantizeError(f"grad and x must have the same leading dimensions, got {tuple(grad.shape)} and {tuple(x.shape)}.")
     wg, wu = w_gate.contiguous(), w_up.contiguous()
-    dx = torch.empty(x2.shape, dtype=x.dtype, device=x.device) if need_input_grad else None
-    dwg = torch.empty(wg.shape, dtype=x.dtype, device=x.device) if need_weight_grad else None
-    dwu = torch.empty(wu.shape, dtype=x.dtype, device=x.device) if need_weight_grad else None
+    dtype, device = x.dtype, x.device
+    dx = empty(x2.shape, dtype, device) if need_input_grad else None
+    dwg = empty(wg.shape, dtype, device) if need_weight_grad else None
+    dwu = empty(wu.shape, dtype, device) if need_weight_grad else None
     vx, vg = ql_view(x2), ql_view(wg)
     out = [ql_view(t) if t is not None else None for t in (dx, dwg, dwu)]
     L = _lib.lib()
 
     def run(stream):   # with the tensors' device current: the plan behind the workspace's size depends on the device
-        size = _workspace_bytes(tuple(x2.shape), tuple(wg.shape), vx.dtype, need_input_grad, need_weight_grad, x.device.index)
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        size = _workspace_bytes(x2.shape, wg.shape, vx.dtype, need_input_grad, need_weight_grad, device.index)
+        ws = empty((size,), torch.uint8, device)
         return L.ql_gated_linear_backward(ql_view(g2), vx, vg, ql_view(wu), act, *out, ws.data_ptr() or None, size, stream)
-    call_on(x.device, run, same_device=(g2, wg, wu))
-    return (dx.reshape(x.shape) if dx is not None else None), dwg, dwu
+    call_on(device, run, same_device=(g2, wg, wu))
+    return (dx.view(x.shape) if dx is not None and x.dim() != 2 else dx), dwg, dwu

@@ -4,13 +4,14 @@ torch.float8_e8m0fnu.  The reference has no such operator; NVFP4 (ops.dynamic_qu
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from . import _lib
 from . import dtypes as dt
 from .ops import QuantizeError
-from .tensor import Float4Tensor, call_on, ql_view, require_cuda
+from .tensor import Float4Tensor, call_on, empty, ql_view, require_cuda
 
 BLOCK = 32
 _FLOATS = frozenset((torch.float32, torch.float16, torch.bfloat16))
@@ -27,8 +28,8 @@ def quantize_mxfp4(input: torch.Tensor):
     if not shape or shape[-1] % BLOCK:
         raise QuantizeError(f"the last dimension must be divisible by {BLOCK}, got shape {shape}.")
     x, device = input.contiguous(), input.device
-    data = Float4Tensor(torch.empty(x.numel() // 2, dtype=torch.uint8, device=device), shape)
-    scales = torch.empty(*shape[:-1], shape[-1] // BLOCK, dtype=torch.float8_e8m0fnu, device=device)
+    data = Float4Tensor.empty(shape, device)
+    scales = empty(shape[:-1] + (shape[-1] // BLOCK,), torch.float8_e8m0fnu, device)
     call_on(device, _lib.lib().ql_quantize_mxfp4, ql_view(x), ql_view(data), ql_view(scales))
     return data, scales
 
@@ -39,10 +40,21 @@ def dequantize_mxfp4(data: Float4Tensor, scales: torch.Tensor, dtype: dt.dtype =
     require_cuda(scales, "scales")
     if dtype not in dt.QUANTIZABLE_DTYPES:
         raise QuantizeError(f"Unsupported data type in dequantize_mxfp4. Supported data types are: {dt.QUANTIZABLE_DTYPES}. Got dtype={dtype}")
-    y = out if out is not None else torch.empty(*data.shape, dtype=dtype.torch, device=data.device)
+    y = out if out is not None else empty(data.shape, dtype.torch, data.device)
     s = scales.contiguous()   # kept alive across the call: a view only borrows the pointer
     call_on(data.device, _lib.lib().ql_dequantize_mxfp4, ql_view(data), ql_view(s), ql_view(y), same_device=(s, y))
     return y
+
+
+@functools.lru_cache(maxsize=256)
+def _padding_bytes(a_shape, b_shape) -> int:
+    """ql_gemm_mxfp4_workspace of operands whose scales are no 16-byte rows (it looks at addresses' alignment only), asked once
+    per shape."""
+    def operand(shape):
+        return _lib.make_tensor(4, _lib.F4E2M1, shape), _lib.make_tensor(4, _lib.F8E8M0, (shape[0], shape[1] // BLOCK))
+    size = ctypes.c_int64()
+    _lib.check(_lib.lib().ql_gemm_mxfp4_workspace(*operand(a_shape), *operand(b_shape), ctypes.byref(size)))
+    return size.value
 
 
 def gemm_mxfp4(a: Float4Tensor, a_scales: torch.Tensor, b: Float4Tensor, b_scales: torch.Tensor, out_dtype: dt.dtype = dt.bfloat16,
@@ -58,17 +70,16 @@ def gemm_mxfp4(a: Float4Tensor, a_scales: torch.Tensor, b: Float4Tensor, b_scale
         raise QuantizeError(f"Unsupported data type in gemm_mxfp4. Supported data types are: {dt.QUANTIZABLE_DTYPES}. Got out_dtype={out_dtype}")
     if len(a.shape) != 2 or len(b.shape) != 2 or a_scales.dim() != 2 or b_scales.dim() != 2:
         raise QuantizeError("gemm_mxfp4: data and scales must be 2-D")
-    y = out if out is not None else torch.empty(a.shape[0], b.shape[0], dtype=out_dtype.torch, device=a.device)
+    y = out if out is not None else empty((a.shape[0], b.shape[0]), out_dtype.torch, a.device)
     # dense, on a multiple of 4 bytes (a slice of rows need not be); kept alive across the call: a view only borrows the pointer
     sa, sb = (s if s.data_ptr() % 4 == 0 else s.clone() for s in (a_scales.contiguous(), b_scales.contiguous()))
     L = _lib.lib()
     va, vsa, vb, vsb = ql_view(a), ql_view(sa), ql_view(b), ql_view(sb)
     ws = None
     if sa.shape[-1] % 16 or (sa.data_ptr() | sb.data_ptr()) % 16:   # rows the kernel for many tokens wants a padded copy of
-        size = ctypes.c_int64()
-        _lib.check(L.ql_gemm_mxfp4_workspace(va, vsa, vb, vsb, ctypes.byref(size)))
-        if size.value:
-            ws = torch.empty(size.value, dtype=torch.uint8, device=a.device)
+        size = _padding_bytes(a.shape, b.shape)
+        if size:
+            ws = empty((size,), torch.uint8, a.device)
     call_on(a.device, L.ql_gemm_mxfp4, va, vsa, vb, vsb, ql_view(y), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
             same_device=(sa, b, sb, y))
     return y

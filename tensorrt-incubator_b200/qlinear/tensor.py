@@ -1,6 +1,7 @@
 """Tensor plumbing between torch (device memory, streams) and the C ABI."""
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -58,6 +59,13 @@ class Float4Tensor:
         assert packed.dtype == torch.uint8 and packed.numel() * 2 == math.prod(self.shape)
         self.packed = packed.contiguous()
 
+    @staticmethod
+    def empty(shape, device) -> "Float4Tensor":
+        """Room for values of `shape` (a tuple with an even number of them)."""
+        t = Float4Tensor.__new__(Float4Tensor)
+        t.shape, t.packed = shape, empty((math.prod(shape) // 2,), torch.uint8, device)
+        return t
+
     @property
     def device(self):
         return self.packed.device
@@ -81,13 +89,38 @@ def dtype_of(t) -> dt.dtype:
     return dt.from_torch(t.dtype)
 
 
+@functools.lru_cache(maxsize=1024)
+def _view_of(dtype, shape) -> bytes:
+    """The bytes of a QlTensor of this type (torch's, or the ABI's number) and shape, without its address."""
+    return bytes(_lib.make_tensor(None, dtype if isinstance(dtype, int) else dt.from_torch(dtype).code, shape))
+
+
 def ql_view(t) -> _lib.QlTensor:
-    """QlTensor over a CUDA torch tensor or Int4Tensor (no copy; the caller keeps `t` alive)."""
+    """QlTensor over a CUDA torch tensor or Int4Tensor (no copy; the caller keeps `t` alive).  Made from the bytes of its kind:
+    0.8 us, 1.8 field by field."""
     if isinstance(t, torch.Tensor):
         if not t.is_contiguous():
             raise _lib.QlError(_lib.ERR_INVALID_ARGUMENT, "tensors must be contiguous (dense row-major)")
-        return _lib.make_tensor(t.data_ptr(), dt.from_torch(t.dtype).code, t.shape)
-    return _lib.make_tensor(t.packed.data_ptr(), _lib.I4 if isinstance(t, Int4Tensor) else _lib.F4E2M1, t.shape)
+        v = _lib.QlTensor.from_buffer_copy(_view_of(t.dtype, t.shape))
+        v.data = t.data_ptr()
+    else:
+        v = _lib.QlTensor.from_buffer_copy(_view_of(_lib.I4 if isinstance(t, Int4Tensor) else _lib.F4E2M1, t.shape))
+        v.data = t.packed.data_ptr()
+    return v
+
+
+@functools.lru_cache(maxsize=1024)
+def _dense_strides(shape):
+    strides, n = [], 1
+    for s in reversed(shape):
+        strides.append(n)
+        n *= max(s, 1)
+    return tuple(reversed(strides))
+
+
+def empty(shape, dtype, device) -> torch.Tensor:
+    """torch.empty of a tuple's shape; with the strides given the allocation takes 1.7 us, without 2.6."""
+    return torch.empty_strided(shape, _dense_strides(shape), dtype=dtype, device=device)
 
 
 def require_cuda(t, what: str) -> None:
