@@ -14,13 +14,14 @@
 //   gated_split     few tokens (decoding): the weights are the 128-row operand (gate rows, then up rows of the same channels),
 //                   up to 128 tokens the other; a cluster of CTAs shares K and adds its parts in rank order through
 //                   distributed shared memory.  Bound by reading the weights once.
-//   gated_pair      many tokens: persistent CTA pairs (cta_group::2) on 256 tokens x 128 channels, six stages; CTA 0 of a
-//                   pair loads the gate rows, CTA 1 the up rows, so each holds half of the B tile.  Bound by the tensor cores.
+//   gated_pair      many tokens: persistent CTA pairs (cta_group::2) on 256 tokens x 128 (or 64) channels, six stages; CTA 0
+//                   of a pair loads the gate rows, CTA 1 the up rows, so each holds half of the B tile.  Bound by the tensor
+//                   cores; small problems by what comes before the first MMA and after the last.
 //   gated_grads     the second products, persistent CTA pairs on 256 x 256 tiles.  dX reads dG, dU along their rows (K-major)
 //                   and the weights across (MN-major); the weight gradients read both operands across.  All through the
 //                   same 128-byte-swizzled tiles: for an operand whose rows run along the reduction a tile is 64 rows of
 //                   128 bytes per 64 columns, and the descriptor says so.  No operand is transposed in memory.
-//   grads_reduce    adds the f32 parts of units whose reduction was cut, in order.
+//   grads_reduce    adds the f32 parts of units whose reduction was cut, in a fixed order.
 // Every wait is bounded, as in the other tensor-core kernels.
 #include <cuda.h>
 #include <string.h>
@@ -147,6 +148,16 @@ struct Parked {
       bulk_commit();
     }
   }
+  __device__ __forceinline__ void send_layer(int buf, const CUtensorMap *map, int lane, int x, int y, int z) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+                   ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(base + buf * 4096)), "r"(x), "r"(y), "r"(z)
+                   : "memory");
+      bulk_commit();
+    }
+  }
   template <int PENDING> __device__ __forceinline__ void reusable(int lane) { // the buffer about to be rewritten has been read
     if (lane == 0) bulk_wait_read<PENDING>();
     __syncwarp();
@@ -156,6 +167,13 @@ struct Parked {
     __syncwarp();
   }
 };
+
+// The backward pass's kernels are launched as soon as all CTAs of the one before have started: they set up barriers and tensor
+// memory where an SM is free, and wait here for its results.  dependents_may_start() comes at the start of a kernel; nothing is
+// written before the wait, and the first kernel of a call is launched in the stream's order.  77 x 2744 x 1032 27.2 us, 29.1
+// with each launched when the one before has ended.
+__device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_results() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // What the two pair kernels share: barriers, tensor memory, the ring.  Both CTAs' loads complete on the leader's barriers.
 struct Pair {
@@ -249,12 +267,14 @@ __device__ __forceinline__ void band_coords(int tile, int tiles_m, int tiles_n, 
   *nt = local / size;
 }
 
-template <typename T, bool BACKWARD>
+// C channels to a tile
+template <typename T, bool BACKWARD, int C>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_gate, const __grid_constant__ CUtensorMap map_up,
                   const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_out2, const ProjArgs args) {
   extern __shared__ uint8_t smem_raw[];
   Pair p;
+  if (BACKWARD) dependents_may_start();
   p.start(smem_raw, args.status);
   const int cluster_id = blockIdx.x >> 1, num_clusters = gridDim.x >> 1, num_tiles = args.tiles_m * args.tiles_n;
 
@@ -268,12 +288,12 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     for (int tile = cluster_id; tile < num_tiles && ok; tile += num_clusters) {
       int mt, nt;
       band_coords(tile, args.tiles_m, args.tiles_n, args.group_m, &mt, &nt);
-      const int m0 = mt * 256 + (int)p.rank * 128, n0 = nt * 128;
+      const int m0 = mt * 256 + (int)p.rank * 128, n0 = nt * C;
       for (int kb = 0; kb < args.num_kb; kb++) {
         if (!warp_wait(p.empty(stage), phase ^ 1, p.abort_flag, p.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
         if (elect_one()) {
           const uint32_t dst = p.base + stage * G_STAGE, bar = map_to_cta(p.full(stage), 0);
-          if (p.rank == 0) mbar_expect_tx(p.full(stage), 2 * G_STAGE);
+          if (p.rank == 0) mbar_expect_tx(p.full(stage), 2 * (G_TILE + C * BK_BYTES));
           tma_load_2d_pair(dst, &map_x, bar, kb * 64, m0);
           tma_load_2d_pair(dst + G_TILE, map_w, bar, kb * 64, n0);
         }
@@ -286,7 +306,7 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
   } else if (p.warp == 1) {
     // ------------------------------------------------------------------ MMA issue (leader only)
     if (p.rank == 0) {
-      const uint32_t idesc = f16_idesc<T>(256, G_N, false, false);
+      const uint32_t idesc = f16_idesc<T>(256, 2 * C, false, false);
       int stage = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -317,7 +337,7 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     // ------------------------------------------------------------------ epilogue (warps 2..5, both CTAs)
     const int quad = p.warp & 3, lane = p.lane;
     Parked out{p.smem + PairSmem::kStaging + quad * 8192};
-    int it = 0;
+    int it = 0, b = 0; // b: the staging buffer whose turn it is (forward)
     bool ok = true;
     for (int tile = cluster_id; tile < num_tiles; tile += num_clusters, it++) {
       const int buf = it & 1;
@@ -326,10 +346,10 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       const int m0 = mt * 256 + (int)p.rank * 128 + quad * 32, m = m0 + lane;
       uint4 ahead[4]; // dH of the next chunk, on its way while this one is worked on
       auto fetch = [&](int c) {
-        const int n = nt * 128 + c * 32;
+        const int n = nt * C + c * 32;
         const T *row = static_cast<const T *>(args.dh) + (size_t)m * (size_t)args.I + n;
 #pragma unroll
-        for (int j = 0; j < 4; j++) ahead[j] = c < 4 && m < args.M && n + 8 * j < args.I ? __ldcs(reinterpret_cast<const uint4 *>(row) + j) : make_uint4(0u, 0u, 0u, 0u);
+        for (int j = 0; j < 4; j++) ahead[j] = c < C / 32 && m < args.M && n + 8 * j < args.I ? __ldcs(reinterpret_cast<const uint4 *>(row) + j) : make_uint4(0u, 0u, 0u, 0u);
       };
       if constexpr (BACKWARD) fetch(0);
       ok = warp_wait(p.tfull(buf), (it >> 1) & 1, p.abort_flag, p.status, ST_TIMEOUT_TMEM_FULL);
@@ -337,8 +357,9 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       tc_fence_after();
       const uint32_t taddr = p.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * G_N);
 #pragma unroll 1
-      for (int c = 0; c < 4; c++) { // 32 channels: gate in columns 32 c, up in columns 128 + 32 c
-        const int n = nt * 128 + c * 32, half = c & 1;
+      for (int c = 0; c < C / 32; c++) { // 32 channels: gate in columns 32 c, up in columns C + 32 c
+        const int n = nt * C + c * 32, half = c & 1;
+        if (m0 >= args.M || (half == 0 && n >= args.I)) break; // nothing left to store
         uint4 dh[4];
         if constexpr (BACKWARD) {
 #pragma unroll
@@ -347,7 +368,7 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
         }
         uint32_t g[32], u[32];
         tmem_load_32(taddr + c * 32, g);
-        tmem_load_32(taddr + 128 + c * 32, u);
+        tmem_load_32(taddr + C + c * 32, u);
         if constexpr (!BACKWARD) {
           if (half == 0) out.reusable<1>(lane);
           with_act(args.act, [&](auto act) {
@@ -355,10 +376,12 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             for (int j = 0; j < 32; j++) g[j] = __float_as_uint(act_value<decltype(act)::value>(__uint_as_float(g[j])) * __uint_as_float(u[j]));
           });
           auto two = [&](int j) { return pack2<T>(__uint_as_float(g[j]), __uint_as_float(g[j + 1])); };
-          const int b = (c >> 1) & 1;
 #pragma unroll
           for (int j = 0; j < 32; j += 8) out.put(b, lane, half * 4 + (j >> 3), make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
-          if (half == 1) out.send(b, &map_out, lane, n - 32, m0);
+          if (half == 1) {
+            out.send(b, &map_out, lane, n - 32, m0);
+            b ^= 1;
+          }
         } else {
           if (half == 0) out.reusable<0>(lane); // both buffers: dG in one, dU in the other
           const T *d = reinterpret_cast<const T *>(dh);
@@ -406,7 +429,8 @@ struct GradArgs {
   int heavy, heavy_w;                                    // which then have `heavy_w` weight units, the others the rest.
   int mixed;                                             // instead: units of one length, all dealt out in turn
   int group_m;
-  float *x_parts, *w_parts;                              // [split][M][K], [split][2][I][K], null where nothing is cut
+  float *x_parts, *w_parts;                              // [split][M][K], [split][2][I][K], null where nothing is cut: then
+                                                         // map_dx or map_dwg lead there, layer by layer
   int *status;
 };
 
@@ -456,7 +480,9 @@ gated_grads_kernel(const __grid_constant__ CUtensorMap map_dg_k, const __grid_co
                    const __grid_constant__ CUtensorMap map_dwu, const GradArgs args) {
   extern __shared__ uint8_t smem_raw[];
   Pair p;
+  dependents_may_start();
   p.start(smem_raw, args.status);
+  wait_for_results();
   const int cluster_id = blockIdx.x >> 1, num_clusters = gridDim.x >> 1;
   Unit u;
 
@@ -531,36 +557,39 @@ gated_grads_kernel(const __grid_constant__ CUtensorMap map_dg_k, const __grid_co
     // ------------------------------------------------------------------ epilogue (warps 2..5, both CTAs)
     const int quad = p.warp & 3, lane = p.lane;
     Parked out{p.smem + PairSmem::kStaging + quad * 8192};
+    int b = 0; // the staging buffer whose turn it is
     bool ok = true;
     for (int j = 0; get_unit(args, cluster_id, num_clusters, j, &u); j++) {
       const int buf = j & 1;
       ok = warp_wait(p.tfull(buf), (j >> 1) & 1, p.abort_flag, p.status, ST_TIMEOUT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after();
-      const int r0 = u.row0 + (int)p.rank * 128 + quad * 32, r = r0 + lane, rows = u.is_x ? args.M : args.I;
+      const int r0 = u.row0 + (int)p.rank * 128 + quad * 32;
       const uint32_t taddr = p.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * G_N);
-      float *parts = u.is_x ? args.x_parts : args.w_parts;
-      if (parts) { // f32 part of a cut reduction: [part][dX, or dWg and dWu]
-        parts += ((size_t)(u.is_x ? u.part : 2 * u.part + (u.up ? 1 : 0)) * (size_t)rows + (size_t)r) * (size_t)args.K;
-      }
-      const CUtensorMap *map = u.is_x ? &map_dx : (u.up ? &map_dwu : &map_dwg);
+      const bool parts = (u.is_x ? args.x_parts : args.w_parts) != nullptr; // f32, a layer for each part of the reduction
+      const int layer = u.is_x ? u.part : 2 * u.part + (u.up ? 1 : 0);
+      const CUtensorMap *map = u.is_x ? &map_dx : (u.up && !parts ? &map_dwu : &map_dwg);
 #pragma unroll 1
       for (int c = 0; c < G_N / 32; c++) {
-        const int n = u.col0 + c * 32, half = c & 1, b = (c >> 1) & 1;
+        const int n = u.col0 + c * 32, half = c & 1;
+        if (r0 >= (u.is_x ? args.M : args.I) || ((parts || half == 0) && n >= args.K)) break; // nothing left to store
         uint32_t v[32];
         tmem_load_32(taddr + c * 32, v);
-        if (parts) {
-          if (r < rows) {
+        if (parts) { // 32 values fill a staged row
+          out.reusable<1>(lane);
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) // K is a multiple of 8
-              if (n + i < args.K) __stcs(reinterpret_cast<uint4 *>(parts + n + i), make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]));
-          }
+          for (int i = 0; i < 32; i += 4) out.put(b, lane, i >> 2, make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+          out.send_layer(b, map, lane, n, r0, layer);
+          b ^= 1;
         } else {
           if (half == 0) out.reusable<1>(lane);
           auto two = [&](int i) { return pack2<T>(__uint_as_float(v[i]), __uint_as_float(v[i + 1])); };
 #pragma unroll
           for (int i = 0; i < 32; i += 8) out.put(b, lane, half * 4 + (i >> 3), make_uint4(two(i), two(i + 2), two(i + 4), two(i + 6)));
-          if (half == 1) out.send(b, map, lane, n - 32, r0);
+          if (half == 1) {
+            out.send(b, map, lane, n - 32, r0);
+            b ^= 1;
+          }
         }
       }
       tc_fence_before();
@@ -573,25 +602,43 @@ gated_grads_kernel(const __grid_constant__ CUtensorMap map_dg_k, const __grid_co
   p.end();
 }
 
-// out[i] = sum over p of parts[p][i], p rising; blocks below `x_blocks` add dX, the others dWg and then dWu
+// out[i] = sum over p of parts[p][i]; the first values are dX's, then come dWg's and dWu's.  1 << slices_log2 threads share four
+// neighbouring values where there are few of them and many parts: thread s adds parts s, s + slices, ... and the sums are
+// added in the order of s, so that the result is the same on every run.
+constexpr int kReduceThreads = 256;
 template <typename T>
-__global__ void __launch_bounds__(256) grads_reduce_kernel(const float4 *__restrict__ x_parts, int x_split, T *__restrict__ dx, int64_t nx4, const float4 *__restrict__ w_parts,
-                                                           int w_split, T *__restrict__ dwg, T *__restrict__ dwu, int64_t nw4) {
+__global__ void __launch_bounds__(kReduceThreads) grads_reduce_kernel(const float4 *__restrict__ x_parts, int x_split, T *__restrict__ dx, int64_t nx4,
+                                                                      const float4 *__restrict__ w_parts, int w_split, T *__restrict__ dwg, T *__restrict__ dwu, int64_t nw4,
+                                                                      int slices_log2) {
+  __shared__ float4 sums[kReduceThreads];
+  const int per_log2 = 8 - slices_log2, at = threadIdx.x & ((1 << per_log2) - 1), slice = threadIdx.x >> per_log2, slices = 1 << slices_log2;
   const int64_t n = (x_parts ? nx4 : 0) + (w_parts ? 2 * nw4 : 0);
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+  wait_for_results();
+  for (int64_t first = (int64_t)blockIdx.x << per_log2; first < n; first += (int64_t)gridDim.x << per_log2) {
+    const int64_t i = first + at;
     const bool is_x = x_parts && i < nx4;
     const int64_t j = is_x ? i : i - (x_parts ? nx4 : 0);
     const float4 *src = is_x ? x_parts + j : w_parts + j;
     const int64_t stride = is_x ? nx4 : 2 * nw4;
-    const int split = is_x ? x_split : w_split;
+    const int split = i < n ? (is_x ? x_split : w_split) : 0;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p = 0; p < split; p++) {
+    for (int p = slice; p < split; p += slices) {
       const float4 w = __ldcs(src + p * stride);
       v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
     }
+    if (slices > 1) {
+      __syncthreads(); // the sums of the round before have been read
+      sums[threadIdx.x] = v;
+      __syncthreads();
+      if (slice != 0) continue;
+      for (int s = 1; s < slices; s++) {
+        const float4 w = sums[(s << per_log2) + at];
+        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+      }
+    }
+    if (i >= n) continue;
     T *out = is_x ? dx : (j < nw4 ? dwg : dwu);
-    const int64_t at = is_x || j < nw4 ? j : j - nw4;
-    reinterpret_cast<uint2 *>(out)[at] = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+    reinterpret_cast<uint2 *>(out)[is_x || j < nw4 ? j : j - nw4] = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
   }
 }
 
@@ -647,6 +694,7 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
   const int ct = tile % args.tiles_c, xt = tile / args.tiles_c;
   const int kb0 = (int)((long long)args.num_kb * rank / split), kb1 = (int)((long long)args.num_kb * (rank + 1) / split);
 
+  if (BACKWARD) dependents_may_start();
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; s++) {
       mbar_init(full_bar(s), 1);
@@ -825,9 +873,9 @@ int band(int64_t row_bytes, int tiles_m) {
   return (int)(g > tiles_m ? (tiles_m < 1 ? 1 : tiles_m) : g);
 }
 
-template <typename T, bool BACKWARD>
+template <typename T, bool BACKWARD, int C>
 int launch_pair(const void *x, const void *wg, const void *wu, const void *dh, void *out, void *out2, int M, int I, int K, int act, cudaStream_t st) {
-  auto kern = gated_pair_kernel<T, BACKWARD>;
+  auto kern = gated_pair_kernel<T, BACKWARD, C>;
   static bool configured[64] = {false};
   static int cache[64] = {0};
   int rc = allow_smem(kern, PairSmem::kDynamic, configured);
@@ -837,17 +885,17 @@ int launch_pair(const void *x, const void *wg, const void *wu, const void *dh, v
   a.M = M, a.I = I, a.K = K, a.act = act;
   a.num_kb = (K + 63) / 64;
   a.tiles_m = (M + 255) / 256;
-  a.tiles_n = (I + 127) / 128;
+  a.tiles_n = (I + C - 1) / C;
   a.group_m = band((int64_t)K * 2, a.tiles_m);
   a.status = device_status_word();
   if (!a.status) return set_error(QL_ERR_CUDA, "gated_linear: could not allocate the device status word");
   CUtensorMap mx, mg, mu, mo, mo2;
   const int kind = kMapKind<T>, dtype = FloatIO<T>::kDtype;
-  if ((rc = make_map(&mx, kind, x, M, K, 128)) != QL_OK) return rc;
-  if ((rc = make_map(&mg, kind, wg, I, K, 128)) != QL_OK) return rc;
-  if ((rc = make_map(&mu, kind, wu, I, K, 128)) != QL_OK) return rc;
-  if ((rc = make_map_out(&mo, dtype, out, M, I, I)) != QL_OK) return rc;
-  if ((rc = make_map_out(&mo2, dtype, out2 ? out2 : out, M, I, I)) != QL_OK) return rc;
+  if ((rc = encode_map(&mx, kind, x, M, K, 128)) != QL_OK) return rc;
+  if ((rc = encode_map(&mg, kind, wg, I, K, C)) != QL_OK) return rc;
+  if ((rc = encode_map(&mu, kind, wu, I, K, C)) != QL_OK) return rc;
+  if ((rc = encode_map_out(&mo, dtype, out, M, I, I)) != QL_OK) return rc;
+  if ((rc = encode_map_out(&mo2, dtype, out2 ? out2 : out, M, I, I)) != QL_OK) return rc;
   const int pairs = resident_cached(kern, kPairThreads, PairSmem::kDynamic, 2, cache), tiles = a.tiles_m * a.tiles_n;
   kern<<<2 * (tiles < pairs ? tiles : pairs), kPairThreads, PairSmem::kDynamic, st>>>(mx, mg, mu, mo, mo2, a);
   count_launches(1);
@@ -906,9 +954,9 @@ int launch_split(const void *x, const void *wg, const void *wu, const void *dh, 
   if (!a.status) return set_error(QL_ERR_CUDA, "gated_linear: could not allocate the device status word");
   CUtensorMap mg, mu, mx;
   const int kind = kMapKind<T>;
-  if ((rc = make_map(&mg, kind, wg, I, K, plan.channels)) != QL_OK) return rc;
-  if ((rc = make_map(&mu, kind, wu, I, K, plan.channels)) != QL_OK) return rc;
-  if ((rc = make_map(&mx, kind, x, M, K, TN)) != QL_OK) return rc;
+  if ((rc = encode_map(&mg, kind, wg, I, K, plan.channels)) != QL_OK) return rc;
+  if ((rc = encode_map(&mu, kind, wu, I, K, plan.channels)) != QL_OK) return rc;
+  if ((rc = encode_map(&mx, kind, x, M, K, TN)) != QL_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(((int64_t)a.tiles_c * ((M + TN - 1) / TN)) << plan.log2), 1, 1);
   cfg.blockDim = dim3(kSplitThreads, 1, 1);
@@ -924,13 +972,19 @@ int launch_split(const void *x, const void *wg, const void *wu, const void *dh, 
   return QL_OK;
 }
 
-// The two projections, by whichever kernel is estimated the faster: a pair takes 8.5 us and 0.28 us per tile and 64 values of
-// K; the split kernel what plan_split says.  Up to 32 tokens a pair's 256 rows are mostly padding.  Forward, us (M x I x K):
-// 256 x 512 x 4096 split 14.4, pairs 24.9; 2314 x 80 x 6296 24.8, 38.8; 211 x 2744 x 1032 20.9, 13.2; 128 x 11008 x 4096 75, 51.
+// The two projections, by whichever kernel is estimated the faster: pairs take 7.2 us and 0.28 us per tile of 128 channels and 64
+// values of K, or 5.2 and 0.23 per tile of 64 channels (half the MMAs and half the epilogue, but as many rows of X to load);
+// the split kernel what plan_split says.  Up to 32 tokens a pair's 256 rows are mostly padding.  Forward, us (M x I x K):
+//   256 x 512 x 4096    split 14.4, pairs 24.9     |  2314 x 80 x 6296  split 24.8, pairs 38.8
+//   211 x 2744 x 1032   split 20.9, pairs 13.3, of 64 channels 10.8  |  256 x 9472 x 4096  pairs 36.1, of 64 channels 41.7
+//   128 x 11008 x 4096  split 75, pairs 51.1, of 64 channels 52.9    |  512 x 2368 x 4096  pairs 25.9, of 64 channels 20.9
 template <typename T, bool BACKWARD>
 int project(const void *x, const void *wg, const void *wu, const void *dh, void *out, void *out2, int M, int I, int K, int act, cudaStream_t st) {
-  const int64_t tiles = (int64_t)((M + 255) / 256) * ((I + 127) / 128), per = (tiles + sm_count() / 2 - 1) / (sm_count() / 2);
-  const double pair_us = M <= 32 ? 1e30 : 8.5 + 0.28 * (double)per * ((K + 63) / 64);
+  const int64_t pairs = sm_count() / 2, rows = (M + 255) / 256;
+  auto per_pair = [&](int c) { return (double)((rows * ((I + c - 1) / c) + pairs - 1) / pairs * ((K + 63) / 64)); };
+  const double wide_us = 7.2 + 0.28 * per_pair(128), narrow_us = 5.2 + 0.23 * per_pair(64);
+  const bool narrow = narrow_us < wide_us;
+  const double pair_us = M <= 32 ? 1e30 : (narrow ? narrow_us : wide_us);
   bool ran = false;
   int rc;
   if (M <= 16) rc = launch_split<T, 16, BACKWARD>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us, &ran, st);
@@ -938,7 +992,7 @@ int project(const void *x, const void *wg, const void *wu, const void *dh, void 
   else if (M <= 64) rc = launch_split<T, 64, BACKWARD>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us, &ran, st);
   else rc = launch_split<T, 128, BACKWARD>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us, &ran, st);
   if (rc != QL_OK || ran) return rc;
-  return launch_pair<T, BACKWARD>(x, wg, wu, dh, out, out2, M, I, K, act, st);
+  return narrow ? launch_pair<T, BACKWARD, 64>(x, wg, wu, dh, out, out2, M, I, K, act, st) : launch_pair<T, BACKWARD, 128>(x, wg, wu, dh, out, out2, M, I, K, act, st);
 }
 
 // How the units of the second products are cut and dealt out (see GradArgs), for `pairs` CTA pairs.
@@ -990,6 +1044,21 @@ GradPlan plan_grads(int M, int I, int K, bool want_x, bool want_w, int pairs) {
   return p;
 }
 
+// f32 [layers, rows, cols], box = [1, 32 rows, 32 columns], 128-byte swizzle: a store is clipped at its own layer's edges
+int encode_map_parts(CUtensorMap *map, const float *ptr, int64_t layers, int64_t rows, int64_t cols) {
+  EncodeTiledFn enc;
+  const int rc = get_encode_fn(&enc);
+  if (rc != QL_OK) return rc;
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)layers};
+  cuuint64_t strides[2] = {(cuuint64_t)cols * 4, (cuuint64_t)(rows * cols) * 4};
+  cuuint32_t box[3] = {32, 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(QL_ERR_CUDA, "cuTensorMapEncodeTiled (parts) failed with code %d", (int)r);
+  return QL_OK;
+}
+
 int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 template <typename T> int grad_pairs() {
@@ -1014,29 +1083,46 @@ int backward(const void *dh, const void *x, const void *wg, const void *wu, void
   if (plan.w_part_floats) a.w_parts = reinterpret_cast<float *>(parts + align256(plan.x_part_floats * 4));
   CUtensorMap dgk, duk, dgm, dum, wgm, wum, xm, mx, mg, mu;
   const int kind = kMapKind<T>, dtype = FloatIO<T>::kDtype;
-  if ((rc = make_map(&dgk, kind, dg, M, I, 128)) != QL_OK) return rc;
-  if ((rc = make_map(&duk, kind, du, M, I, 128)) != QL_OK) return rc;
-  if ((rc = make_map(&dgm, kind, dg, M, I, 64)) != QL_OK) return rc;
-  if ((rc = make_map(&dum, kind, du, M, I, 64)) != QL_OK) return rc;
-  if ((rc = make_map(&wgm, kind, wg, I, K, 64)) != QL_OK) return rc;
-  if ((rc = make_map(&wum, kind, wu, I, K, 64)) != QL_OK) return rc;
-  if ((rc = make_map(&xm, kind, x, M, K, 64)) != QL_OK) return rc;
+  if ((rc = encode_map(&dgk, kind, dg, M, I, 128)) != QL_OK) return rc;
+  if ((rc = encode_map(&duk, kind, du, M, I, 128)) != QL_OK) return rc;
+  if ((rc = encode_map(&dgm, kind, dg, M, I, 64)) != QL_OK) return rc;
+  if ((rc = encode_map(&dum, kind, du, M, I, 64)) != QL_OK) return rc;
+  if ((rc = encode_map(&wgm, kind, wg, I, K, 64)) != QL_OK) return rc;
+  if ((rc = encode_map(&wum, kind, wu, I, K, 64)) != QL_OK) return rc;
+  if ((rc = encode_map(&xm, kind, x, M, K, 64)) != QL_OK) return rc;
   mx = mg = mu = xm; // what is not wanted is not written
-  if (dx && (rc = make_map_out(&mx, dtype, dx, M, K, K)) != QL_OK) return rc;
-  if (dwg && (rc = make_map_out(&mg, dtype, dwg, I, K, K)) != QL_OK) return rc;
-  if (dwu && (rc = make_map_out(&mu, dtype, dwu, I, K, K)) != QL_OK) return rc;
+  if (a.x_parts) rc = encode_map_parts(&mx, a.x_parts, a.x_split, M, K);
+  else if (dx) rc = encode_map_out(&mx, dtype, dx, M, K, K);
+  if (rc != QL_OK) return rc;
+  if (a.w_parts) rc = encode_map_parts(&mg, a.w_parts, 2 * a.w_split, I, K);
+  else if (dwg && (rc = encode_map_out(&mg, dtype, dwg, I, K, K)) == QL_OK) rc = encode_map_out(&mu, dtype, dwu, I, K, K);
+  if (rc != QL_OK) return rc;
   const int pairs = grad_pairs<T>(); // get_unit deals the units out over exactly this many
-  gated_grads_kernel<T><<<2 * pairs, kPairThreads, PairSmem::kDynamic, st>>>(dgk, duk, dgm, dum, wgm, wum, xm, mx, mg, mu, a);
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * pairs), 1, 1);
+  cfg.blockDim = dim3(kPairThreads, 1, 1);
+  cfg.dynamicSmemBytes = PairSmem::kDynamic;
+  cfg.stream = st;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, gated_grads_kernel<T>, dgk, duk, dgm, dum, wgm, wum, xm, mx, mg, mu, a));
   count_launches(1);
-  QL_CUDA_TRY(cudaGetLastError());
   if (a.x_parts || a.w_parts) {
     const int64_t nx4 = (int64_t)M * K / 4, nw4 = (int64_t)I * K / 4, n = (a.x_parts ? nx4 : 0) + (a.w_parts ? 2 * nw4 : 0);
-    const int64_t blocks = (n + 255) / 256, cap = (int64_t)sm_count() * 8;
-    grads_reduce_kernel<T><<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, st>>>(reinterpret_cast<const float4 *>(a.x_parts), a.x_split, static_cast<T *>(dx), nx4,
-                                                                                reinterpret_cast<const float4 *>(a.w_parts), a.w_split, static_cast<T *>(dwg),
-                                                                                static_cast<T *>(dwu), nw4);
+    const int split = a.x_parts && a.w_parts ? (a.x_split > a.w_split ? a.x_split : a.w_split) : (a.x_parts ? a.x_split : a.w_split);
+    const int64_t room = (int64_t)sm_count() * 2048; // threads the device holds
+    int slices_log2 = 0;
+    while (slices_log2 < 3 && (2 << slices_log2) <= split && (n << (slices_log2 + 1)) <= room) slices_log2++;
+    const int64_t per = kReduceThreads >> slices_log2, blocks = (n + per - 1) / per, cap = room / kReduceThreads;
+    cfg.gridDim = dim3((unsigned)(blocks < cap ? blocks : cap), 1, 1);
+    cfg.blockDim = dim3(kReduceThreads, 1, 1);
+    cfg.dynamicSmemBytes = 0;
+    QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, grads_reduce_kernel<T>, reinterpret_cast<const float4 *>(a.x_parts), a.x_split, static_cast<T *>(dx), nx4,
+                                   reinterpret_cast<const float4 *>(a.w_parts), a.w_split, static_cast<T *>(dwg), static_cast<T *>(dwu), nw4, slices_log2));
     count_launches(1);
-    QL_CUDA_TRY(cudaGetLastError());
   }
   return QL_OK;
 }

@@ -831,8 +831,8 @@ template <int TN, bool WIDE> int launch_split_as(const void *w, const void *x, M
   args.tiles_a = (args.N + plan.rows - 1) / plan.rows;
   args.tiles_b = (args.M + TN - 1) / TN;
   CUtensorMap mw, mx;
-  if ((rc = make_map(&mw, KIND_F8, w, args.N, K / 2, plan.rows)) != QL_OK) return rc;
-  if ((rc = make_map(&mx, KIND_F8, x, args.M, K / 2, TN)) != QL_OK) return rc;
+  if ((rc = encode_map(&mw, KIND_F8, w, args.N, K / 2, plan.rows)) != QL_OK) return rc;
+  if ((rc = encode_map(&mx, KIND_F8, x, args.M, K / 2, TN)) != QL_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(((int64_t)args.tiles_a * args.tiles_b) << plan.log2), 1, 1);
   cfg.blockDim = dim3(kSplitThreads, 1, 1);
@@ -905,8 +905,8 @@ template <bool PAIR, bool TURNED> int launch_tiles(const void *a, const void *b,
     args.sfb = args.sfa + (int64_t)args.M * pitch;
   }
   CUtensorMap ma, mb, msa, msb;
-  if ((rc = make_map(&ma, KIND_F8, a, args.M, K / 2, BM)) != QL_OK) return rc;
-  if ((rc = make_map(&mb, KIND_F8, b, args.N, K / 2, L::kRowsB)) != QL_OK) return rc;
+  if ((rc = encode_map(&ma, KIND_F8, a, args.M, K / 2, BM)) != QL_OK) return rc;
+  if ((rc = encode_map(&mb, KIND_F8, b, args.N, K / 2, L::kRowsB)) != QL_OK) return rc;
   if ((rc = make_map_bytes(&msa, args.sfa, args.M, pitch, 32, BM)) != QL_OK) return rc;
   if ((rc = make_map_bytes(&msb, args.sfb, args.N, pitch, 32, TBN)) != QL_OK) return rc;
   args.tiles_a = (args.M + (PAIR ? 2 : 1) * BM - 1) / ((PAIR ? 2 : 1) * BM);

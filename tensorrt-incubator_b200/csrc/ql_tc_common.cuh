@@ -260,6 +260,25 @@ inline int get_encode_fn(EncodeTiledFn *out) {
 }
 
 // [rows, K] row-major matrix of `esize`-byte elements, box = [box_rows, 128 bytes], 128-byte swizzle.
+inline int encode_map(CUtensorMap *map, int kind, const void *ptr, int64_t rows, int64_t K, int box_rows) {
+  EncodeTiledFn enc;
+  int rc = get_encode_fn(&enc);
+  if (rc != QL_OK) return rc;
+  const int esize = (kind == KIND_F8 || kind == KIND_I8) ? 1 : 2;
+  CUtensorMapDataType dt = (kind == KIND_F8 || kind == KIND_I8) ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                           : (kind == KIND_BF16)                ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)K * esize};
+  cuuint32_t box[2] = {(cuuint32_t)(BK_BYTES / esize), (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(map, dt, 2, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(QL_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return QL_OK;
+}
+
+// The same, remembered.
 // A tensor map is a pure function of (address, shape, box, type), so the last few are kept per thread: a decode
 // loop that calls the same layers again and again does not pay the driver's encoder on every launch, and an
 // entry whose buffer was freed and reallocated at the same address with the same shape is still correct.
@@ -278,20 +297,8 @@ inline int make_map(CUtensorMap *map, int kind, const void *ptr, int64_t rows, i
     *map = e.map;
     return QL_OK;
   }
-  EncodeTiledFn enc;
-  int rc = get_encode_fn(&enc);
+  const int rc = encode_map(map, kind, ptr, rows, K, box_rows);
   if (rc != QL_OK) return rc;
-  const int esize = (kind == KIND_F8 || kind == KIND_I8) ? 1 : 2;
-  CUtensorMapDataType dt = (kind == KIND_F8 || kind == KIND_I8) ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                           : (kind == KIND_BF16)                ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)K * esize};
-  cuuint32_t box[2] = {(cuuint32_t)(BK_BYTES / esize), (cuuint32_t)box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(map, dt, 2, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_error(QL_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
   e.ptr = ptr;
   e.rows = rows;
   e.K = K;
@@ -305,6 +312,25 @@ inline int make_map(CUtensorMap *map, int kind, const void *ptr, int64_t rows, i
 // Result matrix [rows, cols] of `esize`-byte elements with `ld` elements between rows, box = [32 rows, 128 bytes],
 // 128-byte swizzle: the epilogue parks 32 rows x 128 bytes in shared memory and one bulk store writes them out as
 // whole 128-byte lines (rows and columns beyond the matrix are clipped by the copy engine).
+inline int encode_map_out(CUtensorMap *map, int dtype, const void *ptr, int64_t rows, int64_t cols, int64_t ld) {
+  EncodeTiledFn enc;
+  int rc = get_encode_fn(&enc);
+  if (rc != QL_OK) return rc;
+  const int esize = dtype == QL_F32 ? 4 : 2;
+  CUtensorMapDataType dt = dtype == QL_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                           : dtype == QL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * esize};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / esize), 32};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(map, dt, 2, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(QL_ERR_CUDA, "cuTensorMapEncodeTiled (result) failed with code %d", (int)r);
+  return QL_OK;
+}
+
+// The same, remembered as make_map's are.
 inline int make_map_out(CUtensorMap *map, int dtype, const void *ptr, int64_t rows, int64_t cols, int64_t ld) {
   struct Entry {
     const void *ptr;
@@ -320,20 +346,8 @@ inline int make_map_out(CUtensorMap *map, int dtype, const void *ptr, int64_t ro
     *map = e.map;
     return QL_OK;
   }
-  EncodeTiledFn enc;
-  int rc = get_encode_fn(&enc);
+  const int rc = encode_map_out(map, dtype, ptr, rows, cols, ld);
   if (rc != QL_OK) return rc;
-  const int esize = dtype == QL_F32 ? 4 : 2;
-  CUtensorMapDataType dt = dtype == QL_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                           : dtype == QL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)ld * esize};
-  cuuint32_t box[2] = {(cuuint32_t)(128 / esize), 32};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(map, dt, 2, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_error(QL_ERR_CUDA, "cuTensorMapEncodeTiled (result) failed with code %d", (int)r);
   e.ptr = ptr;
   e.rows = rows;
   e.cols = cols;
