@@ -172,9 +172,6 @@ struct Parked {
 // memory where an SM is free, and wait here for its results.  dependents_may_start() comes at the start of a kernel; nothing is
 // written before the wait, and the first kernel of a call is launched in the stream's order.  77 x 2744 x 1032 27.2 us, 29.1
 // with each launched when the one before has ended.
-__device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_results() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // What the two pair kernels share: barriers, tensor memory, the ring.  Both CTAs' loads complete on the leader's barriers.
 struct Pair {
   uint8_t *smem;

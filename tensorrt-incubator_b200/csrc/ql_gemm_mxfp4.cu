@@ -411,10 +411,11 @@ gemm_mxfp4_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 // The width leaves tensor memory, beside two accumulators, 96 columns: two slots of the scales of two k steps.  With 224 there
 // is room for two slots of one step, and refilling one (the commit, the hand-over, the store) takes longer than a step.
 constexpr int TBN = 208;
-constexpr int kTileThreads = 320;   // producer, MMA, four epilogue warps, four scale warps
+constexpr int kTileThreads = 448;   // producer, MMA, four epilogue warps, two sets of four scale warps
 constexpr int kScSteps = 4;         // k steps whose scales travel together: 32 bytes, a whole sector, of every row
-constexpr int kSlotSteps = 2;       // k steps of one stage and of one slot: 16 columns of A's scales, then 32 of B's (8 per pair of MMAs, 6.5 used)
-constexpr int kSlotCols = 48;
+constexpr int kStageSteps = 2;      // k steps of one stage
+constexpr int kSlots = 4;           // of one k step: 8 columns of A's scales, then 16 of B's (8 per pair of MMAs, 6.5 used)
+constexpr int kSlotCols = 24;
 constexpr int T_SC_ROWS = BM + TBN;
 constexpr int T_SC_LANES = (T_SC_ROWS + 31) / 32; // rows a lane carries (of the last, half the lanes' are past the tile)
 constexpr int T_SC_BYTES = T_SC_LANES * 32 * 32;  // with room for those
@@ -422,10 +423,10 @@ template <bool PAIR> struct TileSmem {
   static constexpr int kStages = PAIR ? 3 : 2; // of two k steps: half as many barriers to look at and to signal as with one
   static constexpr int kRowsB = PAIR ? TBN / 2 : TBN;                     // rows of the B tile one CTA holds
   static constexpr int kTileB = kRowsB * BK_BYTES;
-  static constexpr int kStageBytes = kSlotSteps * (MX_A_BYTES + kTileB);  // A's tiles, then B's
+  static constexpr int kStageBytes = kStageSteps * (MX_A_BYTES + kTileB);  // A's tiles, then B's
   static constexpr int kScales = kStages * kStageBytes;
-  static constexpr int kBarriers = kScales + 2 * T_SC_BYTES; // full[S], empty[S], tfull[2], tempty[2], scfull[2], scempty[2], sfull[2], sempty[2], drain
-  static constexpr int kTmemPtr = kBarriers + (2 * kStages + 13) * 8;
+  static constexpr int kBarriers = kScales + 2 * T_SC_BYTES; // full[S], empty[S], tfull[2], tempty[2], scfull[2], scempty[2], sfull[4], sempty[4], drain
+  static constexpr int kTmemPtr = kBarriers + (2 * kStages + 9 + 2 * kSlots) * 8;
   static constexpr int kAbort = kTmemPtr + 4;
   static constexpr int kDynamic = kAbort + 4 + 1024;
   static_assert(kDynamic <= 232448 && kStageBytes % 1024 == 0 && T_SC_BYTES % 128 == 0, "tile shape");
@@ -463,7 +464,7 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
   using L = TileSmem<PAIR>;
   constexpr int TSTAGES = L::kStages;
   constexpr uint32_t kTmemCols = 512; // two accumulators, two slots of scales
-  static_assert(2 * TBN + 2 * kSlotCols <= 512, "tensor memory");
+  static_assert(2 * TBN + kSlots * kSlotCols <= 512, "tensor memory");
   constexpr uint32_t kSfCol0 = 2 * TBN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -475,8 +476,8 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
   auto scfull_bar = [&](int b) { return bar_base + 8u * (2 * TSTAGES + 4 + b); };
   auto scempty_bar = [&](int b) { return bar_base + 8u * (2 * TSTAGES + 6 + b); };
   auto sfull_bar = [&](int b) { return bar_base + 8u * (2 * TSTAGES + 8 + b); };
-  auto sempty_bar = [&](int b) { return bar_base + 8u * (2 * TSTAGES + 10 + b); };
-  const uint32_t drain_bar = bar_base + 8u * (2 * TSTAGES + 12);
+  auto sempty_bar = [&](int b) { return bar_base + 8u * (2 * TSTAGES + 8 + kSlots + b); };
+  const uint32_t drain_bar = bar_base + 8u * (2 * TSTAGES + 8 + 2 * kSlots);
   volatile uint32_t *tmem_ptr_smem = reinterpret_cast<volatile uint32_t *>(smem + L::kTmemPtr);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::kAbort);
 
@@ -508,7 +509,9 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
       mbar_init(tfull_bar(b), 1);
       mbar_init(tempty_bar(b), PAIR ? 8 : 4);
       mbar_init(scfull_bar(b), 1);
-      mbar_init(scempty_bar(b), 4);
+      mbar_init(scempty_bar(b), 8); // both sets of scale warps
+    }
+    for (int b = 0; b < kSlots; b++) {
       mbar_init(sfull_bar(b), PAIR ? 8 : 4);
       mbar_init(sempty_bar(b), 1);
     }
@@ -539,9 +542,10 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
     bool ok = true;
     for (int tile = first_tile; tile < num_tiles && ok; tile += tile_stride) {
       const int mt = tile % args.tiles_a, nt = tile / args.tiles_a; // row tiles of one column tile run side by side: B stays in L2
-      for (int ks = 0; ks < args.num_ks; ks += kSlotSteps) { // a second step beyond K is loaded as zeros
+      for (int ks = 0; ks < args.num_ks; ks += kStageSteps) { // a second step beyond K is loaded as zeros
         if (ks % kScSteps == 0) {
           if (!warp_wait(scempty_bar(sc), sc_phase ^ 1, abort_flag, args.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+          if (sc_issued == 0) wait_for_results(); // of the kernel that pads the scales
           if (elect_one()) {
             const uint32_t dst = smem_base + L::kScales + sc * T_SC_BYTES;
             mbar_expect_tx(scfull_bar(sc), T_SC_ROWS * 32);
@@ -554,11 +558,11 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
         }
         if (!warp_wait(empty_bar(stage), phase ^ 1, abort_flag, args.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
         if (elect_one()) {
-          const uint32_t a_dst = smem_base + stage * L::kStageBytes, b_dst = a_dst + kSlotSteps * MX_A_BYTES;
+          const uint32_t a_dst = smem_base + stage * L::kStageBytes, b_dst = a_dst + kStageSteps * MX_A_BYTES;
           const uint32_t bar = PAIR ? map_to_cta(full_bar(stage), 0) : full_bar(stage); // a pair's bytes all land on the leader's barrier
           if (rank == 0) mbar_expect_tx(full_bar(stage), (PAIR ? 2 : 1) * L::kStageBytes);
 #pragma unroll
-          for (int q = 0; q < kSlotSteps; q++) { // coordinates in bytes of packed e2m1
+          for (int q = 0; q < kStageSteps; q++) { // coordinates in bytes of packed e2m1
             const int x = (ks + q) * BK_BYTES;
             if (PAIR) {
               tma_load_2d_pair(a_dst + q * MX_A_BYTES, &map_a, bar, x, (2 * mt + rank) * BM);
@@ -603,34 +607,47 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
         const int buf = it & 1;
         if (!warp_wait(tempty_bar(buf), ((it >> 1) & 1) ^ 1, abort_flag, args.status, ST_TIMEOUT_TMEM_EMPTY)) { ok = false; break; }
         const uint32_t tmem_d = tmem_base + (uint32_t)(buf * TBN);
-        for (int ks = 0; ks < args.num_ks; ks += kSlotSteps) {
-          const int slot = (int)(half & 1);
-          if (!scales_ready && !warp_wait(sfull_bar(slot), (half >> 1) & 1, abort_flag, args.status, ST_TIMEOUT_FULL)) { ok = false; break; }
+        for (int ks = 0; ks < args.num_ks; ks += kStageSteps) {
+          const int slot = (int)(half & 1) * kStageSteps; // of the first step; the second has the next one
+          const uint32_t parity = (half >> 1) & 1;
+          if (!scales_ready && !warp_wait(sfull_bar(slot), parity, abort_flag, args.status, ST_TIMEOUT_FULL)) { ok = false; break; }
           if (!data_ready && !warp_wait(full_bar(stage), phase, abort_flag, args.status, ST_TIMEOUT_FULL)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t a_addr = smem_base + stage * L::kStageBytes, t_sfa = tmem_base + kSfCol0 + kSlotCols * slot, t_sfb = t_sfa + 16;
-          const uint64_t adesc = make_smem_desc(a_addr), bdesc = make_smem_desc(a_addr + kSlotSteps * MX_A_BYTES);
+          const uint32_t a_addr = smem_base + stage * L::kStageBytes, t_sfa = tmem_base + kSfCol0 + kSlotCols * slot, t_sfb = t_sfa + 8;
+          const uint64_t adesc = make_smem_desc(a_addr), bdesc = make_smem_desc(a_addr + kStageSteps * MX_A_BYTES);
           const int cur = stage;
           if (++stage == TSTAGES) { stage = 0; phase ^= 1; }
           half++;
+          auto mma = [&](int q, int j) {
+            mx_k_mma<TBN, PAIR>(j, tmem_d, adesc + q * (MX_A_BYTES >> 4), bdesc + q * (L::kTileB >> 4), t_sfa + q * kSlotCols, t_sfb + q * kSlotCols, 8, (ks | q | j) != 0 ? 1u : 0u);
+          };
           if (leader) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) mx_k_mma<TBN, PAIR>(j, tmem_d, adesc, bdesc, t_sfa, t_sfb, 8, (ks | j) != 0 ? 1u : 0u);
-            mx_k_mma<TBN, PAIR>(0, tmem_d, adesc + (MX_A_BYTES >> 4), bdesc + (L::kTileB >> 4), t_sfa + 8, t_sfb + 16, 8, 1u);
+            for (int j = 0; j < 3; j++) mma(0, j);
           }
+          __syncwarp();
+          const bool second_ready = __all_sync(0xffffffffu, mbar_test_wait(sfull_bar(slot + 1), parity));
+          if (leader) {
+            mma(0, 3);
+            commit_all(sempty_bar(slot));
+          }
+          __syncwarp();
+          if (!second_ready && !warp_wait(sfull_bar(slot + 1), parity, abort_flag, args.status, ST_TIMEOUT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          if (leader) mma(1, 0);
           __syncwarp();
           data_ready = __all_sync(0xffffffffu, mbar_test_wait(full_bar(stage), phase));
           if (leader) {
-            mx_k_mma<TBN, PAIR>(1, tmem_d, adesc + (MX_A_BYTES >> 4), bdesc + (L::kTileB >> 4), t_sfa + 8, t_sfb + 16, 8, 1u);
-            mx_k_mma<TBN, PAIR>(2, tmem_d, adesc + (MX_A_BYTES >> 4), bdesc + (L::kTileB >> 4), t_sfa + 8, t_sfb + 16, 8, 1u);
+            mma(1, 1);
+            mma(1, 2);
           }
           __syncwarp();
-          scales_ready = __all_sync(0xffffffffu, mbar_test_wait(sfull_bar((int)(half & 1)), (half >> 1) & 1));
+          scales_ready = __all_sync(0xffffffffu, mbar_test_wait(sfull_bar((int)(half & 1) * kStageSteps), (half >> 1) & 1));
           if (leader) {
-            mx_k_mma<TBN, PAIR>(3, tmem_d, adesc + (MX_A_BYTES >> 4), bdesc + (L::kTileB >> 4), t_sfa + 8, t_sfb + 16, 8, 1u);
-            commit_all(sempty_bar(slot));
+            mma(1, 3);
+            commit_all(sempty_bar(slot + 1));
             commit_all(empty_bar(cur));
-            if (ks + kSlotSteps >= args.num_ks) commit_all(tfull_bar(buf));
+            if (ks + kStageSteps >= args.num_ks) commit_all(tfull_bar(buf));
           }
           __syncwarp();
         }
@@ -644,49 +661,51 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
       if (!bounded_wait(drain_bar, 0) && lane == 0) atomicCAS(args.status, 0, ST_TIMEOUT_DRAIN);
     }
   } else if (warp >= 6) {
-    // ------------------------------------------------------------------ scales (warps 6..9, one per quarter of the lanes)
+    // ------------------------------------------------------------------ scales (warps 6..13, two for each quarter of the lanes)
+    // The two sets take stages in turn, each with the two slots that are its own.
     const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
-    uint32_t half = 0; // slots filled so far
+    const uint32_t set = warp >= 10 ? 1 : 0;
+    uint32_t half = 0; // stages so far
     bool ok = true;
     const int groups = (args.num_ks + kScSteps - 1) / kScSteps; // of four k steps, in a tile
     auto hand_over = [&](int ks, int sc, uint32_t sc_phase) {
       ok = warp_wait(scfull_bar(sc), sc_phase, abort_flag, args.status, ST_TIMEOUT_FULL);
       if (!ok) return;
       const uint8_t *buf = smem + L::kScales + sc * T_SC_BYTES;
-#pragma unroll 1
-      for (int h = 0; h < kScSteps / kSlotSteps; h++) {
-        const bool more = ok && ks + h * kSlotSteps < args.num_ks;
-        uint32_t w[T_SC_LANES][4]; // rows lane, lane + 32, ... : the words of two k steps
-        if (more) {
+      uint32_t w[T_SC_LANES][4]; // rows lane, lane + 32, ... : the words of two k steps
+      int h = 0;                 // the stage of this group that is this set's, if there is one
+      while (h < kScSteps / kStageSteps && ks + h * kStageSteps < args.num_ks && ((half + h) & 1) != set) h++;
+      const bool mine = h < kScSteps / kStageSteps && ks + h * kStageSteps < args.num_ks;
+      const uint32_t parity = ((half + h) >> 1 & 1) ^ 1u;
+      half += min((args.num_ks - ks + kStageSteps - 1) / kStageSteps, kScSteps / kStageSteps);
+      if (mine) {
+        // 32-byte rows as the copy engine's 32-byte swizzle leaves them: a row's halves changed places in rows 4 to 7 of 8, so that
+        // eight lanes' 16 bytes cover all banks
+        const uint8_t *row = buf + lane * 32 + ((16 * h) ^ ((lane & 4) << 2));
 #pragma unroll
-          for (int c = 0; c < T_SC_LANES; c++) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(buf + (c * 32 + lane) * 32 + 16 * h);
-            w[c][0] = v.x, w[c][1] = v.y, w[c][2] = v.z, w[c][3] = v.w;
-          }
+        for (int c = 0; c < T_SC_LANES; c++) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(row + c * 1024);
+          w[c][0] = v.x, w[c][1] = v.y, w[c][2] = v.z, w[c][3] = v.w;
         }
-        if (h == kScSteps / kSlotSteps - 1) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(scempty_bar(sc));
-        }
-        if (more) {
-          const int slot = (int)(half & 1);
-          ok = warp_wait(sempty_bar(slot), ((half >> 1) & 1) ^ 1u, abort_flag, args.status, ST_TIMEOUT_EMPTY);
-          if (ok) {
-            // of each k step and pair of MMAs (word j): four cells of A's rows, seven of B's
-            const uint32_t t = tmem_base + quarter + kSfCol0 + kSlotCols * slot;
-            tmem_store_16(t, w[0][0], w[1][0], w[2][0], w[3][0], w[0][1], w[1][1], w[2][1], w[3][1], w[0][2], w[1][2], w[2][2], w[3][2], w[0][3], w[1][3], w[2][3], w[3][3]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(scempty_bar(sc));
+      if (!mine) return;
 #pragma unroll
-            for (int q = 0; q < kSlotSteps; q++) {
-              auto v = [&](int c, int j) { return w[4 + c][2 * q + j]; };
-              tmem_store_16(t + 16 + 16 * q, v(0, 0), v(1, 0), v(2, 0), v(3, 0), v(4, 0), v(5, 0), v(6, 0), 0u, v(0, 1), v(1, 1), v(2, 1), v(3, 1), v(4, 1), v(5, 1), v(6, 1), 0u);
-            }
-            tmem_store_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_leader(sfull_bar(slot));
-            half++;
-          }
-        }
+      for (int q = 0; q < kStageSteps; q++) {
+        const int slot = (int)set * kStageSteps + q;
+        ok = warp_wait(sempty_bar(slot), parity, abort_flag, args.status, ST_TIMEOUT_EMPTY);
+        if (!ok) return;
+        // for each pair of MMAs (word j): four cells of A's rows, seven of B's
+        const uint32_t t = tmem_base + quarter + kSfCol0 + kSlotCols * slot;
+        auto v = [&](int c, int j) { return w[c][2 * q + j]; };
+        tmem_store_4(t, v(0, 0), v(1, 0), v(2, 0), v(3, 0));
+        tmem_store_4(t + 4, v(0, 1), v(1, 1), v(2, 1), v(3, 1));
+        tmem_store_16(t + 8, v(4, 0), v(5, 0), v(6, 0), v(7, 0), v(8, 0), v(9, 0), v(10, 0), 0u, v(4, 1), v(5, 1), v(6, 1), v(7, 1), v(8, 1), v(9, 1), v(10, 1), 0u);
+        tmem_store_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_leader(sfull_bar(slot));
       }
     };
     const int mine = first_tile < num_tiles ? (num_tiles - first_tile + tile_stride - 1) / tile_stride : 0;
@@ -860,21 +879,32 @@ template <int TN> int launch_split(const void *w, const void *x, const MxArgs &a
   return wide ? launch_split_as<TN, true>(w, x, args, K, plan, st) : launch_split_as<TN, false>(w, x, args, K, plan, st);
 }
 
-// Rows of scale bytes, `pitch` bytes apart and zero-padded, of both operands: 16 bytes a thread.
+// Rows of scale bytes, `pitch` bytes apart and zero-padded, of both operands: 16 bytes a thread, from the aligned words that hold
+// them (the operands lie on multiples of 4); a word that reaches beyond its operand is read byte by byte.
 __global__ void __launch_bounds__(256) mx_pad_scales_kernel(const uint8_t *__restrict__ a, int rows_a, const uint8_t *__restrict__ b, int rows_b, int kb, int units,
                                                             uint4 *__restrict__ out) {
+  dependents_may_start();
   const int unit = blockIdx.x * 32 + threadIdx.x % 32, b0 = unit * 16; // a warp takes 512 bytes of a row, a block eight rows
   if (unit >= units) return;
   for (int64_t row = (int64_t)blockIdx.y * 8 + threadIdx.x / 32; row < (int64_t)rows_a + rows_b; row += (int64_t)gridDim.y * 8) {
-    const uint8_t *p = (row < rows_a ? a + row * kb : b + (row - rows_a) * kb) + b0;
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
-    if (b0 + 16 <= kb && (reinterpret_cast<uintptr_t>(p) & 3) == 0) {
+    const bool first = row < rows_a;
+    const int64_t at = (first ? row : row - rows_a) * kb + b0, left = (int64_t)(first ? rows_a : rows_b) * kb - at; // bytes of the operand from here on
+    const uint8_t *p = (first ? a : b) + at;
+    const int off = (int)(at & 3), valid = min(16, kb - b0); // of the unit
+    const uint8_t *q = p - off;
+    uint32_t r[5];
 #pragma unroll
-      for (int j = 0; j < 4; j++) w[j] = __ldg(reinterpret_cast<const uint32_t *>(p) + j);
-    } else {
+    for (int i = 0; i < 5; i++) r[i] = ldg32_if(q + 4 * i, 4 * i < valid + off && 4 * i + 4 <= left + off);
+    if (left + off < 4 * ((valid + off + 3) / 4)) { // the operand's last row
 #pragma unroll
-      for (int j = 0; j < 16; j++)
-        if (b0 + j < kb) w[j / 4] |= (uint32_t)__ldg(p + j) << (8 * (j % 4));
+      for (int j = 0; j < 20; j++)
+        if (j >= (int)((left + off) & ~3) && j < left + off) r[j / 4] |= (uint32_t)__ldg(q + j) << (8 * (j % 4));
+    }
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int here = valid - 4 * i;
+      w[i] = __funnelshift_r(r[i], r[i + 1], 8 * off) & (here >= 4 ? 0xFFFFFFFFu : (here <= 0 ? 0u : (1u << (8 * here)) - 1u));
     }
     out[row * units + unit] = make_uint4(w[0], w[1], w[2], w[3]);
   }
@@ -886,6 +916,21 @@ int padded_pitch(int64_t kb) { return (int)((kb + 15) / 16 * 16); }
 bool needs_padding(const MxArgs &args) { return args.kb % 16 != 0 || !aligned16(args.sfa) || !aligned16(args.sfb); }
 int64_t padded_bytes(int64_t M, int64_t N, int64_t kb) { return (M + N) * padded_pitch(kb); }
 
+// scales [rows, pitch] as bytes, box = [box_rows, 32 bytes], 32-byte swizzle
+int encode_map_scales(CUtensorMap *map, const uint8_t *ptr, int64_t rows, int64_t pitch, int box_rows) {
+  EncodeTiledFn enc;
+  const int rc = get_encode_fn(&enc);
+  if (rc != QL_OK) return rc;
+  cuuint64_t dims[2] = {(cuuint64_t)pitch, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)pitch};
+  cuuint32_t box[2] = {32, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_32B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(QL_ERR_CUDA, "cuTensorMapEncodeTiled (scales) failed with code %d", (int)r);
+  return QL_OK;
+}
+
 // args: operands a and b as the kernel takes them (TURNED: the weights first)
 template <bool PAIR, bool TURNED> int launch_tiles(const void *a, const void *b, MxArgs args, int64_t K, void *workspace, cudaStream_t st) {
   using L = TileSmem<PAIR>;
@@ -893,7 +938,8 @@ template <bool PAIR, bool TURNED> int launch_tiles(const void *a, const void *b,
   int rc = allow_smem(gemm_mxfp4_tiles_kernel<PAIR, TURNED>, L::kDynamic, configured);
   if (rc != QL_OK) return rc;
   int pitch = args.kb;
-  if (needs_padding(args)) {
+  const bool padding = needs_padding(args);
+  if (padding) {
     pitch = padded_pitch(args.kb);
     const int units = pitch / 16;
     const int64_t row_blocks = ((int64_t)args.M + args.N + 7) / 8;
@@ -907,8 +953,8 @@ template <bool PAIR, bool TURNED> int launch_tiles(const void *a, const void *b,
   CUtensorMap ma, mb, msa, msb;
   if ((rc = encode_map(&ma, KIND_F8, a, args.M, K / 2, BM)) != QL_OK) return rc;
   if ((rc = encode_map(&mb, KIND_F8, b, args.N, K / 2, L::kRowsB)) != QL_OK) return rc;
-  if ((rc = make_map_bytes(&msa, args.sfa, args.M, pitch, 32, BM)) != QL_OK) return rc;
-  if ((rc = make_map_bytes(&msb, args.sfb, args.N, pitch, 32, TBN)) != QL_OK) return rc;
+  if ((rc = encode_map_scales(&msa, args.sfa, args.M, pitch, BM)) != QL_OK) return rc;
+  if ((rc = encode_map_scales(&msb, args.sfb, args.N, pitch, TBN)) != QL_OK) return rc;
   args.tiles_a = (args.M + (PAIR ? 2 : 1) * BM - 1) / ((PAIR ? 2 : 1) * BM);
   args.tiles_b = (args.N + TBN - 1) / TBN;
   const int64_t tiles = (int64_t)args.tiles_a * args.tiles_b;
@@ -918,11 +964,13 @@ template <bool PAIR, bool TURNED> int launch_tiles(const void *a, const void *b,
   cfg.blockDim = dim3(kTileThreads, 1, 1);
   cfg.dynamicSmemBytes = L::kDynamic;
   cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = PAIR ? 2 : 1, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = PAIR ? 2 : 1, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization; // it starts while the scales are being padded
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = padding ? 2 : 1;
   QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_mxfp4_tiles_kernel<PAIR, TURNED>, ma, mb, msa, msb, args));
   count_launches(1);
   return QL_OK;

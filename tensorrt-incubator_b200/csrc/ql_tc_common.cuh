@@ -231,6 +231,9 @@ __device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity) {
 __device__ __forceinline__ void tc_commit_both(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
+// A kernel launched to start as soon as every CTA of the one before it has said so waits for that one's results itself.
+__device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_results() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Arrival at a barrier of another CTA of the cluster that need not publish this thread's writes: what it announces, stores to
 // tensor memory, is ordered by the tcgen05 fences.  The release at cluster scope of mbar_arrive_cluster takes about 1000 cycles.
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
