@@ -133,41 +133,6 @@ struct PairSmem {
 };
 static_assert(PairSmem::kDynamic <= 232448, "shared memory");
 
-// 32 rows x 128 bytes of a warp, parked with the copy engine's swizzle and written out by one bulk tensor store (whole lines,
-// clipped at the matrix's edges); two buffers.
-struct Parked {
-  uint8_t *base;
-  __device__ __forceinline__ void put(int buf, int lane, int piece, const uint4 &v) {
-    *reinterpret_cast<uint4 *>(base + buf * 4096 + lane * 128 + ((piece ^ (lane & 7)) << 4)) = v;
-  }
-  __device__ __forceinline__ void send(int buf, const CUtensorMap *map, int lane, int x, int y) {
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      tma_store_2d(map, smem_u32(base + buf * 4096), x, y);
-      bulk_commit();
-    }
-  }
-  __device__ __forceinline__ void send_layer(int buf, const CUtensorMap *map, int lane, int x, int y, int z) {
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
-                   ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(base + buf * 4096)), "r"(x), "r"(y), "r"(z)
-                   : "memory");
-      bulk_commit();
-    }
-  }
-  template <int PENDING> __device__ __forceinline__ void reusable(int lane) { // the buffer about to be rewritten has been read
-    if (lane == 0) bulk_wait_read<PENDING>();
-    __syncwarp();
-  }
-  __device__ __forceinline__ void finish(int lane) {
-    if (lane == 0) bulk_wait_all<0>();
-    __syncwarp();
-  }
-};
-
 // The backward pass's kernels are launched as soon as all CTAs of the one before have started: they set up barriers and tensor
 // memory where an SM is free, and wait here for its results.  dependents_may_start() comes at the start of a kernel; nothing is
 // written before the wait, and the first kernel of a call is launched in the stream's order.  77 x 2744 x 1032 27.2 us, 29.1

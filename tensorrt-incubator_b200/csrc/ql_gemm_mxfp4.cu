@@ -7,10 +7,10 @@
 //
 // The tensor core wants the scales of 128 rows as 4 columns of 32 lanes (row r in lane r % 32, column r / 32), repeated in
 // all four lane quarters of tensor memory.  The operands' scales are row-major, a row's bytes in a line.  The NVFP4 kernel
-// re-orders them in a kernel of its own and copies them from shared to tensor memory with tcgen05.cp, one 32-bit cell a
-// cycle and quarter, which is what bounds it.  Here four warps (one per quarter) take the bytes of "their" rows into
-// registers in the layout they already need -- lane l holds rows l, l + 32, ... -- and store them with tcgen05.st, 32 lanes
-// a cycle: no re-ordering pass and no copy instructions between the MMAs.
+// re-orders them in a kernel of its own and copies them from shared to tensor memory between its MMAs.  Here four warps (one
+// per quarter; two such sets in the tiles kernel) take the bytes of "their" rows into registers in the layout they already
+// need -- lane l holds rows l, l + 32, ... -- and store them with tcgen05.st: no re-ordering pass and no copy instructions
+// between the MMAs.
 //
 // Two kernels:
 //   split   few output tiles (decoding, short prompts): the weights are the 128-row operand and up to 128 tokens the other;
@@ -19,7 +19,8 @@
 //   tiles   many output tiles, persistent: one CTA per SM on 128 x 208 tiles, or CTA pairs on 256 x 208 tiles.  In a pair
 //           (tcgen05.mma.cta_group::2, issued by its leader) each CTA holds its own 128 rows of A and half of the B tile, so
 //           per MMA it reads 232 rows of operands from shared memory instead of 336; the scales of all 208 columns are needed
-//           by both.
+//           by both.  Whole 128-byte pieces of Y's rows leave by bulk tensor stores (4096 x 8192 x 512 24 us, 39 with each lane
+//           storing its row).
 // Every wait is bounded, as in the other tensor-core kernels.
 #include <cuda.h>
 #include <string.h>
@@ -408,8 +409,10 @@ gemm_mxfp4_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 // ------------------------------------------------------------------------------------------------------------------
 // tiles kernel: persistent, 128 x 208, or 256 x 208 by CTA pairs
 // ------------------------------------------------------------------------------------------------------------------
-// The width leaves tensor memory, beside two accumulators, 96 columns: two slots of the scales of two k steps.  With 224 there
-// is room for two slots of one step, and refilling one (the commit, the hand-over, the store) takes longer than a step.
+// The width leaves tensor memory, beside two accumulators, 96 columns: four slots of the scales of one k step.  A slot is free
+// when the MMAs of its step are done, and refilled (the commit, the wait, the stores, the arrival at the pair's leader) about
+// 1100 cycles later: three steps (416 cycles each) hide that.  Two slots of two steps, the stage in between hiding it: 8192 x
+// 28672 x 8192 765 us, 715 now.  With 224 columns there is room for two slots of one step.
 constexpr int TBN = 208;
 constexpr int kTileThreads = 448;   // producer, MMA, four epilogue warps, two sets of four scale warps
 constexpr int kScSteps = 4;         // k steps whose scales travel together: 32 bytes, a whole sector, of every row
@@ -425,24 +428,25 @@ template <bool PAIR> struct TileSmem {
   static constexpr int kTileB = kRowsB * BK_BYTES;
   static constexpr int kStageBytes = kStageSteps * (MX_A_BYTES + kTileB);  // A's tiles, then B's
   static constexpr int kScales = kStages * kStageBytes;
-  static constexpr int kBarriers = kScales + 2 * T_SC_BYTES; // full[S], empty[S], tfull[2], tempty[2], scfull[2], scempty[2], sfull[4], sempty[4], drain
+  static constexpr int kStaging = kScales + 2 * T_SC_BYTES;  // the epilogue's, 4096 bytes a warp
+  static constexpr int kBarriers = kStaging + 4 * 4096; // full[S], empty[S], tfull[2], tempty[2], scfull[2], scempty[2], sfull[4], sempty[4], drain
   static constexpr int kTmemPtr = kBarriers + (2 * kStages + 9 + 2 * kSlots) * 8;
   static constexpr int kAbort = kTmemPtr + 4;
   static constexpr int kDynamic = kAbort + 4 + 1024;
-  static_assert(kDynamic <= 232448 && kStageBytes % 1024 == 0 && T_SC_BYTES % 128 == 0, "tile shape");
+  static_assert(kDynamic <= 232448 && kStageBytes % 1024 == 0 && T_SC_BYTES % 1024 == 0, "tile shape");
 };
 
-// `cols` (a multiple of the 16-byte piece, at most 32) columns of one accumulator row a lane, rounded to y's type
+// A tile's last 16 columns, or the `cols` (a multiple of the 16-byte piece) of them that Y has, of one row a lane, rounded to y's type
 template <typename OutT>
 __device__ __forceinline__ void mx_store_chunk(OutT *y, const uint32_t (&r)[32], int cols) {
   if constexpr (sizeof(OutT) == 4) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 4)
+    for (int j = 0; j < 16; j += 4)
       if (j < cols) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]));
   } else {
     auto two = [&](int j) { return pack2<OutT>(__uint_as_float(r[j]), __uint_as_float(r[j + 1])); };
 #pragma unroll
-    for (int j = 0; j < 32; j += 8)
+    for (int j = 0; j < 16; j += 8)
       if (j < cols) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
   }
 }
@@ -460,7 +464,7 @@ __device__ __forceinline__ void mx_store_turned(OutT *y, const uint32_t (&r)[32]
 template <bool PAIR, bool TURNED>
 __global__ void __launch_bounds__(kTileThreads, 1)
 gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sa,
-                        const __grid_constant__ CUtensorMap map_sb, const MxArgs args) {
+                        const __grid_constant__ CUtensorMap map_sb, const __grid_constant__ CUtensorMap map_y, const MxArgs args) {
   using L = TileSmem<PAIR>;
   constexpr int TSTAGES = L::kStages;
   constexpr uint32_t kTmemCols = 512; // two accumulators, two slots of scales
@@ -722,27 +726,46 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
   } else {
     // ------------------------------------------------------------------ epilogue (warps 2..5)
     const int quad = warp & 3;
+    const bool wide = args.y_dtype == QL_F32;
+    Parked out{smem + L::kStaging + quad * 4096};
     int it = 0;
     for (int tile = first_tile; tile < num_tiles; tile += tile_stride, it++) {
       const int buf = it & 1;
       const int mt = tile % args.tiles_a, nt = tile / args.tiles_a;
       if (!warp_wait(tfull_bar(buf), (it >> 1) & 1, abort_flag, args.status, ST_TIMEOUT_TMEM_FULL)) { tell_partner(); break; }
       tc_fence_after();
-      const int m = (row_tile * mt + (int)rank) * BM + quad * 32 + lane;
+      const int m0 = (row_tile * mt + (int)rank) * BM + quad * 32, m = m0 + lane;
       const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * TBN);
 #pragma unroll 1
       for (int c = 0; c < (TBN + 31) / 32; c++) {
+        const int n = nt * TBN + c * 32, cols = min(min(args.N, nt * TBN + TBN) - n, 32);
+        if (m0 >= args.M || (cols <= 0 && (TURNED || wide || (c & 1) == 0))) break; // nothing left to store
         uint32_t r[32];
         tmem_load_32(taddr + c * 32, r); // of the last chunk half the columns are the next accumulator's, or scales: not stored
-        const int n = nt * TBN + c * 32, cols = min(min(args.N, nt * TBN + TBN) - n, 32);
-        if (cols <= 0) break;
-        if (m < args.M) {
+        if (!TURNED && c < TBN / 32) { // 128 bytes of a row: 32 values of f32, or 64 of 16 bits
+          if (wide || (c & 1) == 0) out.reusable<0>(lane);
+          auto put16 = [&](auto type) {
+            using OutT = decltype(type);
+            auto two = [&](int j) { return pack2<OutT>(__uint_as_float(r[j]), __uint_as_float(r[j + 1])); };
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) out.put(0, lane, (c & 1) * 4 + (j >> 3), make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
+          };
+          if (wide) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) out.put(0, lane, j >> 2, make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]));
+          } else if (args.y_dtype == QL_F16) {
+            put16(__half());
+          } else {
+            put16(__nv_bfloat16());
+          }
+          if (wide || (c & 1) == 1) out.send(0, &map_y, lane, wide ? n : n - 32, m0);
+        } else if (m < args.M) { // the tile's last 16 columns, or TURNED
           const size_t at = TURNED ? (size_t)n * (size_t)args.M + m : (size_t)m * (size_t)args.N + n;
           auto store = [&](auto *y) {
             if constexpr (TURNED) mx_store_turned(y, r, cols, (size_t)args.M);
             else mx_store_chunk(y, r, cols);
           };
-          if (args.y_dtype == QL_F32) store(static_cast<float *>(args.Y) + at);
+          if (wide) store(static_cast<float *>(args.Y) + at);
           else if (args.y_dtype == QL_F16) store(static_cast<__half *>(args.Y) + at);
           else store(static_cast<__nv_bfloat16 *>(args.Y) + at);
         }
@@ -751,6 +774,7 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
       __syncwarp();
       if (lane == 0) arrive_leader(tempty_bar(buf));
     }
+    if (!TURNED) out.finish(lane);
   }
 
   tc_fence_before();
@@ -813,7 +837,7 @@ struct SplitPlan {
 // How to cut a product of few tiles: `rows` of the weights per CTA, 2^log2 CTAs sharing K, `co` CTAs per SM.  The estimate
 // of each choice's time comes from measurements on B200 (graph-replayed calls, cold weights): 3.3 us fixed; per k step
 // 0.33 us, 0.0029 us more for every token row beyond 16, or what one SM's share of memory bandwidth (48 KB/us) takes;
-// 1.2 us + 0.033 us per token row to add up the parts of a cluster.  Examples (us; M, N, K):
+// 1.2 us + 0.033 us per token row to add up the parts of a cluster, or half of that to store more than 32 tokens.  Examples (us; M, N, K):
 //   1 x 28672 x 8192    100 rows, 2 CTAs per SM 23.5   |  128 rows, 1 per SM (two waves) 30.8  |  K over 4 CTAs 31.5
 //   1 x 4096 x 4096     128 rows, K over 4 CTAs 6.4    |  28 rows, K whole 9.4
 //   24 x 4096 x 11008   128 rows, K over 4 CTAs 11.0   |  28 rows, K whole 18.3
@@ -831,7 +855,8 @@ template <int TN, bool WIDE> SplitPlan plan_split(int M, int N, int num_ks) {
       const int64_t tiles = (int64_t)((N + rows - 1) / rows) * tiles_x, waves = (tiles + fit - 1) / fit;
       const int steps = (num_ks + (1 << log2) - 1) >> log2;
       const double latency = 0.33 + 0.0029 * (TN - 16), bandwidth = (double)(rows + TN) * BK_BYTES * co / 48e3;
-      const double us = (double)waves * (3.3 + 0.5 * (co - 1) + (log2 ? 1.2 + 0.033 * TN : 0.0) + steps * (latency > bandwidth ? latency : bandwidth));
+      const double join = log2 ? 1.2 + 0.033 * TN : (TN >= 64 ? 1.2 + 0.016 * TN : 0.0);
+      const double us = (double)waves * (3.3 + 0.5 * (co - 1) + join + steps * (latency > bandwidth ? latency : bandwidth));
       if (us < best.us) {
         int stages = (232448 / co - 2048 - (L::kRing + MX_A_BYTES + 1024)) / L::stage_bytes(rows);
         stages = stages > kSplitMaxStages ? kSplitMaxStages : stages;
@@ -911,7 +936,7 @@ __global__ void __launch_bounds__(256) mx_pad_scales_kernel(const uint8_t *__res
 }
 
 // The copy engine takes rows of whole 16-byte units from a 16-byte aligned base.  Other scales are copied into such rows first
-// (in the caller's workspace): 2000 x 4096 x 11040 51 us, against 47 at K = 11264 and 150 with the scale warps loading them.
+// (in the caller's workspace): 2000 x 4096 x 11008 47.5 us, against 45.7 at K = 11264; 150 with the scale warps loading them.
 int padded_pitch(int64_t kb) { return (int)((kb + 15) / 16 * 16); }
 bool needs_padding(const MxArgs &args) { return args.kb % 16 != 0 || !aligned16(args.sfa) || !aligned16(args.sfb); }
 int64_t padded_bytes(int64_t M, int64_t N, int64_t kb) { return (M + N) * padded_pitch(kb); }
@@ -950,11 +975,13 @@ template <bool PAIR, bool TURNED> int launch_tiles(const void *a, const void *b,
     args.sfa = static_cast<const uint8_t *>(workspace);
     args.sfb = args.sfa + (int64_t)args.M * pitch;
   }
-  CUtensorMap ma, mb, msa, msb;
+  CUtensorMap ma, mb, msa, msb, my;
   if ((rc = encode_map(&ma, KIND_F8, a, args.M, K / 2, BM)) != QL_OK) return rc;
   if ((rc = encode_map(&mb, KIND_F8, b, args.N, K / 2, L::kRowsB)) != QL_OK) return rc;
   if ((rc = encode_map_scales(&msa, args.sfa, args.M, pitch, BM)) != QL_OK) return rc;
   if ((rc = encode_map_scales(&msb, args.sfb, args.N, pitch, TBN)) != QL_OK) return rc;
+  my = ma; // TURNED: not used
+  if (!TURNED && (rc = encode_map_out(&my, args.y_dtype, args.Y, args.M, args.N, args.N)) != QL_OK) return rc;
   args.tiles_a = (args.M + (PAIR ? 2 : 1) * BM - 1) / ((PAIR ? 2 : 1) * BM);
   args.tiles_b = (args.N + TBN - 1) / TBN;
   const int64_t tiles = (int64_t)args.tiles_a * args.tiles_b;
@@ -971,7 +998,7 @@ template <bool PAIR, bool TURNED> int launch_tiles(const void *a, const void *b,
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = padding ? 2 : 1;
-  QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_mxfp4_tiles_kernel<PAIR, TURNED>, ma, mb, msa, msb, args));
+  QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_mxfp4_tiles_kernel<PAIR, TURNED>, ma, mb, msa, msb, my, args));
   count_launches(1);
   return QL_OK;
 }
@@ -1028,17 +1055,20 @@ extern "C" int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, cons
   args.tiles_a = args.tiles_b = 0;
   args.status = device_status_word();
   if (!args.status) return set_error(QL_ERR_CUDA, "%s: could not allocate the device status word", op);
-  // Pairs of the tiles kernel take 4.5 us and 0.45 us per k step and tile of a pair, its single CTAs 0.56; the split kernel what
-  // plan_split says.  Up to 32 tokens the tiles are mostly padding and the split kernel is the better one throughout; up to
-  // 128 rows of the first operand a pair's second half would be.  128 x 4096 x 4096: split 11.7 us, tiles 12.7; 128 x 28672 x
-  // 8192: 45.7, 28.0 (pairs 32); 512 x 11008 x 4096: single CTAs 21.9, pairs 20.4; 8192 x 28672 x 8192: 920, 800.
+  // Pairs of the tiles kernel take 4.5 us (3.5 more where scales are padded, 2 of them the host's) and, per tile, 0.45 us per k step, its single CTAs
+  // 0.56, or the 2.2 us that storing a tile takes beside it; the split kernel what plan_split says.  Up to 32 tokens the tiles
+  // are mostly padding and the split kernel is the better one throughout; up to 128 rows of the first operand a pair's second
+  // half would be.  Split and tiles, us: 128 x 1928 x 4736 11.8, 14.1; 1264 x 545 x 4384 14.5, 14.9; 534 x 1617 x 768 8.4, 8.7;
+  // 356 x 4440 x 5088 19.4, 16.2; 458 x 11848 x 480 23.8, 13.5.  Single CTAs and pairs: 128 x 28672 x 8192 28.0, 32; 512 x 11008 x
+  // 4096 21.9, 20.4; 8192 x 28672 x 8192 920, 720.
   const bool turned = N % (y->dtype == QL_F32 ? 4 : 8) != 0 || !aligned16(y->data);
   const int64_t R = turned ? N : M, C = turned ? M : N; // rows of the tiles kernel's operands
   const bool pairs = R > BM;
   const int64_t row_tiles = pairs ? (R + 2 * BM - 1) / (2 * BM) : (R + BM - 1) / BM, units = pairs ? sm_count() / 2 : sm_count();
   const int64_t tiles = row_tiles * ((C + TBN - 1) / TBN);
   if (tiles >= (1ll << 30)) return set_error(QL_ERR_UNSUPPORTED, "%s: too many output tiles", op);
-  const double tiles_us = M <= kSplitOnly ? 1e30 : 4.5 + (need > 0 ? 3.0 : 0.0) + (pairs ? 0.45 : 0.56) * (double)((tiles + units - 1) / units) * args.num_ks;
+  const double main_us = (pairs ? 0.45 : 0.56) * args.num_ks, store_us = C < TBN ? 2.2 * C / TBN : 2.2; // of a tile, one beside the other
+  const double tiles_us = M <= kSplitOnly ? 1e30 : 4.5 + (need > 0 ? 3.5 : 0.0) + (double)((tiles + units - 1) / units) * (main_us > store_us ? main_us : store_us);
   args.sfa = static_cast<const uint8_t *>(b_scales->data); // the weights are the 128-row operand of the split kernel
   args.sfb = static_cast<const uint8_t *>(a_scales->data);
   bool ran = false;
