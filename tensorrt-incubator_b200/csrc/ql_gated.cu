@@ -121,12 +121,13 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t tmem_d, uint64_t adesc, ui
 constexpr int G_TILE = 128 * BK_BYTES;      // 16 KiB: one CTA's half of an operand tile, 128 rows x 64 values or 64 x 128
 constexpr int G_STAGE = 2 * G_TILE;
 constexpr int G_STAGES = 6;
-constexpr int kPairThreads = 192;           // producer, MMA, four epilogue warps
+constexpr int kEpilogueWarps = 8;           // two for each quarter of tensor memory's lanes, which take 32 columns in turn
+constexpr int kPairThreads = 64 + 32 * kEpilogueWarps; // producer, MMA, epilogue
 constexpr int G_N = 256;                    // columns of the pair's accumulator
 
 struct PairSmem {
-  static constexpr int kStaging = G_STAGES * G_STAGE;       // the epilogue's: 4 warps x 2 x 4096 bytes
-  static constexpr int kBarriers = kStaging + 4 * 2 * 4096; // full[S], empty[S], tfull[2], tempty[2], drain
+  static constexpr int kStaging = G_STAGES * G_STAGE;       // the epilogue's, 4096 bytes a warp
+  static constexpr int kBarriers = kStaging + kEpilogueWarps * 4096; // full[S], empty[S], tfull[2], tempty[2], drain
   static constexpr int kTmemPtr = kBarriers + (2 * G_STAGES + 5) * 8;
   static constexpr int kAbort = kTmemPtr + 4;
   static constexpr int kDynamic = kAbort + 4 + 1024;
@@ -167,7 +168,7 @@ struct Pair {
       }
       for (int b = 0; b < 2; b++) {
         mbar_init(tfull(b), 1);
-        mbar_init(tempty(b), 8); // four epilogue warps in each CTA of the pair
+        mbar_init(tempty(b), 2 * kEpilogueWarps); // of both CTAs of the pair
       }
       mbar_init(drain(), 1);
       *abort_flag = 0;
@@ -296,56 +297,57 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       p.drain_mmas();
     }
   } else {
-    // ------------------------------------------------------------------ epilogue (warps 2..5, both CTAs)
-    const int quad = p.warp & 3, lane = p.lane;
-    Parked out{p.smem + PairSmem::kStaging + quad * 8192};
+    // ------------------------------------------------------------------ epilogue (warps 2..9, both CTAs)
+    const int quad = p.warp & 3, turn = (p.warp - 2) >> 2, lane = p.lane;
+    Parked out{p.smem + PairSmem::kStaging + (p.warp - 2) * 4096};
     int it = 0, b = 0; // b: the staging buffer whose turn it is (forward)
     bool ok = true;
+    uint4 ahead[4]; // dH of this warp's next chunk, of the next tile after a tile's last one: on its way while the one before is worked on
+    auto fetch = [&](int tile, int c) {
+      if (tile >= num_tiles) return;
+      int mt, nt;
+      band_coords(tile, args.tiles_m, args.tiles_n, args.group_m, &mt, &nt);
+      const int m = mt * 256 + (int)p.rank * 128 + quad * 32 + lane, n = nt * C + c * 32;
+      const T *row = static_cast<const T *>(args.dh) + (size_t)m * (size_t)args.I + n;
+#pragma unroll
+      for (int j = 0; j < 4; j++) ahead[j] = m < args.M && n + 8 * j < args.I ? __ldcs(reinterpret_cast<const uint4 *>(row) + j) : make_uint4(0u, 0u, 0u, 0u);
+    };
+    if constexpr (BACKWARD) fetch(cluster_id, turn);
     for (int tile = cluster_id; tile < num_tiles; tile += num_clusters, it++) {
       const int buf = it & 1;
       int mt, nt;
       band_coords(tile, args.tiles_m, args.tiles_n, args.group_m, &mt, &nt);
-      const int m0 = mt * 256 + (int)p.rank * 128 + quad * 32, m = m0 + lane;
-      uint4 ahead[4]; // dH of the next chunk, on its way while this one is worked on
-      auto fetch = [&](int c) {
-        const int n = nt * C + c * 32;
-        const T *row = static_cast<const T *>(args.dh) + (size_t)m * (size_t)args.I + n;
-#pragma unroll
-        for (int j = 0; j < 4; j++) ahead[j] = c < C / 32 && m < args.M && n + 8 * j < args.I ? __ldcs(reinterpret_cast<const uint4 *>(row) + j) : make_uint4(0u, 0u, 0u, 0u);
-      };
-      if constexpr (BACKWARD) fetch(0);
+      const int m0 = mt * 256 + (int)p.rank * 128 + quad * 32;
       ok = warp_wait(p.tfull(buf), (it >> 1) & 1, p.abort_flag, p.status, ST_TIMEOUT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after();
       const uint32_t taddr = p.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * G_N);
 #pragma unroll 1
-      for (int c = 0; c < C / 32; c++) { // 32 channels: gate in columns 32 c, up in columns C + 32 c
-        const int n = nt * C + c * 32, half = c & 1;
-        if (m0 >= args.M || (half == 0 && n >= args.I)) break; // nothing left to store
+      for (int c = turn; c < C / 32; c += 2) { // 32 channels: gate in columns 32 c, up in columns C + 32 c
+        const int n = nt * C + c * 32;
         uint4 dh[4];
         if constexpr (BACKWARD) {
 #pragma unroll
           for (int j = 0; j < 4; j++) dh[j] = ahead[j];
-          fetch(c + 1);
+          if (c + 2 < C / 32) fetch(tile, c + 2);
+          else fetch(tile + num_clusters, turn);
         }
+        if (m0 >= args.M || n >= args.I) continue; // nothing to store
         uint32_t g[32], u[32];
         tmem_load_32(taddr + c * 32, g);
         tmem_load_32(taddr + C + c * 32, u);
         if constexpr (!BACKWARD) {
-          if (half == 0) out.reusable<1>(lane);
           with_act(args.act, [&](auto act) {
 #pragma unroll
             for (int j = 0; j < 32; j++) g[j] = __float_as_uint(act_value<decltype(act)::value>(__uint_as_float(g[j])) * __uint_as_float(u[j]));
           });
           auto two = [&](int j) { return pack2<T>(__uint_as_float(g[j]), __uint_as_float(g[j + 1])); };
+          out.reusable<1>(lane);
 #pragma unroll
-          for (int j = 0; j < 32; j += 8) out.put(b, lane, half * 4 + (j >> 3), make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
-          if (half == 1) {
-            out.send(b, &map_out, lane, n - 32, m0);
-            b ^= 1;
-          }
+          for (int j = 0; j < 32; j += 8) out.put64(b, lane, j >> 3, make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
+          out.send64(b, &map_out, lane, n, m0);
+          b ^= 1;
         } else {
-          if (half == 0) out.reusable<0>(lane); // both buffers: dG in one, dU in the other
           const T *d = reinterpret_cast<const T *>(dh);
           with_act(args.act, [&](auto act) {
 #pragma unroll
@@ -358,15 +360,14 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             }
           });
           auto two = [&](const uint32_t (&v)[32], int j) { return pack2<T>(__uint_as_float(v[j]), __uint_as_float(v[j + 1])); };
+          out.reusable<0>(lane); // both buffers: dG in one, dU in the other
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
-            out.put(0, lane, half * 4 + (j >> 3), make_uint4(two(g, j), two(g, j + 2), two(g, j + 4), two(g, j + 6)));
-            out.put(1, lane, half * 4 + (j >> 3), make_uint4(two(u, j), two(u, j + 2), two(u, j + 4), two(u, j + 6)));
+            out.put64(0, lane, j >> 3, make_uint4(two(g, j), two(g, j + 2), two(g, j + 4), two(g, j + 6)));
+            out.put64(1, lane, j >> 3, make_uint4(two(u, j), two(u, j + 2), two(u, j + 4), two(u, j + 6)));
           }
-          if (half == 1) {
-            out.send(0, &map_out, lane, n - 32, m0);
-            out.send(1, &map_out2, lane, n - 32, m0);
-          }
+          out.send64(0, &map_out, lane, n, m0);
+          out.send64(1, &map_out2, lane, n, m0);
         }
       }
       tc_fence_before();
@@ -516,10 +517,9 @@ gated_grads_kernel(const __grid_constant__ CUtensorMap map_dg_k, const __grid_co
       p.drain_mmas();
     }
   } else {
-    // ------------------------------------------------------------------ epilogue (warps 2..5, both CTAs)
-    const int quad = p.warp & 3, lane = p.lane;
-    Parked out{p.smem + PairSmem::kStaging + quad * 8192};
-    int b = 0; // the staging buffer whose turn it is
+    // ------------------------------------------------------------------ epilogue (warps 2..9, both CTAs)
+    const int quad = p.warp & 3, turn = (p.warp - 2) >> 2, lane = p.lane;
+    Parked out{p.smem + PairSmem::kStaging + (p.warp - 2) * 4096};
     bool ok = true;
     for (int j = 0; get_unit(args, cluster_id, num_clusters, j, &u); j++) {
       const int buf = j & 1;
@@ -531,27 +531,26 @@ gated_grads_kernel(const __grid_constant__ CUtensorMap map_dg_k, const __grid_co
       const bool parts = (u.is_x ? args.x_parts : args.w_parts) != nullptr; // f32, a layer for each part of the reduction
       const int layer = u.is_x ? u.part : 2 * u.part + (u.up ? 1 : 0);
       const CUtensorMap *map = u.is_x ? &map_dx : (u.up && !parts ? &map_dwu : &map_dwg);
+      out.reusable<0>(lane); // a part takes the room of both 16-bit buffers
+      int b = 0;             // the buffer whose turn it is
 #pragma unroll 1
-      for (int c = 0; c < G_N / 32; c++) {
-        const int n = u.col0 + c * 32, half = c & 1;
-        if (r0 >= (u.is_x ? args.M : args.I) || ((parts || half == 0) && n >= args.K)) break; // nothing left to store
+      for (int c = turn; c < G_N / 32; c += 2) {
+        const int n = u.col0 + c * 32;
+        if (r0 >= (u.is_x ? args.M : args.I) || n >= args.K) break; // nothing left to store
         uint32_t v[32];
         tmem_load_32(taddr + c * 32, v);
-        if (parts) { // 32 values fill a staged row
+        if (parts) {
+          out.reusable<0>(lane);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) out.put(0, lane, i >> 2, make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+          out.send_layer(0, map, lane, n, r0, layer);
+        } else {
+          auto two = [&](int i) { return pack2<T>(__uint_as_float(v[i]), __uint_as_float(v[i + 1])); };
           out.reusable<1>(lane);
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) out.put(b, lane, i >> 2, make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]));
-          out.send_layer(b, map, lane, n, r0, layer);
+          for (int i = 0; i < 32; i += 8) out.put64(b, lane, i >> 3, make_uint4(two(i), two(i + 2), two(i + 4), two(i + 6)));
+          out.send64(b, map, lane, n, r0);
           b ^= 1;
-        } else {
-          if (half == 0) out.reusable<1>(lane);
-          auto two = [&](int i) { return pack2<T>(__uint_as_float(v[i]), __uint_as_float(v[i + 1])); };
-#pragma unroll
-          for (int i = 0; i < 32; i += 8) out.put(b, lane, half * 4 + (i >> 3), make_uint4(two(i), two(i + 2), two(i + 4), two(i + 6)));
-          if (half == 1) {
-            out.send(b, map, lane, n - 32, r0);
-            b ^= 1;
-          }
         }
       }
       tc_fence_before();
@@ -802,6 +801,21 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
 // ----------------------------------------------------------------------------------------------
 template <typename T> constexpr int kMapKind = FloatIO<T>::kDtype == QL_BF16 ? KIND_BF16 : KIND_F16;
 
+// 16-bit result [rows, cols], box = [32 rows, 32 columns], 64-byte swizzle (Parked::put64)
+int encode_map_narrow(CUtensorMap *map, int dtype, const void *ptr, int64_t rows, int64_t cols) {
+  EncodeTiledFn enc;
+  const int rc = get_encode_fn(&enc);
+  if (rc != QL_OK) return rc;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
+  cuuint32_t box[2] = {32, 32};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(map, dtype == QL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(ptr), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(QL_ERR_CUDA, "cuTensorMapEncodeTiled (16-bit result) failed with code %d", (int)r);
+  return QL_OK;
+}
+
 template <typename K> int resident(K kern, int threads, int smem, int cluster) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * sm_count() * cluster), 1, 1);
@@ -856,8 +870,8 @@ int launch_pair(const void *x, const void *wg, const void *wu, const void *dh, v
   if ((rc = encode_map(&mx, kind, x, M, K, 128)) != QL_OK) return rc;
   if ((rc = encode_map(&mg, kind, wg, I, K, C)) != QL_OK) return rc;
   if ((rc = encode_map(&mu, kind, wu, I, K, C)) != QL_OK) return rc;
-  if ((rc = encode_map_out(&mo, dtype, out, M, I, I)) != QL_OK) return rc;
-  if ((rc = encode_map_out(&mo2, dtype, out2 ? out2 : out, M, I, I)) != QL_OK) return rc;
+  if ((rc = encode_map_narrow(&mo, dtype, out, M, I)) != QL_OK) return rc;
+  if ((rc = encode_map_narrow(&mo2, dtype, out2 ? out2 : out, M, I)) != QL_OK) return rc;
   const int pairs = resident_cached(kern, kPairThreads, PairSmem::kDynamic, 2, cache), tiles = a.tiles_m * a.tiles_n;
   kern<<<2 * (tiles < pairs ? tiles : pairs), kPairThreads, PairSmem::kDynamic, st>>>(mx, mg, mu, mo, mo2, a);
   count_launches(1);
@@ -1054,10 +1068,10 @@ int backward(const void *dh, const void *x, const void *wg, const void *wu, void
   if ((rc = encode_map(&xm, kind, x, M, K, 64)) != QL_OK) return rc;
   mx = mg = mu = xm; // what is not wanted is not written
   if (a.x_parts) rc = encode_map_parts(&mx, a.x_parts, a.x_split, M, K);
-  else if (dx) rc = encode_map_out(&mx, dtype, dx, M, K, K);
+  else if (dx) rc = encode_map_narrow(&mx, dtype, dx, M, K);
   if (rc != QL_OK) return rc;
   if (a.w_parts) rc = encode_map_parts(&mg, a.w_parts, 2 * a.w_split, I, K);
-  else if (dwg && (rc = encode_map_out(&mg, dtype, dwg, I, K, K)) == QL_OK) rc = encode_map_out(&mu, dtype, dwu, I, K, K);
+  else if (dwg && (rc = encode_map_narrow(&mg, dtype, dwg, I, K)) == QL_OK) rc = encode_map_narrow(&mu, dtype, dwu, I, K);
   if (rc != QL_OK) return rc;
   const int pairs = grad_pairs<T>(); // get_unit deals the units out over exactly this many
   cudaLaunchAttribute early;

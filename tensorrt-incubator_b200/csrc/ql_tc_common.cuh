@@ -249,11 +249,17 @@ struct Parked {
   __device__ __forceinline__ void put(int buf, int lane, int piece, const uint4 &v) {
     *reinterpret_cast<uint4 *>(base + buf * 4096 + lane * 128 + ((piece ^ (lane & 7)) << 4)) = v;
   }
-  __device__ __forceinline__ void send(int buf, const CUtensorMap *map, int lane, int x, int y) {
+  __device__ __forceinline__ void send(int buf, const CUtensorMap *map, int lane, int x, int y) { send_from(base + buf * 4096, map, lane, x, y); }
+  // the same with rows of 64 bytes and the engine's 64-byte swizzle, buffers of 2048 bytes
+  __device__ __forceinline__ void put64(int buf, int lane, int piece, const uint4 &v) {
+    *reinterpret_cast<uint4 *>(base + buf * 2048 + lane * 64 + ((piece ^ ((lane >> 1) & 3)) << 4)) = v;
+  }
+  __device__ __forceinline__ void send64(int buf, const CUtensorMap *map, int lane, int x, int y) { send_from(base + buf * 2048, map, lane, x, y); }
+  __device__ __forceinline__ void send_from(const uint8_t *from, const CUtensorMap *map, int lane, int x, int y) {
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
-      tma_store_2d(map, smem_u32(base + buf * 4096), x, y);
+      tma_store_2d(map, smem_u32(from), x, y);
       bulk_commit();
     }
   }
