@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(kReduceThreads) grads_reduce_kernel(const floa
 // ------------------------------------------------------------------------------------------------------------------
 // few tokens: the weights as the 128-row operand, K over the CTAs of a cluster
 // ------------------------------------------------------------------------------------------------------------------
-constexpr int kSplitThreads = 192;
+template <bool WIDE> constexpr int kSplitThreads = WIDE ? 320 : 192; // producer, MMA, four or eight warps on the accumulators
 constexpr int kSplitMaxStages = 16;
 constexpr int kMaxSplit = 8;
 
@@ -622,9 +622,9 @@ struct SplitArgs {
 
 // Fixed parts first, then the ring: `stages` of (channels rounded up to 8) gate rows, as many up rows and TN tokens of 128
 // bytes each.  The MMA reads 128 rows whatever there is of them; the rest lands in accumulator rows nobody looks at.
-template <int TN> struct SplitSmem {
-  static constexpr int kParts = 0;                      // this CTA's tokens, [split][TN / split][128]
-  static constexpr int kBarriers = kParts + TN * BM * 4; // full[16], empty[16], tfull
+template <int TN, bool WIDE> struct SplitSmem {
+  static constexpr int kParts = 0;                                      // this CTA's tokens, [split][TN / split][128]
+  static constexpr int kBarriers = kParts + (WIDE ? 0 : TN * BM * 4); // full[16], empty[16], tfull
   static constexpr int kTmemPtr = kBarriers + (2 * kSplitMaxStages + 1) * 8;
   static constexpr int kAbort = kTmemPtr + 4;
   static constexpr int kRing = (kAbort + 4 + 1023) / 1024 * 1024;
@@ -632,13 +632,16 @@ template <int TN> struct SplitSmem {
   static constexpr int total(int channels, int stages) { return kRing + stages * stage_bytes(channels) + BM * BK_BYTES + 1024; }
 };
 
-template <typename T, int TN, bool BACKWARD>
-__global__ void __launch_bounds__(kSplitThreads)
+// WIDE: up to 128 channels, gate and up rows each as a 128-row operand with an accumulator of its own; a lane then holds both of
+// its channel, and nothing is shared out.  For 33 to 128 tokens, where one wave of CTAs has to take more than 64 channels each to
+// read the weights once.
+template <typename T, int TN, bool BACKWARD, bool WIDE>
+__global__ void __launch_bounds__(kSplitThreads<WIDE>)
 gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_constant__ CUtensorMap map_up, const __grid_constant__ CUtensorMap map_x,
                    const SplitArgs args, int channels, int stages, int split_log2) {
-  using L = SplitSmem<TN>;
+  using L = SplitSmem<TN, WIDE>;
   constexpr int TN_LOG2 = TN == 16 ? 4 : (TN == 32 ? 5 : (TN == 64 ? 6 : 7));
-  constexpr uint32_t kTmemCols = TN < 32 ? 32 : TN;
+  constexpr uint32_t kTmemCols = WIDE ? 2 * TN : (TN < 32 ? 32 : TN);
   const int c8 = (channels + 7) / 8 * 8, stage_bytes = L::stage_bytes(channels), x_off = stage_bytes - TN * BK_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -713,7 +716,10 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
         const uint32_t a = smem_base + L::kRing + stage * stage_bytes;
         const uint64_t adesc = make_smem_desc(a), bdesc = make_smem_desc(a + x_off);
 #pragma unroll
-        for (int k = 0; k < 4; k++) tc_mma<KIND_F16>(tmem_base, adesc + 2 * k, bdesc + 2 * k, idesc, (kb > kb0 || k) ? 1u : 0u);
+        for (int k = 0; k < 4; k++) {
+          tc_mma<KIND_F16>(tmem_base, adesc + 2 * k, bdesc + 2 * k, idesc, (kb > kb0 || k) ? 1u : 0u);
+          if (WIDE) tc_mma<KIND_F16>(tmem_base + TN, make_smem_desc(a + c8 * BK_BYTES) + 2 * k, bdesc + 2 * k, idesc, (kb > kb0 || k) ? 1u : 0u);
+        }
         tc_commit(empty_bar(stage));
       }
       __syncwarp();
@@ -724,6 +730,47 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
     __syncwarp();
     if (!bounded_wait(tfull_bar, 0) && lane == 0) atomicCAS(args.status, 0, ST_TIMEOUT_DRAIN);
     if (split > 1) cluster_wait();
+  } else if (WIDE) {
+    // ------------------------------------------------------------------ the accumulators (warps 2..9): a channel a lane, every
+    // other 16 tokens a warp
+    const int quad = warp & 3, row = quad * 32 + lane, ch = ct * channels + row;
+    const bool mine = row < channels && ch < args.I;
+    const T *dh = static_cast<const T *>(args.dh);
+    T *out = static_cast<T *>(args.out), *out2 = static_cast<T *>(args.out2);
+    warp_wait(tfull_bar, 0, abort_flag, args.status, ST_TIMEOUT_TMEM_FULL);
+    tc_fence_after();
+    const int tokens = min(TN, args.M - xt * TN);
+    with_act(args.act, [&](auto act) {
+#pragma unroll 1
+      for (int c = (warp - 2) >> 2; c * 16 < tokens && quad * 32 < channels; c += 2) {
+        uint32_t g[16], u[16];
+        float d[16];
+        const size_t at = (size_t)(xt * TN + c * 16) * (size_t)args.I + ch;
+        if constexpr (BACKWARD) {
+#pragma unroll
+          for (int j = 0; j < 16; j++) d[j] = mine && c * 16 + j < tokens ? FloatIO<T>::to_f32(dh[at + (size_t)j * (size_t)args.I]) : 0.f;
+        }
+        tmem_load_16(tmem_base + ((uint32_t)(quad * 32) << 16) + c * 16, g);
+        tmem_load_16(tmem_base + ((uint32_t)(quad * 32) << 16) + TN + c * 16, u);
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+          const float z = __uint_as_float(g[j]), up = __uint_as_float(u[j]);
+          const bool on = mine && c * 16 + j < tokens;
+          if constexpr (BACKWARD) {
+            float a, da;
+            act_both<decltype(act)::value>(z, a, da);
+            if (on) {
+              out[at + (size_t)j * (size_t)args.I] = FloatIO<T>::from_f32(d[j] * up * da);
+              out2[at + (size_t)j * (size_t)args.I] = FloatIO<T>::from_f32(d[j] * a);
+            }
+          } else {
+            const float h = act_value<decltype(act)::value>(z) * up;
+            if (on) out[at + (size_t)j * (size_t)args.I] = FloatIO<T>::from_f32(h);
+          }
+        }
+      }
+    });
+    tc_fence_before();
   } else {
     // ------------------------------------------------------------------ the accumulator (warps 2..5)
     const int quad = warp & 3, row = quad * 32 + lane;
@@ -751,19 +798,20 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
   if (split > 1 && warp == 0) cluster_wait();
   __syncthreads();
   if (split > 1) cluster_sync_all(); // every part has arrived
-  {
+  if constexpr (!WIDE) {
+    constexpr int kThreads = kSplitThreads<WIDE>;
     const int per = TN >> split_log2, t0 = rank * per, t1 = min(t0 + per, args.M - xt * TN);
     const float *parts = reinterpret_cast<const float *>(smem + L::kParts);
     T *out = static_cast<T *>(args.out), *out2 = static_cast<T *>(args.out2);
     const int here = min(channels, args.I - ct * channels), items = (t1 - t0) * here;
     with_act(args.act, [&](auto act) {
       constexpr int U = BACKWARD ? 4 : 1; // values a thread works on at once, where it has dH to wait for
-      for (int i0 = threadIdx.x; i0 < items; i0 += U * kSplitThreads) {
+      for (int i0 = threadIdx.x; i0 < items; i0 += U * kThreads) {
         float g[U], u[U], d[U];
         size_t at[U];
 #pragma unroll
         for (int k = 0; k < U; k++) {
-          const int i = min(i0 + k * kSplitThreads, items - 1), t = i / here, ch = i - t * here;
+          const int i = min(i0 + k * kThreads, items - 1), t = i / here, ch = i - t * here;
           at[k] = (size_t)(xt * TN + t0 + t) * (size_t)args.I + ct * channels + ch;
           if constexpr (BACKWARD) d[k] = FloatIO<T>::to_f32(static_cast<const T *>(args.dh)[at[k]]);
           g[k] = u[k] = 0.f;
@@ -777,7 +825,7 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
         }
 #pragma unroll
         for (int k = 0; k < U; k++) {
-          if (i0 + k * kSplitThreads >= items) break;
+          if (i0 + k * kThreads >= items) break;
           if constexpr (BACKWARD) {
             float a, da;
             act_both<decltype(act)::value>(g[k], a, da);
@@ -885,13 +933,13 @@ struct SplitPlan {
 };
 
 template <typename T, int TN, bool BACKWARD> SplitPlan plan_split(int M, int I, int num_kb) {
-  using L = SplitSmem<TN>;
+  using L = SplitSmem<TN, false>;
   static int cache[4][64] = {};
   const int64_t tiles_x = (M + TN - 1) / TN;
   SplitPlan best = {1, 0, 64, 1, 1e30};
   for (int co = 1; co <= (TN <= 32 ? 2 : 1); co++) {
     for (int log2 = 0; log2 < 4 && (log2 == 0 || num_kb >= (4 << log2)); log2++) {
-      const int fit = resident_cached(gated_split_kernel<T, TN, BACKWARD>, kSplitThreads, 232448, 1 << log2, cache[log2]) * co;
+      const int fit = resident_cached(gated_split_kernel<T, TN, BACKWARD, false>, kSplitThreads<false>, 232448, 1 << log2, cache[log2]) * co;
       const int64_t per_x = fit / tiles_x, want = per_x < 1 ? 64 : (I + per_x - 1) / per_x;
       const int channels = (int)(want > 64 ? 64 : (want < 8 ? 8 : want));
       const int64_t tiles = (int64_t)((I + channels - 1) / channels) * tiles_x, waves = (tiles + fit - 1) / fit;
@@ -909,12 +957,24 @@ template <typename T, int TN, bool BACKWARD> SplitPlan plan_split(int M, int I, 
   return best;
 }
 
+// WIDE: as many channels a CTA as let one wave cover them, K whole, one CTA per SM.  5.3 us, 0.03 us per token to store, and per
+// step of 64 values of K 0.30 us for its eight MMAs, or the weights' time at an SM's share of memory bandwidth.
+template <int TN> SplitPlan plan_wide(int M, int I, int num_kb) {
+  const int64_t fit = sm_count(), want = (I + fit - 1) / fit;
+  const int channels = (int)(want > BM ? BM : (want < 8 ? 8 : want));
+  const int64_t tiles = (I + channels - 1) / channels, waves = (tiles + fit - 1) / fit;
+  const double memory = 2.0 * channels * BK_BYTES / 41.5e3, step = memory > 0.30 ? memory : 0.30;
+  int stages = (232448 - 2048 - SplitSmem<TN, true>::total(channels, 0)) / SplitSmem<TN, true>::stage_bytes(channels);
+  stages = stages > kSplitMaxStages ? kSplitMaxStages : stages;
+  return {1, 0, channels, stages > num_kb ? num_kb : stages, (double)waves * (5.3 + 0.03 * M + num_kb * step)};
+}
+
 // Runs the split kernel where its estimate is below `limit_us`, else says so in *ran.
-template <typename T, int TN, bool BACKWARD>
+template <typename T, int TN, bool BACKWARD, bool WIDE>
 int launch_split(const void *x, const void *wg, const void *wu, const void *dh, void *out, void *out2, int M, int I, int K, int act, double limit_us, bool *ran,
                  cudaStream_t st) {
-  using L = SplitSmem<TN>;
-  auto kern = gated_split_kernel<T, TN, BACKWARD>;
+  using L = SplitSmem<TN, WIDE>;
+  auto kern = gated_split_kernel<T, TN, BACKWARD, WIDE>;
   static bool configured[64] = {false};
   int rc = allow_smem(kern, 232448, configured);
   if (rc != QL_OK) return rc;
@@ -922,7 +982,9 @@ int launch_split(const void *x, const void *wg, const void *wu, const void *dh, 
   a.dh = dh, a.out = out, a.out2 = out2;
   a.M = M, a.I = I, a.act = act;
   a.num_kb = (K + 63) / 64;
-  const SplitPlan plan = plan_split<T, TN, BACKWARD>(M, I, a.num_kb);
+  SplitPlan plan;
+  if constexpr (WIDE) plan = plan_wide<TN>(M, I, a.num_kb);
+  else plan = plan_split<T, TN, BACKWARD>(M, I, a.num_kb);
   *ran = plan.us <= limit_us;
   if (!*ran) return QL_OK;
   a.tiles_c = (I + plan.channels - 1) / plan.channels;
@@ -935,7 +997,7 @@ int launch_split(const void *x, const void *wg, const void *wu, const void *dh, 
   if ((rc = encode_map(&mx, kind, x, M, K, TN)) != QL_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(((int64_t)a.tiles_c * ((M + TN - 1) / TN)) << plan.log2), 1, 1);
-  cfg.blockDim = dim3(kSplitThreads, 1, 1);
+  cfg.blockDim = dim3(kSplitThreads<WIDE>, 1, 1);
   cfg.dynamicSmemBytes = L::total(plan.channels, plan.stages);
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -949,24 +1011,40 @@ int launch_split(const void *x, const void *wg, const void *wu, const void *dh, 
 }
 
 // The two projections, by whichever kernel is estimated the faster: pairs take 7.2 us and 0.28 us per tile of 128 channels and 64
-// values of K, or 5.2 and 0.23 per tile of 64 channels (half the MMAs and half the epilogue, but as many rows of X to load);
-// the split kernel what plan_split says.  Up to 32 tokens a pair's 256 rows are mostly padding.  Forward, us (M x I x K):
+// values of K, or 5.2 and 0.23 per tile of 64 channels (half the MMAs and half the epilogue, but as many rows of X to load), or
+// what a wave's weights take at 6 TB/s, and 0.3 (0.8) for every further tile; the split kernels what plan_split and plan_wide say.  Up to 32 tokens a pair's 256 rows
+// are mostly padding.  Forward, us (M x I x K):
 //   256 x 512 x 4096    split 14.4, pairs 24.9     |  2314 x 80 x 6296  split 24.8, pairs 38.8
-//   211 x 2744 x 1032   split 20.9, pairs 13.3, of 64 channels 10.8  |  256 x 9472 x 4096  pairs 36.1, of 64 channels 41.7
-//   128 x 11008 x 4096  split 75, pairs 51.1, of 64 channels 52.9    |  512 x 2368 x 4096  pairs 25.9, of 64 channels 20.9
+//   211 x 2744 x 1032   split 20.9, pairs 13.3, of 64 channels 10.5  |  256 x 9472 x 4096  pairs 36.1, of 64 channels 41.7
+//   128 x 11008 x 4096  pairs 50.1, wide split 39.4  |  64 x 11008 x 4096  pairs 50.1, wide split 36.0
+//   128 x 9472 x 2048   pairs 19.8, wide split 21.9  |  512 x 2368 x 4096  pairs 25.9, of 64 channels 20.9
 template <typename T, bool BACKWARD>
 int project(const void *x, const void *wg, const void *wu, const void *dh, void *out, void *out2, int M, int I, int K, int act, cudaStream_t st) {
-  const int64_t pairs = sm_count() / 2, rows = (M + 255) / 256;
-  auto per_pair = [&](int c) { return (double)((rows * ((I + c - 1) / c) + pairs - 1) / pairs * ((K + 63) / 64)); };
-  const double wide_us = 7.2 + 0.28 * per_pair(128), narrow_us = 5.2 + 0.23 * per_pair(64);
-  const bool narrow = narrow_us < wide_us;
-  const double pair_us = M <= 32 ? 1e30 : (narrow ? narrow_us : wide_us);
+  const int num_kb = (K + 63) / 64;
+  auto pairs_us = [&](int c, double fixed, double step, double next) {
+    const int64_t pairs = sm_count() / 2, rows = (M + 255) / 256, tiles = rows * ((I + c - 1) / c), rest = tiles % pairs;
+    const double bytes = 2.0 * c * BK_BYTES / (double)rows; // of weights from memory, per step and pair; other row tiles find them in L2
+    auto wave = [&](int64_t n) { return n == 0 ? 0.0 : (step > bytes * (double)n / 6e6 ? step : bytes * (double)n / 6e6); };
+    return fixed + next * (double)((tiles - 1) / pairs) + num_kb * ((double)(tiles / pairs) * wave(pairs) + wave(rest));
+  };
+  const double full_us = pairs_us(128, 7.2, 0.28, 0.3), narrow_us = pairs_us(64, 5.2, 0.23, 0.8);
+  const bool narrow = narrow_us < full_us;
+  const double pair_us = M <= 32 ? 1e30 : (narrow ? narrow_us : full_us);
   bool ran = false;
   int rc;
-  if (M <= 16) rc = launch_split<T, 16, BACKWARD>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us, &ran, st);
-  else if (M <= 32) rc = launch_split<T, 32, BACKWARD>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us, &ran, st);
-  else if (M <= 64) rc = launch_split<T, 64, BACKWARD>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us, &ran, st);
-  else rc = launch_split<T, 128, BACKWARD>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us, &ran, st);
+  if (M <= 16) {
+    rc = launch_split<T, 16, BACKWARD, false>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us, &ran, st);
+  } else if (M <= 32) {
+    rc = launch_split<T, 32, BACKWARD, false>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us, &ran, st);
+  } else if (M <= 64) {
+    const double wide_us = plan_wide<64>(M, I, num_kb).us;
+    rc = launch_split<T, 64, BACKWARD, false>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us < wide_us ? pair_us : wide_us, &ran, st);
+    if (rc == QL_OK && !ran) rc = launch_split<T, 64, BACKWARD, true>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us, &ran, st);
+  } else {
+    const double wide_us = M <= 128 ? plan_wide<128>(M, I, num_kb).us : 1e30;
+    rc = launch_split<T, 128, BACKWARD, false>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us < wide_us ? pair_us : wide_us, &ran, st);
+    if (rc == QL_OK && !ran && M <= 128) rc = launch_split<T, 128, BACKWARD, true>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us, &ran, st);
+  }
   if (rc != QL_OK || ran) return rc;
   return narrow ? launch_pair<T, BACKWARD, 64>(x, wg, wu, dh, out, out2, M, I, K, act, st) : launch_pair<T, BACKWARD, 128>(x, wg, wu, dh, out, out2, M, I, K, act, st);
 }

@@ -344,3 +344,11 @@ def test_a_nan_weight_spoils_its_channel_only(activation, M):
     assert torch.equal(h.isnan(), channel.expand(M, 24))
     for g in (dwg, dwu):
         assert torch.equal(g.isnan(), channel[:, None].expand(24, 16))
+
+
+# 33 to 128 tokens through more channels than one wave of 64 a CTA covers: below, at and above a token tile, channels with tails
+@pytest.mark.parametrize("M,I,K", [(33, 9600, 136), (64, 11008, 520), (65, 10000, 72), (128, 18944, 264), (128, 12008, 1032), (100, 19000, 200)])
+@pytest.mark.parametrize("dtype,act", [(torch.bfloat16, "silu"), (torch.float16, "gelu"), (torch.float16, "gelu_tanh"), (torch.bfloat16, "relu")])
+def test_many_channels_of_few_tokens(M, I, K, dtype, act):
+    test_forward(M, I, K, dtype, act)
+    test_backward(M, I, K, dtype, act)
