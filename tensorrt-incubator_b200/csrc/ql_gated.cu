@@ -1064,8 +1064,9 @@ GradPlan plan_grads(int M, int I, int K, bool want_x, bool want_w, int pairs) {
   // A unit costs its steps and about 8 more to start and write out.  With two tiles a pair or more, dX's long units come first,
   // cut to a pair's share of all steps where they are fewer than the pairs, and a pair that has one more of them gets as many
   // fewer of the weights' as that is worth.  With fewer tiles both reductions are cut into units of one length, dealt out in
-  // turn: the length, of the share and fractions of it down to 8, that makes the longest pair's time the shortest.
-  // 8192 x 1024 x 512 84 us so, 153 dealt out the first way; 512 x 11008 x 4096 235 us the first way, 250 the second.
+  // turn: the length, of the share and fractions of it down to 8, or the whole, that makes the longest pair's time the shortest.
+  // 8192 x 1024 x 512 54 us so (67 with the adding of parts thought free), 153 dealt out the first way; 512 x 11008 x 4096 224 us
+  // the first way, 250 the second.
   const int64_t share = (x_tiles * a.x_steps + w_tiles * a.w_steps + pairs - 1) / pairs;
   auto cut = [&](int64_t tiles, int steps, int64_t len) { // what is not wanted has no units and no parts
     if (tiles == 0) return 1;
@@ -1075,11 +1076,13 @@ GradPlan plan_grads(int M, int I, int K, bool want_x, bool want_w, int pairs) {
   a.mixed = x_tiles + w_tiles < 2 * pairs;
   if (a.mixed) {
     int64_t best = INT64_MAX;
-    for (int part = 1; part <= 4; part++) {
-      const int64_t len = share / part < 8 ? 8 : share / part;
+    for (int part = 0; part <= 4; part++) { // 0: nothing is cut
+      const int64_t len = part == 0 ? INT32_MAX : (share / part < 8 ? 8 : share / part);
       const int xs = cut(x_tiles, a.x_steps, len), ws = cut(w_tiles, a.w_steps, len);
       const int64_t x_len = x_tiles ? (a.x_steps + xs - 1) / xs : 0, w_len = w_tiles ? (a.w_steps + ws - 1) / ws : 0;
-      const int64_t cost = (x_tiles * xs + w_tiles * ws + pairs - 1) / pairs * ((x_len > w_len ? x_len : w_len) + 8);
+      const int64_t floats = (xs > 1 ? (int64_t)xs * M * K : 0) + (ws > 1 ? 2ll * ws * I * K : 0);
+      const int64_t join = floats ? 9 + floats * 7 / 1000000 : 0; // adding the parts: 2.5 us and their way to memory and back
+      const int64_t cost = (x_tiles * xs + w_tiles * ws + pairs - 1) / pairs * ((x_len > w_len ? x_len : w_len) + 8) + join;
       if (cost < best) best = cost, a.x_split = xs, a.w_split = ws;
     }
   } else {
@@ -1151,7 +1154,9 @@ int backward(const void *dh, const void *x, const void *wg, const void *wu, void
   if (a.w_parts) rc = encode_map_parts(&mg, a.w_parts, 2 * a.w_split, I, K);
   else if (dwg && (rc = encode_map_narrow(&mg, dtype, dwg, I, K)) == QL_OK) rc = encode_map_narrow(&mu, dtype, dwu, I, K);
   if (rc != QL_OK) return rc;
-  const int pairs = grad_pairs<T>(); // get_unit deals the units out over exactly this many
+  const int units = a.x_units + a.w_units;
+  int pairs = grad_pairs<T>(); // get_unit deals the units out over exactly this many; units dealt out in turn fit any number
+  if (a.mixed && units < pairs) pairs = units;
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
