@@ -5,6 +5,12 @@
 //
 // Forward: both projections are one product with the gate rows as one half of the B operand and the up rows as the other;
 // activation and product are formed from the f32 accumulators, and H is rounded once.  G and U never reach memory.
+// Of few tokens dG and dU are kept as the sum of two values of the operands' type, the rounded one and the rounding's remainder,
+// and the second products take both: the rows of the remainders go where a pair's 256 rows would be empty, and another step
+// over the tokens hides behind writing the weights' gradients.  The gradients' error is then their last rounding's alone.  With
+// many tokens the rounding of dG and dU stays, for the second products would take twice as long: it is of the last one's size
+// (sqrt 2 of it in all), being averaged over many values.
+//
 // Backward: nothing of size M x I is kept from the forward pass.  A first kernel repeats the two projections and forms dG and
 // dU in its epilogue from the f32 accumulators and dH; both are rounded to the operands' type, being the operands of the
 // second kernel, which computes dX and both weight gradients in one launch.  Keeping G and U in 16 bits would save the third
@@ -92,6 +98,12 @@ template <typename F> __device__ __forceinline__ void with_act(int act, F &&f) {
   case ACT_GELU_TANH: f(std::integral_constant<int, ACT_GELU_TANH>{}); break;
   default: f(std::integral_constant<int, ACT_RELU>{}); break;
   }
+}
+
+// What rounding v to T leaves; 0 where that is an infinity.
+template <typename T> __device__ __forceinline__ float remainder_of(float v) {
+  const float h = FloatIO<T>::to_f32(FloatIO<T>::from_f32(v));
+  return fabsf(h) == INFINITY ? 0.f : v - h;
 }
 
 template <typename T> constexpr uint32_t kTypeBits = FloatIO<T>::kDtype == QL_BF16 ? (1u << 7 | 1u << 10) : 0u; // operand formats of kind::f16
@@ -218,6 +230,7 @@ struct ProjArgs {
   const void *dh; // backward: [M, I]
   int M, I, K;
   int act;
+  int layers; // backward: of dG and dU, 2 with the remainders
   int num_kb; // steps of 64 values of K
   int tiles_m, tiles_n, group_m;
   int *status;
@@ -360,14 +373,23 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
             }
           });
           auto two = [&](const uint32_t (&v)[32], int j) { return pack2<T>(__uint_as_float(v[j]), __uint_as_float(v[j + 1])); };
-          out.reusable<0>(lane); // both buffers: dG in one, dU in the other
+          for (int layer = 0; layer < args.layers; layer++) {
+            if (layer > 0) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            out.put64(0, lane, j >> 3, make_uint4(two(g, j), two(g, j + 2), two(g, j + 4), two(g, j + 6)));
-            out.put64(1, lane, j >> 3, make_uint4(two(u, j), two(u, j + 2), two(u, j + 4), two(u, j + 6)));
+              for (int j = 0; j < 32; j++) {
+                g[j] = __float_as_uint(remainder_of<T>(__uint_as_float(g[j])));
+                u[j] = __float_as_uint(remainder_of<T>(__uint_as_float(u[j])));
+              }
+            }
+            out.reusable<0>(lane); // both buffers: dG in one, dU in the other
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+              out.put64(0, lane, j >> 3, make_uint4(two(g, j), two(g, j + 2), two(g, j + 4), two(g, j + 6)));
+              out.put64(1, lane, j >> 3, make_uint4(two(u, j), two(u, j + 2), two(u, j + 4), two(u, j + 6)));
+            }
+            out.send_layer(0, &map_out, lane, n, m0, layer);
+            out.send_layer(2048, &map_out2, lane, n, m0, layer);
           }
-          out.send64(0, &map_out, lane, n, m0);
-          out.send64(1, &map_out2, lane, n, m0);
         }
       }
       tc_fence_before();
@@ -385,15 +407,16 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
 // ------------------------------------------------------------------------------------------------------------------
 struct GradArgs {
   int M, I, K;
+  int layers;                                            // of dG and dU; with 2 (up to 128 tokens) a dX tile's second 128 rows are the remainders'
   // units: a 256 x 256 tile and one of `*_split` parts of its reduction
   int x_tiles_m, x_tiles_n, x_steps, x_split, x_units;   // dX [M, K]: steps of 64 channels, the gate's first, then the up's
-  int w_tiles_m, w_tiles_n, w_steps, w_split, w_units;   // dWg and dWu [I, K] each: steps of 64 tokens
+  int w_tiles_m, w_tiles_n, w_steps, w_split, w_units;   // dWg and dWu [I, K] each: steps of 64 tokens of a layer
   int x_per;                                             // dX units of a cluster; one more for the first `heavy` ones,
   int heavy, heavy_w;                                    // which then have `heavy_w` weight units, the others the rest.
   int mixed;                                             // instead: units of one length, all dealt out in turn
   int group_m;
-  float *x_parts, *w_parts;                              // [split][M][K], [split][2][I][K], null where nothing is cut: then
-                                                         // map_dx or map_dwg lead there, layer by layer
+  float *x_parts, *w_parts;                              // [split][layers][M][K], [split][2][I][K]: map_dx or map_dwg lead there
+                                                         // then; null where there is one part
   int *status;
 };
 
@@ -466,16 +489,18 @@ gated_grads_kernel(const __grid_constant__ CUtensorMap map_dg_k, const __grid_co
           if (u.is_x) {
             const bool up = s >= half_steps;
             const int i0 = (up ? s - half_steps : s) * 64;
-            tma_load_2d_pair(a, up ? &map_du_k : &map_dg_k, bar, i0, r0);
+            if (args.layers == 2) tma_load_3d_pair(a, up ? &map_du_k : &map_dg_k, bar, i0, 0, (int)p.rank);
+            else tma_load_3d_pair(a, up ? &map_du_k : &map_dg_k, bar, i0, r0, 0);
             const CUtensorMap *w = up ? &map_wu_mn : &map_wg_mn;
             tma_load_2d_pair(b, w, bar, c0, i0);
             tma_load_2d_pair(b + 8192, w, bar, c0 + 64, i0);
           } else {
             const CUtensorMap *d = u.up ? &map_du_mn : &map_dg_mn;
-            tma_load_2d_pair(a, d, bar, r0, s * 64);
-            tma_load_2d_pair(a + 8192, d, bar, r0 + 64, s * 64);
-            tma_load_2d_pair(b, &map_x_mn, bar, c0, s * 64);
-            tma_load_2d_pair(b + 8192, &map_x_mn, bar, c0 + 64, s * 64);
+            const int layer = args.layers == 2 ? s & 1 : 0, m = (args.layers == 2 ? s >> 1 : s) * 64;
+            tma_load_3d_pair(a, d, bar, r0, m, layer);
+            tma_load_3d_pair(a + 8192, d, bar, r0 + 64, m, layer);
+            tma_load_2d_pair(b, &map_x_mn, bar, c0, m);
+            tma_load_2d_pair(b + 8192, &map_x_mn, bar, c0 + 64, m);
           }
         }
         __syncwarp();
@@ -526,10 +551,11 @@ gated_grads_kernel(const __grid_constant__ CUtensorMap map_dg_k, const __grid_co
       ok = warp_wait(p.tfull(buf), (j >> 1) & 1, p.abort_flag, p.status, ST_TIMEOUT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after();
-      const int r0 = u.row0 + (int)p.rank * 128 + quad * 32;
+      const bool stacked = u.is_x && args.layers == 2; // this CTA has the rounded values' rows, or the remainders'
+      const int r0 = u.row0 + (stacked ? 0 : (int)p.rank * 128) + quad * 32;
       const uint32_t taddr = p.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * G_N);
-      const bool parts = (u.is_x ? args.x_parts : args.w_parts) != nullptr; // f32, a layer for each part of the reduction
-      const int layer = u.is_x ? u.part : 2 * u.part + (u.up ? 1 : 0);
+      const bool parts = (u.is_x ? args.x_parts : args.w_parts) != nullptr; // f32, a layer for each part of the sum
+      const int layer = stacked ? 2 * u.part + (int)p.rank : (u.is_x ? u.part : 2 * u.part + (u.up ? 1 : 0));
       const CUtensorMap *map = u.is_x ? &map_dx : (u.up && !parts ? &map_dwu : &map_dwg);
       out.reusable<0>(lane); // a part takes the room of both 16-bit buffers
       int b = 0;             // the buffer whose turn it is
@@ -612,9 +638,9 @@ constexpr int kMaxSplit = 8;
 
 struct SplitArgs {
   const void *dh; // backward: [M, I]
-  void *out, *out2; // H, or dG and dU
+  void *out, *out2; // H, or dG and dU, [layers][M][I]
   int M, I;
-  int act;
+  int act, layers;
   int num_kb;
   int tiles_c; // tiles of channels
   int *status;
@@ -760,8 +786,14 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
             float a, da;
             act_both<decltype(act)::value>(z, a, da);
             if (on) {
-              out[at + (size_t)j * (size_t)args.I] = FloatIO<T>::from_f32(d[j] * up * da);
-              out2[at + (size_t)j * (size_t)args.I] = FloatIO<T>::from_f32(d[j] * a);
+              const size_t i = at + (size_t)j * (size_t)args.I;
+              const float vg = d[j] * up * da, vu = d[j] * a;
+              out[i] = FloatIO<T>::from_f32(vg);
+              out2[i] = FloatIO<T>::from_f32(vu);
+              if (args.layers == 2) {
+                out[i + (size_t)args.M * (size_t)args.I] = FloatIO<T>::from_f32(remainder_of<T>(vg));
+                out2[i + (size_t)args.M * (size_t)args.I] = FloatIO<T>::from_f32(remainder_of<T>(vu));
+              }
             }
           } else {
             const float h = act_value<decltype(act)::value>(z) * up;
@@ -829,8 +861,13 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
           if constexpr (BACKWARD) {
             float a, da;
             act_both<decltype(act)::value>(g[k], a, da);
-            out[at[k]] = FloatIO<T>::from_f32(d[k] * u[k] * da);
-            out2[at[k]] = FloatIO<T>::from_f32(d[k] * a);
+            const float vg = d[k] * u[k] * da, vu = d[k] * a;
+            out[at[k]] = FloatIO<T>::from_f32(vg);
+            out2[at[k]] = FloatIO<T>::from_f32(vu);
+            if (args.layers == 2) {
+              out[at[k] + (size_t)args.M * (size_t)args.I] = FloatIO<T>::from_f32(remainder_of<T>(vg));
+              out2[at[k] + (size_t)args.M * (size_t)args.I] = FloatIO<T>::from_f32(remainder_of<T>(vu));
+            }
           } else {
             out[at[k]] = FloatIO<T>::from_f32(act_value<decltype(act)::value>(g[k]) * u[k]);
           }
@@ -849,18 +886,33 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
 // ----------------------------------------------------------------------------------------------
 template <typename T> constexpr int kMapKind = FloatIO<T>::kDtype == QL_BF16 ? KIND_BF16 : KIND_F16;
 
-// 16-bit result [rows, cols], box = [32 rows, 32 columns], 64-byte swizzle (Parked::put64)
-int encode_map_narrow(CUtensorMap *map, int dtype, const void *ptr, int64_t rows, int64_t cols) {
+// 16-bit result [rows, cols], or [layers, rows, cols] where layers > 0, box = [32 rows, 32 columns], 64-byte swizzle (Parked::put64)
+int encode_map_narrow(CUtensorMap *map, int dtype, const void *ptr, int64_t rows, int64_t cols, int layers = 0) {
   EncodeTiledFn enc;
   const int rc = get_encode_fn(&enc);
   if (rc != QL_OK) return rc;
-  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
-  cuuint32_t box[2] = {32, 32};
-  cuuint32_t estr[2] = {1, 1};
-  const CUresult r = enc(map, dtype == QL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(ptr), dims, strides, box, estr,
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)layers};
+  cuuint64_t strides[2] = {(cuuint64_t)cols * 2, (cuuint64_t)(rows * cols) * 2};
+  cuuint32_t box[3] = {32, 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(map, dtype == QL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, layers > 0 ? 3 : 2, const_cast<void *>(ptr), dims, strides, box, estr,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(QL_ERR_CUDA, "cuTensorMapEncodeTiled (16-bit result) failed with code %d", (int)r);
+  return QL_OK;
+}
+
+// 16-bit operand [layers, rows, cols], box = [box_rows, 64 columns], 128-byte swizzle: encode_map's with layers
+int encode_map_layers(CUtensorMap *map, int dtype, const void *ptr, int64_t layers, int64_t rows, int64_t cols, int box_rows) {
+  EncodeTiledFn enc;
+  const int rc = get_encode_fn(&enc);
+  if (rc != QL_OK) return rc;
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)layers};
+  cuuint64_t strides[2] = {(cuuint64_t)cols * 2, (cuuint64_t)(rows * cols) * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(map, dtype == QL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(ptr), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(QL_ERR_CUDA, "cuTensorMapEncodeTiled (layers) failed with code %d", (int)r);
   return QL_OK;
 }
 
@@ -889,6 +941,12 @@ template <typename K> int resident_cached(K kern, int threads, int smem, int clu
   return cache[dev];
 }
 
+// Layers of dG and dU, 2 with the roundings' remainders: up to 64 tokens, and up to 128, half of a pair's rows, where a gradient is
+// of few values over which roundings would average out.  The remainders cost 1 x 64 x 64 1.5 us (7.7 to 9.3) and 16 x 2744 x 1032 0.2
+// (23.3 to 23.5), but 77 x 2744 x 1032 3.5 (24.4 to 27.9) and 128 x 11008 x 4096 20 (121 to 141): four steps of tokens no
+// longer hide behind writing the weights' gradients.
+int grad_layers(int M, int I, int K) { return M <= 64 || (M <= BM && (I <= 256 || K <= 256)) ? 2 : 1; }
+
 // A band of rows of A stays L2-resident: about 32 MiB of it, four row tiles of 256 at the least.  4096 x 28672 x 8192: bands
 // of 16, 32, 64 and 128 MiB 3.00, 2.78, 2.81 and 2.83 ms; 4096 x 11008 x 4096: 522, 501, 504 and 509 us.
 int band(int64_t row_bytes, int tiles_m) {
@@ -907,6 +965,7 @@ int launch_pair(const void *x, const void *wg, const void *wu, const void *dh, v
   ProjArgs a;
   a.dh = dh;
   a.M = M, a.I = I, a.K = K, a.act = act;
+  a.layers = grad_layers(M, I, K);
   a.num_kb = (K + 63) / 64;
   a.tiles_m = (M + 255) / 256;
   a.tiles_n = (I + C - 1) / C;
@@ -918,8 +977,9 @@ int launch_pair(const void *x, const void *wg, const void *wu, const void *dh, v
   if ((rc = encode_map(&mx, kind, x, M, K, 128)) != QL_OK) return rc;
   if ((rc = encode_map(&mg, kind, wg, I, K, C)) != QL_OK) return rc;
   if ((rc = encode_map(&mu, kind, wu, I, K, C)) != QL_OK) return rc;
-  if ((rc = encode_map_narrow(&mo, dtype, out, M, I)) != QL_OK) return rc;
-  if ((rc = encode_map_narrow(&mo2, dtype, out2 ? out2 : out, M, I)) != QL_OK) return rc;
+  if ((rc = encode_map_narrow(&mo, dtype, out, M, I, BACKWARD ? a.layers : 0)) != QL_OK) return rc;
+  mo2 = mo; // forward: not used
+  if (BACKWARD && (rc = encode_map_narrow(&mo2, dtype, out2, M, I, a.layers)) != QL_OK) return rc;
   const int pairs = resident_cached(kern, kPairThreads, PairSmem::kDynamic, 2, cache), tiles = a.tiles_m * a.tiles_n;
   kern<<<2 * (tiles < pairs ? tiles : pairs), kPairThreads, PairSmem::kDynamic, st>>>(mx, mg, mu, mo, mo2, a);
   count_launches(1);
@@ -980,7 +1040,7 @@ int launch_split(const void *x, const void *wg, const void *wu, const void *dh, 
   if (rc != QL_OK) return rc;
   SplitArgs a;
   a.dh = dh, a.out = out, a.out2 = out2;
-  a.M = M, a.I = I, a.act = act;
+  a.M = M, a.I = I, a.act = act, a.layers = grad_layers(M, I, K);
   a.num_kb = (K + 63) / 64;
   SplitPlan plan;
   if constexpr (WIDE) plan = plan_wide<TN>(M, I, a.num_kb);
@@ -1059,7 +1119,8 @@ GradPlan plan_grads(int M, int I, int K, bool want_x, bool want_w, int pairs) {
   GradArgs &a = p.a;
   a.M = M, a.I = I, a.K = K;
   a.x_tiles_m = (M + 255) / 256, a.x_tiles_n = a.w_tiles_n = (K + 255) / 256, a.w_tiles_m = (I + 255) / 256;
-  a.x_steps = 2 * ((I + 63) / 64), a.w_steps = (M + 63) / 64;
+  a.layers = grad_layers(M, I, K);
+  a.x_steps = 2 * ((I + 63) / 64), a.w_steps = a.layers * ((M + 63) / 64);
   const int64_t x_tiles = want_x ? (int64_t)a.x_tiles_m * a.x_tiles_n : 0, w_tiles = want_w ? 2ll * a.w_tiles_m * a.w_tiles_n : 0;
   // A unit costs its steps and about 8 more to start and write out.  With two tiles a pair or more, dX's long units come first,
   // cut to a pair's share of all steps where they are fewer than the pairs, and a pair that has one more of them gets as many
@@ -1080,7 +1141,7 @@ GradPlan plan_grads(int M, int I, int K, bool want_x, bool want_w, int pairs) {
       const int64_t len = part == 0 ? INT32_MAX : (share / part < 8 ? 8 : share / part);
       const int xs = cut(x_tiles, a.x_steps, len), ws = cut(w_tiles, a.w_steps, len);
       const int64_t x_len = x_tiles ? (a.x_steps + xs - 1) / xs : 0, w_len = w_tiles ? (a.w_steps + ws - 1) / ws : 0;
-      const int64_t floats = (xs > 1 ? (int64_t)xs * M * K : 0) + (ws > 1 ? 2ll * ws * I * K : 0);
+      const int64_t floats = (x_tiles && xs * a.layers > 1 ? (int64_t)xs * a.layers * M * K : 0) + (ws > 1 ? 2ll * ws * I * K : 0);
       const int64_t join = floats ? 9 + floats * 7 / 1000000 : 0; // adding the parts: 2.5 us and their way to memory and back
       const int64_t cost = (x_tiles * xs + w_tiles * ws + pairs - 1) / pairs * ((x_len > w_len ? x_len : w_len) + 8) + join;
       if (cost < best) best = cost, a.x_split = xs, a.w_split = ws;
@@ -1096,7 +1157,7 @@ GradPlan plan_grads(int M, int I, int K, bool want_x, bool want_w, int pairs) {
   a.heavy_w = hw < 0 ? 0 : (int)(hw + 0.5);
   a.group_m = 8; // row tiles walked together; 4, 8, 16, 32 on 4096 x 11008 x 4096: 1.62, 1.55, 1.59, 1.54 ms; on 1024 x 28672 x 8192: 2.12, 2.10, 2.10, 2.20
   a.x_parts = a.w_parts = nullptr;
-  p.x_part_floats = x_tiles > 0 && a.x_split > 1 ? (int64_t)a.x_split * M * K : 0;
+  p.x_part_floats = x_tiles > 0 && a.x_split * a.layers > 1 ? (int64_t)a.x_split * a.layers * M * K : 0;
   p.w_part_floats = w_tiles > 0 && a.w_split > 1 ? 2ll * a.w_split * I * K : 0;
   return p;
 }
@@ -1129,7 +1190,7 @@ int pairs_of(int dtype) { return dtype == QL_BF16 ? grad_pairs<__nv_bfloat16>() 
 template <typename T>
 int backward(const void *dh, const void *x, const void *wg, const void *wu, void *dx, void *dwg, void *dwu, int M, int I, int K, int act, uint8_t *ws, const GradPlan &plan,
              cudaStream_t st) {
-  const int64_t mi = align256((int64_t)M * I * 2);
+  const int64_t mi = align256((int64_t)plan.a.layers * M * I * 2);
   void *dg = ws, *du = ws + mi;
   int rc = project<T, true>(x, wg, wu, dh, dg, du, M, I, K, act, st);
   if (rc != QL_OK || (!dx && !dwg)) return rc;
@@ -1138,17 +1199,18 @@ int backward(const void *dh, const void *x, const void *wg, const void *wu, void
   uint8_t *parts = ws + 2 * mi;
   if (plan.x_part_floats) a.x_parts = reinterpret_cast<float *>(parts);
   if (plan.w_part_floats) a.w_parts = reinterpret_cast<float *>(parts + align256(plan.x_part_floats * 4));
+  const int x_layers = a.x_split * a.layers;
   CUtensorMap dgk, duk, dgm, dum, wgm, wum, xm, mx, mg, mu;
   const int kind = kMapKind<T>, dtype = FloatIO<T>::kDtype;
-  if ((rc = encode_map(&dgk, kind, dg, M, I, 128)) != QL_OK) return rc;
-  if ((rc = encode_map(&duk, kind, du, M, I, 128)) != QL_OK) return rc;
-  if ((rc = encode_map(&dgm, kind, dg, M, I, 64)) != QL_OK) return rc;
-  if ((rc = encode_map(&dum, kind, du, M, I, 64)) != QL_OK) return rc;
+  if ((rc = encode_map_layers(&dgk, dtype, dg, a.layers, M, I, 128)) != QL_OK) return rc;
+  if ((rc = encode_map_layers(&duk, dtype, du, a.layers, M, I, 128)) != QL_OK) return rc;
+  if ((rc = encode_map_layers(&dgm, dtype, dg, a.layers, M, I, 64)) != QL_OK) return rc;
+  if ((rc = encode_map_layers(&dum, dtype, du, a.layers, M, I, 64)) != QL_OK) return rc;
   if ((rc = encode_map(&wgm, kind, wg, I, K, 64)) != QL_OK) return rc;
   if ((rc = encode_map(&wum, kind, wu, I, K, 64)) != QL_OK) return rc;
   if ((rc = encode_map(&xm, kind, x, M, K, 64)) != QL_OK) return rc;
   mx = mg = mu = xm; // what is not wanted is not written
-  if (a.x_parts) rc = encode_map_parts(&mx, a.x_parts, a.x_split, M, K);
+  if (a.x_parts) rc = encode_map_parts(&mx, a.x_parts, x_layers, M, K);
   else if (dx) rc = encode_map_narrow(&mx, dtype, dx, M, K);
   if (rc != QL_OK) return rc;
   if (a.w_parts) rc = encode_map_parts(&mg, a.w_parts, 2 * a.w_split, I, K);
@@ -1171,7 +1233,7 @@ int backward(const void *dh, const void *x, const void *wg, const void *wu, void
   count_launches(1);
   if (a.x_parts || a.w_parts) {
     const int64_t nx4 = (int64_t)M * K / 4, nw4 = (int64_t)I * K / 4, n = (a.x_parts ? nx4 : 0) + (a.w_parts ? 2 * nw4 : 0);
-    const int split = a.x_parts && a.w_parts ? (a.x_split > a.w_split ? a.x_split : a.w_split) : (a.x_parts ? a.x_split : a.w_split);
+    const int split = a.x_parts && a.w_parts ? (x_layers > a.w_split ? x_layers : a.w_split) : (a.x_parts ? x_layers : a.w_split);
     const int64_t room = (int64_t)sm_count() * 2048; // threads the device holds
     int slices_log2 = 0;
     while (slices_log2 < 3 && (2 << slices_log2) <= split && (n << (slices_log2 + 1)) <= room) slices_log2++;
@@ -1179,7 +1241,7 @@ int backward(const void *dh, const void *x, const void *wg, const void *wu, void
     cfg.gridDim = dim3((unsigned)(blocks < cap ? blocks : cap), 1, 1);
     cfg.blockDim = dim3(kReduceThreads, 1, 1);
     cfg.dynamicSmemBytes = 0;
-    QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, grads_reduce_kernel<T>, reinterpret_cast<const float4 *>(a.x_parts), a.x_split, static_cast<T *>(dx), nx4,
+    QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, grads_reduce_kernel<T>, reinterpret_cast<const float4 *>(a.x_parts), x_layers, static_cast<T *>(dx), nx4,
                                    reinterpret_cast<const float4 *>(a.w_parts), a.w_split, static_cast<T *>(dwg), static_cast<T *>(dwu), nw4, slices_log2));
     count_launches(1);
   }
@@ -1239,7 +1301,7 @@ extern "C" int ql_gated_linear_backward_workspace(const ql_tensor *x, const ql_t
   *bytes = 0;
   if (M == 0 || K == 0 || I == 0) return QL_OK;
   const GradPlan p = plan_grads((int)M, (int)I, (int)K, want_dx != 0, want_dw != 0, pairs_of(x->dtype));
-  *bytes = 2 * align256(M * I * 2) + align256(p.x_part_floats * 4) + align256(p.w_part_floats * 4);
+  *bytes = 2 * align256(p.a.layers * M * I * 2) + align256(p.x_part_floats * 4) + align256(p.w_part_floats * 4);
   return QL_OK;
 }
 

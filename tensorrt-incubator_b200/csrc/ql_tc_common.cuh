@@ -198,6 +198,11 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
                ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(leader_bar), "r"(x), "r"(y)
                : "memory");
 }
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap *map, uint32_t leader_bar, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(leader_bar), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
 // A role that gave up tells the pair's other CTA, whose roles would otherwise each run into their own limit.
 __device__ __forceinline__ void signal_partner_abort(uint32_t abort_addr, uint32_t rank) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to_cta(abort_addr, rank ^ 1u)), "r"(1u) : "memory");
@@ -263,12 +268,12 @@ struct Parked {
       bulk_commit();
     }
   }
-  __device__ __forceinline__ void send_layer(int buf, const CUtensorMap *map, int lane, int x, int y, int z) {
+  __device__ __forceinline__ void send_layer(uint32_t offset, const CUtensorMap *map, int lane, int x, int y, int z) { // from base + offset
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
       asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
-                   ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(base + buf * 4096)), "r"(x), "r"(y), "r"(z)
+                   ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(base) + offset), "r"(x), "r"(y), "r"(z)
                    : "memory");
       bulk_commit();
     }

@@ -352,3 +352,20 @@ def test_a_nan_weight_spoils_its_channel_only(activation, M):
 def test_many_channels_of_few_tokens(M, I, K, dtype, act):
     test_forward(M, I, K, dtype, act)
     test_backward(M, I, K, dtype, act)
+
+
+@pytest.mark.parametrize("M,I,K", [(1, 64, 64), (2, 264, 136), (16, 64, 128), (33, 64, 64), (40, 4104, 520), (100, 12000, 72), (128, 136, 1032)])
+@pytest.mark.parametrize("dtype,act", [(torch.bfloat16, "silu"), (torch.float16, "gelu"), (torch.bfloat16, "relu")])
+def test_few_tokens_gradients_are_rounded_once(M, I, K, dtype, act):
+    """Up to 128 tokens the roundings of dG and dU are carried along: what is left is the last rounding, whose error is measured
+    on the exact gradients.  Beside it stand the remainders' own roundings, 2^-8 of a rounding (f16: 2^-11, and for remainders
+    below its normal range at most 2^-25 of absolute size against gradients of 0.01 and more), and f32 sums and functions, a
+    few 2^-22: together below a twentieth of it."""
+    c = [randn((M, K), dtype, 8600), randn((I, K), dtype, 8601, K ** -0.5), randn((I, K), dtype, 8602, K ** -0.5), randn((M, I), dtype, 8603)]
+    x, wg, wu, d = [t.double() for t in c]
+    g, u = x @ wg.T, x @ wu.T
+    a, da = act_both(g, act)
+    dg, du = d * u * da, d * a
+    for got, want in zip(ql.gated_linear_backward(c[3], c[0], c[1], c[2], act), (dg @ wg + du @ wu, dg.T @ x, du.T @ x)):
+        off, rounding = float((got.double() - want).norm()), float((want.to(dtype).double() - want).norm())
+        assert off < 1.05 * rounding, f"{off / rounding:.3f} of one rounding"
