@@ -70,16 +70,22 @@ def gemm_mxfp4(a: Float4Tensor, a_scales: torch.Tensor, b: Float4Tensor, b_scale
         raise QuantizeError(f"Unsupported data type in gemm_mxfp4. Supported data types are: {dt.QUANTIZABLE_DTYPES}. Got out_dtype={out_dtype}")
     if len(a.shape) != 2 or len(b.shape) != 2 or a_scales.dim() != 2 or b_scales.dim() != 2:
         raise QuantizeError("gemm_mxfp4: data and scales must be 2-D")
-    y = out if out is not None else empty((a.shape[0], b.shape[0]), out_dtype.torch, a.device)
+    device = a.packed.device
     # dense, on a multiple of 4 bytes (a slice of rows need not be); kept alive across the call: a view only borrows the pointer
-    sa, sb = (s if s.data_ptr() % 4 == 0 else s.clone() for s in (a_scales.contiguous(), b_scales.contiguous()))
-    L = _lib.lib()
-    va, vsa, vb, vsb = ql_view(a), ql_view(sa), ql_view(b), ql_view(sb)
-    ws = None
-    if sa.shape[-1] % 16 or (sa.data_ptr() | sb.data_ptr()) % 16:   # rows the kernel for many tokens wants a padded copy of
+    sa, sb = a_scales.contiguous(), b_scales.contiguous()
+    where = sa.data_ptr() | sb.data_ptr()
+    if where % 4:
+        sa, sb = sa.clone(), sb.clone()
+        where = sa.data_ptr() | sb.data_ptr()
+    other, y = (b, sa, sb), out
+    if out is None:
+        y = empty((a.shape[0], b.shape[0]), out_dtype.torch, device)
+    else:
+        other += (out,)
+    ws, size = None, 0
+    if where % 16 or a.shape[1] % 512:   # scale rows the kernel for many tokens wants a padded copy of
         size = _padding_bytes(a.shape, b.shape)
         if size:
-            ws = empty((size,), torch.uint8, a.device)
-    call_on(a.device, L.ql_gemm_mxfp4, va, vsa, vb, vsb, ql_view(y), ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-            same_device=(sa, b, sb, y))
+            ws = empty((size,), torch.uint8, device)
+    call_on(device, _lib.lib().ql_gemm_mxfp4, ql_view(a), ql_view(sa), ql_view(b), ql_view(sb), ql_view(y), ws.data_ptr() if size else None, size, same_device=other)
     return y
