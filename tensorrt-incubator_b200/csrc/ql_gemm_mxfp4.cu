@@ -16,7 +16,8 @@
 //   split   few output tiles (decoding, short prompts): the weights are the 128-row operand and up to 128 tokens the other;
 //           a cluster of up to 8 CTAs shares the K axis of one tile and adds its parts through distributed shared memory,
 //           in rank order (the same bits on every run).
-//   tiles   many output tiles, persistent: one CTA per SM on 128 x 208 tiles, or CTA pairs on 256 x 208 tiles.  In a pair
+//   tiles   many output tiles, persistent: one CTA per SM on 128 x 208 tiles, or CTA pairs on 256 x 208 tiles (x 112 where the wider
+//           ones would leave SMs without work).  In a pair
 //           (tcgen05.mma.cta_group::2, issued by its leader) each CTA holds its own 128 rows of A and half of the B tile, so
 //           per MMA it reads 232 rows of operands from shared memory instead of 336; the scales of all 208 columns are needed
 //           by both.  Whole 128-byte pieces of Y's rows leave by bulk tensor stores (4096 x 8192 x 512 24 us, 39 with each lane
@@ -407,46 +408,46 @@ gemm_mxfp4_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// tiles kernel: persistent, 128 x 208, or 256 x 208 by CTA pairs
+// tiles kernel: persistent, 128 x 208 or 128 x 112, or twice the rows by CTA pairs
 // ------------------------------------------------------------------------------------------------------------------
-// The width leaves tensor memory, beside two accumulators, 96 columns: four slots of the scales of one k step.  A slot is free
+// TBN, columns of a tile: 208 leaves tensor memory, beside two accumulators, 96 columns: four slots of the scales of one k step.  A slot is free
 // when the MMAs of its step are done, and refilled (the commit, the wait, the stores, the arrival at the pair's leader) about
 // 1100 cycles later: three steps (416 cycles each) hide that.  Two slots of two steps, the stage in between hiding it: 8192 x
 // 28672 x 8192 765 us, 715 now.  With 224 columns there is room for two slots of one step.
-constexpr int TBN = 208;
 constexpr int kTileThreads = 448;   // producer, MMA, four epilogue warps, two sets of four scale warps
 constexpr int kScSteps = 4;         // k steps whose scales travel together: 32 bytes, a whole sector, of every row
 constexpr int kStageSteps = 2;      // k steps of one stage
-constexpr int kSlots = 4;           // of one k step: 8 columns of A's scales, then 16 of B's (8 per pair of MMAs, 6.5 used)
-constexpr int kSlotCols = 24;
-constexpr int T_SC_ROWS = BM + TBN;
-constexpr int T_SC_LANES = (T_SC_ROWS + 31) / 32; // rows a lane carries (of the last, half the lanes' are past the tile)
-constexpr int T_SC_BYTES = T_SC_LANES * 32 * 32;  // with room for those
-template <bool PAIR> struct TileSmem {
-  static constexpr int kStages = PAIR ? 3 : 2; // of two k steps: half as many barriers to look at and to signal as with one
+constexpr int kSlots = 4;           // of one k step: 8 columns of A's scales, then 16 (8) of B's: 8 (4) per pair of MMAs, 6.5 (3.5) used
+template <bool PAIR, int TBN> struct TileSmem {
+  static constexpr int kScRows = BM + TBN, kScLanes = (kScRows + 31) / 32; // rows of scales, and of them those a lane carries
+  static constexpr int kScBytes = kScLanes * 32 * 32;                      // with room for the last lanes' rows past the tile
+  static constexpr int kCellsB = (TBN + 31) / 32, kColsB = kCellsB > 4 ? 8 : 4;
+  static constexpr int kSlotCols = 8 + 2 * kColsB;
+  static constexpr int kStages = (PAIR ? 3 : 2) + (TBN <= 128 ? 1 : 0); // of two k steps: half as many barriers to look at and to signal as with one
   static constexpr int kRowsB = PAIR ? TBN / 2 : TBN;                     // rows of the B tile one CTA holds
   static constexpr int kTileB = kRowsB * BK_BYTES;
   static constexpr int kStageBytes = kStageSteps * (MX_A_BYTES + kTileB);  // A's tiles, then B's
   static constexpr int kScales = kStages * kStageBytes;
-  static constexpr int kStaging = kScales + 2 * T_SC_BYTES;  // the epilogue's, 4096 bytes a warp
+  static constexpr int kStaging = kScales + 2 * kScBytes;  // the epilogue's, 4096 bytes a warp
   static constexpr int kBarriers = kStaging + 4 * 4096; // full[S], empty[S], tfull[2], tempty[2], scfull[2], scempty[2], sfull[4], sempty[4], drain
   static constexpr int kTmemPtr = kBarriers + (2 * kStages + 9 + 2 * kSlots) * 8;
   static constexpr int kAbort = kTmemPtr + 4;
   static constexpr int kDynamic = kAbort + 4 + 1024;
-  static_assert(kDynamic <= 232448 && kStageBytes % 1024 == 0 && T_SC_BYTES % 1024 == 0, "tile shape");
+  static_assert(kDynamic <= 232448 && kStageBytes % 1024 == 0 && kScBytes % 1024 == 0, "tile shape");
 };
 
-// A tile's last 16 columns, or the `cols` (a multiple of the 16-byte piece) of them that Y has, of one row a lane, rounded to y's type
+// The `cols` (a multiple of the 16-byte piece, at most 32) columns behind a tile's whole 128 bytes, of one row a lane, rounded to y's
+// type
 template <typename OutT>
 __device__ __forceinline__ void mx_store_chunk(OutT *y, const uint32_t (&r)[32], int cols) {
   if constexpr (sizeof(OutT) == 4) {
 #pragma unroll
-    for (int j = 0; j < 16; j += 4)
+    for (int j = 0; j < 32; j += 4)
       if (j < cols) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]));
   } else {
     auto two = [&](int j) { return pack2<OutT>(__uint_as_float(r[j]), __uint_as_float(r[j + 1])); };
 #pragma unroll
-    for (int j = 0; j < 16; j += 8)
+    for (int j = 0; j < 32; j += 8)
       if (j < cols) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
   }
 }
@@ -461,14 +462,14 @@ __device__ __forceinline__ void mx_store_turned(OutT *y, const uint32_t (&r)[32]
 // TURNED: operand a are the weights and operand b the activations (args.M, args.N: rows of a and b; Y is [N, M]).  For rows of
 // Y that are no multiple of 16 bytes, where a lane that holds a row of Y could only store it value by value, far apart:
 // 4571 x 5597 x 160 takes 39 us turned, 88 through a staging buffer in shared memory.
-template <bool PAIR, bool TURNED>
+template <bool PAIR, bool TURNED, int TBN>
 __global__ void __launch_bounds__(kTileThreads, 1)
 gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sa,
                         const __grid_constant__ CUtensorMap map_sb, const __grid_constant__ CUtensorMap map_y, const MxArgs args) {
-  using L = TileSmem<PAIR>;
+  using L = TileSmem<PAIR, TBN>;
   constexpr int TSTAGES = L::kStages;
   constexpr uint32_t kTmemCols = 512; // two accumulators, two slots of scales
-  static_assert(2 * TBN + kSlots * kSlotCols <= 512, "tensor memory");
+  static_assert(2 * TBN + kSlots * L::kSlotCols <= 512, "tensor memory");
   constexpr uint32_t kSfCol0 = 2 * TBN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -551,8 +552,8 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
           if (!warp_wait(scempty_bar(sc), sc_phase ^ 1, abort_flag, args.status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
           if (sc_issued == 0) wait_for_results(); // of the kernel that pads the scales
           if (elect_one()) {
-            const uint32_t dst = smem_base + L::kScales + sc * T_SC_BYTES;
-            mbar_expect_tx(scfull_bar(sc), T_SC_ROWS * 32);
+            const uint32_t dst = smem_base + L::kScales + sc * L::kScBytes;
+            mbar_expect_tx(scfull_bar(sc), L::kScRows * 32);
             tma_load_2d(dst, &map_sa, scfull_bar(sc), ks * kScaleBytes, (row_tile * mt + rank) * BM);
             tma_load_2d(dst + BM * 32, &map_sb, scfull_bar(sc), ks * kScaleBytes, nt * TBN);
           }
@@ -617,13 +618,13 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
           if (!scales_ready && !warp_wait(sfull_bar(slot), parity, abort_flag, args.status, ST_TIMEOUT_FULL)) { ok = false; break; }
           if (!data_ready && !warp_wait(full_bar(stage), phase, abort_flag, args.status, ST_TIMEOUT_FULL)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t a_addr = smem_base + stage * L::kStageBytes, t_sfa = tmem_base + kSfCol0 + kSlotCols * slot, t_sfb = t_sfa + 8;
+          const uint32_t a_addr = smem_base + stage * L::kStageBytes, t_sfa = tmem_base + kSfCol0 + L::kSlotCols * slot, t_sfb = t_sfa + 8;
           const uint64_t adesc = make_smem_desc(a_addr), bdesc = make_smem_desc(a_addr + kStageSteps * MX_A_BYTES);
           const int cur = stage;
           if (++stage == TSTAGES) { stage = 0; phase ^= 1; }
           half++;
           auto mma = [&](int q, int j) {
-            mx_k_mma<TBN, PAIR>(j, tmem_d, adesc + q * (MX_A_BYTES >> 4), bdesc + q * (L::kTileB >> 4), t_sfa + q * kSlotCols, t_sfb + q * kSlotCols, 8, (ks | q | j) != 0 ? 1u : 0u);
+            mx_k_mma<TBN, PAIR>(j, tmem_d, adesc + q * (MX_A_BYTES >> 4), bdesc + q * (L::kTileB >> 4), t_sfa + q * L::kSlotCols, t_sfb + q * L::kSlotCols, L::kColsB, (ks | q | j) != 0 ? 1u : 0u);
           };
           if (leader) {
 #pragma unroll
@@ -675,8 +676,8 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
     auto hand_over = [&](int ks, int sc, uint32_t sc_phase) {
       ok = warp_wait(scfull_bar(sc), sc_phase, abort_flag, args.status, ST_TIMEOUT_FULL);
       if (!ok) return;
-      const uint8_t *buf = smem + L::kScales + sc * T_SC_BYTES;
-      uint32_t w[T_SC_LANES][4]; // rows lane, lane + 32, ... : the words of two k steps
+      const uint8_t *buf = smem + L::kScales + sc * L::kScBytes;
+      uint32_t w[L::kScLanes][4]; // rows lane, lane + 32, ... : the words of two k steps
       int h = 0;                 // the stage of this group that is this set's, if there is one
       while (h < kScSteps / kStageSteps && ks + h * kStageSteps < args.num_ks && ((half + h) & 1) != set) h++;
       const bool mine = h < kScSteps / kStageSteps && ks + h * kStageSteps < args.num_ks;
@@ -687,7 +688,7 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
         // eight lanes' 16 bytes cover all banks
         const uint8_t *row = buf + lane * 32 + ((16 * h) ^ ((lane & 4) << 2));
 #pragma unroll
-        for (int c = 0; c < T_SC_LANES; c++) {
+        for (int c = 0; c < L::kScLanes; c++) {
           const uint4 v = *reinterpret_cast<const uint4 *>(row + c * 1024);
           w[c][0] = v.x, w[c][1] = v.y, w[c][2] = v.z, w[c][3] = v.w;
         }
@@ -700,12 +701,18 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
         const int slot = (int)set * kStageSteps + q;
         ok = warp_wait(sempty_bar(slot), parity, abort_flag, args.status, ST_TIMEOUT_EMPTY);
         if (!ok) return;
-        // for each pair of MMAs (word j): four cells of A's rows, seven of B's
-        const uint32_t t = tmem_base + quarter + kSfCol0 + kSlotCols * slot;
+        // for each pair of MMAs (word j): four cells of A's rows, seven (four) of B's
+        const uint32_t t = tmem_base + quarter + kSfCol0 + L::kSlotCols * slot;
         auto v = [&](int c, int j) { return w[c][2 * q + j]; };
         tmem_store_4(t, v(0, 0), v(1, 0), v(2, 0), v(3, 0));
         tmem_store_4(t + 4, v(0, 1), v(1, 1), v(2, 1), v(3, 1));
-        tmem_store_16(t + 8, v(4, 0), v(5, 0), v(6, 0), v(7, 0), v(8, 0), v(9, 0), v(10, 0), 0u, v(4, 1), v(5, 1), v(6, 1), v(7, 1), v(8, 1), v(9, 1), v(10, 1), 0u);
+        if constexpr (L::kCellsB == 7) {
+          tmem_store_16(t + 8, v(4, 0), v(5, 0), v(6, 0), v(7, 0), v(8, 0), v(9, 0), v(10, 0), 0u, v(4, 1), v(5, 1), v(6, 1), v(7, 1), v(8, 1), v(9, 1), v(10, 1), 0u);
+        } else {
+          static_assert(L::kCellsB == 4, "cells of B's scales");
+          tmem_store_4(t + 8, v(4, 0), v(5, 0), v(6, 0), v(7, 0));
+          tmem_store_4(t + 12, v(4, 1), v(5, 1), v(6, 1), v(7, 1));
+        }
         tmem_store_wait();
         tc_fence_before();
         __syncwarp();
@@ -742,7 +749,7 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
         if (m0 >= args.M || (cols <= 0 && (TURNED || wide || (c & 1) == 0))) break; // nothing left to store
         uint32_t r[32];
         tmem_load_32(taddr + c * 32, r); // of the last chunk half the columns are the next accumulator's, or scales: not stored
-        if (!TURNED && c < TBN / 32) { // 128 bytes of a row: 32 values of f32, or 64 of 16 bits
+        if (!TURNED && c < (wide ? TBN / 32 : TBN / 64 * 2)) { // 128 bytes of a row: 32 values of f32, or 64 of 16 bits
           if (wide || (c & 1) == 0) out.reusable<0>(lane);
           auto put16 = [&](auto type) {
             using OutT = decltype(type);
@@ -759,7 +766,7 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
             put16(__nv_bfloat16());
           }
           if (wide || (c & 1) == 1) out.send(0, &map_y, lane, wide ? n : n - 32, m0);
-        } else if (m < args.M) { // the tile's last 16 columns, or TURNED
+        } else if (m < args.M && cols > 0) { // the tile's last columns, or TURNED
           const size_t at = TURNED ? (size_t)n * (size_t)args.M + m : (size_t)m * (size_t)args.N + n;
           auto store = [&](auto *y) {
             if constexpr (TURNED) mx_store_turned(y, r, cols, (size_t)args.M);
@@ -957,10 +964,10 @@ int encode_map_scales(CUtensorMap *map, const uint8_t *ptr, int64_t rows, int64_
 }
 
 // args: operands a and b as the kernel takes them (TURNED: the weights first)
-template <bool PAIR, bool TURNED> int launch_tiles(const void *a, const void *b, MxArgs args, int64_t K, void *workspace, cudaStream_t st) {
-  using L = TileSmem<PAIR>;
+template <bool PAIR, bool TURNED, int TBN> int launch_tiles(const void *a, const void *b, MxArgs args, int64_t K, void *workspace, cudaStream_t st) {
+  using L = TileSmem<PAIR, TBN>;
   static bool configured[64] = {false};
-  int rc = allow_smem(gemm_mxfp4_tiles_kernel<PAIR, TURNED>, L::kDynamic, configured);
+  int rc = allow_smem(gemm_mxfp4_tiles_kernel<PAIR, TURNED, TBN>, L::kDynamic, configured);
   if (rc != QL_OK) return rc;
   int pitch = args.kb;
   const bool padding = needs_padding(args);
@@ -998,9 +1005,13 @@ template <bool PAIR, bool TURNED> int launch_tiles(const void *a, const void *b,
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = padding ? 2 : 1;
-  QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_mxfp4_tiles_kernel<PAIR, TURNED>, ma, mb, msa, msb, my, args));
+  QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, gemm_mxfp4_tiles_kernel<PAIR, TURNED, TBN>, ma, mb, msa, msb, my, args));
   count_launches(1);
   return QL_OK;
+}
+template <bool TURNED> int launch_tiles_as(bool pairs, bool narrow, const void *a, const void *b, const MxArgs &args, int64_t K, void *workspace, cudaStream_t st) {
+  if (pairs) return narrow ? launch_tiles<true, TURNED, 112>(a, b, args, K, workspace, st) : launch_tiles<true, TURNED, 208>(a, b, args, K, workspace, st);
+  return narrow ? launch_tiles<false, TURNED, 112>(a, b, args, K, workspace, st) : launch_tiles<false, TURNED, 208>(a, b, args, K, workspace, st);
 }
 
 } // namespace
@@ -1055,33 +1066,40 @@ extern "C" int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, cons
   args.tiles_a = args.tiles_b = 0;
   args.status = device_status_word();
   if (!args.status) return set_error(QL_ERR_CUDA, "%s: could not allocate the device status word", op);
-  // Pairs of the tiles kernel take 4.5 us (3.5 more where scales are padded, 2 of them the host's) and, per tile, 0.45 us per k step, its single CTAs
-  // 0.56, or the 2.2 us that storing a tile takes beside it; the split kernel what plan_split says.  Up to 32 tokens the tiles
-  // are mostly padding and the split kernel is the better one throughout; up to 128 rows of the first operand a pair's second
-  // half would be.  Split and tiles, us: 128 x 1928 x 4736 11.8, 14.1; 1264 x 545 x 4384 14.5, 14.9; 534 x 1617 x 768 8.4, 8.7;
-  // 356 x 4440 x 5088 19.4, 16.2; 458 x 11848 x 480 23.8, 13.5.  Single CTAs and pairs: 128 x 28672 x 8192 28.0, 32; 512 x 11008 x
-  // 4096 21.9, 20.4; 8192 x 28672 x 8192 920, 720.
+  // Pairs of the tiles kernel take 6.7 us and 0.29 us per tile and k step, with tiles of 112 columns 5.6 and 0.243; its single CTAs
+  // 6.0 and 0.43, or 4.0 and 0.36; a tile at least the 2.2 (1.7) us that storing it takes beside the next; 3 more where scales are
+  // padded, half of them the host's.  The split kernel takes what plan_split says.  Up to 32 tokens the tiles are mostly padding
+  // and the split kernel is the better one throughout; up to 128 rows of the first operand a pair's second half would be.  us,
+  // split and tiles: 128 x 1928 x 4736 11.8, 14.1; 534 x 1617 x 768 8.4, 8.7; 356 x 4440 x 5088 19.4, 16.2; 458 x 11848 x 480 23.8, 13.5.
+  // Tiles of 208 and of 112 columns: 512 x 4096 x 4096 11.9, 10.0; 4490 x 384 x 22528 32.5, 26.9; 70 x 9000 x 4096 12.9, 9.7;
+  // 2048 x 1024 x 4096 11.5, 12.7; 1403 x 7344 x 768 14.5, 16.9; 4096 x 4096 x 8192 55, 68.5.  Single CTAs and pairs: 128 x 28672 x
+  // 8192 28.0, 32; 8192 x 28672 x 8192 920, 720.
   const bool turned = N % (y->dtype == QL_F32 ? 4 : 8) != 0 || !aligned16(y->data);
   const int64_t R = turned ? N : M, C = turned ? M : N; // rows of the tiles kernel's operands
   const bool pairs = R > BM;
   const int64_t row_tiles = pairs ? (R + 2 * BM - 1) / (2 * BM) : (R + BM - 1) / BM, units = pairs ? sm_count() / 2 : sm_count();
-  const int64_t tiles = row_tiles * ((C + TBN - 1) / TBN);
-  if (tiles >= (1ll << 30)) return set_error(QL_ERR_UNSUPPORTED, "%s: too many output tiles", op);
-  const double main_us = (pairs ? 0.45 : 0.56) * args.num_ks, store_us = C < TBN ? 2.2 * C / TBN : 2.2; // of a tile, one beside the other
-  const double tiles_us = M <= kSplitOnly ? 1e30 : 4.5 + (need > 0 ? 3.5 : 0.0) + (double)((tiles + units - 1) / units) * (main_us > store_us ? main_us : store_us);
+  if (row_tiles * ((C + 111) / 112) >= (1ll << 30)) return set_error(QL_ERR_UNSUPPORTED, "%s: too many output tiles", op);
+  auto tiles_us = [&](int width, double fixed, double step, double store) {
+    const int64_t tiles = row_tiles * ((C + width - 1) / width);
+    const double main_us = step * args.num_ks, store_us = C < width ? store * C / width : store; // of a tile, one beside the other
+    return fixed + (need > 0 ? 3.0 : 0.0) + (double)((tiles + units - 1) / units) * (main_us > store_us ? main_us : store_us);
+  };
+  const double wide_us = tiles_us(208, pairs ? 6.7 : 6.0, pairs ? 0.29 : 0.43, 2.2), narrow_us = tiles_us(112, pairs ? 5.6 : 4.0, pairs ? 0.243 : 0.36, 1.7);
+  const bool narrow = narrow_us < wide_us;
+  const double limit_us = M <= kSplitOnly ? 1e30 : (narrow ? narrow_us : wide_us);
   args.sfa = static_cast<const uint8_t *>(b_scales->data); // the weights are the 128-row operand of the split kernel
   args.sfb = static_cast<const uint8_t *>(a_scales->data);
   bool ran = false;
-  rc = M <= 16   ? launch_split<16>(b->data, a->data, args, K, tiles_us, &ran, st)
-       : M <= 32 ? launch_split<32>(b->data, a->data, args, K, tiles_us, &ran, st)
-       : M <= 64 ? launch_split<64>(b->data, a->data, args, K, tiles_us, &ran, st)
-                 : launch_split<128>(b->data, a->data, args, K, tiles_us, &ran, st);
+  rc = M <= 16   ? launch_split<16>(b->data, a->data, args, K, limit_us, &ran, st)
+       : M <= 32 ? launch_split<32>(b->data, a->data, args, K, limit_us, &ran, st)
+       : M <= 64 ? launch_split<64>(b->data, a->data, args, K, limit_us, &ran, st)
+                 : launch_split<128>(b->data, a->data, args, K, limit_us, &ran, st);
   if (rc != QL_OK || ran) return rc;
   if (turned) {
     args.M = (int)N, args.N = (int)M;
-    return pairs ? launch_tiles<true, true>(b->data, a->data, args, K, workspace, st) : launch_tiles<false, true>(b->data, a->data, args, K, workspace, st);
+    return launch_tiles_as<true>(pairs, narrow, b->data, a->data, args, K, workspace, st);
   }
   args.sfa = static_cast<const uint8_t *>(a_scales->data);
   args.sfb = static_cast<const uint8_t *>(b_scales->data);
-  return pairs ? launch_tiles<true, false>(a->data, b->data, args, K, workspace, st) : launch_tiles<false, false>(a->data, b->data, args, K, workspace, st);
+  return launch_tiles_as<false>(pairs, narrow, a->data, b->data, args, K, workspace, st);
 }

@@ -63,7 +63,8 @@ def test_few_tiles(M, N, K, out):
 
 # many tiles: scales of whole 16-byte rows and padded ones, rows of Y of whole 16-byte pieces and of odd lengths
 @pytest.mark.parametrize("M,N,K", [(2048, 4096, 512), (1700, 2600, 1056), (4100, 1120, 32), (2048, 2300, 2048), (640, 6700, 4640), (1701, 2601, 1280), (2047, 2305, 11008), (130, 4099, 544), (257, 2001, 1024), (2048, 1000, 4096), (70, 9000, 4096),
-                                   (128, 11000, 8192), (3000, 101, 8192), (33, 9001, 4128), (40000, 101, 1024), (20000, 3, 4096)])
+                                   (128, 11000, 8192), (3000, 101, 8192), (33, 9001, 4128), (40000, 101, 1024), (20000, 3, 4096),
+                                   (512, 4096, 4096), (1024, 545, 2112), (500, 304, 8192), (130, 7777, 96)])
 @pytest.mark.parametrize("out", [torch.float32, torch.float16, torch.bfloat16])
 def test_many_tiles(M, N, K, out):
     a, sa = operand(M, K, 5100 + M)
