@@ -369,3 +369,37 @@ def test_few_tokens_gradients_are_rounded_once(M, I, K, dtype, act):
     for got, want in zip(ql.gated_linear_backward(c[3], c[0], c[1], c[2], act), (dg @ wg + du @ wu, dg.T @ x, du.T @ x)):
         off, rounding = float((got.double() - want).norm()), float((want.to(dtype).double() - want).norm())
         assert off < 1.05 * rounding, f"{off / rounding:.3f} of one rounding"
+
+
+def test_calls_from_several_threads_and_a_replayed_one():
+    """Host threads on streams of their own, shapes of every kernel, while a captured backward pass is replayed beside them."""
+    import threading
+    shapes = [(1, 512, 264), (40, 9600, 136), (100, 264, 1032), (300, 1000, 328), (700, 2056, 264)]
+    ops = [(randn((M, I), torch.bfloat16, 8700 + M), randn((M, K), torch.bfloat16, 8701 + M), randn((I, K), torch.bfloat16, 8702 + M, K ** -0.5),
+            randn((I, K), torch.bfloat16, 8703 + M, K ** -0.5)) for M, I, K in shapes]
+    want = [(ql.gated_linear(x, wg, wu), *ql.gated_linear_backward(d, x, wg, wu)) for d, x, wg, wu in ops]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        replayed = ql.gated_linear_backward(*ops[3])
+    wrong = []
+
+    def work(seed):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for k in range(10):
+                i = (seed + k) % len(ops)
+                d, x, wg, wu = ops[i]
+                got = (ql.gated_linear(x, wg, wu), *ql.gated_linear_backward(d, x, wg, wu))
+                torch.cuda.current_stream().synchronize()
+                wrong.extend((i, j) for j, (a, b) in enumerate(zip(got, want[i])) if not torch.equal(a, b))
+    threads = [threading.Thread(target=work, args=(s,)) for s in range(4)]
+    for t in threads:
+        t.start()
+    for _ in range(20):
+        graph.replay()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong
+    assert all(torch.equal(a, b) for a, b in zip(replayed, want[3][1:]))
+    assert ql.lib().ql_gemm_status(None) == 0
