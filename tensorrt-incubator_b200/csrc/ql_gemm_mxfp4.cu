@@ -20,7 +20,7 @@
 //           ones would leave SMs without work).  In a pair
 //           (tcgen05.mma.cta_group::2, issued by its leader) each CTA holds its own 128 rows of A and half of the B tile, so
 //           per MMA it reads 232 rows of operands from shared memory instead of 336; the scales of all 208 columns are needed
-//           by both.  Whole 128-byte pieces of Y's rows leave by bulk tensor stores (4096 x 8192 x 512 24 us, 39 with each lane
+//           by both.  Y leaves by bulk tensor stores of 32 columns (4096 x 8192 x 512 24 us, 39 with each lane
 //           storing its row).
 // Every wait is bounded, as in the other tensor-core kernels.
 #include <cuda.h>
@@ -436,18 +436,17 @@ template <bool PAIR, int TBN> struct TileSmem {
   static_assert(kDynamic <= 232448 && kStageBytes % 1024 == 0 && kScBytes % 1024 == 0, "tile shape");
 };
 
-// The `cols` (a multiple of the 16-byte piece, at most 32) columns behind a tile's whole 128 bytes, of one row a lane, rounded to y's
-// type
+// A tile's last 16 columns, or the `cols` (a multiple of the 16-byte piece) of them that Y has, of one row a lane, rounded to y's type
 template <typename OutT>
 __device__ __forceinline__ void mx_store_chunk(OutT *y, const uint32_t (&r)[32], int cols) {
   if constexpr (sizeof(OutT) == 4) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 4)
+    for (int j = 0; j < 16; j += 4)
       if (j < cols) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]));
   } else {
     auto two = [&](int j) { return pack2<OutT>(__uint_as_float(r[j]), __uint_as_float(r[j + 1])); };
 #pragma unroll
-    for (int j = 0; j < 32; j += 8)
+    for (int j = 0; j < 16; j += 8)
       if (j < cols) __stcs(reinterpret_cast<uint4 *>(y + j), make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
   }
 }
@@ -735,7 +734,7 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
     const int quad = warp & 3;
     const bool wide = args.y_dtype == QL_F32;
     Parked out{smem + L::kStaging + quad * 4096};
-    int it = 0;
+    int it = 0, b = 0; // b: the staging buffer whose turn it is
     for (int tile = first_tile; tile < num_tiles; tile += tile_stride, it++) {
       const int buf = it & 1;
       const int mt = tile % args.tiles_a, nt = tile / args.tiles_a;
@@ -746,27 +745,29 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
 #pragma unroll 1
       for (int c = 0; c < (TBN + 31) / 32; c++) {
         const int n = nt * TBN + c * 32, cols = min(min(args.N, nt * TBN + TBN) - n, 32);
-        if (m0 >= args.M || (cols <= 0 && (TURNED || wide || (c & 1) == 0))) break; // nothing left to store
+        if (m0 >= args.M || cols <= 0) break; // nothing left to store
         uint32_t r[32];
         tmem_load_32(taddr + c * 32, r); // of the last chunk half the columns are the next accumulator's, or scales: not stored
-        if (!TURNED && c < (wide ? TBN / 32 : TBN / 64 * 2)) { // 128 bytes of a row: 32 values of f32, or 64 of 16 bits
-          if (wide || (c & 1) == 0) out.reusable<0>(lane);
+        if (!TURNED && c < TBN / 32) { // rows of 64 bytes in two buffers, of 128 (f32) in the room of both
           auto put16 = [&](auto type) {
             using OutT = decltype(type);
             auto two = [&](int j) { return pack2<OutT>(__uint_as_float(r[j]), __uint_as_float(r[j + 1])); };
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) out.put(0, lane, (c & 1) * 4 + (j >> 3), make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
+            for (int j = 0; j < 32; j += 8) out.put64(b, lane, j >> 3, make_uint4(two(j), two(j + 2), two(j + 4), two(j + 6)));
           };
           if (wide) {
+            out.reusable<0>(lane);
 #pragma unroll
             for (int j = 0; j < 32; j += 4) out.put(0, lane, j >> 2, make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]));
-          } else if (args.y_dtype == QL_F16) {
-            put16(__half());
+            out.send(0, &map_y, lane, n, m0);
           } else {
-            put16(__nv_bfloat16());
+            out.reusable<1>(lane);
+            if (args.y_dtype == QL_F16) put16(__half());
+            else put16(__nv_bfloat16());
+            out.send64(b, &map_y, lane, n, m0);
+            b ^= 1;
           }
-          if (wide || (c & 1) == 1) out.send(0, &map_y, lane, wide ? n : n - 32, m0);
-        } else if (m < args.M && cols > 0) { // the tile's last columns, or TURNED
+        } else if (m < args.M) { // the tile's last 16 columns, or TURNED
           const size_t at = TURNED ? (size_t)n * (size_t)args.M + m : (size_t)m * (size_t)args.N + n;
           auto store = [&](auto *y) {
             if constexpr (TURNED) mx_store_turned(y, r, cols, (size_t)args.M);
@@ -988,7 +989,8 @@ template <bool PAIR, bool TURNED, int TBN> int launch_tiles(const void *a, const
   if ((rc = encode_map_scales(&msa, args.sfa, args.M, pitch, BM)) != QL_OK) return rc;
   if ((rc = encode_map_scales(&msb, args.sfb, args.N, pitch, TBN)) != QL_OK) return rc;
   my = ma; // TURNED: not used
-  if (!TURNED && (rc = encode_map_out(&my, args.y_dtype, args.Y, args.M, args.N, args.N)) != QL_OK) return rc;
+  if (!TURNED && (rc = args.y_dtype == QL_F32 ? encode_map_out(&my, QL_F32, args.Y, args.M, args.N, args.N) : encode_map_narrow(&my, args.y_dtype, args.Y, args.M, args.N)) != QL_OK)
+    return rc;
   args.tiles_a = (args.M + (PAIR ? 2 : 1) * BM - 1) / ((PAIR ? 2 : 1) * BM);
   args.tiles_b = (args.N + TBN - 1) / TBN;
   const int64_t tiles = (int64_t)args.tiles_a * args.tiles_b;

@@ -422,6 +422,21 @@ inline int make_map_bytes(CUtensorMap *map, const void *ptr, int64_t rows, int64
   return QL_OK;
 }
 
+// 16-bit result [rows, cols], or [layers, rows, cols] where layers > 0, box = [32 rows, 32 columns], 64-byte swizzle (Parked::put64)
+inline int encode_map_narrow(CUtensorMap *map, int dtype, const void *ptr, int64_t rows, int64_t cols, int layers = 0) {
+  EncodeTiledFn enc;
+  const int rc = get_encode_fn(&enc);
+  if (rc != QL_OK) return rc;
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)layers};
+  cuuint64_t strides[2] = {(cuuint64_t)cols * 2, (cuuint64_t)(rows * cols) * 2};
+  cuuint32_t box[3] = {32, 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(map, dtype == QL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, layers > 0 ? 3 : 2, const_cast<void *>(ptr), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(QL_ERR_CUDA, "cuTensorMapEncodeTiled (16-bit result) failed with code %d", (int)r);
+  return QL_OK;
+}
+
 // Raises a kernel's dynamic shared-memory limit on the current device, once.
 template <typename K> inline int allow_smem(K kern, int bytes, bool (&configured)[64]) {
   int dev = 0;
