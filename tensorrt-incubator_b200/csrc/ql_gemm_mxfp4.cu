@@ -28,6 +28,7 @@
 
 #include "ql_common.cuh"
 #include "ql_tc_common.cuh"
+#include "ql_together.cuh"
 
 namespace ql {
 namespace {
@@ -119,6 +120,12 @@ __device__ __forceinline__ uint32_t ldg8_if(const void *p, bool on) {
   uint32_t v;
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.nc.u8 %0, [%1];\n\t}" : "=r"(v) : "l"(p), "r"((int)on));
   return v;
+}
+// The barrier of the 128 threads that hand scales over (warps as wholes, converged): do all of them go on?
+__device__ __forceinline__ bool all_of_128(bool go) {
+  uint32_t all;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((int)go) : "memory");
+  return all != 0;
 }
 // The scale bytes of four k steps of one row: the first `n` of 32 bytes from p on, zeros beyond.  Loading and shifting are
 // apart, so that the loads of several rows are in flight together, and the loads are predicated, not branched around: a
@@ -311,18 +318,19 @@ gemm_mxfp4_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
       fa.load(args.sfa + at_a, has_a ? n : 0, (long long)args.N * args.kb - at_a);
       fb.load(args.sfb + at_b, has_b ? n : 0, (long long)args.M * args.kb - at_b);
     };
-    bool ok = true;
-    auto hand_over = [&](int ks, int slot, uint32_t parity, RowScales<WIDE> &fa, RowScales<WIDE> &fb) {
+    auto meet = [&](auto slot, int, bool go) { // this thread's rows, then the barrier behind which all rows are there
       uint8_t *buf = smem + L::kScales + slot * L::kScaleGroup;
 #pragma unroll
       for (int q = 0; q < kFetchSteps; q++) {
-        *reinterpret_cast<uint2 *>(buf + tid * kScPitch + q * 8) = make_uint2(fa.word(2 * q), fa.word(2 * q + 1));
-        if (tid < TN) *reinterpret_cast<uint2 *>(buf + (BM + tid) * kScPitch + q * 8) = make_uint2(fb.word(2 * q), fb.word(2 * q + 1));
+        *reinterpret_cast<uint2 *>(buf + tid * kScPitch + q * 8) = make_uint2(a[slot].word(2 * q), a[slot].word(2 * q + 1));
+        if (tid < TN) *reinterpret_cast<uint2 *>(buf + (BM + tid) * kScPitch + q * 8) = make_uint2(b[slot].word(2 * q), b[slot].word(2 * q + 1));
       }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      fetch(ks + 2 * kFetchSteps, fa, fb);
-      ok = warp_wait(sempty_bar(slot), parity, abort_flag, args.status, ST_TIMEOUT_EMPTY);
-      if (!ok) return;
+      return all_of_128(go);
+    };
+    auto take = [&](auto slot, int group) {
+      const uint8_t *buf = smem + L::kScales + slot * L::kScaleGroup;
+      fetch(ks0 + (group + 2) * kFetchSteps, a[slot], b[slot]);
+      if (!warp_wait(sempty_bar(slot), ((group >> 1) & 1) ^ 1u, abort_flag, args.status, ST_TIMEOUT_EMPTY)) return false;
       const uint32_t t = tmem_base + quarter + kSfCol0 + slot * kSlotCols;
 #pragma unroll
       for (int q = 0; q < kFetchSteps; q++) {
@@ -342,14 +350,11 @@ gemm_mxfp4_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(sfull_bar(slot));
+      return true;
     };
     fetch(ks0, a[0], b[0]);
     fetch(ks0 + kFetchSteps, a[1], b[1]);
-    uint32_t parity = 1;
-    for (int ks = ks0; ks < ks1 && ok; ks += 2 * kFetchSteps, parity ^= 1) {
-      hand_over(ks, 0, parity, a[0], b[0]);
-      if (ok && ks + kFetchSteps < ks1) hand_over(ks + kFetchSteps, 1, parity, a[1], b[1]);
-    }
+    steps_together((ks1 - ks0 + kFetchSteps - 1) / kFetchSteps, meet, take);
     warp_wait(tfull_bar, 0, abort_flag, args.status, ST_TIMEOUT_TMEM_FULL);
     tc_fence_after();
     // lane = row of the weights = column of Y, so a warp's store of one token is contiguous
@@ -467,7 +472,7 @@ gemm_mxfp4_tiles_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_
                         const __grid_constant__ CUtensorMap map_sb, const __grid_constant__ CUtensorMap map_y, const MxArgs args) {
   using L = TileSmem<PAIR, TBN>;
   constexpr int TSTAGES = L::kStages;
-  constexpr uint32_t kTmemCols = 512; // two accumulators, two slots of scales
+  constexpr uint32_t kTmemCols = 512; // two accumulators, four slots of scales
   static_assert(2 * TBN + kSlots * L::kSlotCols <= 512, "tensor memory");
   constexpr uint32_t kSfCol0 = 2 * TBN;
   extern __shared__ uint8_t smem_raw[];
