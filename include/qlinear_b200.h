@@ -181,7 +181,9 @@ QL_API int ql_gated_linear(const ql_tensor *x, const ql_tensor *w_gate, const ql
 /* Its backward pass: the gradients of x, w_gate and w_up from grad = the gradient of h [M,I], all of x's type.  dx may be
  * null, and so may dw_gate and dw_up together.  Nothing is kept from the forward pass: both projections are computed again;
  * their gradients are formed in f32 and rounded to x's type as operands of the second products, which sum in f32 (of up to 64
- * tokens the rounding's remainder is kept beside it, so that only the results' own rounding is left).
+ * tokens the rounding's remainder is kept beside it, so that only the results' own rounding is left).  f16: they are held times
+ * a power of two that suits their largest magnitude, chosen on the device, so gradients may be of any size and the intermediate
+ * ones beyond f16's range; a token's keep all their digits down to 2^-16 of the largest.
  * `workspace`: 256-byte aligned device memory of at least the bytes the query gives; free again when the call's work on the
  * stream is done. */
 QL_API int ql_gated_linear_backward_workspace(const ql_tensor *x, const ql_tensor *w_gate, int32_t want_dx, int32_t want_dw,

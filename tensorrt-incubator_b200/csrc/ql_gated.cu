@@ -12,14 +12,15 @@
 // (sqrt 2 of it in all), being averaged over many values.
 //
 // Backward: nothing of size M x I is kept from the forward pass.  A first kernel repeats the two projections and forms dG and
-// dU in its epilogue from the f32 accumulators and dH; both are rounded to the operands' type, being the operands of the
-// second kernel, which computes dX and both weight gradients in one launch.  Keeping G and U in 16 bits would save the third
+// dU in its epilogue from the f32 accumulators and dH; both are rounded to the operands' type (f16: times a power of two), being
+// the operands of the second kernel, which computes dX and both weight gradients in one launch.  Keeping G and U in 16 bits would save the third
 // of the backward pass that repeats them and would add their two roundings to the one of dG and dU.
 //
 // Kernels:
 //   gated_split     few tokens (decoding): the weights are the 128-row operand (gate rows, then up rows of the same channels),
 //                   up to 128 tokens the other; a cluster of CTAs shares K and adds its parts in rank order through
 //                   distributed shared memory.  Bound by reading the weights once.
+//                   (each runs a second time where f16 needs another power of two, see kRanged)
 //   gated_pair      many tokens: persistent CTA pairs (cta_group::2) on 256 tokens x 128 (or 64) channels, six stages; CTA 0
 //                   of a pair loads the gate rows, CTA 1 the up rows, so each holds half of the B tile.  Bound by the tensor
 //                   cores; small problems by what comes before the first MMA and after the last.
@@ -106,6 +107,42 @@ template <typename T> __device__ __forceinline__ float remainder_of(float v) {
   return fabsf(h) == INFINITY ? 0.f : v - h;
 }
 
+// dG and dU in f16 are held times a power of two, undone in f32 where the second products leave their accumulators: f16 ends at
+// 65504, and below 2^-14 its digits fade, while gradients come in every size.  The first stage multiplies dH by 2^6 and notes the
+// largest finite magnitude it then met, before rounding; where that is not between 2^2 and 65504 it is run again (the launch is
+// there on every call and ends at once otherwise) with the power that takes it to 2^14 .. 2^15.  So digits are lost below 2^-16
+// of the largest value at the earliest.  bf16 has f32's range and none of this.
+// Beside one launch without any of it: 16 x 2744 x 1032 22.0 us, 24.4 with the second launch, 31 where it runs; 77 x 2744 x 1032
+// 23.6, 26.5 and 35; 128 x 11008 x 4096 133, 136 and 185; 512 x 2744 x 1032 43, 45 and 56; 4096 x 11008 x 4096 1.66, 1.69 and 2.17 ms.
+// Noting the largest takes 0.3 to 0.7 of the 2.5 us, the launch the rest.  An exponent from the largest |dH| alone would need no
+// second run but for gates and projections far from 1, where it would be as wrong as none.
+template <typename T> constexpr bool kRanged = FloatIO<T>::kDtype == QL_F16;
+constexpr int kFirstExponent = 6;
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// The largest of what the first stage's CTAs met, for every lane of a warp; bits of floats that are not negative order as these do.
+__device__ __forceinline__ float largest_of(const float *largest, int n, int lane) {
+  uint32_t m = 0;
+#pragma unroll 8
+  for (int i = lane; i < n; i += 32) m = max(m, __float_as_uint(largest[i]));
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, m));
+}
+__device__ __forceinline__ bool first_exponent_fits(float largest) { return largest == 0.f || (largest >= 4.f && largest <= 65504.f); }
+__device__ __forceinline__ int range_exponent(float largest) {
+  // 60 at the most: beyond, every gradient is 0 in f16, and a product on the way would leave f32's range
+  return first_exponent_fits(largest) ? kFirstExponent : min(kFirstExponent + 14 + 127 - (int)(__float_as_uint(largest) >> 23), 60);
+}
+// The larger of `top` and the values' magnitudes, a NaN or an infinity aside
+template <int N> __device__ __forceinline__ float finite_top(float top, const uint32_t (&bits)[N]) {
+  auto magnitude = [&](int i) { return fabsf(__uint_as_float(bits[i])); };
+  float all = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; i++) all = fmaxf(all, magnitude(i)); // passes over a NaN
+  if (all < INFINITY) return fmaxf(top, all);
+#pragma unroll
+  for (int i = 0; i < N; i++) top = fmaxf(top, magnitude(i) < INFINITY ? magnitude(i) : 0.f);
+  return top;
+}
+
 template <typename T> constexpr uint32_t kTypeBits = FloatIO<T>::kDtype == QL_BF16 ? (1u << 7 | 1u << 10) : 0u; // operand formats of kind::f16
 
 // Instruction descriptor of kind::f16: f32 accumulation, N >> 3 at bit 17, M >> 4 at bit 24, operand A (bit 15) or B (bit 16)
@@ -142,7 +179,8 @@ struct PairSmem {
   static constexpr int kBarriers = kStaging + kEpilogueWarps * 4096; // full[S], empty[S], tfull[2], tempty[2], drain
   static constexpr int kTmemPtr = kBarriers + (2 * G_STAGES + 5) * 8;
   static constexpr int kAbort = kTmemPtr + 4;
-  static constexpr int kDynamic = kAbort + 4 + 1024;
+  static constexpr int kLargest = kAbort + 4; // kRanged
+  static constexpr int kDynamic = kLargest + 4 + 1024;
 };
 static_assert(PairSmem::kDynamic <= 232448, "shared memory");
 
@@ -161,6 +199,7 @@ struct Pair {
   __device__ __forceinline__ uint32_t empty(int s) const { return bars + 8u * (G_STAGES + s); }
   __device__ __forceinline__ uint32_t tfull(int b) const { return bars + 8u * (2 * G_STAGES + b); }
   __device__ __forceinline__ uint32_t tempty(int b) const { return bars + 8u * (2 * G_STAGES + 2 + b); }
+  __device__ __forceinline__ float *largest() const { return reinterpret_cast<float *>(smem + PairSmem::kLargest); }
   __device__ __forceinline__ uint32_t drain() const { return bars + 8u * (2 * G_STAGES + 4); }
 
   __device__ __forceinline__ void start(uint8_t *raw, int *status_) {
@@ -184,6 +223,7 @@ struct Pair {
       }
       mbar_init(drain(), 1);
       *abort_flag = 0;
+      *largest() = 0.f;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -231,6 +271,8 @@ struct ProjArgs {
   int M, I, K;
   int act;
   int layers; // backward: of dG and dU, 2 with the remainders
+  float *largest;    // backward, kRanged: what each CTA of the first run met
+  int again;         // this is the second run, of as many CTAs
   int num_kb; // steps of 64 values of K
   int tiles_m, tiles_n, group_m;
   int *status;
@@ -251,6 +293,14 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
   extern __shared__ uint8_t smem_raw[];
   Pair p;
   if (BACKWARD) dependents_may_start();
+  constexpr bool RANGED = BACKWARD && kRanged<T>;
+  float scale = pow2(kFirstExponent);
+  if (RANGED && args.again) {
+    wait_for_results();
+    const float seen = largest_of(args.largest, gridDim.x, threadIdx.x & 31);
+    if (first_exponent_fits(seen)) return; // all CTAs alike
+    scale = pow2(range_exponent(seen));
+  }
   p.start(smem_raw, args.status);
   const int cluster_id = blockIdx.x >> 1, num_clusters = gridDim.x >> 1, num_tiles = args.tiles_m * args.tiles_n;
 
@@ -315,6 +365,7 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
     Parked out{p.smem + PairSmem::kStaging + (p.warp - 2) * 4096};
     int it = 0, b = 0; // b: the staging buffer whose turn it is (forward)
     bool ok = true;
+    float top = 0.f;
     uint4 ahead[4]; // dH of this warp's next chunk, of the next tile after a tile's last one: on its way while the one before is worked on
     auto fetch = [&](int tile, int c) {
       if (tile >= num_tiles) return;
@@ -366,12 +417,16 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
 #pragma unroll
             for (int j = 0; j < 32; j++) {
               float a, da;
-              const float dv = FloatIO<T>::to_f32(d[j]);
+              const float dv = FloatIO<T>::to_f32(d[j]) * (RANGED ? scale : 1.f);
               act_both<decltype(act)::value>(__uint_as_float(g[j]), a, da);
               g[j] = __float_as_uint(dv * __uint_as_float(u[j]) * da);
               u[j] = __float_as_uint(dv * a);
             }
           });
+          if constexpr (RANGED) {
+            top = finite_top(top, g);
+            top = finite_top(top, u);
+          }
           auto two = [&](const uint32_t (&v)[32], int j) { return pack2<T>(__uint_as_float(v[j]), __uint_as_float(v[j + 1])); };
           for (int layer = 0; layer < args.layers; layer++) {
             if (layer > 0) {
@@ -397,9 +452,14 @@ gated_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
       if (lane == 0) mbar_arrive_remote(map_to_cta(p.tempty(buf), 0)); // the leader owns the accumulator hand-over
     }
     out.finish(lane);
+    if (RANGED) {
+      const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+      if (lane == 0) atomicMax(reinterpret_cast<uint32_t *>(p.largest()), bits);
+    }
     if (!ok && lane == 0) signal_partner_abort(smem_u32((const void *)p.abort_flag), p.rank);
   }
   p.end();
+  if (RANGED && !args.again && threadIdx.x == 0) args.largest[blockIdx.x] = *p.largest();
 }
 
 // ------------------------------------------------------------------------------------------------------------------
@@ -417,6 +477,8 @@ struct GradArgs {
   int group_m;
   float *x_parts, *w_parts;                              // [split][layers][M][K], [split][2][I][K]: map_dx or map_dwg lead there
                                                          // then; null where there is one part
+  const float *largest;                                  // kRanged: what the first stage's CTAs met
+  int num_largest;
   int *status;
 };
 
@@ -546,6 +608,8 @@ gated_grads_kernel(const __grid_constant__ CUtensorMap map_dg_k, const __grid_co
     const int quad = p.warp & 3, turn = (p.warp - 2) >> 2, lane = p.lane;
     Parked out{p.smem + PairSmem::kStaging + (p.warp - 2) * 4096};
     bool ok = true;
+    float back = 1.f; // what dG and dU were multiplied by, undone
+    if constexpr (kRanged<T>) back = pow2(-range_exponent(largest_of(args.largest, args.num_largest, lane)));
     for (int j = 0; get_unit(args, cluster_id, num_clusters, j, &u); j++) {
       const int buf = j & 1;
       ok = warp_wait(p.tfull(buf), (j >> 1) & 1, p.abort_flag, p.status, ST_TIMEOUT_TMEM_FULL);
@@ -565,6 +629,10 @@ gated_grads_kernel(const __grid_constant__ CUtensorMap map_dg_k, const __grid_co
         if (r0 >= (u.is_x ? args.M : args.I) || n >= args.K) break; // nothing left to store
         uint32_t v[32];
         tmem_load_32(taddr + c * 32, v);
+        if constexpr (kRanged<T>) {
+#pragma unroll
+          for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * back);
+        }
         if (parts) {
           out.reusable<0>(lane);
 #pragma unroll
@@ -641,6 +709,8 @@ struct SplitArgs {
   void *out, *out2; // H, or dG and dU, [layers][M][I]
   int M, I;
   int act, layers;
+  float *largest; // as in ProjArgs
+  int again;
   int num_kb;
   int tiles_c; // tiles of channels
   int *status;
@@ -653,7 +723,8 @@ template <int TN, bool WIDE> struct SplitSmem {
   static constexpr int kBarriers = kParts + (WIDE ? 0 : TN * BM * 4); // full[16], empty[16], tfull
   static constexpr int kTmemPtr = kBarriers + (2 * kSplitMaxStages + 1) * 8;
   static constexpr int kAbort = kTmemPtr + 4;
-  static constexpr int kRing = (kAbort + 4 + 1023) / 1024 * 1024;
+  static constexpr int kLargest = kAbort + 4;
+  static constexpr int kRing = (kLargest + 4 + 1023) / 1024 * 1024;
   static constexpr int stage_bytes(int channels) { return ((channels + 7) / 8 * 16 + TN) * BK_BYTES; }
   static constexpr int total(int channels, int stages) { return kRing + stages * stage_bytes(channels) + BM * BK_BYTES + 1024; }
 };
@@ -677,6 +748,7 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
   const uint32_t tfull_bar = bar_base + 8u * (2 * kSplitMaxStages);
   volatile uint32_t *tmem_ptr_smem = reinterpret_cast<volatile uint32_t *>(smem + L::kTmemPtr);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::kAbort);
+  float *largest = reinterpret_cast<float *>(smem + L::kLargest);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int split = 1 << split_log2;
@@ -685,6 +757,18 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
   const int kb0 = (int)((long long)args.num_kb * rank / split), kb1 = (int)((long long)args.num_kb * (rank + 1) / split);
 
   if (BACKWARD) dependents_may_start();
+  constexpr bool RANGED = BACKWARD && kRanged<T>;
+  float scale = pow2(kFirstExponent), top = 0.f;
+  if (RANGED && args.again) {
+    wait_for_results();
+    const float seen = largest_of(args.largest, gridDim.x, lane);
+    if (first_exponent_fits(seen)) return; // all CTAs alike
+    scale = pow2(range_exponent(seen));
+  }
+  auto met = [&](float vg, float vu) { // values of dG and dU
+    const float m = fmaxf(fabsf(vg), fabsf(vu));
+    if constexpr (RANGED) top = fmaxf(top, m < INFINITY ? m : fminf(fabsf(vg), fabsf(vu)) < INFINITY ? fminf(fabsf(vg), fabsf(vu)) : 0.f);
+  };
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; s++) {
       mbar_init(full_bar(s), 1);
@@ -692,6 +776,7 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
     }
     mbar_init(tfull_bar, 1);
     *abort_flag = 0;
+    *largest = 0.f;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -774,7 +859,7 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
         const size_t at = (size_t)(xt * TN + c * 16) * (size_t)args.I + ch;
         if constexpr (BACKWARD) {
 #pragma unroll
-          for (int j = 0; j < 16; j++) d[j] = mine && c * 16 + j < tokens ? FloatIO<T>::to_f32(dh[at + (size_t)j * (size_t)args.I]) : 0.f;
+          for (int j = 0; j < 16; j++) d[j] = mine && c * 16 + j < tokens ? FloatIO<T>::to_f32(dh[at + (size_t)j * (size_t)args.I]) * (RANGED ? scale : 1.f) : 0.f;
         }
         tmem_load_16(tmem_base + ((uint32_t)(quad * 32) << 16) + c * 16, g);
         tmem_load_16(tmem_base + ((uint32_t)(quad * 32) << 16) + TN + c * 16, u);
@@ -788,6 +873,7 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
             if (on) {
               const size_t i = at + (size_t)j * (size_t)args.I;
               const float vg = d[j] * up * da, vu = d[j] * a;
+              met(vg, vu);
               out[i] = FloatIO<T>::from_f32(vg);
               out2[i] = FloatIO<T>::from_f32(vu);
               if (args.layers == 2) {
@@ -845,7 +931,7 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
         for (int k = 0; k < U; k++) {
           const int i = min(i0 + k * kThreads, items - 1), t = i / here, ch = i - t * here;
           at[k] = (size_t)(xt * TN + t0 + t) * (size_t)args.I + ct * channels + ch;
-          if constexpr (BACKWARD) d[k] = FloatIO<T>::to_f32(static_cast<const T *>(args.dh)[at[k]]);
+          if constexpr (BACKWARD) d[k] = FloatIO<T>::to_f32(static_cast<const T *>(args.dh)[at[k]]) * (RANGED ? scale : 1.f);
           g[k] = u[k] = 0.f;
 #pragma unroll
           for (int p = 0; p < kMaxSplit; p++) {
@@ -862,6 +948,7 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
             float a, da;
             act_both<decltype(act)::value>(g[k], a, da);
             const float vg = d[k] * u[k] * da, vu = d[k] * a;
+            met(vg, vu);
             out[at[k]] = FloatIO<T>::from_f32(vg);
             out2[at[k]] = FloatIO<T>::from_f32(vu);
             if (args.layers == 2) {
@@ -878,6 +965,13 @@ gated_split_kernel(const __grid_constant__ CUtensorMap map_gate, const __grid_co
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemCols) : "memory");
+  }
+  if (RANGED && !args.again) {
+    __syncwarp();
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    if (lane == 0) atomicMax(reinterpret_cast<uint32_t *>(largest), bits);
+    __syncthreads();
+    if (threadIdx.x == 0) args.largest[blockIdx.x] = *largest;
   }
 }
 
@@ -940,43 +1034,25 @@ int band(int64_t row_bytes, int tiles_m) {
   return (int)(g > tiles_m ? (tiles_m < 1 ? 1 : tiles_m) : g);
 }
 
-template <typename T, bool BACKWARD, int C>
-int launch_pair(const void *x, const void *wg, const void *wu, const void *dh, void *out, void *out2, int M, int I, int K, int act, cudaStream_t st) {
-  auto kern = gated_pair_kernel<T, BACKWARD, C>;
-  static bool configured[64] = {false};
-  static int cache[64] = {0};
-  int rc = allow_smem(kern, PairSmem::kDynamic, configured);
-  if (rc != QL_OK) return rc;
-  ProjArgs a;
-  a.dh = dh;
-  a.M = M, a.I = I, a.K = K, a.act = act;
-  a.layers = grad_layers(M, I, K);
-  a.num_kb = (K + 63) / 64;
-  a.tiles_m = (M + 255) / 256;
-  a.tiles_n = (I + C - 1) / C;
-  a.group_m = band((int64_t)K * 2, a.tiles_m);
-  a.status = device_status_word();
-  if (!a.status) return set_error(QL_ERR_CUDA, "gated_linear: could not allocate the device status word");
-  CUtensorMap mx, mg, mu, mo, mo2;
-  const int kind = kMapKind<T>, dtype = FloatIO<T>::kDtype;
-  if ((rc = encode_map(&mx, kind, x, M, K, 128)) != QL_OK) return rc;
-  if ((rc = encode_map(&mg, kind, wg, I, K, C)) != QL_OK) return rc;
-  if ((rc = encode_map(&mu, kind, wu, I, K, C)) != QL_OK) return rc;
-  if ((rc = encode_map_narrow(&mo, dtype, out, M, I, BACKWARD ? a.layers : 0)) != QL_OK) return rc;
-  mo2 = mo; // forward: not used
-  if (BACKWARD && (rc = encode_map_narrow(&mo2, dtype, out2, M, I, a.layers)) != QL_OK) return rc;
-  const int pairs = resident_cached(kern, kPairThreads, PairSmem::kDynamic, 2, cache), tiles = a.tiles_m * a.tiles_n;
-  kern<<<2 * (tiles < pairs ? tiles : pairs), kPairThreads, PairSmem::kDynamic, st>>>(mx, mg, mu, mo, mo2, a);
-  count_launches(1);
-  QL_CUDA_TRY(cudaGetLastError());
-  return QL_OK;
-}
-
 struct SplitPlan {
   int co, log2, channels, stages;
   double us;
 };
 
+template <typename T, int TN, bool BACKWARD, bool WIDE> int allow_split() {
+  static bool configured[64] = {false};
+  return allow_smem(gated_split_kernel<T, TN, BACKWARD, WIDE>, 232448, configured);
+}
+template <typename T, bool BACKWARD, int C> int allow_pair() {
+  static bool configured[64] = {false};
+  return allow_smem(gated_pair_kernel<T, BACKWARD, C>, PairSmem::kDynamic, configured);
+}
+template <typename T, bool BACKWARD, int C> int resident_pairs() {
+  static int cache[64] = {0};
+  return resident_cached(gated_pair_kernel<T, BACKWARD, C>, kPairThreads, PairSmem::kDynamic, 2, cache);
+}
+
+// (the occupancy query needs allow_split first)
 template <typename T, int TN, bool BACKWARD> SplitPlan plan_split(int M, int I, int num_kb) {
   using L = SplitSmem<TN, false>;
   static int cache[4][64] = {};
@@ -1014,44 +1090,95 @@ template <int TN> SplitPlan plan_wide(int M, int I, int num_kb) {
   return {1, 0, channels, stages > num_kb ? num_kb : stages, (double)waves * (5.3 + 0.03 * M + num_kb * step)};
 }
 
-// Runs the split kernel where its estimate is below `limit_us`, else says so in *ran.
-template <typename T, int TN, bool BACKWARD, bool WIDE>
-int launch_split(const void *x, const void *wg, const void *wu, const void *dh, void *out, void *out2, int M, int I, int K, int act, double limit_us, bool *ran,
-                 cudaStream_t st) {
-  using L = SplitSmem<TN, WIDE>;
-  auto kern = gated_split_kernel<T, TN, BACKWARD, WIDE>;
-  static bool configured[64] = {false};
-  int rc = allow_smem(kern, 232448, configured);
+// The first stage: its operands, and by which kernel it is done.
+struct Projection {
+  const void *x, *wg, *wu, *dh;
+  void *out, *out2;  // H, or dG and dU
+  float *largest;    // as in ProjArgs
+  int M, I, K, act;
+};
+struct Choice {
+  int tokens;   // of the split kernels' tile; 0: pairs
+  bool wide;    // split kernel
+  int channels; // of the pairs' tile
+  SplitPlan split;
+  int ctas;
+};
+
+// Backward, kRanged: launched twice, the second time to be run where the first one's exponent did not fit.
+template <typename T, bool BACKWARD, int C> int launch_pair(const Projection &p, const Choice &choice, cudaStream_t st) {
+  auto kern = gated_pair_kernel<T, BACKWARD, C>;
+  int rc = allow_pair<T, BACKWARD, C>();
   if (rc != QL_OK) return rc;
+  ProjArgs a;
+  a.dh = p.dh;
+  a.M = p.M, a.I = p.I, a.K = p.K, a.act = p.act;
+  a.layers = grad_layers(p.M, p.I, p.K);
+  a.largest = p.largest;
+  a.num_kb = (p.K + 63) / 64;
+  a.tiles_m = (p.M + 255) / 256;
+  a.tiles_n = (p.I + C - 1) / C;
+  a.group_m = band((int64_t)p.K * 2, a.tiles_m);
+  a.status = device_status_word();
+  if (!a.status) return set_error(QL_ERR_CUDA, "gated_linear: could not allocate the device status word");
+  CUtensorMap mx, mg, mu, mo, mo2;
+  const int kind = kMapKind<T>, dtype = FloatIO<T>::kDtype;
+  if ((rc = encode_map(&mx, kind, p.x, p.M, p.K, 128)) != QL_OK) return rc;
+  if ((rc = encode_map(&mg, kind, p.wg, p.I, p.K, C)) != QL_OK) return rc;
+  if ((rc = encode_map(&mu, kind, p.wu, p.I, p.K, C)) != QL_OK) return rc;
+  if ((rc = encode_map_narrow(&mo, dtype, p.out, p.M, p.I, BACKWARD ? a.layers : 0)) != QL_OK) return rc;
+  mo2 = mo; // forward: not used
+  if (BACKWARD && (rc = encode_map_narrow(&mo2, dtype, p.out2, p.M, p.I, a.layers)) != QL_OK) return rc;
+  for (a.again = 0; a.again < (BACKWARD && kRanged<T> ? 2 : 1); a.again++) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)choice.ctas, 1, 1);
+    cfg.blockDim = dim3(kPairThreads, 1, 1);
+    cfg.dynamicSmemBytes = PairSmem::kDynamic;
+    cfg.stream = st;
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &early;
+    cfg.numAttrs = a.again;
+    QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, mx, mg, mu, mo, mo2, a));
+    count_launches(1);
+  }
+  return QL_OK;
+}
+template <typename T, int TN, bool BACKWARD, bool WIDE> int launch_split(const Projection &p, const Choice &choice, cudaStream_t st) {
+  using L = SplitSmem<TN, WIDE>;
+  int rc = allow_split<T, TN, BACKWARD, WIDE>();
+  if (rc != QL_OK) return rc;
+  const SplitPlan &plan = choice.split;
   SplitArgs a;
-  a.dh = dh, a.out = out, a.out2 = out2;
-  a.M = M, a.I = I, a.act = act, a.layers = grad_layers(M, I, K);
-  a.num_kb = (K + 63) / 64;
-  SplitPlan plan;
-  if constexpr (WIDE) plan = plan_wide<TN>(M, I, a.num_kb);
-  else plan = plan_split<T, TN, BACKWARD>(M, I, a.num_kb);
-  *ran = plan.us <= limit_us;
-  if (!*ran) return QL_OK;
-  a.tiles_c = (I + plan.channels - 1) / plan.channels;
+  a.dh = p.dh, a.out = p.out, a.out2 = p.out2;
+  a.M = p.M, a.I = p.I, a.act = p.act, a.layers = grad_layers(p.M, p.I, p.K);
+  a.largest = p.largest;
+  a.num_kb = (p.K + 63) / 64;
+  a.tiles_c = (p.I + plan.channels - 1) / plan.channels;
   a.status = device_status_word();
   if (!a.status) return set_error(QL_ERR_CUDA, "gated_linear: could not allocate the device status word");
   CUtensorMap mg, mu, mx;
   const int kind = kMapKind<T>;
-  if ((rc = encode_map(&mg, kind, wg, I, K, plan.channels)) != QL_OK) return rc;
-  if ((rc = encode_map(&mu, kind, wu, I, K, plan.channels)) != QL_OK) return rc;
-  if ((rc = encode_map(&mx, kind, x, M, K, TN)) != QL_OK) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(((int64_t)a.tiles_c * ((M + TN - 1) / TN)) << plan.log2), 1, 1);
-  cfg.blockDim = dim3(kSplitThreads<WIDE>, 1, 1);
-  cfg.dynamicSmemBytes = L::total(plan.channels, plan.stages);
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = 1u << plan.log2, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, mg, mu, mx, a, plan.channels, plan.stages, plan.log2));
-  count_launches(1);
+  if ((rc = encode_map(&mg, kind, p.wg, p.I, p.K, plan.channels)) != QL_OK) return rc;
+  if ((rc = encode_map(&mu, kind, p.wu, p.I, p.K, plan.channels)) != QL_OK) return rc;
+  if ((rc = encode_map(&mx, kind, p.x, p.M, p.K, TN)) != QL_OK) return rc;
+  for (a.again = 0; a.again < (BACKWARD && kRanged<T> ? 2 : 1); a.again++) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)choice.ctas, 1, 1);
+    cfg.blockDim = dim3(kSplitThreads<WIDE>, 1, 1);
+    cfg.dynamicSmemBytes = L::total(plan.channels, plan.stages);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1u << plan.log2, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1 + a.again;
+    QL_CUDA_TRY(cudaLaunchKernelEx(&cfg, gated_split_kernel<T, TN, BACKWARD, WIDE>, mg, mu, mx, a, plan.channels, plan.stages, plan.log2));
+    count_launches(1);
+  }
   return QL_OK;
 }
 
@@ -1063,8 +1190,7 @@ int launch_split(const void *x, const void *wg, const void *wu, const void *dh, 
 //   211 x 2744 x 1032   split 20.9, pairs 13.3, of 64 channels 10.5  |  256 x 9472 x 4096  pairs 36.1, of 64 channels 41.7
 //   128 x 11008 x 4096  pairs 50.1, wide split 39.4  |  64 x 11008 x 4096  pairs 50.1, wide split 36.0
 //   128 x 9472 x 2048   pairs 19.8, wide split 21.9  |  512 x 2368 x 4096  pairs 25.9, of 64 channels 20.9
-template <typename T, bool BACKWARD>
-int project(const void *x, const void *wg, const void *wu, const void *dh, void *out, void *out2, int M, int I, int K, int act, cudaStream_t st) {
+template <typename T, bool BACKWARD> Choice choose(int M, int I, int K) {
   const int num_kb = (K + 63) / 64;
   auto pairs_us = [&](int c, double fixed, double step, double next) {
     const int64_t pairs = sm_count() / 2, rows = (M + 255) / 256, tiles = rows * ((I + c - 1) / c), rest = tiles % pairs;
@@ -1075,23 +1201,43 @@ int project(const void *x, const void *wg, const void *wu, const void *dh, void 
   const double full_us = pairs_us(128, 7.2, 0.28, 0.3), narrow_us = pairs_us(64, 5.2, 0.23, 0.8);
   const bool narrow = narrow_us < full_us;
   const double pair_us = M <= 32 ? 1e30 : (narrow ? narrow_us : full_us);
-  bool ran = false;
-  int rc;
-  if (M <= 16) {
-    rc = launch_split<T, 16, BACKWARD, false>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us, &ran, st);
-  } else if (M <= 32) {
-    rc = launch_split<T, 32, BACKWARD, false>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us, &ran, st);
-  } else if (M <= 64) {
-    const double wide_us = plan_wide<64>(M, I, num_kb).us;
-    rc = launch_split<T, 64, BACKWARD, false>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us < wide_us ? pair_us : wide_us, &ran, st);
-    if (rc == QL_OK && !ran) rc = launch_split<T, 64, BACKWARD, true>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us, &ran, st);
-  } else {
-    const double wide_us = M <= 128 ? plan_wide<128>(M, I, num_kb).us : 1e30;
-    rc = launch_split<T, 128, BACKWARD, false>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us < wide_us ? pair_us : wide_us, &ran, st);
-    if (rc == QL_OK && !ran && M <= 128) rc = launch_split<T, 128, BACKWARD, true>(x, wg, wu, dh, out, out2, M, I, K, act, pair_us, &ran, st);
+  Choice ch = {};
+  // the split kernel of TN tokens, where its estimate is no larger than `limit_us`
+  auto split = [&](auto tn, auto wide, double limit_us) {
+    constexpr int TN = decltype(tn)::value;
+    constexpr bool WIDE = decltype(wide)::value;
+    allow_split<T, TN, BACKWARD, WIDE>(); // where it fails, so does the launch
+    if constexpr (WIDE) ch.split = plan_wide<TN>(M, I, num_kb);
+    else ch.split = plan_split<T, TN, BACKWARD>(M, I, num_kb);
+    ch.tokens = ch.split.us <= limit_us ? TN : 0, ch.wide = WIDE;
+    ch.ctas = (int)(((int64_t)((I + ch.split.channels - 1) / ch.split.channels) * ((M + TN - 1) / TN)) << ch.split.log2);
+    return ch.tokens != 0;
+  };
+  auto either = [&](auto tn) { // split or wide
+    const double wide_us = M <= 128 ? plan_wide<decltype(tn)::value>(M, I, num_kb).us : 1e30;
+    return split(tn, std::false_type{}, pair_us < wide_us ? pair_us : wide_us) || (M <= 128 && split(tn, std::true_type{}, pair_us));
+  };
+  if (M <= 16) split(std::integral_constant<int, 16>{}, std::false_type{}, pair_us);
+  else if (M <= 32) split(std::integral_constant<int, 32>{}, std::false_type{}, pair_us);
+  else if (M <= 64) either(std::integral_constant<int, 64>{});
+  else either(std::integral_constant<int, 128>{});
+  if (ch.tokens == 0) {
+    ch.channels = narrow ? 64 : 128;
+    (void)(narrow ? allow_pair<T, BACKWARD, 64>() : allow_pair<T, BACKWARD, 128>());
+    const int tiles = ((M + 255) / 256) * ((I + ch.channels - 1) / ch.channels);
+    const int pairs = narrow ? resident_pairs<T, BACKWARD, 64>() : resident_pairs<T, BACKWARD, 128>();
+    ch.ctas = 2 * (tiles < pairs ? tiles : pairs);
   }
-  if (rc != QL_OK || ran) return rc;
-  return narrow ? launch_pair<T, BACKWARD, 64>(x, wg, wu, dh, out, out2, M, I, K, act, st) : launch_pair<T, BACKWARD, 128>(x, wg, wu, dh, out, out2, M, I, K, act, st);
+  return ch;
+}
+template <typename T, bool BACKWARD> int project(const Projection &p, const Choice &ch, cudaStream_t st) {
+  switch (ch.tokens) {
+  case 16: return launch_split<T, 16, BACKWARD, false>(p, ch, st);
+  case 32: return launch_split<T, 32, BACKWARD, false>(p, ch, st);
+  case 64: return ch.wide ? launch_split<T, 64, BACKWARD, true>(p, ch, st) : launch_split<T, 64, BACKWARD, false>(p, ch, st);
+  case 128: return ch.wide ? launch_split<T, 128, BACKWARD, true>(p, ch, st) : launch_split<T, 128, BACKWARD, false>(p, ch, st);
+  default: return ch.channels == 64 ? launch_pair<T, BACKWARD, 64>(p, ch, st) : launch_pair<T, BACKWARD, 128>(p, ch, st);
+  }
 }
 
 // How the units of the second products are cut and dealt out (see GradArgs), for `pairs` CTA pairs.
@@ -1142,6 +1288,7 @@ GradPlan plan_grads(int M, int I, int K, bool want_x, bool want_w, int pairs) {
   a.heavy_w = hw < 0 ? 0 : (int)(hw + 0.5);
   a.group_m = 8; // row tiles walked together; 4, 8, 16, 32 on 4096 x 11008 x 4096: 1.62, 1.55, 1.59, 1.54 ms; on 1024 x 28672 x 8192: 2.12, 2.10, 2.10, 2.20
   a.x_parts = a.w_parts = nullptr;
+  a.largest = nullptr, a.num_largest = 0;
   p.x_part_floats = x_tiles > 0 && a.x_split * a.layers > 1 ? (int64_t)a.x_split * a.layers * M * K : 0;
   p.w_part_floats = w_tiles > 0 && a.w_split > 1 ? 2ll * a.w_split * I * K : 0;
   return p;
@@ -1172,18 +1319,36 @@ template <typename T> int grad_pairs() {
 }
 int pairs_of(int dtype) { return dtype == QL_BF16 ? grad_pairs<__nv_bfloat16>() : grad_pairs<__half>(); }
 
+// A backward call: the first stage's kernel, the second's plan, and where things lie in the workspace.
+struct BackwardPlan {
+  Choice first;
+  GradPlan grads;
+  int64_t mi, x_parts, w_parts, largest, bytes; // offsets; dG at 0, dU at mi
+};
+BackwardPlan plan_backward(int dtype, int M, int I, int K, bool want_x, bool want_w) {
+  BackwardPlan p;
+  p.first = dtype == QL_BF16 ? choose<__nv_bfloat16, true>(M, I, K) : choose<__half, true>(M, I, K);
+  p.grads = plan_grads(M, I, K, want_x, want_w, pairs_of(dtype));
+  p.mi = align256((int64_t)p.grads.a.layers * M * I * 2);
+  p.x_parts = 2 * p.mi;
+  p.w_parts = p.x_parts + align256(p.grads.x_part_floats * 4);
+  p.largest = p.w_parts + align256(p.grads.w_part_floats * 4);
+  p.bytes = p.largest + (dtype == QL_F16 ? align256((int64_t)p.first.ctas * 4) : 0);
+  return p;
+}
+
 template <typename T>
-int backward(const void *dh, const void *x, const void *wg, const void *wu, void *dx, void *dwg, void *dwu, int M, int I, int K, int act, uint8_t *ws, const GradPlan &plan,
+int backward(const void *dh, const void *x, const void *wg, const void *wu, void *dx, void *dwg, void *dwu, int M, int I, int K, int act, uint8_t *ws, const BackwardPlan &plan,
              cudaStream_t st) {
-  const int64_t mi = align256((int64_t)plan.a.layers * M * I * 2);
-  void *dg = ws, *du = ws + mi;
-  int rc = project<T, true>(x, wg, wu, dh, dg, du, M, I, K, act, st);
-  if (rc != QL_OK || (!dx && !dwg)) return rc;
-  GradArgs a = plan.a;
+  void *dg = ws, *du = ws + plan.mi;
+  float *largest = reinterpret_cast<float *>(ws + plan.largest);
+  int rc = project<T, true>({x, wg, wu, dh, dg, du, largest, M, I, K, act}, plan.first, st);
+  if (rc != QL_OK) return rc;
+  GradArgs a = plan.grads.a;
   a.status = device_status_word();
-  uint8_t *parts = ws + 2 * mi;
-  if (plan.x_part_floats) a.x_parts = reinterpret_cast<float *>(parts);
-  if (plan.w_part_floats) a.w_parts = reinterpret_cast<float *>(parts + align256(plan.x_part_floats * 4));
+  if (plan.grads.x_part_floats) a.x_parts = reinterpret_cast<float *>(ws + plan.x_parts);
+  if (plan.grads.w_part_floats) a.w_parts = reinterpret_cast<float *>(ws + plan.w_parts);
+  a.largest = largest, a.num_largest = plan.first.ctas;
   const int x_layers = a.x_split * a.layers;
   CUtensorMap dgk, duk, dgm, dum, wgm, wum, xm, mx, mg, mu;
   const int kind = kMapKind<T>, dtype = FloatIO<T>::kDtype;
@@ -1274,8 +1439,8 @@ extern "C" int ql_gated_linear(const ql_tensor *x, const ql_tensor *w_gate, cons
     QL_CUDA_TRY(cudaMemsetAsync(h->data, 0, (size_t)numel(h) * 2, st));
     return QL_OK;
   }
-  return x->dtype == QL_BF16 ? project<__nv_bfloat16, false>(x->data, w_gate->data, w_up->data, nullptr, h->data, nullptr, M, I, K, activation, st)
-                             : project<__half, false>(x->data, w_gate->data, w_up->data, nullptr, h->data, nullptr, M, I, K, activation, st);
+  const Projection p = {x->data, w_gate->data, w_up->data, nullptr, h->data, nullptr, nullptr, M, I, K, activation};
+  return x->dtype == QL_BF16 ? project<__nv_bfloat16, false>(p, choose<__nv_bfloat16, false>(M, I, K), st) : project<__half, false>(p, choose<__half, false>(M, I, K), st);
 }
 
 extern "C" int ql_gated_linear_backward_workspace(const ql_tensor *x, const ql_tensor *w_gate, int32_t want_dx, int32_t want_dw, int64_t *bytes) {
@@ -1285,8 +1450,7 @@ extern "C" int ql_gated_linear_backward_workspace(const ql_tensor *x, const ql_t
   if (M < 0 || K < 0 || I < 0 || M > (1 << 30) || K > (1 << 30) || I > (1 << 30)) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: bad shape", op);
   *bytes = 0;
   if (M == 0 || K == 0 || I == 0) return QL_OK;
-  const GradPlan p = plan_grads((int)M, (int)I, (int)K, want_dx != 0, want_dw != 0, pairs_of(x->dtype));
-  *bytes = 2 * align256(p.a.layers * M * I * 2) + align256(p.x_part_floats * 4) + align256(p.w_part_floats * 4);
+  *bytes = plan_backward(x->dtype, (int)M, (int)I, (int)K, want_dx != 0, want_dw != 0).bytes;
   return QL_OK;
 }
 
@@ -1313,9 +1477,9 @@ extern "C" int ql_gated_linear_backward(const ql_tensor *grad, const ql_tensor *
     return QL_OK;
   }
   if (!dx && !dw_gate) return QL_OK;
-  int64_t need = 0;
-  if ((rc = ql_gated_linear_backward_workspace(x, w_gate, dx != nullptr, dw_gate != nullptr, &need)) != QL_OK) return rc;
-  if (!workspace || workspace_bytes < need) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %lld bytes, got %lld", op, (long long)need, (long long)(workspace ? workspace_bytes : 0));
+  const BackwardPlan plan = plan_backward(x->dtype, M, I, K, dx != nullptr, dw_gate != nullptr);
+  if (!workspace || workspace_bytes < plan.bytes)
+    return set_error(QL_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %lld bytes, got %lld", op, (long long)plan.bytes, (long long)(workspace ? workspace_bytes : 0));
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return set_error(QL_ERR_UNSUPPORTED, "%s: the workspace must be 256-byte aligned", op);
   const ql_tensor *in[4] = {grad, x, w_gate, w_up};
   for (int i = 0; i < 3; i++) {
@@ -1325,7 +1489,6 @@ extern "C" int ql_gated_linear_backward(const ql_tensor *grad, const ql_tensor *
       if (overlap(out[i], out[j])) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: %s and %s must not overlap", op, name[j], name[i]);
   }
   if (!device_status_word()) return set_error(QL_ERR_CUDA, "%s: could not allocate the device status word", op);
-  const GradPlan plan = plan_grads(M, I, K, dx != nullptr, dw_gate != nullptr, pairs_of(x->dtype));
   void *p[3] = {dx ? dx->data : nullptr, dw_gate ? dw_gate->data : nullptr, dw_up ? dw_up->data : nullptr};
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   return x->dtype == QL_BF16 ? backward<__nv_bfloat16>(grad->data, x->data, w_gate->data, w_up->data, p[0], p[1], p[2], M, I, K, activation, ws, plan, st)

@@ -63,7 +63,9 @@ def gated_linear_backward(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Ten
     """(dx, dw_gate, dw_up) of gated_linear from `grad`, the gradient of its result [..., I]; None for what is not needed.
     Nothing is kept from the forward pass: the projections are computed again, their gradients are formed in f32 and rounded
     to the operands' type for the second products (of up to 64 tokens with the rounding's remainder beside it, so that only
-    the results' own rounding is left).  Gradients have the type of what they belong to."""
+    the results' own rounding is left).  In float16 they are held times a power of two chosen on the device from their largest
+    magnitude: gradients may be of any size, and a token's keep all their digits down to 2^-16 of the largest.  Gradients have
+    the type of what they belong to."""
     act = _activation(activation)
     x2, g2 = _rows(x, "x"), _rows(grad, "grad")
     if grad.shape[:-1] != x.shape[:-1]:
