@@ -150,8 +150,8 @@ QL_API int ql_gemm_nvfp4(const ql_tensor *a, const ql_tensor *a_scales, const ql
  * a NaN gets the scale NaN and zero data: it dequantizes to NaN.  input: f32 | f16 | bf16 [..., K], K % 32 == 0;
  * data: QL_F4E2M1 of the input's shape (buffer of numel / 2 bytes); scales: QL_F8E8M0 [..., K / 32].
  * ql_dequantize_mxfp4: output = data * scale, rounded to f32 | f16 | bf16.
- * 16-byte aligned floating-point buffers and 4-byte aligned data (QL_ERR_UNSUPPORTED otherwise); results overlap nothing
- * else (QL_ERR_INVALID_ARGUMENT, as in the three entries below). */
+ * 16-byte aligned floating-point buffers and 4-byte aligned data (QL_ERR_UNSUPPORTED otherwise); results and workspaces
+ * overlap nothing else (QL_ERR_INVALID_ARGUMENT, as in the three entries below). */
 QL_API int ql_quantize_mxfp4(const ql_tensor *input, ql_tensor *data, ql_tensor *scales, void *stream);
 QL_API int ql_dequantize_mxfp4(const ql_tensor *data, const ql_tensor *scales, ql_tensor *output, void *stream);
 

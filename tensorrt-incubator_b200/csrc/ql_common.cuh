@@ -47,6 +47,13 @@ static inline bool overlap(const ql_tensor *a, const ql_tensor *b) {
   return pa < pb + (uintptr_t)byte_size(b) && pb < pa + (uintptr_t)byte_size(a);
 }
 
+// A caller's workspace as a tensor, for overlap().
+static inline ql_tensor workspace_view(void *p, int64_t bytes) {
+  ql_tensor t = {};
+  t.data = p, t.dtype = QL_I8, t.rank = 1, t.shape[0] = bytes;
+  return t;
+}
+
 // Where the scale of element i lives:  idx(i) = ((i / a) % b) * c + (i % d) / e
 //   per-tensor            a=1 b=1 c=0 d=1 e=1
 //   per-channel           a=inner b=C c=1 d=1 e=1          (tensor seen as [outer, C, inner])

@@ -1482,6 +1482,9 @@ extern "C" int ql_gated_linear_backward(const ql_tensor *grad, const ql_tensor *
     return set_error(QL_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %lld bytes, got %lld", op, (long long)plan.bytes, (long long)(workspace ? workspace_bytes : 0));
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return set_error(QL_ERR_UNSUPPORTED, "%s: the workspace must be 256-byte aligned", op);
   const ql_tensor *in[4] = {grad, x, w_gate, w_up};
+  const ql_tensor scratch = workspace_view(workspace, plan.bytes);
+  for (int i = 0; i < 4; i++)
+    if (overlap(&scratch, in[i]) || (i < 3 && overlap(&scratch, out[i]))) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: the workspace must not overlap an operand or a gradient", op);
   for (int i = 0; i < 3; i++) {
     for (int j = 0; j < 4; j++)
       if (overlap(out[i], in[j])) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: %s must not overlap an operand", op, name[i]);

@@ -1061,6 +1061,9 @@ extern "C" int ql_gemm_mxfp4(const ql_tensor *a, const ql_tensor *a_scales, cons
     return set_error(QL_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %lld bytes, got %lld", op, (long long)need, (long long)(workspace ? workspace_bytes : 0));
   if (need > 0 && !aligned16(workspace)) return set_error(QL_ERR_UNSUPPORTED, "%s: the workspace must be 16-byte aligned", op);
   if (overlap(y, a) || overlap(y, a_scales) || overlap(y, b) || overlap(y, b_scales)) return set_error(QL_ERR_INVALID_ARGUMENT, "%s: y must not overlap an operand", op);
+  const ql_tensor scratch = workspace_view(workspace, need);
+  if (overlap(&scratch, y) || overlap(&scratch, a) || overlap(&scratch, a_scales) || overlap(&scratch, b) || overlap(&scratch, b_scales))
+    return set_error(QL_ERR_INVALID_ARGUMENT, "%s: the workspace must not overlap y or an operand", op);
   cudaStream_t st = (cudaStream_t)stream;
 
   MxArgs args;
