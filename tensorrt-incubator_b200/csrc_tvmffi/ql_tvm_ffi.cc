@@ -55,6 +55,9 @@ bool int_arg(const TVMFFIAny &a, int64_t *out) {
   return false;
 }
 
+// The number of a ql_activation; what 32 bits do not hold is none of them.
+int32_t activation(int64_t v) { return v == (int32_t)v ? (int32_t)v : -1; }
+
 // DLTensor -> ql_tensor.  `packed` reinterprets a uint8 [..., K/2] tensor as int4 (1) or e2m1 (2) [..., K], or takes uint8 for
 // e8m0 (kE8M0).
 constexpr int kE8M0 = 3;
@@ -350,7 +353,7 @@ TVM_FFI_DLL_EXPORT int __tvm_ffi_ql_gated_linear(void *, const TVMFFIAny *args, 
   int64_t act;
   if (!int_arg(args[3], &act)) return fail("activation must be an integer");
   QL_TENSOR(4, h, 0)
-  return finish(ql_gated_linear(&x, &wg, &wu, (int32_t)act, &h, stream_of(x_dl)));
+  return finish(ql_gated_linear(&x, &wg, &wu, activation(act), &h, stream_of(x_dl)));
 }
 
 TVM_FFI_DLL_EXPORT int __tvm_ffi_ql_gated_linear_backward_workspace(void *, const TVMFFIAny *args, int32_t n, TVMFFIAny *ret) {
@@ -377,7 +380,7 @@ TVM_FFI_DLL_EXPORT int __tvm_ffi_ql_gated_linear_backward(void *, const TVMFFIAn
   QL_OPTIONAL(6, dwg)
   QL_OPTIONAL(7, dwu)
   QL_OPTIONAL(8, ws)
-  return finish(ql_gated_linear_backward(&grad, &x, &wg, &wu, (int32_t)act, dx_p ? &dx : nullptr, dwg_p ? &dwg : nullptr, dwu_p ? &dwu : nullptr, ws_p ? ws.data : nullptr,
+  return finish(ql_gated_linear_backward(&grad, &x, &wg, &wu, activation(act), dx_p ? &dx : nullptr, dwg_p ? &dwg : nullptr, dwu_p ? &dwu : nullptr, ws_p ? ws.data : nullptr,
                                          byte_count(ws_p), stream_of(x_dl)));
 }
 }
