@@ -135,10 +135,11 @@ def check(rc: int) -> None:
 
 
 def make_tensor(ptr: int, dtype: int, shape) -> QlTensor:
+    shape = tuple(map(int, shape))
     rank = len(shape)
     if rank > QL_MAX_RANK:
         raise QlError(ERR_INVALID_ARGUMENT, f"rank {rank} exceeds {QL_MAX_RANK}")
-    return QlTensor(ptr, dtype, rank, tuple(shape))   # one call: the rest of the shape is zero
+    return QlTensor(ptr, dtype, rank, shape)   # one call: the rest of the shape is zero
 
 
 def make_attrs(axis=None, fp8_mode="direct") -> QlQdqAttrs:
