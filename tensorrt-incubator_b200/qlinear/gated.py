@@ -1,6 +1,9 @@
 """Gated projection of a feed-forward block in 16 bits, and its backward pass: the unquantized counterpart of the fp8 block's
 gate/up projection (mlp.gemm_fp8_swiglu), for the block that a quantized one is made from, compared with or trained as.  The
-reference has no such operator; its pieces are tp.Linear and the activations of its frontend."""
+reference has no such operator; its pieces are tp.Linear and the activations of its frontend.
+
+As all of the package, both functions work on plain tensors and record nothing for automatic differentiation: their results require
+no gradient, whatever the operands do, and a training step calls gated_linear_backward itself."""
 from __future__ import annotations
 
 import ctypes
@@ -41,7 +44,8 @@ def _workspace_bytes(x_shape, w_shape, dtype: int, want_dx: bool, want_dw: bool,
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu", *, out=None) -> torch.Tensor:
     """act(x @ w_gate^T) * (x @ w_up^T): x [..., K], w_gate and w_up [I, K], all float16 or all bfloat16; both products,
     `activation` ("silu", "gelu", "gelu_tanh" or "relu") and the gate's product in one kernel, f32 sums, one rounding.  K and
-    I are multiples of 8; any number of rows from none up."""
+    I are multiples of 8; any number of rows from none up.  The result is detached from operands that require gradients:
+    gated_linear_backward gives theirs."""
     act = _activation(activation)
     x2 = _rows(x, "x")
     wg, wu = w_gate.contiguous(), w_up.contiguous()   # kept alive across the call: a view only borrows the pointer

@@ -49,7 +49,8 @@ class Int4Tensor:
 
 class Float4Tensor:
     """e2m1 values, two per byte with the first element in the low nibble; `packed` is a flat uint8 tensor of
-    numel / 2 bytes, `shape` the logical shape (last dimension a multiple of 16: NVFP4 blocks)."""
+    numel / 2 bytes, `shape` the logical shape.  The scales beside it say which format it belongs to: e4m3 for each 16 values
+    along the last dimension (NVFP4, dynamic_quantize), or e8m0 for each 32 (MXFP4, quantize_mxfp4)."""
 
     dtype = dt.float4
     _VALUES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
